@@ -75,7 +75,7 @@ void q8_destroy(q8_ctx *ctx);
  * streams are not ordered, except that one that uses the context's scratch
  * (q8_linear of more than 4 rows or of unaligned ones, q8_linear_bf16act, _swiglu
  * and _rmsnorm, q8_head_argmax, q8_decode_attention, q8_attention from 16
- * rows on, q8_graph_launch) starts behind the last such call on another
+ * rows on, q8_kv8_attention, q8_pages_reserve and _compact, q8_graph_launch) starts behind the last such call on another
  * stream; for that, a stream stays valid until another one is set, or
  * until q8_sync has returned on it.  A graph that the caller captured and
  * launches by itself is not seen by this. */
@@ -392,6 +392,126 @@ int q8_pos_advance(q8_ctx *ctx, q8_buf *posbuf, uint64_t opos_i32, int64_t s);
 int q8_token_begin(q8_ctx *ctx, q8_buf *ids, uint64_t oid_i32, int32_t id, q8_buf *posbuf,
                    uint64_t opos_i32, int32_t pos, q8_buf *w, uint64_t oemb_u16, q8_buf *a,
                    uint64_t ox_f32, int64_t d, int64_t vocab, int G, int scale_dtype);
+
+/* ---- several sequences at once --------------------------------------------------
+ * Prompts and token steps of many sequences in one call, and a KV cache held in
+ * 8 bits in pages.  (No counterpart in the reference, which serves one sequence
+ * over a dense f32 cache.)
+ *
+ * Rows.  Sequence i has the rows cu[i] .. cu[i+1]-1 of the packed arrays; cu are
+ * nseq + 1 ascending int32 at element offset ocu of `ix`, from 0 to at most
+ * `rows`, on the device like every int32 array here, so that captured steps
+ * serve all lengths.  A sequence may have no rows; rows from cu[nseq] on are
+ * left as they are.  The calls keep to their buffers whatever the arrays hold.
+ *
+ * Cache.  A page holds `page` (16, 32, 64 or 128) tokens of one layer,
+ * q8_kv8_page_bytes() bytes: K codes [nkv][page][head_dim] and V codes
+ * [nkv][head_dim][page] (int8), then the K scales [nkv] and the V scales [nkv]
+ * (f32; one number per page and KV head), padded to 16 bytes; a stored value is
+ * code * scale.  The npages pages of a layer lie one after the other at byte
+ * offset opages of `pages` (16-byte aligned).  Token t of sequence i is in page
+ * table[i][t / page] (int32 [nseq][maxpages]); len[i] tokens are cached before
+ * the call, whose rows follow at positions len[i], len[i] + 1, ...  All layers
+ * share the table and the lengths; q8_pages_set_len advances them after the
+ * last layer.  head_dim 64 or 128, any nheads / nkv; up to 4096 sequences. */
+
+/* out [rows, nheads*head_dim] = causal attention of each packed prompt over its
+ * own rows: row r of sequence i attends rows cu[i] .. r, query head h reads KV
+ * head h / (nheads / nkv), scores scaled by 1/sqrt(head_dim).  q and out are f32
+ * or bf16 (act_dtype Q8_SRC_F32 / Q8_SRC_BF16; offsets oq and oy in elements of
+ * that type), row r of q at oq + r*ldq (ldq = 0: nheads*head_dim, dense), out
+ * dense; K and V are binary16 rows [rows, nkv*head_dim] at okc and ovc of kv, as
+ * q8_rope_kv and q8_kv8_append write them.  f32 q keeps f32 accuracy (<= 1e-5),
+ * bf16 q rounds the probabilities to binary16.  head_dim 64 or 128, nheads / nkv
+ * up to 128, rows up to 2^24; q, out, K and V rows start 16-byte aligned
+ * (Q8_ERR_UNSUPPORTED otherwise).  Values that a row does not see, infinities
+ * and NaN included, do not reach it. */
+int q8_attention_packed(q8_ctx *ctx, q8_buf *q, uint64_t oq, int act_dtype, int64_t ldq, q8_buf *kv,
+                        uint64_t okc_f16, uint64_t ovc_f16, q8_buf *out, uint64_t oy, q8_buf *ix,
+                        uint64_t ocu_i32, int64_t nseq, int64_t rows, int nheads, int nkv,
+                        int head_dim);
+
+/* Bytes of a cache page, 0 for sizes that the cache does not take. */
+uint64_t q8_kv8_page_bytes(int page, int nkv, int head_dim);
+
+/* RoPE (rotate_half; head_dim/2 inverse frequencies at oinv) of q and k at each
+ * row's position, and the append of the rotated k and of v to the cache.  Row r
+ * of q, k and v at oq, ok, ov + r*ld (ld = 0: each dense); the rotated q goes to
+ * oqr + r*ldr (ldr = 0: dense; oqr = oq at the same stride: in place), k and v
+ * are left as they were.  With kv non-null the rotated k and v are also stored
+ * as binary16 rows [rows, nkv*head_dim] at okc and ovc of kv (the prompt rows
+ * that q8_attention_packed reads).
+ * Angles are formed to 64 bits and a rotated key is rounded to f32 once.  A
+ * page's scale of a head is s = max(s_old, max |x| / 127) over the new rows x
+ * (s_old counts where the page holds older tokens of the sequence), codes are
+ * the quotients x / s rounded to the nearest, ties to even; where the scale
+ * grows, the older tokens' codes become code * s_old / s rounded likewise.  A
+ * page that takes a NaN or an infinity gets the scale NaN: every row that sees
+ * one of its tokens is NaN from then on.  Rows whose page is missing (an id
+ * outside [0, npages), positions from maxpages*page on) are not stored.  Pages
+ * that are written must belong to one sequence alone (q8_pages_reserve). */
+int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint64_t ov_f32,
+                  uint64_t oinv_f32, uint64_t oqr_f32, int64_t ld, int64_t ldr, q8_buf *kv,
+                  uint64_t okc_f16, uint64_t ovc_f16, q8_buf *pages, uint64_t opages,
+                  int64_t npages, int page, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32,
+                  uint64_t otab_i32, int64_t nseq, int64_t rows, int64_t maxpages, int nheads,
+                  int nkv, int head_dim);
+
+/* out [rows, nheads*head_dim] at oy = causal attention of the rotated q at oq
+ * (row stride ldq, 0: dense) over the 8-bit cache: row j of sequence i attends
+ * its cached tokens 0 .. len[i] + j (those of this call's rows included, so
+ * q8_kv8_append comes first), one row a sequence or several (drafted tokens, a
+ * prompt's next chunk).  Within 1e-5 of float64 over the stored values.  A row
+ * that sees a missing page is NaN.  The split records live in the context's
+ * scratch (q8_set_stream). */
+int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
+                     q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+                     uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
+                     int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim);
+
+/* Pages.  The state of nslots slots (sequences) over a pool of npages pages is
+ * four int32 arrays of `ix`: table [nslots][maxpages], -1 behind the held pages;
+ * len [nslots] tokens; held [nslots] pages; ref [npages], the table entries that
+ * name a page (0: free).  A new state is table -1 and the rest 0.  Every call is
+ * asynchronous, reads no result on the host and depends on its inputs alone:
+ * pages are taken from the lowest free id up, slots served in ascending order.
+ * `page` is the tokens of a page.  Up to 4096 slots.  A pool is `layers` runs of
+ * npages pages of page_bytes, layer_stride bytes apart, at byte opages of
+ * `pages`: any paged cache in multiples of 16 bytes, the 8-bit one among them. */
+
+/* Room for want[s] tokens in each slot s (at most maxpages*page): the pages it
+ * lacks are taken from the free ones; and a slot that is to grow (want > len) and
+ * whose last page is partly filled and shared gets a page of its own in its
+ * place, with the contents copied in every layer.  (Slots that share a page and
+ * grow in the same call each get a copy.)  Where the free pages do not reach,
+ * the slots from the first that does not fit on get nothing: held says so. */
+int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
+                     uint64_t oheld_i32, uint64_t oref_i32, uint64_t owant_i32, int64_t nslots,
+                     int64_t maxpages, int64_t npages, int page, q8_buf *pages, uint64_t opages,
+                     uint64_t page_bytes, int64_t layers, uint64_t layer_stride);
+
+/* len[s] = new[s] (at most what the held pages hold; new[s] < 0 leaves the slot
+ * alone), and the pages behind it are released: the advance after a step, the
+ * return of rejected tokens and, with 0, the end of a sequence. */
+int q8_pages_set_len(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
+                     uint64_t oheld_i32, uint64_t oref_i32, uint64_t onew_i32, int64_t nslots,
+                     int64_t maxpages, int64_t npages, int page);
+
+/* Slot s becomes a fork of slot source[s], as that was before the call (an id
+ * outside [0, nslots) leaves the slot alone): it names the same pages, and what
+ * it held is released.  Nothing is copied until one of them grows
+ * (q8_pages_reserve). */
+int q8_pages_fork(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32, uint64_t oheld_i32,
+                  uint64_t oref_i32, uint64_t osource_i32, int64_t nslots, int64_t maxpages,
+                  int64_t npages);
+
+/* Moves the pages in use to the ids 0 .. n-1 (those from n on, ascending, to the
+ * free ids below n, ascending), their contents in every layer, and the tables and
+ * counts with them; n goes to `live`.  Up to about 5.5 million pages. */
+int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_i32,
+                     uint64_t oref_i32, uint64_t olive_i32, int64_t nslots, int64_t maxpages,
+                     int64_t npages, q8_buf *pages, uint64_t opages, uint64_t page_bytes,
+                     int64_t layers, uint64_t layer_stride);
 
 /* ---- HIP graphs ------------------------------------------------------------ */
 

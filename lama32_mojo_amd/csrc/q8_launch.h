@@ -251,4 +251,69 @@ struct TokenBeginArgs {
 };
 hipError_t launch_token_begin(const TokenBeginArgs &a, hipStream_t st);
 
+
+// ---- several sequences at once (q8_packed.hip, q8_kv8.hip, q8_pages.hip) ------
+// Sequence i has the rows cu[i] .. cu[i+1]-1 (q8_ragged.h).
+struct PackedAttnArgs {
+  const void *q;           // row r at q + r * ldq elements (f32 or bf16)
+  bool bf16;               // type of q and out
+  const __half *kc, *vc;   // [rows, nkv * head_dim]
+  void *out;               // [rows, nheads * head_dim]
+  const int *cu;
+  int64_t nseq, rows;
+  int nheads, nkv, head_dim;
+  int64_t ldq;
+};
+hipError_t launch_attention_packed(const PackedAttnArgs &a, hipStream_t st);
+
+// A layer's pages and the int32 state of the sequences (kv8_page_bytes).
+struct Kv8Args {
+  uint8_t *pages;
+  int64_t npages;
+  int page;                // tokens of a page: 16, 32, 64 or 128
+  const int *cu, *len, *tab;
+  int64_t nseq, rows, maxpages;
+  int nheads, nkv, head_dim;
+};
+struct Kv8AppendArgs {
+  Kv8Args c;
+  const float *q, *k, *v;  // row r of q at q + r * ldq, of k and v at + r * ldk
+  const float *inv;        // head_dim / 2 inverse frequencies
+  float *qr;               // rotated q, row r at qr + r * ldr (qr == q: in place)
+  int64_t ldq, ldk, ldr;
+  __half *krow, *vrow;     // binary16 rows [rows, nkv * head_dim] or null
+};
+hipError_t launch_kv8_append(const Kv8AppendArgs &a, hipStream_t st);
+struct Kv8AttnArgs {
+  Kv8Args c;
+  const float *q;          // rotated, row r at q + r * ldq
+  int64_t ldq;
+  float *out;              // [rows, nheads * head_dim]
+  float *ws;               // split records, 16-byte aligned
+  int64_t ws_floats;
+};
+// Sequences of one call: their unit counts are summed in LDS.
+constexpr int kKv8MaxSeq = 4096;
+hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st);
+
+struct PagesArgs {
+  int *tab, *len, *held, *ref;   // [nslots][maxpages], [nslots], [nslots], [npages]
+  int64_t nslots, maxpages, npages;
+  int page;
+};
+// Layers of pages, `stride` bytes apart.
+struct PagePool {
+  uint8_t *pages;
+  int64_t page_bytes, layers, stride;
+};
+constexpr int kPagesMaxSlots = 4096;   // lengths and tables of a column in LDS
+// ws: 2 * nslots + 1 ints (the copies to make).
+hipError_t launch_pages_reserve(const PagesArgs &a, const int *want, const PagePool &pool, int *ws,
+                                hipStream_t st);
+hipError_t launch_pages_set_len(const PagesArgs &a, const int *new_len, hipStream_t st);
+hipError_t launch_pages_fork(const PagesArgs &a, const int *source, hipStream_t st);
+// ws: 3 * npages + 2 ints.
+hipError_t launch_pages_compact(const PagesArgs &a, int *live, const PagePool &pool, int *ws,
+                                hipStream_t st);
+
 }  // namespace q8

@@ -20,6 +20,7 @@
 
 #include "../../include/q8hip.h"
 #include "q8_launch.h"
+#include "q8_ragged.h"
 
 struct q8_ctx {
   int device = -1;
@@ -1608,6 +1609,453 @@ int q8_token_begin(q8_ctx *ctx, q8_buf *ids, uint64_t oid_i32, int32_t id, q8_bu
   t.x = w ? fptr(a, ox_f32) : nullptr;
   hipError_t e = q8::launch_token_begin(t, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "q8_token_begin launch");
+  return ok(ctx);
+}
+
+// ---- several sequences at once -----------------------------------------------------
+
+namespace {
+
+// Byte ranges of two tensors share memory (views of one allocation included).
+bool share(const q8_buf *x, uint64_t x0, uint64_t xn, const q8_buf *y, uint64_t y0, uint64_t yn) {
+  if (xn == 0 || yn == 0) return false;
+  if (x == y) return overlaps(x0, x0 + xn, y0, y0 + yn);
+  if (!x->ptr || !y->ptr) return false;
+  const uint64_t xp = reinterpret_cast<uint64_t>(x->ptr) + x0;
+  const uint64_t yp = reinterpret_cast<uint64_t>(y->ptr) + y0;
+  return overlaps(xp, xp + xn, yp, yp + yn);
+}
+
+uintptr_t at(const q8_buf *b, uint64_t off) { return reinterpret_cast<uintptr_t>(b->ptr) + off; }
+
+// An int32 array of `ix`.
+struct Ints {
+  const char *name;
+  uint64_t off, count;
+  bool written;
+};
+// All inside the buffer, and no written one over another.
+int check_ints(q8_ctx *ctx, const q8_buf *ix, const Ints *v, int n, const char *what) {
+  for (int i = 0; i < n; ++i) {
+    if (!fits(v[i].off, v[i].count, 4, ix->size))
+      return fail(ctx, Q8_ERR_RANGE, "%s: %s [%llu, +%llu) i32 exceeds its buffer", what, v[i].name,
+                  (unsigned long long)v[i].off, (unsigned long long)v[i].count);
+    for (int j = 0; j < i; ++j)
+      if ((v[i].written || v[j].written) &&
+          overlaps(v[i].off, v[i].off + v[i].count, v[j].off, v[j].off + v[j].count))
+        return fail(ctx, Q8_ERR_ARG, "%s: %s and %s overlap", what, v[j].name, v[i].name);
+  }
+  return Q8_OK;
+}
+
+int *iptr(q8_buf *b, uint64_t off) { return reinterpret_cast<int *>(bytes(b, off * 4)); }
+
+int check_head_dim(q8_ctx *ctx, int nheads, int nkv, int head_dim, const char *what) {
+  if (int rc = check_heads(ctx, nheads, nkv, head_dim, what)) return rc;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: head_dim=%d (supported: 64 or 128)", what, head_dim);
+  if (nheads > 65535)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nheads=%d (at most 65535)", what, nheads);
+  return Q8_OK;
+}
+
+// The rows and sequences of a call: cu at ocu of ix.
+int check_seqs(q8_ctx *ctx, int64_t nseq, int64_t rows, const char *what) {
+  if (nseq < 0 || rows < 0 || rows > ((int64_t)1 << 24) || nseq > ((int64_t)1 << 24))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: nseq=%lld, rows=%lld (0 .. 2^24)", what, (long long)nseq,
+                (long long)rows);
+  return Q8_OK;
+}
+
+// The paged cache of q8_kv8_append and q8_kv8_attention, and the int32 arrays
+// that say whose pages they are.
+int check_kv8(q8_ctx *ctx, q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+              uint64_t ocu, uint64_t olen, uint64_t otab, int64_t nseq, int64_t rows,
+              int64_t maxpages, int nheads, int nkv, int head_dim, const char *what,
+              q8::Kv8Args *out) {
+  if (!pages || !ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (int rc = check_head_dim(ctx, nheads, nkv, head_dim, what)) return rc;
+  if (int rc = check_seqs(ctx, nseq, rows, what)) return rc;
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: page=%d tokens (supported: 16, 32, 64 or 128)", what, page);
+  if (nseq > q8::kKv8MaxSeq)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nseq=%lld (at most %d sequences a call)", what,
+                (long long)nseq, q8::kKv8MaxSeq);
+  if (npages <= 0 || npages > INT32_MAX || maxpages <= 0 || maxpages * page > ((int64_t)1 << 30))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: npages=%lld, maxpages=%lld (at least 1, maxpages * page at "
+                "most 2^30)", what, (long long)npages, (long long)maxpages);
+  const uint64_t pb = (uint64_t)q8::kv8_page_bytes(page, nkv, head_dim);
+  if (!fits(opages, (uint64_t)npages * pb, 1, pages->size))
+    return fail(ctx, Q8_ERR_RANGE, "%s: %lld pages of %llu bytes exceed their buffer", what,
+                (long long)npages, (unsigned long long)pb);
+  if (at(pages, opages) % 16 != 0)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: the pages must start 16-byte aligned", what);
+  const Ints v[] = {{"cu", ocu, (uint64_t)nseq + 1, false},
+                    {"len", olen, (uint64_t)nseq, false},
+                    {"table", otab, (uint64_t)nseq * (uint64_t)maxpages, false}};
+  if (int rc = check_ints(ctx, ix, v, 3, what)) return rc;
+  out->pages = bytes(pages, opages);
+  out->npages = npages;
+  out->page = page;
+  out->cu = iptr(ix, ocu);
+  out->len = iptr(ix, olen);
+  out->tab = iptr(ix, otab);
+  out->nseq = nseq;
+  out->rows = rows;
+  out->maxpages = maxpages;
+  out->nheads = nheads;
+  out->nkv = nkv;
+  out->head_dim = head_dim;
+  return Q8_OK;
+}
+
+}  // namespace
+
+int q8_attention_packed(q8_ctx *ctx, q8_buf *q, uint64_t oq, int act_dtype, int64_t ldq, q8_buf *kv,
+                        uint64_t okc_f16, uint64_t ovc_f16, q8_buf *out, uint64_t oy, q8_buf *ix,
+                        uint64_t ocu_i32, int64_t nseq, int64_t rows, int nheads, int nkv,
+                        int head_dim) {
+  const char *what = "q8_attention_packed";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!q || !kv || !out || !ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (act_dtype != Q8_SRC_F32 && act_dtype != Q8_SRC_BF16)
+    return fail(ctx, Q8_ERR_ARG, "%s: act_dtype=%d (Q8_SRC_F32 or Q8_SRC_BF16)", what, act_dtype);
+  if (int rc = check_head_dim(ctx, nheads, nkv, head_dim, what)) return rc;
+  if (nheads / nkv > 128)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nheads/nkv=%d (at most 128)", what, nheads / nkv);
+  if (int rc = check_seqs(ctx, nseq, rows, what)) return rc;
+  const uint64_t es = act_dtype == Q8_SRC_F32 ? 4 : 2;
+  const int64_t qdim = (int64_t)nheads * head_dim, kvdim = (int64_t)nkv * head_dim;
+  if (ldq != 0 && (ldq < qdim || ldq > INT32_MAX))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: q row stride %lld (0, or at least %lld)", what, (long long)ldq,
+                (long long)qdim);
+  if (ldq == 0) ldq = qdim;
+  const uint64_t qspan = rows_span(rows, ldq, (uint64_t)qdim), on = (uint64_t)rows * (uint64_t)qdim;
+  const uint64_t cn = (uint64_t)rows * (uint64_t)kvdim;
+  if (!fits(oq, qspan, es, q->size) || !fits(oy, on, es, out->size))
+    return fail(ctx, Q8_ERR_RANGE, "%s: q or out exceeds its buffer", what);
+  if (!fits(okc_f16, cn, 2, kv->size) || !fits(ovc_f16, cn, 2, kv->size))
+    return fail(ctx, Q8_ERR_RANGE, "%s: the K or V rows exceed their buffer", what);
+  const Ints v[] = {{"cu", ocu_i32, (uint64_t)nseq + 1, false}};
+  if (int rc = check_ints(ctx, ix, v, 1, what)) return rc;
+  if (share(out, oy * es, on * es, q, oq * es, qspan * es) ||
+      share(out, oy * es, on * es, kv, okc_f16 * 2, cn * 2) ||
+      share(out, oy * es, on * es, kv, ovc_f16 * 2, cn * 2) ||
+      share(out, oy * es, on * es, ix, ocu_i32 * 4, ((uint64_t)nseq + 1) * 4))
+    return fail(ctx, Q8_ERR_ARG, "%s: out overlaps an input", what);
+  if (at(q, oq * es) % 16 != 0 || at(out, oy * es) % 16 != 0 || at(kv, okc_f16 * 2) % 16 != 0 ||
+      at(kv, ovc_f16 * 2) % 16 != 0 || (uint64_t)ldq * es % 16 != 0)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: q, out, K and V rows must start 16-byte aligned", what);
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0 || nseq == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  q8::PackedAttnArgs a;
+  a.q = bytes(q, oq * es);
+  a.bf16 = act_dtype == Q8_SRC_BF16;
+  a.kc = reinterpret_cast<const __half *>(bytes(kv, okc_f16 * 2));
+  a.vc = reinterpret_cast<const __half *>(bytes(kv, ovc_f16 * 2));
+  a.out = bytes(out, oy * es);
+  a.cu = iptr(ix, ocu_i32);
+  a.nseq = nseq;
+  a.rows = rows;
+  a.nheads = nheads;
+  a.nkv = nkv;
+  a.head_dim = head_dim;
+  a.ldq = ldq;
+  const hipError_t e = q8::launch_attention_packed(a, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_attention_packed launch");
+  return ok(ctx);
+}
+
+uint64_t q8_kv8_page_bytes(int page, int nkv, int head_dim) {
+  if ((page != 16 && page != 32 && page != 64 && page != 128) || nkv <= 0 || nkv > 65535 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return (uint64_t)q8::kv8_page_bytes(page, nkv, head_dim);
+}
+
+int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint64_t ov_f32,
+                  uint64_t oinv_f32, uint64_t oqr_f32, int64_t ld, int64_t ldr, q8_buf *kv,
+                  uint64_t okc_f16, uint64_t ovc_f16, q8_buf *pages, uint64_t opages,
+                  int64_t npages, int page, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32,
+                  uint64_t otab_i32, int64_t nseq, int64_t rows, int64_t maxpages, int nheads,
+                  int nkv, int head_dim) {
+  const char *what = "q8_kv8_append";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!a) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  q8::Kv8AppendArgs p;
+  if (int rc = check_kv8(ctx, pages, opages, npages, page, ix, ocu_i32, olen_i32, otab_i32, nseq,
+                         rows, maxpages, nheads, nkv, head_dim, what, &p.c))
+    return rc;
+  const int64_t qdim = (int64_t)nheads * head_dim, kvdim = (int64_t)nkv * head_dim;
+  if ((ld != 0 && (ld < qdim || ld < kvdim || ld > INT32_MAX)) ||
+      (ldr != 0 && (ldr < qdim || ldr > INT32_MAX)))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: row stride %lld or %lld (0, or at least the row widths %lld, "
+                "%lld)", what, (long long)ld, (long long)ldr, (long long)qdim, (long long)kvdim);
+  const int64_t ldq = ld ? ld : qdim, ldk = ld ? ld : kvdim, lr = ldr ? ldr : qdim;
+  const uint64_t qn = rows_span(rows, ldq, (uint64_t)qdim), kn = rows_span(rows, ldk, (uint64_t)kvdim);
+  const uint64_t rn = rows_span(rows, lr, (uint64_t)qdim), ni = (uint64_t)head_dim / 2;
+  if (int rc = check_f32(ctx, a, oq_f32, qn, what, "q")) return rc;
+  if (int rc = check_f32(ctx, a, ok_f32, kn, what, "k")) return rc;
+  if (int rc = check_f32(ctx, a, ov_f32, kn, what, "v")) return rc;
+  if (int rc = check_f32(ctx, a, oinv_f32, ni, what, "inv_freq")) return rc;
+  if (int rc = check_f32(ctx, a, oqr_f32, rn, what, "rotated q")) return rc;
+  // The rotated q is the only f32 output: q itself at its own stride, or apart
+  // from all inputs.
+  const uint64_t o = oqr_f32;
+  if (overlaps(o, o + rn, oinv_f32, oinv_f32 + ni))
+    return fail(ctx, Q8_ERR_ARG, "%s: inv_freq overlaps the rotated q", what);
+  if (o == oq_f32 && (lr == ldq || rows == 1)) {
+    const bool apart = ld == 0 ? !overlaps(o, o + rn, ok_f32, ok_f32 + kn) &&
+                                     !overlaps(o, o + rn, ov_f32, ov_f32 + kn)
+                               : stride_disjoint(o, qdim, ok_f32, kvdim, ld) &&
+                                     stride_disjoint(o, qdim, ov_f32, kvdim, ld);
+    if (rows > 0 && !apart)
+      return fail(ctx, Q8_ERR_ARG, "%s: k or v overlaps the q rows rotated in place", what);
+  } else if (overlaps(o, o + rn, oq_f32, oq_f32 + qn) || overlaps(o, o + rn, ok_f32, ok_f32 + kn) ||
+             overlaps(o, o + rn, ov_f32, ov_f32 + kn)) {
+    return fail(ctx, Q8_ERR_ARG, "%s: the rotated q overlaps q, k or v (q at its own stride "
+                "excepted)", what);
+  }
+  const uint64_t cn = (uint64_t)rows * (uint64_t)kvdim;
+  if (kv) {
+    if (!fits(okc_f16, cn, 2, kv->size) || !fits(ovc_f16, cn, 2, kv->size))
+      return fail(ctx, Q8_ERR_RANGE, "%s: the binary16 rows exceed their buffer", what);
+    if (overlaps(okc_f16, okc_f16 + cn, ovc_f16, ovc_f16 + cn))
+      return fail(ctx, Q8_ERR_ARG, "%s: the binary16 K and V rows overlap", what);
+  }
+  const uint64_t pn = (uint64_t)npages * (uint64_t)q8::kv8_page_bytes(page, nkv, head_dim);
+  struct {
+    q8_buf *b;
+    uint64_t off, n;
+  } outs[] = {{a, o * 4, rn * 4}, {pages, opages, pn}, {kv, okc_f16 * 2, cn * 2}, {kv, ovc_f16 * 2, cn * 2}},
+    ins[] = {{a, ok_f32 * 4, kn * 4}, {a, ov_f32 * 4, kn * 4}, {a, oq_f32 * 4, qn * 4},
+             {a, oinv_f32 * 4, ni * 4}, {ix, ocu_i32 * 4, ((uint64_t)nseq + 1) * 4},
+             {ix, olen_i32 * 4, (uint64_t)nseq * 4},
+             {ix, otab_i32 * 4, (uint64_t)nseq * (uint64_t)maxpages * 4}};
+  for (int i = 0; i < 4; ++i) {
+    if (!outs[i].b) continue;
+    for (int j = 0; j < i; ++j)
+      if (outs[j].b && !(i == 3 && j == 2) &&
+          share(outs[i].b, outs[i].off, outs[i].n, outs[j].b, outs[j].off, outs[j].n))
+        return fail(ctx, Q8_ERR_ARG, "%s: two outputs overlap", what);
+    for (int j = i == 0 ? 4 : 0; j < 7; ++j)    // (the rotated q against the arena: above)
+      if (share(outs[i].b, outs[i].off, outs[i].n, ins[j].b, ins[j].off, ins[j].n))
+        return fail(ctx, Q8_ERR_ARG, "%s: an output overlaps an input", what);
+  }
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0 || nseq == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  p.q = fptr(a, oq_f32);
+  p.k = fptr(a, ok_f32);
+  p.v = fptr(a, ov_f32);
+  p.inv = fptr(a, oinv_f32);
+  p.qr = fptr(a, oqr_f32);
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldr = lr;
+  p.krow = kv ? reinterpret_cast<__half *>(bytes(kv, okc_f16 * 2)) : nullptr;
+  p.vrow = kv ? reinterpret_cast<__half *>(bytes(kv, ovc_f16 * 2)) : nullptr;
+  const hipError_t e = q8::launch_kv8_append(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_kv8_append launch");
+  return ok(ctx);
+}
+
+int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
+                     q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+                     uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
+                     int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim) {
+  const char *what = "q8_kv8_attention";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!a) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  q8::Kv8AttnArgs p;
+  if (int rc = check_kv8(ctx, pages, opages, npages, page, ix, ocu_i32, olen_i32, otab_i32, nseq,
+                         rows, maxpages, nheads, nkv, head_dim, what, &p.c))
+    return rc;
+  const int64_t qdim = (int64_t)nheads * head_dim;
+  if (ldq != 0 && (ldq < qdim || ldq > INT32_MAX))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: q row stride %lld (0, or at least %lld)", what, (long long)ldq,
+                (long long)qdim);
+  if (ldq == 0) ldq = qdim;
+  // units of 64 keys are counted in int32
+  const double units = ((double)rows * (nheads / nkv) / 16 + (double)nseq) *
+                       ((double)maxpages * page / q8::kKv8Unit + 1);
+  if (units >= (double)q8::kKv8MaxUnits)
+    return fail(ctx, Q8_ERR_SHAPE, "%s: %lld rows over %lld pages each are too many for one call", what,
+                (long long)rows, (long long)maxpages);
+  const uint64_t qspan = rows_span(rows, ldq, (uint64_t)qdim), on = (uint64_t)rows * (uint64_t)qdim;
+  if (int rc = check_f32(ctx, a, oq_f32, qspan, what, "q")) return rc;
+  if (int rc = check_f32(ctx, a, oy_f32, on, what, "out")) return rc;
+  const uint64_t pn = (uint64_t)npages * (uint64_t)q8::kv8_page_bytes(page, nkv, head_dim);
+  if (overlaps(oy_f32, oy_f32 + on, oq_f32, oq_f32 + qspan) ||
+      share(a, oy_f32 * 4, on * 4, pages, opages, pn) ||
+      share(a, oy_f32 * 4, on * 4, ix, ocu_i32 * 4, ((uint64_t)nseq + 1) * 4) ||
+      share(a, oy_f32 * 4, on * 4, ix, olen_i32 * 4, (uint64_t)nseq * 4) ||
+      share(a, oy_f32 * 4, on * 4, ix, otab_i32 * 4, (uint64_t)nseq * (uint64_t)maxpages * 4))
+    return fail(ctx, Q8_ERR_ARG, "%s: out overlaps an input", what);
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0 || nseq == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  p.q = fptr(a, oq_f32);
+  p.ldq = ldq;
+  p.out = fptr(a, oy_f32);
+  p.ws = static_cast<float *>(ctx->act16);
+  p.ws_floats = kAct16Bytes / 4;
+  const hipError_t e = with_scratch(ctx, [&] { return q8::launch_kv8_attention(p, ctx->stream); });
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_kv8_attention launch");
+  return ok(ctx);
+}
+
+namespace {
+
+int check_pages(q8_ctx *ctx, q8_buf *ix, int64_t nslots, int64_t maxpages, int64_t npages, int page,
+                const char *what) {
+  if (!ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (nslots < 0 || maxpages <= 0 || npages <= 0 || npages > INT32_MAX || page <= 0 ||
+      maxpages > ((int64_t)1 << 30) / page)
+    return fail(ctx, Q8_ERR_SHAPE, "%s: nslots=%lld, maxpages=%lld, npages=%lld, page=%d", what,
+                (long long)nslots, (long long)maxpages, (long long)npages, page);
+  if (nslots > q8::kPagesMaxSlots || nslots * maxpages > INT32_MAX)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nslots=%lld (at most %d slots, 2^31 table entries)",
+                what, (long long)nslots, q8::kPagesMaxSlots);
+  return Q8_OK;
+}
+
+int check_pool(q8_ctx *ctx, q8_buf *pages, uint64_t opages, uint64_t page_bytes, int64_t layers,
+               uint64_t layer_stride, int64_t npages, q8_buf *ix, const Ints *v, int nv,
+               const char *what, q8::PagePool *out) {
+  if (!pages) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (page_bytes == 0 || page_bytes > ((uint64_t)1 << 40) || layers <= 0 || layers > 65535)
+    return fail(ctx, Q8_ERR_SHAPE, "%s: page_bytes=%llu, layers=%lld", what,
+                (unsigned long long)page_bytes, (long long)layers);
+  const unsigned __int128 layer = (unsigned __int128)npages * page_bytes;
+  if (layers > 1 && layer_stride < layer)
+    return fail(ctx, Q8_ERR_SHAPE, "%s: layers of %lld pages overlap at a stride of %llu bytes", what,
+                (long long)npages, (unsigned long long)layer_stride);
+  const unsigned __int128 end =
+      (unsigned __int128)opages + (unsigned __int128)(layers - 1) * layer_stride + layer;
+  if (end > pages->size) return fail(ctx, Q8_ERR_RANGE, "%s: the pages exceed their buffer", what);
+  if (at(pages, opages) % 16 != 0 || page_bytes % 16 != 0 || (layers > 1 && layer_stride % 16 != 0))
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: the pages, their size and the layer stride must be "
+                "multiples of 16 bytes", what);
+  for (int i = 0; i < nv; ++i)
+    if (share(pages, opages, (uint64_t)end - opages, ix, v[i].off * 4, v[i].count * 4))
+      return fail(ctx, Q8_ERR_ARG, "%s: the pages overlap %s", what, v[i].name);
+  out->pages = bytes(pages, opages);
+  out->page_bytes = (int64_t)page_bytes;
+  out->layers = layers;
+  out->stride = layers > 1 ? (int64_t)layer_stride : 0;
+  return Q8_OK;
+}
+
+}  // namespace
+
+int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
+                     uint64_t oheld_i32, uint64_t oref_i32, uint64_t owant_i32, int64_t nslots,
+                     int64_t maxpages, int64_t npages, int page, q8_buf *pages, uint64_t opages,
+                     uint64_t page_bytes, int64_t layers, uint64_t layer_stride) {
+  const char *what = "q8_pages_reserve";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (int rc = check_pages(ctx, ix, nslots, maxpages, npages, page, what)) return rc;
+  const uint64_t ns = (uint64_t)nslots;
+  const Ints v[] = {{"table", otab_i32, ns * (uint64_t)maxpages, true},
+                    {"len", olen_i32, ns, false},
+                    {"held", oheld_i32, ns, true},
+                    {"ref", oref_i32, (uint64_t)npages, true},
+                    {"want", owant_i32, ns, false}};
+  if (int rc = check_ints(ctx, ix, v, 5, what)) return rc;
+  q8::PagePool pool;
+  if (int rc = check_pool(ctx, pages, opages, page_bytes, layers, layer_stride, npages, ix, v, 5, what,
+                          &pool))
+    return rc;
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (nslots == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  const q8::PagesArgs a = {iptr(ix, otab_i32), iptr(ix, olen_i32), iptr(ix, oheld_i32),
+                           iptr(ix, oref_i32), nslots, maxpages, npages, page};
+  const hipError_t e = with_scratch(ctx, [&] {
+    return q8::launch_pages_reserve(a, iptr(ix, owant_i32), pool,
+                                    reinterpret_cast<int *>(ctx->gemm_ws), ctx->stream);
+  });
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_pages_reserve launch");
+  return ok(ctx);
+}
+
+int q8_pages_set_len(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
+                     uint64_t oheld_i32, uint64_t oref_i32, uint64_t onew_i32, int64_t nslots,
+                     int64_t maxpages, int64_t npages, int page) {
+  const char *what = "q8_pages_set_len";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (int rc = check_pages(ctx, ix, nslots, maxpages, npages, page, what)) return rc;
+  const uint64_t ns = (uint64_t)nslots;
+  const Ints v[] = {{"table", otab_i32, ns * (uint64_t)maxpages, true},
+                    {"len", olen_i32, ns, true},
+                    {"held", oheld_i32, ns, true},
+                    {"ref", oref_i32, (uint64_t)npages, true},
+                    {"new lengths", onew_i32, ns, false}};
+  if (int rc = check_ints(ctx, ix, v, 5, what)) return rc;
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (nslots == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  const q8::PagesArgs a = {iptr(ix, otab_i32), iptr(ix, olen_i32), iptr(ix, oheld_i32),
+                           iptr(ix, oref_i32), nslots, maxpages, npages, page};
+  const hipError_t e = q8::launch_pages_set_len(a, iptr(ix, onew_i32), ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_pages_set_len launch");
+  return ok(ctx);
+}
+
+int q8_pages_fork(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32, uint64_t oheld_i32,
+                  uint64_t oref_i32, uint64_t osource_i32, int64_t nslots, int64_t maxpages,
+                  int64_t npages) {
+  const char *what = "q8_pages_fork";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (int rc = check_pages(ctx, ix, nslots, maxpages, npages, 1, what)) return rc;
+  const uint64_t ns = (uint64_t)nslots;
+  const Ints v[] = {{"table", otab_i32, ns * (uint64_t)maxpages, true},
+                    {"len", olen_i32, ns, true},
+                    {"held", oheld_i32, ns, true},
+                    {"ref", oref_i32, (uint64_t)npages, true},
+                    {"source", osource_i32, ns, false}};
+  if (int rc = check_ints(ctx, ix, v, 5, what)) return rc;
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (nslots == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  const q8::PagesArgs a = {iptr(ix, otab_i32), iptr(ix, olen_i32), iptr(ix, oheld_i32),
+                           iptr(ix, oref_i32), nslots, maxpages, npages, 1};
+  const hipError_t e = q8::launch_pages_fork(a, iptr(ix, osource_i32), ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_pages_fork launch");
+  return ok(ctx);
+}
+
+int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_i32,
+                     uint64_t oref_i32, uint64_t olive_i32, int64_t nslots, int64_t maxpages,
+                     int64_t npages, q8_buf *pages, uint64_t opages, uint64_t page_bytes,
+                     int64_t layers, uint64_t layer_stride) {
+  const char *what = "q8_pages_compact";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (int rc = check_pages(ctx, ix, nslots, maxpages, npages, 1, what)) return rc;
+  const uint64_t ns = (uint64_t)nslots;
+  const Ints v[] = {{"table", otab_i32, ns * (uint64_t)maxpages, true},
+                    {"held", oheld_i32, ns, false},
+                    {"ref", oref_i32, (uint64_t)npages, true},
+                    {"live", olive_i32, 1, true}};
+  if (int rc = check_ints(ctx, ix, v, 4, what)) return rc;
+  q8::PagePool pool;
+  if (int rc = check_pool(ctx, pages, opages, page_bytes, layers, layer_stride, npages, ix, v, 4, what,
+                          &pool))
+    return rc;
+  if (3 * npages + 2 > kAct16Bytes / 4)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: npages=%lld (at most %lld)", what, (long long)npages,
+                (long long)((kAct16Bytes / 4 - 2) / 3));
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (int rc = set_device(ctx)) return rc;
+  const q8::PagesArgs a = {iptr(ix, otab_i32), nullptr, iptr(ix, oheld_i32), iptr(ix, oref_i32),
+                           nslots, maxpages, npages, 1};
+  const hipError_t e = with_scratch(ctx, [&] {
+    return q8::launch_pages_compact(a, iptr(ix, olive_i32), pool, static_cast<int *>(ctx->act16),
+                                    ctx->stream);
+  });
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_pages_compact launch");
   return ok(ctx);
 }
 

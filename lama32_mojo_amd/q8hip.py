@@ -117,6 +117,19 @@ SIGNATURES = {
     "q8_pos_advance": (_I, [_P, _P, _U64, _I64]),
     "q8_token_begin": (_I, [_P, _P, _U64, ctypes.c_int32, _P, _U64, ctypes.c_int32, _P, _U64, _P,
                             _U64, _I64, _I64, _I, _I]),
+    "q8_attention_packed": (_I, [_P, _P, _U64, _I, _I64, _P, _U64, _U64, _P, _U64, _P, _U64, _I64,
+                                 _I64, _I, _I, _I]),
+    "q8_kv8_page_bytes": (_U64, [_I, _I, _I]),
+    "q8_kv8_append": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _P, _U64, _U64, _P,
+                           _U64, _I64, _I, _P, _U64, _U64, _U64, _I64, _I64, _I64, _I, _I, _I]),
+    "q8_kv8_attention": (_I, [_P, _P, _U64, _I64, _U64, _P, _U64, _I64, _I, _P, _U64, _U64, _U64,
+                              _I64, _I64, _I64, _I, _I, _I]),
+    "q8_pages_reserve": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _I, _P, _U64,
+                              _U64, _I64, _U64]),
+    "q8_pages_set_len": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _I]),
+    "q8_pages_fork": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64]),
+    "q8_pages_compact": (_I, [_P, _P, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _P, _U64, _U64,
+                              _I64, _U64]),
     "q8_graph_begin": (_I, [_P]),
     "q8_graph_end": (_I, [_P, ctypes.POINTER(_P)]),
     "q8_graph_launch": (_I, [_P, _P]),
@@ -484,3 +497,92 @@ def token_begin(ctx: Context, ids: Buffer, oid_i32: int, token: int, posbuf: Buf
     ctx.check(ctx._lib.q8_token_begin(ctx.h, ids.h, int(oid_i32), token, posbuf.h, int(opos_i32),
                                       pos, _h(w), int(oemb_u16), _h(a), int(ox_f32), int(d),
                                       int(vocab), int(G), scale_code(scale)))
+
+
+# ---- several sequences at once ---------------------------------------------------------
+# (int32 arrays at element offsets of `ix`; see include/q8hip.h for the layouts)
+
+ACT = {"f32": Q8_SRC_F32, "bf16": Q8_SRC_BF16}
+
+
+def attention_packed(ctx: Context, q: Buffer, oq: int, kv: Buffer, okc_f16: int, ovc_f16: int,
+                     out: Buffer, oy: int, ix: Buffer, ocu_i32: int, nseq: int, rows: int,
+                     nheads: int, nkv: int, head_dim: int, act="f32", ldq: int = 0) -> None:
+    """Causal attention of packed prompts over their own binary16 K and V rows;
+    q and out f32 or bf16 ("f32" / "bf16"): q8_attention_packed."""
+    ctx.check(ctx._lib.q8_attention_packed(
+        ctx.h, q.h, int(oq), act if isinstance(act, int) else ACT[act], int(ldq), kv.h,
+        int(okc_f16), int(ovc_f16), out.h, int(oy), ix.h, int(ocu_i32), int(nseq), int(rows),
+        int(nheads), int(nkv), int(head_dim)))
+
+
+def kv8_page_bytes(page: int, nkv: int, head_dim: int) -> int:
+    """Bytes of a page of the 8-bit cache: q8_kv8_page_bytes."""
+    n = int(lib().q8_kv8_page_bytes(int(page), int(nkv), int(head_dim)))
+    if n == 0:
+        raise Q8Error(Q8_ERR_UNSUPPORTED, f"no cache of page={page} nkv={nkv} head_dim={head_dim}")
+    return n
+
+
+def kv8_append(ctx: Context, a: Buffer, oq: int, ok: int, ov: int, oinv: int, oqr: int,
+               pages: Buffer, opages: int, npages: int, page: int, ix: Buffer, ocu: int, olen: int,
+               otab: int, nseq: int, rows: int, maxpages: int, nheads: int, nkv: int,
+               head_dim: int, ld: int = 0, ldr: int | None = None, kv: Buffer | None = None,
+               okc_f16: int = 0, ovc_f16: int = 0) -> None:
+    """RoPE at each row's position and the append to the 8-bit cache, with kv
+    also binary16 rows; ldr: row stride of the rotated q (None: ld in place,
+    else dense): q8_kv8_append."""
+    if ldr is None:
+        ldr = ld if oqr == oq else 0
+    ctx.check(ctx._lib.q8_kv8_append(
+        ctx.h, a.h, int(oq), int(ok), int(ov), int(oinv), int(oqr), int(ld), int(ldr), _h(kv),
+        int(okc_f16), int(ovc_f16), pages.h, int(opages), int(npages), int(page), ix.h, int(ocu),
+        int(olen), int(otab), int(nseq), int(rows), int(maxpages), int(nheads), int(nkv),
+        int(head_dim)))
+
+
+def kv8_attention(ctx: Context, a: Buffer, oq: int, oy: int, pages: Buffer, opages: int,
+                  npages: int, page: int, ix: Buffer, ocu: int, olen: int, otab: int, nseq: int,
+                  rows: int, maxpages: int, nheads: int, nkv: int, head_dim: int,
+                  ldq: int = 0) -> None:
+    """Causal attention of the rows of several sequences over the 8-bit cache:
+    q8_kv8_attention."""
+    ctx.check(ctx._lib.q8_kv8_attention(
+        ctx.h, a.h, int(oq), int(ldq), int(oy), pages.h, int(opages), int(npages), int(page), ix.h,
+        int(ocu), int(olen), int(otab), int(nseq), int(rows), int(maxpages), int(nheads),
+        int(nkv), int(head_dim)))
+
+
+def pages_reserve(ctx: Context, ix: Buffer, otab: int, olen: int, oheld: int, oref: int,
+                  owant: int, nslots: int, maxpages: int, npages: int, page: int, pages: Buffer,
+                  opages: int, page_bytes: int, layers: int = 1, layer_stride: int = 0) -> None:
+    """Room for want[s] tokens in every slot, shared partly filled last pages
+    copied: q8_pages_reserve."""
+    ctx.check(ctx._lib.q8_pages_reserve(
+        ctx.h, ix.h, int(otab), int(olen), int(oheld), int(oref), int(owant), int(nslots),
+        int(maxpages), int(npages), int(page), pages.h, int(opages), int(page_bytes), int(layers),
+        int(layer_stride)))
+
+
+def pages_set_len(ctx: Context, ix: Buffer, otab: int, olen: int, oheld: int, oref: int,
+                  onew: int, nslots: int, maxpages: int, npages: int, page: int) -> None:
+    """Lengths of the slots, the pages behind them released: q8_pages_set_len."""
+    ctx.check(ctx._lib.q8_pages_set_len(ctx.h, ix.h, int(otab), int(olen), int(oheld), int(oref),
+                                        int(onew), int(nslots), int(maxpages), int(npages),
+                                        int(page)))
+
+
+def pages_fork(ctx: Context, ix: Buffer, otab: int, olen: int, oheld: int, oref: int,
+               osource: int, nslots: int, maxpages: int, npages: int) -> None:
+    """Slot s continues slot source[s]: q8_pages_fork."""
+    ctx.check(ctx._lib.q8_pages_fork(ctx.h, ix.h, int(otab), int(olen), int(oheld), int(oref),
+                                     int(osource), int(nslots), int(maxpages), int(npages)))
+
+
+def pages_compact(ctx: Context, ix: Buffer, otab: int, oheld: int, oref: int, olive: int,
+                  nslots: int, maxpages: int, npages: int, pages: Buffer, opages: int,
+                  page_bytes: int, layers: int = 1, layer_stride: int = 0) -> None:
+    """The pages in use moved to the lowest ids: q8_pages_compact."""
+    ctx.check(ctx._lib.q8_pages_compact(
+        ctx.h, ix.h, int(otab), int(oheld), int(oref), int(olive), int(nslots), int(maxpages),
+        int(npages), pages.h, int(opages), int(page_bytes), int(layers), int(layer_stride)))
