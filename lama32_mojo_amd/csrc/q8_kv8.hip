@@ -274,24 +274,31 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
 //
 // Bound: HBM (2 HD bytes a key and KV head), as long as a tile's columns are
 // few.  The units of work (64 keys of one sequence's row tile) of all sequences
-// are laid end to end and cut into equal runs, one per block of a KV head, so
-// ragged contexts leave no block behind; a run that ends inside a row tile
-// leaves a record for kv8_merge_kernel.  Within a run the block's four waves
-// take the units in turn, each with its own online softmax, and meet in LDS.
+// are laid end to end and cut into equal runs, one per wave of a KV head, so
+// ragged contexts leave no wave behind (a row tile of 16 MT columns: one per MT
+// waves, which go through the same keys side by side).  A wave streams its run through
+// registers without a barrier: page ids are read two units ahead, codes one,
+// across the ends of row tiles, so the loads never wait for a sum to be
+// written.  A run that ends inside a row tile leaves a record for
+// kv8_merge_kernel.  Tables of up to 1024 tokens take a block of 8 waves per
+// row tile instead (WHOLE), which meet in LDS, and no merge.
 //
-// A wave holds a unit's codes in registers: S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_16x16x32_bf16, the codes as bf16 (exact), q and p as three bf16
-// terms each whose sum is the f32 value, so products are exact and scores and
-// sums carry f32-level error whatever the sizes of q's dims or the scales; the
-// scales are applied to scores and probabilities in f32.  Lane layout (lane l,
-// g4 = l / 16): A element i is A[l % 16][8 g4 + i], B element i is
-// B[8 g4 + i][l % 16], accumulator element i is D[4 g4 + i][l % 16].  Which key
-// is row r of score tile tt, and which dim is element (step, g4, i), is free;
-// taking key 16 (r / 4) + 4 tt + r % 4 makes the four accumulators of a lane
-// hold 16 consecutive keys of its column, the ones its V operand loads as one
-// 16-byte run of a V column, and taking dim 64 h + 16 g4 + 8 e + i for step
-// 2 h + e makes its K operands two halves of one 16-byte run of a K row.
-typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+// Scores: S^T = K Q^T on v_mfma_i32_16x16x64_i8 with the codes as they are and
+// q as four signed base-256 digits of 2^30 q / 2^e (2^e the power of two above
+// the column's largest |q|): exact integer sums, joined in f32, so q is carried
+// to 2^-31 of the column's largest and nothing is lost in the sum.  Outputs:
+// O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, the codes as bf16 (exact) and
+// p vs as three bf16 terms whose sum is the f32 value, whatever the scales.
+// (Codes as bf16 in both products cost 192 more conversions of a unit's 700
+// VALU operations, and 16 more matrix instructions.)
+// Lane layout (lane l, g4 = l / 16), n = 16 (i8) or 8 (bf16) elements: A element
+// i is A[l % 16][n g4 + i], B element i is B[n g4 + i][l % 16], accumulator
+// element i is D[4 g4 + i][l % 16].  Which key is row r of score tile tt, and
+// which dims are the elements of a step, is free: key 16 (r / 4) + 4 tt + r % 4
+// makes the accumulators of a lane hold 16 consecutive keys of its column, the
+// ones its V operand loads as one 16-byte run of a V column, and dims 64 h + 16
+// g4 + i make its K operand one 16-byte run of a K row.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // x as three bf16 terms (truncations, exact): the upper halves of h, m, l.
 __device__ __forceinline__ void split3(float x, float &h, float &m, float &l) {
@@ -312,19 +319,44 @@ __device__ __forceinline__ void split3x8(const float (&x)[8], u32x4 (&o)[3]) {
   }
 }
 
-// Prefix sums of the sequences' units in LDS (pre[0] = 0 .. pre[nseq]); all
-// 256 threads.
-__device__ __forceinline__ int kv8_plan(const Kv8Args &c, int cols, int *pre, int *wsum) {
+// Four values' base-256 digits: byte i of digit k's word is digit k of x[i]
+// (k = 3 the highest; digits 0 to 2 in [-128, 127]).
+__device__ __forceinline__ void digits4(const float (&x)[4], uint32_t (&o)[4]) {
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = ((uint32_t)(int)__builtin_rintf(x[i]) + 0x00808080u) ^ 0x00808080u;
+  const uint32_t a = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);   // bytes 0, 1 of y0, y1
+  const uint32_t b = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);   // bytes 2, 3
+  const uint32_t d = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
+  o[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  o[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  o[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  o[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// The plan of a call in LDS: the prefix sums of the sequences' units (WHOLE: row
+// tiles), pre[0] = 0 .. pre[nseq], and their first rows, row counts and cached
+// tokens; all NT threads.
+struct Kv8Plan {
+  int *pre, *row0, *n, *old;
+};
+template <bool WHOLE, int NT>
+__device__ __forceinline__ int kv8_plan(const Kv8Args &c, int cols, const Kv8Plan &pl, int *wsum) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, nseq = (int)c.nseq;
   const int grp = c.nheads / c.nkv;
   int base = 0;
-  if (t == 0) pre[0] = 0;
-  for (int i0 = 0; i0 < nseq; i0 += 256) {
+  if (t == 0) pl.pre[0] = 0;
+  for (int i0 = 0; i0 < nseq; i0 += NT) {
     const int i = i0 + t;
     int u = 0;
     if (i < nseq) {
-      const Kv8Seq s = kv8_seq(c.cu[i], c.cu[i + 1], c.len[i], c.rows, c.maxpages * c.page, grp, cols);
-      u = kv8_units_of(s);
+      const int a = c.cu[i];
+      const Kv8Seq s = kv8_seq(a, c.cu[i + 1], c.len[i], c.rows, c.maxpages * c.page, grp, cols);
+      u = WHOLE ? s.row_tiles : kv8_units_of(s);
+      pl.row0[i] = clamp_i(a, 0, c.rows);
+      pl.n[i] = s.n;
+      pl.old[i] = s.old;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -335,11 +367,11 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &c, int cols, int *pre, in
     __syncthreads();
     int all = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < NT / 64; ++x) {
       u = kv8_add(u, x < w ? wsum[x] : 0);
       all = kv8_add(all, wsum[x]);
     }
-    if (i < nseq) pre[i + 1] = kv8_add(base, u);
+    if (i < nseq) pl.pre[i + 1] = kv8_add(base, u);
     base = kv8_add(base, all);
     __syncthreads();
   }
@@ -357,354 +389,418 @@ __device__ __forceinline__ int kv8_seq_of(const int *pre, int nseq, int u) {
   return lo;
 }
 
-constexpr int kKv8Least = 4;              // units a block serves at least: one per wave
+constexpr int kKv8WholeUnits = 16;        // tables of up to 1024 tokens: no splits
+constexpr int kKv8Waves = 4;              // waves of a block (WHOLE: 8)
+constexpr int kKv8PlanSeq = 1024;         // sequences of a launch (16 KB of LDS for the plan)
 
-// Record of a block and KV head: o[NC][HD] unnormalised, m[NC], l[NC]; slot 0
-// for a run that begins inside a row tile, slot 1 for one that ends inside.
+// Record of a run and KV head: o[NC][HD] unnormalised, m[NC], l[NC] (of the
+// columns that exist); slot 0 for a run that begins inside a row tile, slot 1
+// for one that ends inside.
 template <int HD, int NC> constexpr int kv8_record() { return NC * (HD + 2); }
+// The prefix sums, behind the records of the call's runs.
+template <int HD, int NC>
+__device__ __forceinline__ int *kv8_plan_at(const Kv8AttnArgs &a, int runs) {
+  return reinterpret_cast<int *>(a.ws + (int64_t)runs * a.c.nkv * 2 * kv8_record<HD, NC>());
+}
 
-template <int HD, int MT>
-__global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8AttnArgs a) {
-  constexpr int KS = HD / 32, DT = HD / 16, HH = HD / 64, NC = 16 * MT;
+// A place in a run of units: unit u of row tile rt of sequence i, its keys kt,
+// the row tile's units of the run ending at t1.
+struct Kv8Place {
+  int u, i, rt, kt, t0, t1, units;       // units: the row tile's
+  int ctx;                               // keys its last row sees
+};
+
+//
+// WIDE (pages of 128 tokens, runs): a V column of a page is one 128-byte line,
+// of which a unit takes half.  The even unit's load brings the odd unit's half
+// into registers too; fetched a unit later, the line had left the L2 by then
+// (4 contexts of up to 131000 tokens 142 -> 128 us).
+template <int HD, int MT, bool WHOLE, bool WIDE>
+__global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kernel(Kv8AttnArgs a) {
+  constexpr int DT = HD / 16, HH = HD / 64, NC = 16 * MT, NW = WHOLE ? 8 : kKv8Waves;
+  constexpr int RW = NW / MT;             // runs of a block
   constexpr int OST = HD + 4;             // floats of a column's sums in LDS
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  // q fragments [term][step][tile][lane], then (at the end of a segment) the
-  // sums of two waves; behind them the prefix sums
-  u32x4 *qf = reinterpret_cast<u32x4 *>(lds);
+  // WHOLE: the sums of four waves; the plan behind them
   float *ob = reinterpret_cast<float *>(lds);
-  constexpr int kQBytes = 3 * KS * MT * 64 * 16, kOBytes = 2 * NC * OST * 4;
-  int *pre = reinterpret_cast<int *>(lds + (kQBytes > kOBytes ? kQBytes : kOBytes));
-  __shared__ int wsum[4];
-  __shared__ float wm[4][NC], wl[4][NC];
+  constexpr int kOBytes = WHOLE ? (RW / 2) * NC * OST * 4 : 0;
+  __shared__ int wsum[NW];
+  __shared__ float wm[RW][NC], wl[RW][NC];
   const Kv8Args &c = a.c;
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63, col = lane & 15, g4 = lane >> 4;
+  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6) / MT;    // run of the block
+  const int cc = 16 * (__builtin_amdgcn_readfirstlane(t >> 6) % MT) + col;   // this lane's column
   const int g = blockIdx.y, grp = c.nheads / c.nkv, nseq = (int)c.nseq, P = c.page;
-  const int64_t cap = c.maxpages * P;
+  const int psh = 31 - __builtin_clz(P);  // page = 2^psh
+  const int cap = (int)(c.maxpages * P);
   const int64_t pbytes = kv8_page_bytes(P, c.nkv, HD);
   const int64_t scales_at = kv8_scales_at(P, c.nkv, HD);
   const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
   const float qscale = 1.44269504088896341f / sqrtf((float)HD);
+  Kv8Plan pl;
+  pl.pre = reinterpret_cast<int *>(lds + kOBytes);
+  pl.row0 = pl.pre + nseq + 1;
+  pl.n = pl.row0 + nseq;
+  pl.old = pl.n + nseq;
 
-  const int units = kv8_plan(c, NC, pre, wsum);
-  const int per = kv8_units_per_block(units, gridDim.x, kKv8Least);
-  int u = blockIdx.x * per;
-  const int uend = min(u + per, units);
-  while (u < uend) {
-    const int i = kv8_seq_of(pre, nseq, u);
-    const Kv8Seq sq = kv8_seq(c.cu[i], c.cu[i + 1], c.len[i], c.rows, cap, grp, NC);
-    const int local = u - pre[i], rt = local / sq.key_units, t0 = local % sq.key_units;
-    const int t1 = min(sq.key_units, t0 + (uend - u));
-    u += t1 - t0;
-    const int row0 = clamp_i(c.cu[i], 0, c.rows);
-    const int *tab = c.tab + (int64_t)i * c.maxpages;
-    const int ctx = (int)min((int64_t)sq.old + sq.n, cap);
+  const int units = kv8_plan<WHOLE, 64 * NW>(c, NC, pl, wsum);
+  const int runs = gridDim.x * RW, run = blockIdx.x * RW + w;
+  const int per = WHOLE ? 1 : kv8_units_per_block(units, runs, 1);
+  // the merge reads the plan behind the records
+  if (!WHOLE && blockIdx.x == 0 && g == 0)
+    for (int i = t; i <= nseq; i += 64 * NW) kv8_plan_at<HD, NC>(a, runs)[i] = pl.pre[i];
+  const int u0 = WHOLE ? (int)blockIdx.x : run * per;
+  const int uend = WHOLE ? min((int)blockIdx.x + 1, units) : min(u0 + per, units);
+  if (u0 >= uend) return;                 // (WHOLE: the whole block)
 
-    // ---- q of the tile's columns, scaled, as three bf16 terms
-    __syncthreads();                      // the last segment's sums are read
-    for (int n = t; n < NC * (HD / 8); n += 256) {
-      const int cc = n / (HD / 8), d8 = n % (HD / 8);
-      const int lin = rt * NC + cc, j = lin / grp;
-      float x[8];
+  // the place of unit u, in sequence i or behind it
+  auto place = [&](int u, int i) {
+    Kv8Place p;
+    while (pl.pre[i + 1] <= u) ++i;
+    const int local = u - pl.pre[i], ctx = min(pl.old[i] + pl.n[i], cap);
+    p.units = (ctx + kKv8Unit - 1) / kKv8Unit;
+    p.u = u;
+    p.i = i;
+    p.ctx = ctx;
+    p.rt = WHOLE ? local : local / p.units;
+    p.t0 = p.kt = WHOLE ? 0 : local % p.units;
+    p.t1 = WHOLE ? p.units : min(p.units, p.t0 + (uend - u));
+    return p;
+  };
+
+  // The unit that is loaded next; its page ids are there already.  Lanes of a
+  // unit's 16-key groups: K rows by col / 4, V columns by g4; page 0 stands
+  // behind the context (those keys are masked).
+  u32x4 kr[4][HH], vr[DT], vr2[WIDE ? DT : 1];
+  float ks = 0.0f, vs = 0.0f;
+  int idk = 0, idv = 0;
+  bool second = false;                    // vr2 holds the V of the unit loaded next
+  const int step = WHOLE ? RW : 1;
+  Kv8Place nx = place(u0, kv8_seq_of(pl.pre, nseq, u0));
+  Kv8Place cu = nx;
+  if (WHOLE) nx.kt = w;
+  auto have = [&]() { return nx.kt < nx.t1; };
+  auto load_ids = [&]() {
+    if (!have()) return;
+    const int *tab = c.tab + (int64_t)nx.i * c.maxpages;
+    const int kk = nx.kt * kKv8Unit + 16 * (col >> 2), kv = nx.kt * kKv8Unit + 16 * g4;
+    idk = kk < nx.ctx ? tab[kk >> psh] : 0;
+    idv = kv < nx.ctx ? tab[kv >> psh] : 0;
+  };
+  auto load_k = [&]() {
+    if (!have()) return;
+    const int id = page_or_none(idk, (int)c.npages);
+    const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
+                       (int64_t)(((nx.kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD +
+                       16 * g4;
 #pragma unroll
-      for (int v = 0; v < 8; ++v) x[v] = 0.0f;
-      if (j < sq.n) {
-        const float *q = a.q + (int64_t)(row0 + j) * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 8 * d8;
-        const f32x4 x0 = *reinterpret_cast<const f32x4_u *>(q);
-        const f32x4 x1 = *reinterpret_cast<const f32x4_u *>(q + 4);
+    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          x[v] = x0[v] * qscale;
-          x[4 + v] = x1[v] * qscale;
-        }
-      }
-      u32x4 f[3];
-      split3x8(x, f);
-      const int h = d8 >> 3, gg = (d8 & 7) >> 1, e = d8 & 1;
+      for (int h = 0; h < HH; ++h)
+        kr[tt][h] = *reinterpret_cast<const u32x4 *>(p + 4 * tt * HD + 64 * h);
+  };
+  auto load_v = [&]() {
+    if (!have()) return;
+    if (WIDE && second) {                 // (an even unit of the same page came before it)
 #pragma unroll
-      for (int k = 0; k < 3; ++k)
-        qf[((k * KS + 2 * h + e) * MT + cc / 16) * 64 + gg * 16 + cc % 16] = f[k];
+      for (int d = 0; d < DT; ++d) vr[d] = vr2[WIDE ? d : 0];
+      second = false;
+      return;
     }
-    // keys each of this lane's columns sees: 0 .. kend-1 (0: no such column)
-    int kend[MT];
-    int kmin = INT32_MAX;
+    const int id = page_or_none(idv, (int)c.npages);
+    const uint8_t *base = c.pages + (id < 0 ? 0 : id) * pbytes;
+    const float *sc = reinterpret_cast<const float *>(base + scales_at);
+    ks = id < 0 ? __builtin_nanf("") : sc[g];
+    vs = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
+    const uint8_t *p = base + v_at + (int64_t)col * P + ((nx.kt * kKv8Unit + 16 * g4) & (P - 1));
+    // non-temporal where a load takes whole lines (64 sequences, pages of 64
+    // tokens, 71 -> 67 us; with WIDE's two loads a line 124 -> 132)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int j = (rt * NC + 16 * mt + col) / grp;
-      kend[mt] = j < sq.n ? (int)min((int64_t)sq.old + j + 1, cap) : 0;
-      if (j < sq.n) kmin = min(kmin, kend[mt]);
+    for (int d = 0; d < DT; ++d) {
+      const u32x4 *q = reinterpret_cast<const u32x4 *>(p + (int64_t)16 * d * P);
+      vr[d] = WIDE ? *q : __builtin_nontemporal_load(q);
     }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) kmin = min(kmin, __shfl_xor(kmin, d));
-    __syncthreads();
-
-    // ---- the wave's units
-    u32x4 kr[4][HH], vr[DT];
-    float ks = 0.0f, vs = 0.0f;
-    // page of the 16 keys from key0 on (reads page 0 where there is none)
-    auto page_at = [&](int key0) -> int {
-      return key0 < ctx ? page_or_none(tab[key0 / P], (int)c.npages) : 0;
-    };
-    auto load_k = [&](int kt) {
-      const int key0 = kt * kKv8Unit + 16 * (col >> 2);
-      const int id = page_at(key0);
-      const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
-                         (int64_t)(key0 % P + (col & 3)) * HD + 16 * g4;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int h = 0; h < HH; ++h)
-          kr[tt][h] = *reinterpret_cast<const u32x4 *>(p + 4 * tt * HD + 64 * h);
-    };
-    auto load_v = [&](int kt) {
-      const int key0 = kt * kKv8Unit + 16 * g4;
-      const int id = page_at(key0);
-      const uint8_t *base = c.pages + (id < 0 ? 0 : id) * pbytes;
-      const float *sc = reinterpret_cast<const float *>(base + scales_at);
-      ks = id < 0 ? __builtin_nanf("") : sc[g];
-      vs = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
-      const uint8_t *p = base + v_at + (int64_t)col * P + key0 % P;
+    if (WIDE && (nx.kt & 1) == 0 && nx.kt + 1 < nx.t1) {
+      second = true;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
-        vr[d] = *reinterpret_cast<const u32x4 *>(p + (int64_t)16 * d * P);
-    };
-    f32x4 o[DT][MT];
-    float m[MT], l[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt] = -INFINITY;
-      l[mt] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d][mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        vr2[WIDE ? d : 0] = *reinterpret_cast<const u32x4 *>(p + (int64_t)16 * d * P + kKv8Unit);
     }
-    int kt = t0 + w;
-    if (kt < t1) {
-      load_k(kt);
-      load_v(kt);
-    }
-    for (; kt < t1; kt += 4) {
-      f32x4 s[4][MT];
+  };
+  auto advance = [&]() {
+    nx.kt += step;
+    if (WHOLE || nx.kt < nx.t1) return;
+    const int u = nx.u + (nx.t1 - nx.t0);
+    if (u < uend) nx = place(u, nx.i);
+  };
+  load_ids();
+  load_k();
+  load_v();
+  advance();
+  load_ids();
+
+  for (;;) {                              // row tiles of the run
+    const int row0 = pl.row0[cu.i], n = pl.n[cu.i], old = pl.old[cu.i];
+    // ---- this lane's digits of q: column col, dims 64 h + 16 g4 ..; the keys
+    // its columns see: 0 .. kend-1 (0: no such column)
+    const int lin = cu.rt * NC + cc, j = lin / grp;
+    const int kend = j < n ? min(old + j + 1, cap) : 0;
+    int kmin = j < n ? kend : INT32_MAX;
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
+    for (int d = 1; d < 16; d <<= 1) kmin = min(kmin, __shfl_xor(kmin, d));
+    u32x4 qd[4][HH];
+    float qs;                             // score = ks qs (256^3 d3 + 256^2 d2 + 256 d1 + d0)
+    {
+      float x[HH][16];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[tt][mt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int h = 0; h < HH; ++h) {
+        const float *q = a.q + (int64_t)(row0 + (j < n ? j : 0)) * a.ldq +
+                         (int64_t)(g * grp + lin % grp) * HD + 64 * h + 16 * g4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const f32x4 y = *reinterpret_cast<const f32x4_u *>(q + 4 * v);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) x[h][4 * v + z] = y[z];
+        }
+      }
+      uint32_t bits = 0;                  // |q| as bits: NaN and infinity above all
 #pragma unroll
       for (int h = 0; h < HH; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          bf16x8_t ka[4];
+        for (int v = 0; v < 16; ++v)
+          bits = max(bits, __builtin_bit_cast(uint32_t, x[h][v]) & 0x7fffffffu);
+      bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16));
+      bits = max(bits, (uint32_t)__shfl_xor((int)bits, 32));
+      const bool fine = bits < 0x7f800000u;
+      const int e = max((int)(bits >> 23) - 126, -90);     // |q| < 2^e
+      const float up = __builtin_ldexpf(1.0f, 30 - e);
+      qs = fine ? __builtin_ldexpf(qscale, e - 30) : __builtin_nanf("");
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) ka[tt] = codes_to_bf16(kr[tt][h][2 * e], kr[tt][h][2 * e + 1]);
+      for (int h = 0; h < HH; ++h)
 #pragma unroll
-          for (int k = 0; k < 3; ++k)
+        for (int v = 0; v < 4; ++v) {
+          float y[4];
+          uint32_t d[4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              const bf16x8_t b =
-                  __builtin_bit_cast(bf16x8_t, qf[((k * KS + 2 * h + e) * MT + mt) * 64 + lane]);
+          for (int z = 0; z < 4; ++z) y[z] = fine ? x[h][4 * v + z] * up : 0.0f;
+          digits4(y, d);
 #pragma unroll
-              for (int tt = 0; tt < 4; ++tt)
-                s[tt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[tt], b, s[tt][mt], 0, 0, 0);
-            }
+          for (int k = 0; k < 4; ++k) qd[k][h][v] = d[k];
         }
-      const float ksc = ks, vsc = vs;
-      if (kt + 4 < t1) load_k(kt + 4);
-      const int key0 = kt * kKv8Unit + 16 * g4;
-      const bool masked = kt * kKv8Unit + kKv8Unit > kmin;
-      u32x4 pf[2][MT][3];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float tmax = -INFINITY;
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            float x = s[tt][mt][v] * ksc;
-            if (masked) x = key0 + 4 * tt + v < kend[mt] ? x : -INFINITY;
-            s[tt][mt][v] = x;
-            tmax = fmaxf(tmax, x);
-          }
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
-        // the maximum rounded to an integer: alpha is a power of two, and 1
-        // for most units
-        const float mnew = fmaxf(m[mt], __builtin_rintf(tmax));
-        const float ms = mnew == -INFINITY ? 0.0f : mnew;
-        const float alpha = __builtin_amdgcn_exp2f(m[mt] - ms);
-        m[mt] = mnew;
-        float ps = 0.0f;
-        float pv[2][8];
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float p = __builtin_amdgcn_exp2f(s[tt][mt][v] - ms);
-            ps += p;
-            // (a page of NaN scale counts for the rows that see one of its keys)
-            float x = p * vsc;
-            if (masked) x = key0 + 4 * tt + v < kend[mt] ? x : 0.0f;
-            pv[tt >> 1][4 * (tt & 1) + v] = x;
-          }
-        l[mt] = __builtin_fmaf(l[mt], alpha, ps);
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[d][mt] *= alpha;
-        }
-        split3x8(pv[0], pf[0][mt]);
-        split3x8(pv[1], pf[1][mt]);
-      }
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bf16x8_t va = codes_to_bf16(vr[d][2 * e], vr[d][2 * e + 1]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-              o[d][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  va, __builtin_bit_cast(bf16x8_t, pf[e][mt][k]), o[d][mt], 0, 0, 0);
-        }
-      if (kt + 4 < t1) load_v(kt + 4);
     }
 
-    // ---- the four waves meet
+    // ---- the wave's units
+    f32x4 o[DT];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      l[mt] += __shfl_xor(l[mt], 16);
-      l[mt] += __shfl_xor(l[mt], 32);
-      if (g4 == 0) {
-        wm[w][16 * mt + col] = m[mt];
-        wl[w][16 * mt + col] = l[mt];
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kt = WHOLE ? w : cu.t0; kt < cu.t1; kt += step) {
+      f32x4 s[4];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        i32x4 d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          d[k] = i32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int h = 0; h < HH; ++h)
+            d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[tt][h]),
+                                                         __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0,
+                                                         0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v)       // (|d| < 2^21 each: the pairs fit)
+          s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
+                                    (float)((d[1][v] << 8) + d[0][v]));
       }
-    }
-    __syncthreads();                      // (and q's fragments are done with)
-    float mall[MT], lall[MT];
+      const float sc = qs * ks, vsc = vs;
+      load_k();
+      const int key0 = kt * kKv8Unit + 16 * g4;
+      const bool masked = kt * kKv8Unit + kKv8Unit > kmin;
+      float tmax = -INFINITY;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int cc = 16 * mt + col;
-      float mx = -INFINITY;
+      for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mx = fmaxf(mx, wm[x][cc]);
-      const float ms = mx == -INFINITY ? 0.0f : mx;
-      float sum = 0.0f;
+        for (int v = 0; v < 4; ++v) {
+          float x = s[tt][v] * sc;
+          if (masked) x = key0 + 4 * tt + v < kend ? x : -INFINITY;
+          s[tt][v] = x;
+          tmax = fmaxf(tmax, x);
+        }
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+      // the maximum rounded to an integer: alpha is a power of two, and 1 for
+      // most units
+      const float mnew = fmaxf(m, __builtin_rintf(tmax));
+      const float ms = mnew == -INFINITY ? 0.0f : mnew;
+      const float alpha = __builtin_amdgcn_exp2f(m - ms);
+      m = mnew;
+      float ps = 0.0f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        sum = __builtin_fmaf(wl[x][cc], __builtin_amdgcn_exp2f(wm[x][cc] - ms), sum);
-      mall[mt] = mx;
-      lall[mt] = sum;
-      const float f = __builtin_amdgcn_exp2f(m[mt] - ms);
+      for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d][mt] *= f;
-    }
-    auto put = [&](float *dst) {
+        for (int v = 0; v < 4; ++v) {
+          const float p = __builtin_amdgcn_exp2f(s[tt][v] - ms);
+          ps += p;
+          // (a page of NaN scale counts for the rows that see one of its keys)
+          float x = p * vsc;
+          if (masked) x = key0 + 4 * tt + v < kend ? x : 0.0f;
+          s[tt][v] = x;
+        }
+      l = __builtin_fmaf(l, alpha, ps);
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+        for (int d = 0; d < DT; ++d) o[d] *= alpha;
+      }
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          *reinterpret_cast<f32x4 *>(dst + (16 * mt + col) * OST + 16 * d + 4 * g4) = o[d][mt];
-    };
-    auto take = [&](const float *src) {
+      for (int e = 0; e < 2; ++e) {
+        u32x4 pf[3];
+        float x[8];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+        for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3];
+        split3x8(x, pf);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d][mt] += *reinterpret_cast<const f32x4 *>(src + (16 * mt + col) * OST + 16 * d + 4 * g4);
-    };
-    // (a wave without units adds zeros; its order in the sum is fixed)
-    if (w >= 2) put(ob + (w - 2) * NC * OST);
-    __syncthreads();
-    if (w < 2) take(ob + w * NC * OST);
-    __syncthreads();
-    if (w == 1) put(ob);
-    __syncthreads();
-    if (w == 0) {
-      take(ob);
-      const bool whole = t0 == 0 && t1 == sq.key_units;
-      float *rec = a.ws + (((int64_t)blockIdx.x * c.nkv + g) * 2 + (t0 == 0)) * kv8_record<HD, NC>();
+        for (int d = 0; d < DT; ++d) {
+          const bf16x8_t va = codes_to_bf16(vr[d][2 * e], vr[d][2 * e + 1]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int cc = 16 * mt + col, lin = rt * NC + cc, j = lin / grp;
-        if (whole) {
-          if (j >= sq.n) continue;
-          const float il = 1.0f / lall[mt];
-          float *out = a.out + ((int64_t)(row0 + j) * c.nheads + g * grp + lin % grp) * HD + 4 * g4;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            *reinterpret_cast<f32x4_u *>(out + 16 * d) = o[d][mt] * il;
-        } else {
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            *reinterpret_cast<f32x4 *>(rec + cc * HD + 16 * d + 4 * g4) = o[d][mt];
-          if (g4 == 0) {
-            rec[NC * HD + cc] = mall[mt];
-            rec[NC * HD + NC + cc] = lall[mt];
-          }
+          for (int k = 0; k < 3; ++k)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, pf[k]), o[d],
+                                                           0, 0, 0);
         }
       }
+      load_v();
+      advance();
+      load_ids();
     }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    if (WHOLE) {                          // the runs of the row tile meet
+      if (g4 == 0) {
+        wm[w][cc] = m;
+        wl[w][cc] = l;
+      }
+      __syncthreads();
+      float mx = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < RW; ++x) mx = fmaxf(mx, wm[x][cc]);
+      const float ms = mx == -INFINITY ? 0.0f : mx;
+      l = 0.0f;
+#pragma unroll
+      for (int x = 0; x < RW; ++x) l = __builtin_fmaf(wl[x][cc], __builtin_amdgcn_exp2f(wm[x][cc] - ms), l);
+      const float f = __builtin_amdgcn_exp2f(m - ms);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+      // (a run without units adds zeros; the order of the sum is fixed)
+      for (int half = RW / 2; half > 0; half >>= 1) {
+        f32x4 *at = reinterpret_cast<f32x4 *>(ob + ((w % half) * NC + cc) * OST + 4 * g4);
+        if (w >= half && w < 2 * half) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) at[4 * d] = o[d];
+        }
+        __syncthreads();
+        if (w < half) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[d] += at[4 * d];
+        }
+        __syncthreads();
+      }
+      if (w != 0) return;
+    }
+    if (j < n) {
+      const bool whole = WHOLE || (cu.t0 == 0 && cu.t1 == cu.units);
+      float *rec = a.ws + (((int64_t)run * c.nkv + g) * 2 + (cu.t0 == 0)) * kv8_record<HD, NC>();
+      const float il = whole ? 1.0f / l : 1.0f;
+      float *out = whole ? a.out + ((int64_t)(row0 + j) * c.nheads + g * grp + lin % grp) * HD
+                         : rec + cc * HD;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(out + 16 * d + 4 * g4) = o[d] * il;
+      if (!whole && g4 == 0) {
+        rec[NC * HD + cc] = m;
+        rec[NC * HD + NC + cc] = l;
+      }
+    }
+    const int u = cu.u + (cu.t1 - cu.t0);
+    if (WHOLE || u >= uend) return;
+    cu = place(u, cu.i);
   }
 }
 
-// Joins the records of the row tiles that several blocks served: grid
-// (rows, nkv), the block's threads over the group's heads x HD / 4 dims.
+// Joins the records of the row tiles that several runs served: grid
+// (rows, nkv, heads of a group / hb).  The block's threads are groups over hb
+// heads x HD / 4 dims; the groups take the records in turn and meet in LDS.
 template <int HD, int MT>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int nblocks) {
-  constexpr int NC = 16 * MT;
-  extern __shared__ __attribute__((aligned(16))) int pre[];
-  __shared__ int wsum[4];
+__global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs, int hb) {
+  constexpr int NC = 16 * MT, NT = 512;
+  __shared__ __attribute__((aligned(16))) float so[NT * 4];
+  __shared__ float sm[NT], sl[NT];
   const Kv8Args &c = a.c;
   const int g = blockIdx.y, grp = c.nheads / c.nkv, nseq = (int)c.nseq;
-  const int row = blockIdx.x;
-  const int units = kv8_plan(c, NC, pre, wsum);
-  const int per = kv8_units_per_block(units, nblocks, kKv8Least);
-  __syncthreads();
-  // the sequence of this row
-  int lo = 0, hi = nseq;
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (c.cu[m] <= row) lo = m;
-    else hi = m;
-  }
+  const int row = blockIdx.x, t = threadIdx.x;
+  const int *pre = kv8_plan_at<HD, NC>(a, runs);
+  const int per = kv8_units_per_block(pre[nseq], runs, 1);
+  // the sequence of this row: the last one that begins at it or before
+  const int lo = find_seq(c.cu, nseq, c.rows, row, 1, 0);
   const Kv8Seq sq = kv8_seq(c.cu[lo], c.cu[lo + 1], c.len[lo], c.rows, c.maxpages * c.page, grp, NC);
   const int j = row - clamp_i(c.cu[lo], 0, c.rows);
   if (j < 0 || j >= sq.n) return;             // behind the last sequence
-  for (int n = threadIdx.x; n < grp * (HD / 4); n += 256) {
-    const int hh = n / (HD / 4), d = 4 * (n % (HD / 4));
+  constexpr int IPH = HD / 4;
+  const int sg = NT / (hb * IPH);             // groups of threads
+  const int grp_id = t / (hb * IPH), item = t % (hb * IPH);
+  {
+    const int hh = blockIdx.z * hb + item / IPH, d = 4 * (item % IPH);
     const int lin = j * grp + hh, rt = lin / NC, cc = lin % NC;
     const int64_t ua = pre[lo] + (int64_t)rt * sq.key_units;
-    const int b0 = clamp_i(ua / per, 0, nblocks - 1);
-    const int b1 = clamp_i((ua + sq.key_units - 1) / per, 0, nblocks - 1);
-    if (b0 == b1) continue;                   // written whole
-    auto rec = [&](int b) {
-      return a.ws + (((int64_t)b * c.nkv + g) * 2 + (b == b0)) * kv8_record<HD, NC>();
-    };
+    const int b0 = clamp_i(ua / per, 0, runs - 1);
+    const int b1 = clamp_i((ua + sq.key_units - 1) / per, 0, runs - 1);
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int z0 = b0; z0 <= b1; z0 += 8) {
-      float zm[8], zl[8];
-      f32x4 zo[8];
+    const bool on = grp_id < sg && hh < grp && b0 != b1;   // (b0 == b1: written whole)
+    for (int z0 = b0 + grp_id; on && z0 <= b1; z0 += 4 * sg) {
+      float zm[4], zl[4];
+      f32x4 zo[4];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float *r = rec(z0 + x <= b1 ? z0 + x : b1);
+      for (int x = 0; x < 4; ++x) {
+        const int z = z0 + x * sg <= b1 ? z0 + x * sg : z0;
+        const float *r = a.ws + (((int64_t)z * c.nkv + g) * 2 + (z == b0)) * kv8_record<HD, NC>();
         zm[x] = r[NC * HD + cc];
         zl[x] = r[NC * HD + NC + cc];
         zo[x] = *reinterpret_cast<const f32x4 *>(r + cc * HD + d);
       }
       float mx = m;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) mx = fmaxf(mx, z0 + x <= b1 ? zm[x] : -INFINITY);
+      for (int x = 0; x < 4; ++x) mx = fmaxf(mx, z0 + x * sg <= b1 ? zm[x] : -INFINITY);
       const float ms = mx == -INFINITY ? 0.0f : mx;
       const float f0 = __builtin_amdgcn_exp2f(m - ms);
       l *= f0;
       o *= f0;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float f = z0 + x <= b1 ? __builtin_amdgcn_exp2f(zm[x] - ms) : 0.0f;
-        if (z0 + x > b1) continue;
+      for (int x = 0; x < 4; ++x) {
+        if (z0 + x * sg > b1) continue;
+        const float f = __builtin_amdgcn_exp2f(zm[x] - ms);
         l = __builtin_fmaf(f, zl[x], l);
 #pragma unroll
         for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(f, zo[x][v], o[v]);
       }
       m = mx;
+    }
+    sm[t] = m;
+    sl[t] = l;
+    *reinterpret_cast<f32x4 *>(so + 4 * t) = o;
+    __syncthreads();
+    if (grp_id != 0 || !on) return;
+    float mx = m;
+    for (int x = 1; x < sg; ++x) mx = fmaxf(mx, sm[x * hb * IPH + item]);
+    const float ms = mx == -INFINITY ? 0.0f : mx;
+    const float f0 = __builtin_amdgcn_exp2f(m - ms);
+    l *= f0;
+    o *= f0;
+    for (int x = 1; x < sg; ++x) {
+      const int y = x * hb * IPH + item;
+      const float f = __builtin_amdgcn_exp2f(sm[y] - ms);
+      l = __builtin_fmaf(f, sl[y], l);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(f, so[4 * y + v], o[v]);
     }
     const float il = 1.0f / l;
     *reinterpret_cast<f32x4_u *>(a.out + ((int64_t)row * c.nheads + g * grp + hh) * HD + d) = o * il;
@@ -713,25 +809,37 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int nbloc
 
 template <int HD, int MT>
 hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
-  constexpr int NC = 16 * MT, KS = HD / 32, OST = HD + 4;
-  constexpr int kQBytes = 3 * KS * MT * 64 * 16, kOBytes = 2 * NC * OST * 4;
+  constexpr int NC = 16 * MT, RW = kKv8Waves / MT;
   const Kv8Args &c = a.c;
   const int grp = c.nheads / c.nkv;
+  const size_t plan = (size_t)(4 * c.nseq + 1) * 4;
+  const int64_t tiles = c.rows * grp / NC + c.nseq;
+  const int64_t key_units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit;
+  if (key_units <= kKv8WholeUnits) {
+    const size_t lds = (size_t)(8 / MT / 2) * NC * (HD + 4) * 4 + plan;
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, true, false>), dim3((unsigned)tiles, (unsigned)c.nkv),
+                       dim3(512), lds, st, a);
+    return hipGetLastError();
+  }
   // two blocks per CU over all KV heads, as far as the work (by its bound)
   // and the records' space reach
-  const int64_t units = (c.rows * grp / NC + c.nseq) * ((c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit);
   int64_t nb = (512 + c.nkv - 1) / c.nkv;
-  nb = std::min(nb, (units + kKv8Least - 1) / kKv8Least);
-  nb = std::min(nb, a.ws_floats / (2 * (int64_t)c.nkv * kv8_record<HD, NC>()));
-  if (nb < 1) nb = 1;
-  const size_t plan = (size_t)(c.nseq + 1) * 4;
-  const size_t lds = (size_t)std::max(kQBytes, kOBytes) + plan;
-  hipLaunchKernelGGL((kv8_attn_kernel<HD, MT>), dim3((unsigned)nb, (unsigned)c.nkv), dim3(256), lds,
-                     st, a);
+  nb = std::min(nb, (tiles * key_units + RW - 1) / RW);
+  nb = std::min(nb, (a.ws_floats - c.nseq - 1) / (RW * 2 * (int64_t)c.nkv * kv8_record<HD, NC>()));
+  if (nb < 1) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)nb, (unsigned)c.nkv), block(64 * kKv8Waves);
+  if (c.page == 128)
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, true>), grid, block, plan, st, a);
+  else
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, false>), grid, block, plan, st, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || nb == 1) return e;
-  hipLaunchKernelGGL((kv8_merge_kernel<HD, MT>), dim3((unsigned)c.rows, (unsigned)c.nkv), dim3(256),
-                     plan, st, a, (int)nb);
+  if (e != hipSuccess) return e;
+  // few rows: more blocks, with more groups of threads over a row's records
+  int hb = std::min(grp, 512 / (HD / 4));
+  while (hb > 1 && c.rows * c.nkv * ((grp + hb - 1) / hb) < 256) hb = (hb + 1) / 2;
+  hipLaunchKernelGGL((kv8_merge_kernel<HD, MT>),
+                     dim3((unsigned)c.rows, (unsigned)c.nkv, (unsigned)((grp + hb - 1) / hb)),
+                     dim3(512), 0, st, a, (int)(nb * RW), hb);
   return hipGetLastError();
 }
 
@@ -753,12 +861,27 @@ hipError_t launch_kv8_append(const Kv8AppendArgs &a, hipStream_t st) {
   return a.c.head_dim == 64 ? launch_append_t<64>(a, st) : launch_append_t<128>(a, st);
 }
 
+template <int MT>
+static hipError_t launch_kv8_cols(const Kv8AttnArgs &a, hipStream_t st) {
+  return a.c.head_dim == 64 ? launch_kv8_attn_t<64, MT>(a, st) : launch_kv8_attn_t<128, MT>(a, st);
+}
+
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
-  // one 16-column tile where a sequence's rows fill no more on average
-  const bool one = a.c.rows * (a.c.nheads / a.c.nkv) <= 16 * a.c.nseq;
-  if (a.c.head_dim == 64)
-    return one ? launch_kv8_attn_t<64, 1>(a, st) : launch_kv8_attn_t<64, 2>(a, st);
-  return one ? launch_kv8_attn_t<128, 1>(a, st) : launch_kv8_attn_t<128, 2>(a, st);
+  // row tiles of 16, 32 or 64 columns, as the sequences' rows fill them on
+  // average (a tile's keys are read once)
+  const int64_t cols = a.c.rows * (a.c.nheads / a.c.nkv);
+  for (int64_t i = 0; i < a.c.nseq; i += kKv8PlanSeq) {
+    Kv8AttnArgs p = a;
+    p.c.cu += i;
+    p.c.len += i;
+    p.c.tab += i * a.c.maxpages;
+    p.c.nseq = std::min<int64_t>(kKv8PlanSeq, a.c.nseq - i);
+    const hipError_t e = cols <= 16 * a.c.nseq   ? launch_kv8_cols<1>(p, st)
+                         : cols <= 32 * a.c.nseq ? launch_kv8_cols<2>(p, st)
+                                                 : launch_kv8_cols<4>(p, st);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace q8
