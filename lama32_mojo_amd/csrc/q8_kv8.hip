@@ -18,23 +18,30 @@ namespace {
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // any f32 address
 
-// The sequence of block b: the last i with seq_first_block(cu[i], i) <= b.
-// The whole wave searches, 64 candidates a step.
-__device__ __forceinline__ int find_seq(const int *__restrict__ cu, int nseq, int64_t rows,
-                                        int64_t b, int tile, int spare) {
+// The sequence of block b: the last i with seq_first_block(cu[i], i) <= b, with
+// its rows and length.  The whole wave searches, 64 candidates a step, and reads
+// the candidates' rows and lengths along, so up to 64 sequences take one round
+// trip.
+struct SeqAt {
+  int i, r0, r1, len;
+};
+__device__ __forceinline__ SeqAt find_seq(const int *__restrict__ cu, const int *__restrict__ len,
+                                          int nseq, int64_t rows, int64_t b, int tile, int spare) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = nseq;                     // the answer lies in [lo, lo + n)
-  while (n > 1) {
+  for (;;) {
     const int step = (n + 63) / 64;         // candidates lo, lo + step, ...
-    const int i = lo + lane * step;
-    const bool le = lane * step < n &&
-                    seq_first_block(clamp_i(cu[i < nseq ? i : nseq - 1], 0, rows), i, tile, spare) <= b;
+    const int i = min(lo + lane * step, nseq - 1);
+    const int c0 = clamp_i(cu[i], 0, rows), c1 = clamp_i(cu[i + 1], 0, rows), ln = len[i];
+    const bool le = lane * step < n && seq_first_block(c0, i, tile, spare) <= b;
     const uint64_t m = __builtin_amdgcn_ballot_w64(le);
     const int k = m ? 63 - __builtin_clzll(m) : 0;
-    n = n - k * step < step ? n - k * step : step;
+    n = min(n - k * step, step);
     lo += k * step;
+    if (n <= 1)
+      return {lo, __builtin_amdgcn_readlane(c0, k), __builtin_amdgcn_readlane(c1, k),
+              __builtin_amdgcn_readlane(ln, k)};
   }
-  return lo;
 }
 
 // cos and sin of pos * inv to f64 accuracy: the angle as an exact f64
@@ -86,15 +93,38 @@ __device__ __forceinline__ void sincos_pos(int pos, float inv, double &sn, doubl
 // Bound: HBM for prompts (q read and written, k and v read, codes written),
 // the chain of dependent loads for a token per sequence.
 
-// rint(x / s), half to even, as if divided exactly: c = rint(x * (1/s)) is off
-// by one at most, next to a border; x - c s is exact (a multiple of ulp(s) below
-// 2^24 of them), so its side of s / 2 settles it.
-__device__ __forceinline__ float code_of(float x, float s, float inv) {
-  float c = __builtin_rintf(x * inv);
-  const float r = __builtin_fmaf(-c, s, x), h = 0.5f * s;
-  const bool odd = ((int)c & 1) != 0;
-  c += (r > h || (r == h && odd)) ? 1.0f : (r < -h || (r == -h && odd)) ? -1.0f : 0.0f;
-  return __builtin_fminf(__builtin_fmaxf(c, -127.0f), 127.0f);
+// rint(x / s), half to even, as if divided exactly, of four values, as bytes:
+// c = rint(x * (1/s)) is off by one at most, next to a border; x - c s is exact
+// (a multiple of ulp(s) below 2^24 of them), so its side of s / 2 settles it.
+// s from 2^-100 on; below, the f64 quotient is far enough from any border that
+// it does not hit.
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s, float inv) {
+  float c[4];
+  if (s <= 0x1p-100f) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[u] = s == 0.0f ? 0.0f : (float)rint((double)x[u] / (double)s);
+  } else {
+    const float h = 0.5f * s;
+    float r[4], worst = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      c[u] = __builtin_rintf(x[u] * inv);
+      r[u] = __builtin_fmaf(-c[u], s, x[u]);
+      worst = fmaxf(worst, fabsf(r[u]));
+    }
+    if (worst >= h) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool odd = ((int)c[u] & 1) != 0;
+        c[u] += (r[u] > h || (r[u] == h && odd)) ? 1.0f : (r[u] < -h || (r[u] == -h && odd)) ? -1.0f : 0.0f;
+      }
+    }
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    w |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(c[u], -127.0f, 127.0f) & 255u) << (8 * u);
+  return w;
 }
 
 template <int HD, int P>
@@ -103,15 +133,14 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   constexpr int IPT = HD / 8;                 // items per token
   constexpr int TPP = 256 / IPT;              // tokens per pass
   constexpr int NP = (P + TPP - 1) / TPP;     // passes
-  constexpr int VST = P + 4;                  // bytes of a V column in LDS
+  constexpr int VST = P + 16;                 // bytes of a V column in LDS
   __shared__ __attribute__((aligned(16))) uint8_t vt[HD * VST];
   __shared__ uint32_t red[2][4];
   const Kv8Args &c = a.c;
   const int t = threadIdx.x, g = blockIdx.y, grp = c.nheads / c.nkv;
   const int nseq = (int)c.nseq;
-  const int i = find_seq(c.cu, nseq, c.rows, blockIdx.x, P, 2);
-  const int r0 = clamp_i(c.cu[i], 0, c.rows), r1 = clamp_i(c.cu[i + 1], 0, c.rows);
-  const int len = clamp_i(c.len[i], 0, (int64_t)1 << 30);
+  const SeqAt sq = find_seq(c.cu, c.len, nseq, c.rows, blockIdx.x, P, 2);
+  const int i = sq.i, r0 = sq.r0, r1 = sq.r1, len = clamp_i(sq.len, 0, (int64_t)1 << 30);
   const int64_t b = (int64_t)blockIdx.x - seq_first_block(r0, i, P, 2);
   const int64_t pg = len / P + b;             // page of the sequence
   const int64_t p0 = pg * P;                  // its first position
@@ -121,6 +150,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const int row0 = r0 + (int)(p0 - len);      // row of the page's token 0
   int id = pg < c.maxpages ? c.tab[(int64_t)i * c.maxpages + pg] : -1;
   id = page_or_none(id, (int)c.npages);
+  uint8_t *page = c.pages + (int64_t)(id < 0 ? 0 : id) * kv8_page_bytes(P, c.nkv, HD);
+  float *scale = reinterpret_cast<float *>(page + kv8_scales_at(P, c.nkv, HD));
+  const float old0 = scale[g], old1 = scale[c.nkv + g];
   const int64_t kvdim = (int64_t)c.nkv * HD;
 
   float kx[NP][8], vx[NP][8];
@@ -200,70 +232,99 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
     red[1][t >> 6] = vmax;
   }
   __syncthreads();
-  uint8_t *page = c.pages + (int64_t)id * kv8_page_bytes(P, c.nkv, HD);
-  float *scale = reinterpret_cast<float *>(page + kv8_scales_at(P, c.nkv, HD));
   float s0[2], s1[2], inv[2];
   bool fine[2], grew[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const uint32_t mx = max(max(red[x][0], red[x][1]), max(red[x][2], red[x][3]));
     const float am = __builtin_bit_cast(float, mx) / 127.0f;
-    s0[x] = e > 0 ? scale[x * c.nkv + g] : 0.0f;
+    s0[x] = e > 0 ? (x ? old1 : old0) : 0.0f;
     s1[x] = am > s0[x] || am != am ? am : s0[x];          // (a NaN s0 stays)
     fine[x] = __builtin_isfinite(s1[x]);
     if (!fine[x]) s1[x] = __builtin_nanf("");
     grew[x] = e > 0 && fine[x] && s1[x] > s0[x];
-    // 1 / s1 and x - c s1 keep their bits while s1 is well inside the normal
-    // range; below, the codes are formed from the f64 quotient
     inv[x] = 1.0f / s1[x];
   }
-  __syncthreads();                            // every thread has read s0
   if (t < 2) scale[t * c.nkv + g] = s1[t];
   uint8_t *kc = page + (int64_t)g * P * HD, *vc = page + (int64_t)(c.nkv + g) * P * HD;
-  auto code = [&](float x, int w) -> uint32_t {
-    if (!fine[w] || s1[w] == 0.0f) return 0;
-    const float q = s1[w] > 0x1p-100f
-                        ? code_of(x, s1[w], inv[w])
-                        : (float)fmin(fmax(rint((double)x / (double)s1[w]), -127.0), 127.0);
+  // The old codes that stay around new ones in a V run of 16 tokens, or that
+  // change: all loads go out together.
+  constexpr int KI = (HD * P / 16 + 255) / 256;          // 16-byte runs per thread
+  constexpr int RPC = P / 16;                            // runs of a V column
+  u32x4 kold[KI], vold[KI];
+#pragma unroll
+  for (int u = 0; u < KI; ++u) {
+    const int n = t + 256 * u, x = 16 * (n % RPC);
+    if (grew[0] && n < e * (HD / 16)) kold[u] = *reinterpret_cast<const u32x4 *>(kc + 16 * n);
+    if (n < HD * RPC && x < z && (x < e ? x + 16 > e || grew[1] : x + 16 > z))
+      vold[u] = *reinterpret_cast<const u32x4 *>(vc + 16 * n);
+  }
+  // An old token's code at a larger scale: rint(c s0 / s1).  The f32 quotient is
+  // within 127 2^-22 of it; next to a border the remainder decides, exact in f64
+  // (c s0 and q s1 have 31 bits).
+  float ratio[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) ratio[x] = grew[x] ? s0[x] / s1[x] : 1.0f;
+  auto again = [&](uint32_t byte, int w) -> uint32_t {
+    const float c = (float)(int8_t)byte, y = c * ratio[w];
+    float q = __builtin_rintf(y);
+    if (__builtin_fabsf(__builtin_fabsf(y - q) - 0.5f) < 1e-4f) {
+      const double r = __builtin_fma(-(double)q, (double)s1[w], (double)c * (double)s0[w]);
+      const double h = 0.5 * (double)s1[w];
+      const bool odd = ((int)q & 1) != 0;
+      q += (r > h || (r == h && odd)) ? 1.0f : (r < -h || (r == -h && odd)) ? -1.0f : 0.0f;
+    }
     return (uint32_t)(int)q & 255u;
   };
-  // the old tokens' codes at a larger scale
-  auto again = [&](uint8_t *at, int w) {
-    const double d = (double)(int8_t)*at * (double)s0[w] / (double)s1[w];
-    *at = (uint8_t)(int8_t)(int)rint(d);
+  auto again4 = [&](uint32_t x, int w) -> uint32_t {
+    return again(x & 255u, w) | again(x >> 8 & 255u, w) << 8 | again(x >> 16 & 255u, w) << 16 |
+           again(x >> 24, w) << 24;
   };
-  if (grew[0])
-    for (int n = t; n < e * HD; n += 256) again(kc + n, 0);
-  if (grew[1])
-    for (int n = t; n < e * HD; n += 256) again(vc + (n / e) * P + n % e, 1);
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     const int tok = p * TPP + t / IPT;
     if (tok < e || tok >= z) continue;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t w = 0;
+      const float k4[4] = {kx[p][4 * h], kx[p][4 * h + 1], kx[p][4 * h + 2], kx[p][4 * h + 3]};
+      const float v4[4] = {vx[p][4 * h], vx[p][4 * h + 1], vx[p][4 * h + 2], vx[p][4 * h + 3]};
+      const uint32_t kw = fine[0] ? codes4(k4, s1[0], inv[0]) : 0;
+      const uint32_t vw = fine[1] ? codes4(v4, s1[1], inv[1]) : 0;
+      *reinterpret_cast<uint32_t *>(kc + tok * HD + h * half + 4 * j) = kw;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        w |= code(kx[p][4 * h + u], 0) << (8 * u);
-        vt[(h * half + 4 * j + u) * VST + tok] = (uint8_t)code(vx[p][4 * h + u], 1);
-      }
-      *reinterpret_cast<uint32_t *>(kc + tok * HD + h * half + 4 * j) = w;
+      for (int u = 0; u < 4; ++u) vt[(h * half + 4 * j + u) * VST + tok] = (uint8_t)(vw >> (8 * u));
+    }
+  }
+  if (grew[0]) {
+#pragma unroll
+    for (int u = 0; u < KI; ++u) {
+      const int n = t + 256 * u;
+      if (n >= e * (HD / 16)) continue;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) kold[u][x] = again4(kold[u][x], 0);
+      *reinterpret_cast<u32x4 *>(kc + 16 * n) = kold[u];
     }
   }
   __syncthreads();
-  if (e == 0 && z == P) {                     // a whole page: 4 tokens a store
-    for (int n = t; n < HD * P / 4; n += 256) {
-      const int d = n / (P / 4), x = 4 * (n % (P / 4));
-      *reinterpret_cast<uint32_t *>(vc + d * P + x) =
-          *reinterpret_cast<const uint32_t *>(&vt[d * VST + x]);
+  // V runs that hold a new token or an old one whose code changes; a run is one
+  // thread's, which keeps what is around them
+#pragma unroll
+  for (int u = 0; u < KI; ++u) {
+    const int n = t + 256 * u, x = 16 * (n % RPC);
+    if (n >= HD * RPC || x >= z || (x + 16 <= e && !grew[1])) continue;
+    u32x4 y = *reinterpret_cast<const u32x4 *>(&vt[(n / RPC) * VST + x]);
+    if (x < e || x + 16 > z) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // bytes of tokens before e and from z on
+        const int lo = min(max(e - x - 4 * i, 0), 4), hi = min(max(z - x - 4 * i, 0), 4);
+        const uint32_t om = (uint32_t)((1ull << (8 * lo)) - 1);
+        const uint32_t zm = ~(uint32_t)((1ull << (8 * hi)) - 1);
+        const uint32_t o = grew[1] && lo > 0 ? again4(vold[u][i], 1) : vold[u][i];
+        y[i] = (y[i] & ~(om | zm)) | (o & om) | (vold[u][i] & zm);
+      }
     }
-  } else {
-    const int m = z - e;
-    for (int n = t; n < HD * m; n += 256) {
-      const int d = n / m, x = e + n % m;
-      vc[d * P + x] = vt[d * VST + x];
-    }
+    *reinterpret_cast<u32x4 *>(vc + 16 * n) = y;
   }
 }
 
@@ -740,9 +801,9 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   const int *pre = kv8_plan_at<HD, NC>(a, runs);
   const int per = kv8_units_per_block(pre[nseq], runs, 1);
   // the sequence of this row: the last one that begins at it or before
-  const int lo = find_seq(c.cu, nseq, c.rows, row, 1, 0);
-  const Kv8Seq sq = kv8_seq(c.cu[lo], c.cu[lo + 1], c.len[lo], c.rows, c.maxpages * c.page, grp, NC);
-  const int j = row - clamp_i(c.cu[lo], 0, c.rows);
+  const SeqAt at = find_seq(c.cu, c.len, nseq, c.rows, row, 1, 0);
+  const int lo = at.i, j = row - at.r0;
+  const Kv8Seq sq = kv8_seq(at.r0, at.r1, at.len, c.rows, c.maxpages * c.page, grp, NC);
   if (j < 0 || j >= sq.n) return;             // behind the last sequence
   constexpr int IPH = HD / 4;
   const int sg = NT / (hb * IPH);             // groups of threads

@@ -49,22 +49,56 @@ __device__ __forceinline__ void refs4(const int *ref, int64_t p, int64_t npages,
   for (int u = 0; u < 4; ++u) r[u] = p + u < npages ? ref[p + u] : 1;
 }
 
+// Free pages as a wave reads them: bit r of a lane is page first + 64 r + lane,
+// r < rows <= 32.  The loads are coalesced, and independent within a group of 8.
+__device__ __forceinline__ uint32_t free_pages(const int *ref, int64_t first, int rows,
+                                               int64_t npages) {
+  const int lane = threadIdx.x & 63;
+  uint32_t bits = 0;
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    int v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int64_t p = first + 64 * (r0 + r) + lane;
+      v[r] = r0 + r < rows && p < npages ? ref[p] : 1;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) bits |= (uint32_t)(v[r] == 0) << (r0 + r);
+  }
+  return bits;
+}
+// Free pages of the wave.
+__device__ __forceinline__ int count_free(uint32_t bits, int rows) {
+  int n = 0;
+  for (int r = 0; r < rows; ++r) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(bits >> r & 1u));
+  return n;
+}
+constexpr int kList = 4096;
+
 // One block.  Slots in ascending order ask for the pages they lack (and one
 // more where their partly filled last page is shared); an exclusive sum of
 // the needs gives each slot a run of ranks, and the free page of rank r, found
 // by a second sum over the pages, goes to the slot whose run holds r.  When
 // the free pages do not reach, the slots behind the last run that fits get
-// nothing.  copies: their number, then (from, to) pairs.
+// nothing.  copies: their number, then (from, to) pairs.  Bound: the chain
+// length, page id, reference count, sums; the free pages are looked up beside it.
 __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a,
                                                                      const int *__restrict__ want,
                                                                      int *__restrict__ copies) {
   __shared__ int off[kPagesMaxSlots + 1];
   __shared__ uint8_t cow[kPagesMaxSlots];
+  __shared__ int list[kList];
   __shared__ int wsum[kScanThreads / 64];
   __shared__ int ncopy, granted_end;
-  const int t = threadIdx.x, npages = (int)a.npages;
+  const int t = threadIdx.x, npages = (int)a.npages, wave = t >> 6;
   const int64_t cap = a.maxpages * a.page;
   if (t == 0) ncopy = granted_end = 0;
+  // pages in goes of 16 waves x rows x 64; the first go's counts are in flight
+  // beside the slots' reads
+  const int rows = (int)(a.npages < 32 * kScanThreads ? (a.npages + kScanThreads - 1) / kScanThreads : 32);
+  const int64_t go = (int64_t)rows * kScanThreads;
+  const int64_t first = (int64_t)64 * rows * wave;
+  uint32_t bits = free_pages(a.ref, first, rows, a.npages);
   int need[kSlotsPerThread], mine = 0;
 #pragma unroll
   for (int u = 0; u < kSlotsPerThread; ++u) {
@@ -84,77 +118,95 @@ __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a
     mine += need[u];
   }
   int total, at = block_scan(mine, wsum, &total);
+  if (total == 0) {
+    if (t == 0) copies[0] = 0;
+    return;
+  }
 #pragma unroll
   for (int u = 0; u < kSlotsPerThread; ++u) {
     const int s = t * kSlotsPerThread + u;
-    if (s <= a.nslots) off[s] = at;
+    if (s < a.nslots) off[s] = at;
     at += need[u];
   }
   if (t == 0) off[a.nslots] = total;
-  if (total > 0) {
-    int mfree = 0, nfree;
-    for (int64_t p = 4 * t; p < a.npages; p += 4 * kScanThreads) {
-      int r[4];
-      refs4(a.ref, p, a.npages, r);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) mfree += r[u] == 0;
+  // free pages: as many as are needed, or all there are
+  // (of the first go: rank of the wave's first free page, and how many there are)
+  int nfree = 0, base0 = 0, got0 = 0;
+  for (int64_t p0 = 0; p0 < a.npages && nfree < total; p0 += go) {
+    const int n = count_free(p0 ? free_pages(a.ref, p0 + first, rows, a.npages) : bits, rows);
+    int got;
+    const int r = block_scan((t & 63) == 0 ? n : 0, wsum, &got);
+    if (p0 == 0) {
+      base0 = __builtin_amdgcn_readfirstlane(r);
+      got0 = got;
     }
-    block_scan(mfree, wsum, &nfree);
-    int end = 0;
+    nfree += got;
+  }
+  int end = 0;
 #pragma unroll
-    for (int u = 0; u < kSlotsPerThread; ++u) {
-      const int s = t * kSlotsPerThread + u;
-      if (s < a.nslots && need[u] > 0 && off[s] + need[u] <= nfree) end = off[s] + need[u];
+  for (int u = 0; u < kSlotsPerThread; ++u) {
+    const int s = t * kSlotsPerThread + u;
+    if (s < a.nslots && need[u] > 0 && off[s] + need[u] <= nfree) end = off[s] + need[u];
+  }
+  if (end) atomicMax(&granted_end, end);
+  __syncthreads();
+  // The free pages' ids by rank, kList at a time in LDS, then a thread per rank.
+  const int take = granted_end;
+  int done = 0;                               // ranks handed out
+  for (int64_t p0 = 0, run = 0; p0 < a.npages && run < take; p0 += go) {
+    int got = got0, base = base0;
+    if (p0) {
+      bits = free_pages(a.ref, p0 + first, rows, a.npages);
+      const int n = count_free(bits, rows);
+      base = (int)run + __builtin_amdgcn_readfirstlane(block_scan((t & 63) == 0 ? n : 0, wsum, &got));
     }
-    if (end) atomicMax(&granted_end, end);
-    __syncthreads();
-    const int take = granted_end;
-    int run = 0;
-    for (int64_t p0 = 0; p0 < a.npages && run < take; p0 += 4 * kScanThreads) {
-      const int64_t p = p0 + 4 * t;
-      int r[4], n = 0, got;
-      refs4(a.ref, p, a.npages, r);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) n += r[u] == 0;
-      int rank = run + block_scan(n, wsum, &got);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (r[u] != 0) continue;
-        if (rank < take) {
-          int lo = 0, hi = (int)a.nslots;       // the slot with off[lo] <= rank < off[lo + 1]
-          while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if (off[m] <= rank) lo = m;
-            else hi = m;
-          }
-          const int id = (int)(p + u), k = rank - off[lo];
-          int *row = a.tab + (int64_t)lo * a.maxpages;
-          if (cow[lo] && k == 0) {
-            int *e = row + clamp_i(a.len[lo], 0, cap) / a.page;
-            const int x = atomicAdd(&ncopy, 1);
-            copies[1 + 2 * x] = *e;
-            copies[2 + 2 * x] = id;
-            *e = id;
-          } else {
-            row[clamp_i(a.held[lo], 0, a.maxpages) + k - cow[lo]] = id;
-          }
-          a.ref[id] = 1;
-        }
-        ++rank;
+    run += got;
+    const int upto = (int)(run < take ? run : take);
+    while (done < upto) {
+      const int stop = done + kList < upto ? done + kList : upto;
+      int rank = base;
+      for (int r = 0; r < rows && rank < stop; ++r) {
+        const uint64_t m = __builtin_amdgcn_ballot_w64(bits >> r & 1u);
+        const int at = rank + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        if ((bits >> r & 1u) && at >= done && at < stop)
+          list[at - done] = (int)(p0 + first + 64 * r) + (t & 63);
+        rank += __builtin_popcountll(m);
       }
-      run += got;
-    }
-    __syncthreads();
-    // (only now: a page that this call gives up is not handed out by it)
-    for (int x = t; x < ncopy; x += kScanThreads) atomicSub(&a.ref[copies[1 + 2 * x]], 1);
-#pragma unroll
-    for (int u = 0; u < kSlotsPerThread; ++u) {
-      const int s = t * kSlotsPerThread + u;
-      if (s < a.nslots && need[u] > 0 && off[s] + need[u] <= nfree)
-        a.held[s] = clamp_i(a.held[s], 0, a.maxpages) + need[u] - cow[s];
+      __syncthreads();
+      for (int x = t; x < stop - done; x += kScanThreads) {
+        int lo = 0, hi = (int)a.nslots;       // the slot with off[lo] <= rank < off[lo + 1]
+        while (hi - lo > 1) {
+          const int m = (lo + hi) >> 1;
+          if (off[m] <= done + x) lo = m;
+          else hi = m;
+        }
+        const int id = list[x], k = done + x - off[lo];
+        int *row = a.tab + (int64_t)lo * a.maxpages;
+        if (cow[lo] && k == 0) {
+          int *e = row + clamp_i(a.len[lo], 0, cap) / a.page;
+          const int y = atomicAdd(&ncopy, 1);
+          copies[1 + 2 * y] = *e;
+          copies[2 + 2 * y] = id;
+          *e = id;
+        } else {
+          row[clamp_i(a.held[lo], 0, a.maxpages) + k - cow[lo]] = id;
+        }
+        a.ref[id] = 1;
+      }
+      __syncthreads();
+      done = stop;
     }
   }
   __syncthreads();
+  // (only now: a page that this call gives up is not handed out by it)
+  for (int x = t; x < ncopy; x += kScanThreads) atomicSub(&a.ref[copies[1 + 2 * x]], 1);
+#pragma unroll
+  for (int u = 0; u < kSlotsPerThread; ++u) {
+    const int s = t * kSlotsPerThread + u;
+    if (s < a.nslots && need[u] > 0 && off[s] + need[u] <= nfree)
+      a.held[s] = clamp_i(a.held[s], 0, a.maxpages) + need[u] - cow[s];
+  }
   if (t == 0) copies[0] = ncopy;
 }
 
@@ -366,8 +418,12 @@ hipError_t launch_pages_set_len(const PagesArgs &a, const int *new_len, hipStrea
 }
 
 hipError_t launch_pages_fork(const PagesArgs &a, const int *source, hipStream_t st) {
+  // columns of a block: at most 4 entries a thread where there are columns
+  // enough, and 64 KB of LDS (64 slots of 34 pages: one block of 64 columns
+  // 16.0 us, nine of 4 3.8)
   int cols = 64;
-  while (cols > 4 && a.nslots * cols * 4 > 65536) cols >>= 1;
+  while (cols > 4 && a.nslots * cols > 1024) cols >>= 1;
+  while (cols > 4 && (a.maxpages + cols - 1) / cols < 64) cols >>= 1;
   hipLaunchKernelGGL(pages_fork_kernel, dim3((unsigned)((a.maxpages + cols - 1) / cols)),
                      dim3(256), (size_t)(a.nslots * cols * 4), st, a, source, cols);
   return hipGetLastError();
