@@ -16,7 +16,12 @@
 // f32, have f32-level error.  bf16 q fits one binary16 after the scaling, and
 // p is rounded to one (2^-12 of itself, a sixteenth of the bf16 output's own
 // rounding): half the matrix work.
-// Bound: MFMA (4 hd flops per (row, head, key seen), twice issued for f32).
+// Bound: MFMA (4 hd flops per (row, head, key seen), twice issued for f32) with
+// the softmax's VALU work and the LDS traffic beside it; of 16001 rows in bf16
+// (2.1 ms, 1000 TFLOP/s) the staging of the tiles costs 0.5 ms and the LDS reads of
+// the operands 0.4.  Blocks of 4 waves, two to a CU, raise their priority in the
+// matrix phases, so one block's softmax falls beside the other's products (8
+// ragged f32 prompts 361 -> 349 us).
 //
 // Lane layout of the 32x32x16 MFMA (lane l, h = l / 32): A element i is
 // A[l % 32][8h + i], B element i is B[8h + i][l % 32], accumulator element v is
@@ -32,10 +37,18 @@ namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 constexpr int kBK = 64;                // keys per staged tile
-constexpr int kCols = 128;             // columns per block
 constexpr float kPScale = 16384.0f;    // 2^14 on p in binary16
+// Rows per sequence from which heads of 128 take 8 waves a block, which halves the
+// loads and LDS writes a column costs (one sequence of 8192 rows, 32 / 8 heads:
+// f32 1014 -> 968 us, bf16 634 -> 572; of 2048 rows 96 -> 104 and 64 -> 67, for
+// the tiles are twice as tall and fewer; 8 sequences of 700 rows, bf16, 64 ->
+// 73).  Heads of 64 gain nothing (579 -> 595).
+constexpr int kWideRows = 4096;
+// Sequences up to which the row tiles are served longest first.
+constexpr int kSorted = 16;
 
-__host__ __device__ inline int rows_per_block(int grp) { return kCols / grp; }
+// Rows of a block of nw waves, 32 columns each.
+__host__ __device__ inline int rows_per_block(int grp, int nw) { return 32 * nw / grp; }
 
 template <bool BF16> struct QType { typedef float T; };
 template <> struct QType<true> { typedef __bf16 T; };
@@ -104,41 +117,85 @@ __device__ __forceinline__ void row_f32(const T *__restrict__ q, const __half *_
   for (int e = 0; e < HD / 64; ++e) o[e] /= l;
 }
 
+// The row tile of block b of nb: tile `tile` of the sequence with the rows r0 ..
+// r1-1 (none: tile < 0 or past the rows).  Up to 16 sequences: all tiles in
+// descending order of their place in their sequence, which is the order of
+// their key runs, so the longest start first whatever the sequences' order: tile
+// k (and with it a sequence) of block b is the last k for which more than b
+// tiles have a place from k on, searched by the lanes side by side (8 sequences
+// of 700 rows, 32 / 8 heads of 64, 56.4 -> 51.5 us; 3000 rows between 600 and 40,
+// of 128, 164 -> 160).  More sequences: the last ones' last tiles first, since the
+// search grows with them and such tiles are short (61 sequences of 100 rows 33.6
+// us, sorted 41.5).
+struct PackedTile {
+  int r0, r1;
+  int64_t tile;
+};
+__device__ __forceinline__ PackedTile packed_tile(const int *__restrict__ cu, int nseq, int64_t rows,
+                                                  int PB, int nb, int b) {
+  const int lane = threadIdx.x & 63;
+  if (nseq <= kSorted) {
+    const int x = min(lane, nseq - 1);
+    const int c0 = clamp_i(cu[x], 0, rows), c1 = clamp_i(cu[x + 1], 0, rows);
+    const int tiles = lane < nseq && c1 > c0 ? (c1 - c0 + PB - 1) / PB : 0;
+    int k0 = 0, step = nb, from = 0;             // k lies in [k0, k0 + step)
+    do {
+      step = (step + 63) / 64;
+      const int k = k0 + lane * step;
+      int c = 0;                                 // tiles with a place from k on
+      for (int i = 0; i < nseq; ++i) c += max(__builtin_amdgcn_readlane(tiles, i) - k, 0);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(c > b);
+      if (m == 0) return {0, 0, -1};
+      const int z = 63 - __builtin_clzll(m);
+      k0 += z * step;
+      from = __builtin_amdgcn_readlane(c, z);
+    } while (step > 1);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(tiles > k0);
+    const int r = b - (from - (int)__builtin_popcountll(m));   // of the sequences that have a tile k0
+    const int mine = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    const uint64_t at = __builtin_amdgcn_ballot_w64((m >> lane & 1) && mine == r);
+    const int i = at ? __builtin_ctzll(at) : 0;
+    return {__builtin_amdgcn_readlane(c0, i), __builtin_amdgcn_readlane(c1, i), at ? k0 : -1};
+  }
+  b = nb - 1 - b;
+  int i0 = 0, n = nseq;                          // the last i with seq_first_block(cu[i], i) <= b
+  while (n > 1) {
+    const int step = (n + 63) / 64, x = i0 + lane * step;
+    const bool le = lane * step < n &&
+                    seq_first_block(clamp_i(cu[x < nseq ? x : nseq - 1], 0, rows), x, PB, 1) <= b;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(le);
+    const int k = m ? 63 - __builtin_clzll(m) : 0;
+    n = min(n - k * step, step);
+    i0 += k * step;
+  }
+  const int r0 = clamp_i(cu[i0], 0, rows);
+  return {r0, clamp_i(cu[i0 + 1], 0, rows), b - seq_first_block(r0, i0, PB, 1)};
+}
+
 // Grid seq_blocks(rows, nseq, rows_per_block, 1) x nkv, the KV heads of a tile
-// side by side (8 of them: one per XCD, whose L2 then holds that head); the blocks of a
-// sequence's last rows come first, since their key runs are the longest.
-template <int HD, bool BF16>
-__global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
+// side by side (8 of them: one per XCD, whose L2 then holds that head).
+template <int HD, bool BF16, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedAttnArgs a) {
   typedef typename QType<BF16>::T T;
   constexpr int KS = HD / 16;                    // 16-dim steps of a score tile
   constexpr int DT = HD / 32;                    // 32-dim tiles of the output
   constexpr int KST = HD + 8;                    // K row stride in LDS (halves)
   constexpr int VST = kBK + 8;                   // V^T row stride in LDS (halves)
-  constexpr int KCH = kBK * (HD / 8) / 256;      // 16-byte K chunks per thread
-  constexpr int VCH = (kBK / 2) * (HD / 8) / 256; // V key pairs x 8 dims per thread
+  constexpr int NTH = 64 * NW;                   // threads
+  constexpr int KCH = (kBK * (HD / 8) + NTH - 1) / NTH;        // 16-byte K chunks per thread
+  constexpr int VALL = (kBK / 2) * (HD / 8);     // V key pairs x 8 dims
+  constexpr int VCH = (VALL + NTH - 1) / NTH;
   constexpr int NT = BF16 ? 1 : 2;               // binary16 terms of q and p
-  __shared__ __attribute__((aligned(16))) _Float16 ks[kBK * KST];
-  __shared__ __attribute__((aligned(16))) _Float16 vt[HD * VST];
+  constexpr int NB = NW == 8 ? 2 : 1;            // staged tiles
+  __shared__ __attribute__((aligned(16))) _Float16 ks_[NB][kBK * KST];
+  __shared__ __attribute__((aligned(16))) _Float16 vt_[NB][HD * VST];
   const int g = blockIdx.x % a.nkv, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = lane & 31, hf = lane >> 5;
-  const int grp = a.nheads / a.nkv, PB = rows_per_block(grp), nseq = (int)a.nseq;
-  const int64_t b = (int64_t)(gridDim.x - 1 - blockIdx.x) / a.nkv;
-  // the sequence of block b: the last i with seq_first_block(cu[i], i) <= b
-  int i0 = 0;
-  {
-    int n = nseq;
-    while (n > 1) {
-      const int step = (n + 63) / 64, x = i0 + lane * step;
-      const bool le = lane * step < n &&
-                      seq_first_block(clamp_i(a.cu[x < nseq ? x : nseq - 1], 0, a.rows), x, PB, 1) <= b;
-      const uint64_t m = __builtin_amdgcn_ballot_w64(le);
-      const int k = m ? 63 - __builtin_clzll(m) : 0;
-      n = min(n - k * step, step);
-      i0 += k * step;
-    }
-  }
-  const int r0 = clamp_i(a.cu[i0], 0, a.rows), r1 = clamp_i(a.cu[i0 + 1], 0, a.rows);
-  const int64_t tile = b - seq_first_block(r0, i0, PB, 1);
+  const int grp = a.nheads / a.nkv, PB = rows_per_block(grp, NW), nseq = (int)a.nseq;
+  const PackedTile pt = packed_tile(a.cu, nseq, a.rows, PB, (int)(gridDim.x / a.nkv), (int)(blockIdx.x / a.nkv));
+  const int r0 = pt.r0, r1 = pt.r1;
+  const int64_t tile = pt.tile;
   if (tile < 0 || tile * PB >= r1 - r0) return;  // (the whole block)
   const int n = r1 - r0, row0 = (int)tile * PB;  // rows and keys count within the sequence
   const int nkeys = min(row0 + PB, n);
@@ -194,26 +251,28 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
     const uint32_t kvd = (uint32_t)kvdim;
 #pragma unroll
     for (int u = 0; u < KCH; ++u) {
-      const uint32_t c = threadIdx.x + 256 * u, key = c / (HD / 8), dg = c % (HD / 8);
+      const uint32_t c = threadIdx.x + NTH * u, key = c / (HD / 8), dg = c % (HD / 8);
       kreg[u] = bload16(rk, (key * kvd + dg * 8) * 2);
     }
 #pragma unroll
     for (int u = 0; u < VCH; ++u) {
-      const uint32_t c = threadIdx.x + 256 * u, kp = c % (kBK / 2), dg = c / (kBK / 2);
-      const uint32_t off = (2 * kp * kvd + dg * 8) * 2;
+      const uint32_t c = threadIdx.x + NTH * u, kp = c % (kBK / 2), dg = c / (kBK / 2);
+      const uint32_t off = c < VALL ? (2 * kp * kvd + dg * 8) * 2 : kOutOfRange;
       vreg[u][0] = bload16(rv, off);
       vreg[u][1] = bload16(rv, off + kvd * 2);
     }
   };
-  auto store_tile = [&]() {
+  auto store_tile = [&](int buf) {
+    _Float16 *ks = ks_[buf], *vt = vt_[buf];
 #pragma unroll
     for (int u = 0; u < KCH; ++u) {
-      const int c = threadIdx.x + 256 * u, key = c / (HD / 8), dg = c % (HD / 8);
+      const int c = threadIdx.x + NTH * u, key = c / (HD / 8), dg = c % (HD / 8);
       *reinterpret_cast<u32x4 *>(&ks[key * KST + dg * 8]) = kreg[u];
     }
 #pragma unroll
     for (int u = 0; u < VCH; ++u) {
-      const int c = threadIdx.x + 256 * u, kp = c % (kBK / 2), dg = c / (kBK / 2);
+      const int c = threadIdx.x + NTH * u, kp = c % (kBK / 2), dg = c / (kBK / 2);
+      if (VALL % NTH && c >= VALL) continue;
       const int key = 2 * kp, r = key & 15;
       const int at = (key & ~15) + 8 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
 #pragma unroll
@@ -235,13 +294,26 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
     for (int v = 0; v < 16; ++v) o[t][v] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   load_tile(0);
+  if (NB == 2) {
+    store_tile(0);
+    if (ntiles > 1) load_tile(1);
+  }
   for (int kt = 0; kt < ntiles; ++kt) {
+    const _Float16 *ks = ks_[kt % NB], *vt = vt_[kt % NB];
     __syncthreads();                             // every wave is done with the last tile
-    store_tile();
-    __syncthreads();
-    if (kt + 1 < ntiles) load_tile(kt + 1);
+    if (NB == 2) {                               // (and this one is staged)
+      if (kt + 1 < ntiles) {
+        store_tile((kt + 1) % NB);
+        if (kt + 2 < ntiles) load_tile(kt + 2);
+      }
+    } else {
+      store_tile(0);
+      __syncthreads();
+      if (kt + 1 < ntiles) load_tile(kt + 1);
+    }
     const int k0 = kt * kBK;
     if (!wlive || k0 >= wlast) continue;         // past every row of this wave
+    if (NB == 1) __builtin_amdgcn_s_setprio(1);
     f32x16 sc[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -255,6 +327,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
           sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[z][k], sc[t], 0, 0, 0);
       }
     }
+    if (NB == 1) __builtin_amdgcn_s_setprio(0);
     // m is the running maximum of the scores in the log2 domain rounded to an
     // integer: p = exp2(s cs - m) takes one FMA, and alpha is a power of two
     // that is 1 for most tiles
@@ -276,14 +349,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
     // (key 0 is visible to every column, so m is -inf only for scores of -inf:
     // then p is NaN, as the formula has it)
     const float mn = fmaxf(m, __builtin_rintf(tmax * cs));
-    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn), mp = BF16 ? mn - 14.0f : mn;
     m = mn;
     float ps = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v], cs, -mn));
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v], cs, -mp));
         sc[t][v] = p;
         ps += p;
       }
@@ -294,6 +367,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
     }
+    if (NB == 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -302,7 +376,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const float p = sc[t][8 * j + c];
-          pf[0][c] = (_Float16)(p * kPScale);
+          pf[0][c] = (_Float16)(BF16 ? p : p * kPScale);
           if constexpr (NT == 2) pf[1][c] = (_Float16)__builtin_fmaf(p, kPScale, -(float)pf[0][c]);
         }
 #pragma unroll
@@ -314,6 +388,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pf[z], o[d], 0, 0, 0);
         }
       }
+    if (NB == 1) __builtin_amdgcn_s_setprio(0);
   }
   l += __shfl_xor(l, 32);
   // The MFMAs multiply every key of a tile into every column: 0 times an
@@ -330,7 +405,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
   T *out = static_cast<T *>(a.out);
   const int64_t qdim = (int64_t)a.nheads * HD;
   if (live && !bad) {
-    const float il = 1.0f / (l * kPScale);
+    const float il = 1.0f / (BF16 ? l : l * kPScale);
     T *orow = out + (int64_t)(r0 + i) * qdim + (int64_t)head * HD + 4 * hf;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -354,21 +429,22 @@ __global__ __launch_bounds__(256, 2) void packed_attn_kernel(PackedAttnArgs a) {
   }
 }
 
-template <int HD>
+template <int HD, int NW>
 hipError_t launch_packed_t(const PackedAttnArgs &a, hipStream_t st) {
-  const int64_t nb = seq_blocks(a.rows, a.nseq, rows_per_block(a.nheads / a.nkv), 1);
+  const int64_t nb = seq_blocks(a.rows, a.nseq, rows_per_block(a.nheads / a.nkv, NW), 1);
   const dim3 grid((unsigned)(nb * a.nkv));
   if (a.bf16)
-    hipLaunchKernelGGL((packed_attn_kernel<HD, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((packed_attn_kernel<HD, true, NW>), grid, dim3(64 * NW), 0, st, a);
   else
-    hipLaunchKernelGGL((packed_attn_kernel<HD, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((packed_attn_kernel<HD, false, NW>), grid, dim3(64 * NW), 0, st, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_attention_packed(const PackedAttnArgs &a, hipStream_t st) {
-  return a.head_dim == 64 ? launch_packed_t<64>(a, st) : launch_packed_t<128>(a, st);
+  if (a.head_dim == 64) return launch_packed_t<64, 4>(a, st);
+  return a.rows >= kWideRows * a.nseq ? launch_packed_t<128, 8>(a, st) : launch_packed_t<128, 4>(a, st);
 }
 
 }  // namespace q8
