@@ -619,3 +619,154 @@ def test_graphs_share_scratch(ctx):
         assert np.array_equal(run_cache(ps[i % 2], arenas[i % 2].download((2, nh, hd), np.float32)), eager[i % 2])
     for g in graphs:
         g.destroy()
+
+
+# ---- a model over several sequences ------------------------------------------------------
+
+class OracleBatch:
+    """The float64 model (oracle/model_oracle.py) over the slots of a Q8Batch.  Its
+    attention reads the codes that the batch stored, after each has been checked
+    against the float64 key or value (a code beside its border may fall either
+    way by the linears' error, and would differ for good in a cache of its own)."""
+
+    def __init__(self, spec, tensors, inv, batch):
+        from oracle import model_oracle as mo
+        self.mo, self.m = mo, mo.OracleModel(spec, tensors, inv, 1)
+        self.sp, self.inv, self.b = spec, inv, batch
+        self.kv = {}                          # slot -> [layer] -> (k, v) as computed
+
+    def cache(self, L):
+        p = self.b.pages
+        raw = p.pool.download((p.npages, p.page_bytes), np.uint8, L * p.npages * p.page_bytes)
+        return bo.Cache.from_bytes(raw, p.page, p.nkv, p.head_dim)
+
+    def forward(self, slot, ids, packed):
+        """Logits of every row of one slot, after the batch's call."""
+        from oracle.q8_oracle import embed_gather_np
+        sp, mo, lin, t, p = self.sp, self.mo, self.m.lin, self.m.tensors, self.b.pages
+        s, hd = len(ids), sp.head_dim
+        kv = self.kv.setdefault(slot, [(np.zeros((0, sp.n_kv, hd)),) * 2 for _ in range(sp.layers)])
+        n = len(kv[0][0])
+        assert p.length[slot] == n + s
+        table = p.ix.download((p.slots, p.maxpages), np.int32, 4 * p.at["table"])[slot]
+        x = embed_gather_np(t["model.embed_tokens.weight"], np.asarray(ids), sp.hidden, sp.G,
+                            sp.scale).astype(np.float64)
+        for L in range(sp.layers):
+            w = f"model.layers.{L}."
+            xn = mo.rmsnorm(x, t[w + "input_layernorm.weight"], sp.eps)
+            q, k, v = (lin(w + f"self_attn.{y}_proj.weight", xn) for y in "qkv")
+            if sp.qk_norm:
+                q = mo.head_rmsnorm(q, t[w + "self_attn.q_norm.weight"], sp.n_heads, hd, sp.eps)
+                k = mo.head_rmsnorm(k, t[w + "self_attn.k_norm.weight"], sp.n_kv, hd, sp.eps)
+            q, k, v = (y.reshape(s, -1, hd) for y in (q, k, v))
+            q, k = (bo.rotate(y, np.arange(n, n + s), self.inv) for y in (q, k))
+            kv[L] = tuple(np.concatenate(y) for y in zip(kv[L], (k, v)))
+            c = self.cache(L)
+            stored = c.values(table, n + s)
+            for which, (have, want) in enumerate(zip(stored, kv[L])):
+                # half a step of the page's scale for the code, half for each time
+                # the scale grew since (3 at most here), one for the border
+                step = np.stack([c.s[table[i // p.page], which] for i in range(n + s)])[..., None]
+                assert (np.abs(have - want) <= 3 * step + 1e-3 * np.abs(want).max()).all(), (L, which)
+            if packed:
+                ao = bo.attention_packed(q, k.astype(np.float16), v.astype(np.float16), [0, s])
+            else:
+                ao = bo.attend(q, *stored, n)
+            h = x + lin(w + "self_attn.o_proj.weight", ao.reshape(s, -1))
+            z = mo.rmsnorm(h, t[w + "post_attention_layernorm.weight"], sp.eps)
+            g, u = lin(w + "mlp.gate_proj.weight", z), lin(w + "mlp.up_proj.weight", z)
+            x = h + lin(w + "mlp.down_proj.weight", mo.swiglu(g, u))
+        xn = mo.rmsnorm(x, t["model.norm.weight"], sp.eps)
+        return lin("model.embed_tokens.weight" if sp.tied else "lm_head.weight", xn)
+
+    def fork(self, dst, src):
+        self.kv[dst] = list(self.kv[src])
+
+    def truncate(self, slot, n):
+        self.kv[slot] = [(k[:n], v[:n]) for k, v in self.kv[slot]]
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_model_batch(ctx, kind):
+    """Prompts of three slots in one pass, token steps of all, a fork, drafts
+    with their return, a late prompt beside running slots, release, compaction,
+    against the float64 model.
+
+    The bar: from 32 rows on a linear is within 2e-4 of its largest output
+    (q8_linear), 4 * 2 + 1 of them follow each other, 1.8e-3; and a score s of q
+    and k 2e-4 off each is 4e-4 |s| off, |s| up to 8 here, which a probability
+    carries as a factor, 3.2e-3 in each of two layers: together 8.2e-3.  Fewer rows:
+    linears within 1e-5, a twentieth of it.  A row at a wrong position, page, head
+    or slot is off by its whole size."""
+    import sys
+    sys.path.insert(0, __file__.rsplit("/", 1)[0])
+    from test_model_oracle import qwen_tiny, tiny_model
+    from lama32_mojo_amd import batch, model as gm
+    say("model batch", kind)
+    spec, t, inv = tiny_model() if kind == "llama" else qwen_tiny()
+    cfg = gm.Config(spec.hidden, spec.layers, spec.n_heads, spec.n_kv, spec.head_dim, spec.inter,
+                    spec.vocab, spec.eps, 500000.0 if kind == "llama" else 1000000.0, 32.0, 1.0, 4.0,
+                    8192.0, tied=spec.tied, qk_norm=spec.qk_norm,
+                    rope="llama3" if kind == "llama" else "plain")
+    m = gm.Q8Llama(ctx, cfg, 16, weights=t)
+    b = batch.Q8Batch(m, slots=4, npages=24, maxlen=160, page=16, max_rows=128)
+    o = OracleBatch(spec, t, inv, b)
+    rng = np.random.default_rng(1)
+
+    def run(tokens, every=False):
+        packed = all(b.pages.length[s] == 0 for s in tokens)
+        rows = sum(len(x) for x in tokens.values())
+        got = b.forward(tokens, every=every, logits=True)
+        for s, ids in tokens.items():
+            ref = o.forward(s, ids, packed)
+            err = max_rel_err(got[s], ref if every else ref[-1])
+            say("slot", s, "rows", len(ids), "of", rows, "err %.1e" % err)
+            assert err <= (8.2e-3 if rows >= 32 else 4.1e-4), (s, len(ids))
+    draw = lambda n: rng.integers(0, spec.vocab, n).tolist()
+    run({0: draw(37), 1: draw(5), 3: draw(20)})              # packed prompts, 62 rows
+    for _ in range(3):
+        run({s: draw(1) for s in (0, 1, 3)})
+    b.fork({2: 0})
+    o.fork(2, 0)
+    run({s: draw(1) for s in range(4)})
+    run({0: draw(4), 2: draw(3), 3: draw(1)}, every=True)    # drafts; slot 0 keeps 2 of 4
+    b.truncate({0: b.pages.length[0] - 2})
+    o.truncate(0, b.pages.length[0])
+    run({0: draw(2), 1: draw(30)})                           # a chunk beside a step
+    b.truncate({1: 0})
+    o.truncate(1, 0)
+    live = b.compact()
+    assert live == sum(-(-b.pages.length[s] // 16) for s in (0, 2, 3)) - 2    # two shared pages
+    run({1: draw(40)})
+    run({s: draw(1) for s in range(4)})
+    # the ids are the argmax of the logits
+    ids = b.forward({0: [3], 2: [5]})
+    assert set(ids) == {0, 2} and all(0 <= x < spec.vocab for x in ids.values())
+    with pytest.raises(RuntimeError, match="pages full"):
+        b.forward({0: draw(120)})
+    assert b.pages.length[0] == b.pages.ix.download((1,), np.int32, 4 * b.pages.at["len"])[0]
+    with pytest.raises(ValueError):
+        b.forward({0: draw(129)})
+    with pytest.raises(ValueError):
+        b.forward({0: []})
+    b.close()
+    m.close()
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_packed_long(ctx, act):
+    """A prompt long enough for the 8-wave blocks, beside 17 and more sequences."""
+    say("packed long", act)
+    rng = np.random.default_rng(40)
+    for lens in ([4500], [1] * 20):
+        q, k, v = packed_inputs(rng, lens, 2, 1, 128)
+        q = bf16_to_f32(bf16_bits(q)) if act == "bf16" else q
+        pick = np.unique(np.r_[0:3, 60:70, 2040:2050, 4490:4500]) if len(lens) == 1 else np.arange(20)
+        y = run_packed(ctx, q, k, v, offsets(lens), act)
+        for r in pick:
+            a = 0 if len(lens) == 1 else r
+            ref = bo.attend(q[r:r + 1].astype(np.float64), k[a:r + 1].astype(np.float64),
+                            v[a:r + 1].astype(np.float64), r - a)[0]
+            bar = 1e-5 * np.abs(ref).max() if act == "f32" else \
+                2.0 ** -8 * np.abs(ref) + 2.0 ** -11 * np.abs(v.astype(np.float64)).max() + 1e-5
+            assert (np.abs(y[r] - ref) <= bar).all(), r
