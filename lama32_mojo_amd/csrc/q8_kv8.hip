@@ -341,8 +341,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
 // registers without a barrier: page ids are read two units ahead, codes one,
 // across the ends of row tiles, so the loads never wait for a sum to be
 // written.  A run that ends inside a row tile leaves a record for
-// kv8_merge_kernel.  Tables of up to 1024 tokens take a block of 8 waves per
-// row tile instead (WHOLE), which meet in LDS, and no merge.
+// kv8_merge_kernel.  A few short tables take a block of 8 waves per row tile
+// instead (WHOLE), which meet in LDS, and no merge.
 //
 // Scores: S^T = K Q^T on v_mfma_i32_16x16x64_i8 with the codes as they are and
 // q as four signed base-256 digits of 2^30 q / 2^e (2^e the power of two above
@@ -450,7 +450,13 @@ __device__ __forceinline__ int kv8_seq_of(const int *pre, int nseq, int u) {
   return lo;
 }
 
-constexpr int kKv8WholeUnits = 16;        // tables of up to 1024 tokens: no splits
+// Tables of up to this many units, and no more blocks of 8 waves than about one
+// per CU, take a block per row tile: the merge launch costs 4 us, a second
+// round of blocks more (heads of 128 in groups of 4, us whole / split: 1 sequence
+// of 500 tokens 11.4 / 13.3, of 900 15.4 / 13.5; 32 of 500 12.9 / 16.2; 64 of
+// 500 23.6 / 18.1).
+constexpr int kKv8WholeUnits = 12;
+constexpr int kKv8WholeBlocks = 384;
 constexpr int kKv8Waves = 4;              // waves of a block (WHOLE: 8)
 constexpr int kKv8PlanSeq = 1024;         // sequences of a launch (16 KB of LDS for the plan)
 
@@ -876,7 +882,7 @@ hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
   const size_t plan = (size_t)(4 * c.nseq + 1) * 4;
   const int64_t tiles = c.rows * grp / NC + c.nseq;
   const int64_t key_units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit;
-  if (key_units <= kKv8WholeUnits) {
+  if (key_units <= kKv8WholeUnits && tiles * c.nkv <= kKv8WholeBlocks) {
     const size_t lds = (size_t)(8 / MT / 2) * NC * (HD + 4) * 4 + plan;
     hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, true, false>), dim3((unsigned)tiles, (unsigned)c.nkv),
                        dim3(512), lds, st, a);
