@@ -423,7 +423,7 @@ int q8_token_begin(q8_ctx *ctx, q8_buf *ids, uint64_t oid_i32, int32_t id, q8_bu
  * dense; K and V are binary16 rows [rows, nkv*head_dim] at okc and ovc of kv, as
  * q8_rope_kv and q8_kv8_append write them.  f32 q keeps f32 accuracy (<= 1e-5),
  * bf16 q rounds the probabilities to binary16.  head_dim 64 or 128, nheads / nkv
- * up to 128, rows up to 2^24; q, out, K and V rows start 16-byte aligned
+ * up to 128, rows up to 2^24 (row tiles times KV heads below 2^24); q, out, K and V rows start 16-byte aligned
  * (Q8_ERR_UNSUPPORTED otherwise).  Values that a row does not see, infinities
  * and NaN included, do not reach it. */
 int q8_attention_packed(q8_ctx *ctx, q8_buf *q, uint64_t oq, int act_dtype, int64_t ldq, q8_buf *kv,
@@ -462,8 +462,8 @@ int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint
  * its cached tokens 0 .. len[i] + j (those of this call's rows included, so
  * q8_kv8_append comes first), one row a sequence or several (drafted tokens, a
  * prompt's next chunk).  Within 1e-5 of float64 over the stored values.  A row
- * that sees a missing page is NaN.  The split records live in the context's
- * scratch (q8_set_stream). */
+ * that sees a missing page is NaN.  Up to 512 KV heads and 2^22 rows.  The split
+ * records live in the context's scratch (q8_set_stream). */
 int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
                      q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
                      uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
@@ -480,11 +480,12 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
  * `pages`: any paged cache in multiples of 16 bytes, the 8-bit one among them. */
 
 /* Room for want[s] tokens in each slot s (at most maxpages*page): the pages it
- * lacks are taken from the free ones; and a slot that is to grow (want > len) and
- * whose last page is partly filled and shared gets a page of its own in its
- * place, with the contents copied in every layer.  (Slots that share a page and
- * grow in the same call each get a copy.)  Where the free pages do not reach,
- * the slots from the first that does not fit on get nothing: held says so. */
+ * lacks are taken from the free ones; and a slot that is to grow (want > len)
+ * gets a page of its own in the place of each shared one that its tokens len ..
+ * want-1 go to, the partly filled one with its contents copied in every layer.
+ * (Slots that share a page and grow in the same call each get one.)  Where the
+ * free pages do not reach, the slots from the first that does not fit on get
+ * nothing: held and table stay.  Up to about 5.5 million pages. */
 int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
                      uint64_t oheld_i32, uint64_t oref_i32, uint64_t owant_i32, int64_t nslots,
                      int64_t maxpages, int64_t npages, int page, q8_buf *pages, uint64_t opages,

@@ -210,24 +210,26 @@ class Q8Batch:
         p.ix.upload(cu, 4 * p.at["cu"])
         self.ids.upload(np.concatenate([np.asarray(tokens[s], np.int32) for s in slots]))
         mark = self.a.mark()
-        self.a.align(4)
-        ox = self.a.alloc(rows * H)
-        m, cfg = self.m, self.m.cfg
-        q8hip.embed_gather(self.ctx, m.w.buf, m.w.o("model.embed_tokens.weight"), self.ids, 0, self.a.buf,
-                           ox, rows, H, cfg.vocab, m.G, m.scale)
-        for L in range(cfg.layers):
-            at = self.a.mark()
-            self._layer(L, ox, rows, packed)
-            self.a.reset(at)
-        p.set_len([n + c for n, c in zip(old, counts)])
-        olg = self._head(ox, out_rows)
-        if logits:
-            flat = self.a.read(olg, len(out_rows) * cfg.vocab).reshape(-1, cfg.vocab)
-        else:
-            for i in range(len(out_rows)):
-                q8hip.argmax(self.ctx, self.a.buf, olg + i * cfg.vocab, cfg.vocab, self.ids, i)
-            flat = self.ids.download((len(out_rows),), np.int32).tolist()
-        self.a.reset(mark)
+        m, cfg, V = self.m, self.m.cfg, self.m.cfg.vocab
+        try:
+            self.a.align(4)
+            ox = self.a.alloc(rows * H)
+            q8hip.embed_gather(self.ctx, m.w.buf, m.w.o("model.embed_tokens.weight"), self.ids, 0,
+                               self.a.buf, ox, rows, H, V, m.G, m.scale)
+            for L in range(cfg.layers):
+                at = self.a.mark()
+                self._layer(L, ox, rows, packed)
+                self.a.reset(at)
+            p.set_len([n + c for n, c in zip(old, counts)])
+            olg = self._head(ox, out_rows)
+            if logits:
+                flat = self.a.read(olg, len(out_rows) * V).reshape(-1, V)
+            else:
+                for i in range(len(out_rows)):
+                    q8hip.argmax(self.ctx, self.a.buf, olg + i * V, V, self.ids, i)
+                flat = self.ids.download((len(out_rows),), np.int32).tolist()
+        finally:
+            self.a.reset(mark)
         if every:
             return {s: flat[cu[s]:cu[s + 1]] for s in slots}
         return dict(zip(slots, flat))

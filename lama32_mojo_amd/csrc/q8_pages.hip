@@ -75,24 +75,46 @@ __device__ __forceinline__ int count_free(uint32_t bits, int rows) {
 }
 constexpr int kList = 4096;
 
-// One block.  Slots in ascending order ask for the pages they lack (and one
-// more where their partly filled last page is shared); an exclusive sum of
-// the needs gives each slot a run of ranks, and the free page of rank r, found
-// by a second sum over the pages, goes to the slot whose run holds r.  When
-// the free pages do not reach, the slots behind the last run that fits get
-// nothing.  copies: their number, then (from, to) pairs.  Bound: the chain
-// length, page id, reference count, sums; the free pages are looked up beside it.
+// The pages of a slot that growing from len to want tokens writes to and that
+// other slots name too: places len / page .. to pages_of(want) of what it holds.
+// visit(place, id) for each, in order; returns their number.
+template <class F>
+__device__ __forceinline__ int shared_pages(const PagesArgs &a, int s, int len, int want, int held,
+                                            F visit) {
+  int n = 0;
+  if (want <= len) return 0;
+  const int to = min(held, pages_of(want, a.page));
+  for (int j = len / a.page; j < to; ++j) {
+    const int id = page_or_none(a.tab[(int64_t)s * a.maxpages + j], (int)a.npages);
+    if (id >= 0 && a.ref[id] > 1) {
+      if (visit(j, id, n)) return n + 1;
+      ++n;
+    }
+  }
+  return n;
+}
+
+// One block.  Slots in ascending order ask for the pages they lack and for one
+// in the place of each shared page they are to write to (the first of which may
+// be partly filled: its contents are copied); an exclusive sum of the needs
+// gives each slot a run of ranks, and the free page of rank r, found by a second
+// sum over the pages, goes to the slot whose run holds r.  When the free pages
+// do not reach, the slots behind the last run that fits get nothing.  ws: the
+// number of copies and (from, to) pairs, at most one per slot; behind them the
+// pages replaced as (table entry, old, new).  Bound: the chain length, page id, reference count, sums; the
+// free pages are looked up beside it.
 __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a,
                                                                      const int *__restrict__ want,
-                                                                     int *__restrict__ copies) {
+                                                                     int *__restrict__ ws) {
   __shared__ int off[kPagesMaxSlots + 1];
-  __shared__ uint8_t cow[kPagesMaxSlots];
+  __shared__ int cow[kPagesMaxSlots];          // shared pages replaced
   __shared__ int list[kList];
   __shared__ int wsum[kScanThreads / 64];
-  __shared__ int ncopy, granted_end;
-  const int t = threadIdx.x, npages = (int)a.npages, wave = t >> 6;
+  __shared__ int ncopy, nswap, granted_end;
+  int *copies = ws, *swaps = ws + 1 + 2 * a.nslots;
+  const int t = threadIdx.x, wave = t >> 6;
   const int64_t cap = a.maxpages * a.page;
-  if (t == 0) ncopy = granted_end = 0;
+  if (t == 0) ncopy = nswap = granted_end = 0;
   // pages in goes of 16 waves x rows x 64; the first go's counts are in flight
   // beside the slots' reads
   const int rows = (int)(a.npages < 32 * kScanThreads ? (a.npages + kScanThreads - 1) / kScanThreads : 32);
@@ -107,11 +129,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a
     if (s >= a.nslots) continue;
     const int len = clamp_i(a.len[s], 0, cap), w = clamp_i(want[s], 0, cap);
     const int held = clamp_i(a.held[s], 0, a.maxpages);
-    bool c = false;
-    if (w > len && len % a.page != 0 && len / a.page < held) {
-      const int id = page_or_none(a.tab[(int64_t)s * a.maxpages + len / a.page], npages);
-      c = id >= 0 && a.ref[id] > 1;
-    }
+    const int c = shared_pages(a, s, len, w, held, [](int, int, int) { return false; });
     cow[s] = c;
     const int more = pages_of(w, a.page) - held;
     need[u] = (more > 0 ? more : 0) + c;
@@ -183,14 +201,27 @@ __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a
         }
         const int id = list[x], k = done + x - off[lo];
         int *row = a.tab + (int64_t)lo * a.maxpages;
-        if (cow[lo] && k == 0) {
-          int *e = row + clamp_i(a.len[lo], 0, cap) / a.page;
-          const int y = atomicAdd(&ncopy, 1);
-          copies[1 + 2 * y] = *e;
-          copies[2 + 2 * y] = id;
-          *e = id;
+        const int held = clamp_i(a.held[lo], 0, a.maxpages);
+        if (k < cow[lo]) {                    // the k-th shared page
+          const int len = clamp_i(a.len[lo], 0, cap);
+          int place = 0, was = 0;
+          shared_pages(a, lo, len, clamp_i(want[lo], 0, cap), held, [&](int j, int old, int n) {
+            place = j;
+            was = old;
+            return n == k;
+          });
+          if (place == len / a.page && len % a.page != 0) {
+            const int y = atomicAdd(&ncopy, 1);
+            copies[1 + 2 * y] = was;
+            copies[2 + 2 * y] = id;
+          }
+          // entered below, once no thread counts a row's shared pages any more
+          int *e = swaps + 3 * (int64_t)atomicAdd(&nswap, 1);
+          e[0] = (int)((int64_t)lo * a.maxpages) + place;
+          e[1] = was;
+          e[2] = id;
         } else {
-          row[clamp_i(a.held[lo], 0, a.maxpages) + k - cow[lo]] = id;
+          row[held + k - cow[lo]] = id;
         }
         a.ref[id] = 1;
       }
@@ -200,7 +231,10 @@ __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(PagesArgs a
   }
   __syncthreads();
   // (only now: a page that this call gives up is not handed out by it)
-  for (int x = t; x < ncopy; x += kScanThreads) atomicSub(&a.ref[copies[1 + 2 * x]], 1);
+  for (int x = t; x < nswap; x += kScanThreads) {
+    a.tab[swaps[3 * (int64_t)x]] = swaps[3 * (int64_t)x + 2];
+    atomicSub(&a.ref[swaps[3 * (int64_t)x + 1]], 1);
+  }
 #pragma unroll
   for (int u = 0; u < kSlotsPerThread; ++u) {
     const int s = t * kSlotsPerThread + u;

@@ -1746,6 +1746,10 @@ int q8_attention_packed(q8_ctx *ctx, q8_buf *q, uint64_t oq, int act_dtype, int6
   if (at(q, oq * es) % 16 != 0 || at(out, oy * es) % 16 != 0 || at(kv, okc_f16 * 2) % 16 != 0 ||
       at(kv, ovc_f16 * 2) % 16 != 0 || (uint64_t)ldq * es % 16 != 0)
     return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: q, out, K and V rows must start 16-byte aligned", what);
+  // one block per row tile (of at least 128 / group rows) and KV head, 2^32 threads
+  if (q8::seq_blocks(rows, nseq, 128 / (nheads / nkv), 1) * nkv >= ((int64_t)1 << 24))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: %lld rows of %lld sequences, %d heads, are too many for one "
+                "call", what, (long long)rows, (long long)nseq, nheads);
   if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
   if (rows == 0 || nseq == 0) return ok(ctx);
   if (int rc = set_device(ctx)) return rc;
@@ -1877,6 +1881,10 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
     return fail(ctx, Q8_ERR_SHAPE, "%s: q row stride %lld (0, or at least %lld)", what, (long long)ldq,
                 (long long)qdim);
   if (ldq == 0) ldq = qdim;
+  if (nkv > 512)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nkv=%d (at most 512)", what, nkv);
+  if (rows > (1 << 22))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: rows=%lld (at most 2^22)", what, (long long)rows);
   // units of 64 keys are counted in int32
   const double units = ((double)rows * (nheads / nkv) / 16 + (double)nseq) *
                        ((double)maxpages * page / q8::kKv8Unit + 1);
@@ -1911,8 +1919,8 @@ namespace {
 int check_pages(q8_ctx *ctx, q8_buf *ix, int64_t nslots, int64_t maxpages, int64_t npages, int page,
                 const char *what) {
   if (!ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
-  if (nslots < 0 || maxpages <= 0 || npages <= 0 || npages > INT32_MAX || page <= 0 ||
-      maxpages > ((int64_t)1 << 30) / page)
+  if (nslots < 0 || maxpages <= 0 || maxpages > (1 << 24) || npages <= 0 || npages > INT32_MAX ||
+      page <= 0 || maxpages > ((int64_t)1 << 30) / page)
     return fail(ctx, Q8_ERR_SHAPE, "%s: nslots=%lld, maxpages=%lld, npages=%lld, page=%d", what,
                 (long long)nslots, (long long)maxpages, (long long)npages, page);
   if (nslots > q8::kPagesMaxSlots || nslots * maxpages > INT32_MAX)
@@ -1921,10 +1929,17 @@ int check_pages(q8_ctx *ctx, q8_buf *ix, int64_t nslots, int64_t maxpages, int64
   return Q8_OK;
 }
 
+// q8_pages_reserve and _compact keep up to three ints a page, and two a slot, in
+// the context's scratch.
+constexpr int64_t kMaxPoolPages = (kAct16Bytes / 4 - 2 * q8::kPagesMaxSlots - 2) / 3;
+
 int check_pool(q8_ctx *ctx, q8_buf *pages, uint64_t opages, uint64_t page_bytes, int64_t layers,
                uint64_t layer_stride, int64_t npages, q8_buf *ix, const Ints *v, int nv,
                const char *what, q8::PagePool *out) {
   if (!pages) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (npages > kMaxPoolPages)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: npages=%lld (at most %lld)", what, (long long)npages,
+                (long long)kMaxPoolPages);
   if (page_bytes == 0 || page_bytes > ((uint64_t)1 << 40) || layers <= 0 || layers > 65535)
     return fail(ctx, Q8_ERR_SHAPE, "%s: page_bytes=%llu, layers=%lld", what,
                 (unsigned long long)page_bytes, (long long)layers);
@@ -1975,7 +1990,7 @@ int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i
                            iptr(ix, oref_i32), nslots, maxpages, npages, page};
   const hipError_t e = with_scratch(ctx, [&] {
     return q8::launch_pages_reserve(a, iptr(ix, owant_i32), pool,
-                                    reinterpret_cast<int *>(ctx->gemm_ws), ctx->stream);
+                                    static_cast<int *>(ctx->act16), ctx->stream);
   });
   if (e != hipSuccess) return hip_fail(ctx, e, "q8_pages_reserve launch");
   return ok(ctx);
@@ -2044,9 +2059,6 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
   if (int rc = check_pool(ctx, pages, opages, page_bytes, layers, layer_stride, npages, ix, v, 4, what,
                           &pool))
     return rc;
-  if (3 * npages + 2 > kAct16Bytes / 4)
-    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: npages=%lld (at most %lld)", what, (long long)npages,
-                (long long)((kAct16Bytes / 4 - 2) / 3));
   if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
   if (int rc = set_device(ctx)) return rc;
   const q8::PagesArgs a = {iptr(ix, otab_i32), nullptr, iptr(ix, oheld_i32), iptr(ix, oref_i32),

@@ -182,12 +182,12 @@ class Pages:
         plan = []
         for s, row in enumerate(self.rows):
             w = min(max(want[s], 0), self.maxpages * self.P)
-            j = self.len[s] // self.P
-            cow = w > self.len[s] and self.len[s] % self.P != 0 and j < len(row) and ref[row[j]] > 1
-            plan.append((cow, max(0, -(-w // self.P) - len(row))))
+            to = min(len(row), -(-w // self.P)) if w > self.len[s] else 0
+            own = [j for j in range(self.len[s] // self.P, to) if ref[row[j]] > 1]
+            plan.append((own, max(0, -(-w // self.P) - len(row))))
         at = 0
-        for s, (cow, more) in enumerate(plan):
-            n = cow + more
+        for s, (own, more) in enumerate(plan):
+            n = len(own) + more
             if n == 0:
                 continue
             short = short or at + n > len(free)
@@ -195,11 +195,11 @@ class Pages:
                 continue
             got = free[at:at + n]
             at += n
-            if cow:
-                j = self.len[s] // self.P
-                copies.append((self.rows[s][j], got[0]))
-                self.rows[s][j] = got[0]
-            self.rows[s] += got[cow:]
+            for j, p in zip(own, got):
+                if j == self.len[s] // self.P and self.len[s] % self.P:
+                    copies.append((self.rows[s][j], p))
+                self.rows[s][j] = p
+            self.rows[s] += got[len(own):]
         return copies
 
     def set_len(self, new):

@@ -54,6 +54,11 @@ def test_attention_packed(hctx):
     assert call(hd=96, rows=4) == call(hd=32) == Q8_ERR_UNSUPPORTED
     assert call(nh=129, nkv=1, rows=1) == Q8_ERR_UNSUPPORTED
     assert call(rows=1 << 25) == Q8_ERR_SHAPE
+    # more row tiles than a launch has blocks
+    q, out, kv = (hctx.alloc(1 << 41) for _ in range(3))
+    T = 1 << 24
+    assert call(nh=8, nkv=1, rows=T, ovc=T * 64, o=out) == Q8_ERR_NODEVICE
+    assert call(nh=128, nkv=1, rows=T, ovc=T * 64, o=out) == Q8_ERR_SHAPE
 
 
 def cache(hctx, npages=5, page=16, nkv=2, hd=64, nseq=3, maxpages=4, rows=9):
@@ -104,6 +109,8 @@ def test_kv8_attention(hctx):
     assert call(npages=6) == call(olen=19) == Q8_ERR_RANGE
     assert call(page=8) == call(nseq=4097) == call(hd=32) == Q8_ERR_UNSUPPORTED
     assert call(npages=0) == call(nh=5) == call(ldq=8) == Q8_ERR_SHAPE
+    assert call(rows=(1 << 22) + 1) == Q8_ERR_SHAPE
+    assert call(nkv=513, nh=513, p=hctx.alloc(1 << 30)) == Q8_ERR_UNSUPPORTED
     # more units of work than an int32 counts
     big = hctx.alloc(8 << 32)
     assert call(ix=big, maxpages=1 << 26, nseq=50, otab=100, olen=52, ocu=0) == Q8_ERR_NODEVICE
@@ -144,4 +151,6 @@ def test_pages(hctx):
         assert f(pb=24, ls=npg * 32) == f(layers=1, op=8) == Q8_ERR_UNSUPPORTED, f
         assert f(pool=ix, pb=16, layers=1, npg=2) == Q8_ERR_ARG, f   # the pool over the state
         assert f(layers=1, ls=0) == Q8_ERR_NODEVICE, f
-    assert reserve(page=0) == set_len(page=-1) == Q8_ERR_SHAPE
+    assert reserve(page=0) == set_len(page=-1) == set_len(mp=1 << 25) == Q8_ERR_SHAPE
+    ix = hctx.alloc(1 << 30)
+    assert reserve(npg=6 << 20, ox=7 << 20) == compact(npg=6 << 20, ox=7 << 20) == Q8_ERR_UNSUPPORTED

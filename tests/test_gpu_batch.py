@@ -373,6 +373,31 @@ def test_cache_attention_long(ctx):
     assert max_rel_err(run_cache(p, q), ref) <= 1e-5
 
 
+@pytest.mark.parametrize("nh,hd,P", [(2, 128, 128), (5, 64, 128), (20, 128, 32), (40, 64, 64)])
+def test_cache_attention_splits(ctx, nh, hd, P):
+    """Split contexts at every page size and column tile (16, 32, 64 columns), odd
+    first units among them, some units of a wave's run in the next sequence."""
+    say("cache splits", nh, hd, P)
+    rng = np.random.default_rng(nh + P)
+    lens, old = [1, 2, 1, 1], [1500, 700, 64 * 7, 3333]
+    p = Paged(ctx, rng, lens, old, P, 1, hd)
+    q = rng.standard_normal((p.rows, nh, hd)).astype(np.float32)
+    assert max_rel_err(run_cache(p, q), p.c.attention(q, p.cu, p.old, p.table)) <= 1e-5
+
+
+def test_cache_attention_many_sequences(ctx):
+    """More sequences than one launch plans for."""
+    say("cache many")
+    rng = np.random.default_rng(50)
+    n = 1100
+    p = Paged(ctx, rng, [1 + i % 2 if i % 7 else 0 for i in range(n)], [i % 40 for i in range(n)], 16, 1, 64)
+    q = rng.standard_normal((p.rows, 2, 64)).astype(np.float32)
+    ref = p.c.attention(q, p.cu, p.old, p.table)
+    assert max_rel_err(run_cache(p, q), ref) <= 1e-5
+    q, k, v = (rng.standard_normal((p.rows, h, 64)).astype(np.float32) for h in (2, 1, 1))
+    check_append(p, q, k, v)
+
+
 def test_cache_attention_hidden(ctx):
     """A NaN scale reaches the rows that see a token of its page and head, no
     others; missing pages make NaN; rows past the table see what it holds; rows
@@ -479,6 +504,14 @@ def test_pages(ctx, nslots, maxpages, npages, P, pb):
             if rng.random() < 0.2:
                 want[rng.integers(0, nslots)] = cap + 100
             s.reserve(want.tolist())
+            if rng.random() < 0.3:               # fork slots that hold pages ahead, grow both
+                src = np.where(rng.random(nslots) < 0.3, rng.integers(0, nslots, nslots), -1)
+                s.fork(src.tolist())
+                s.check()
+                ln = np.array(s.o.len)
+                want = ln + rng.integers(0, 3 * P, nslots)
+                s.reserve(want.tolist())
+                s.check()
             grown = np.minimum(np.maximum(ln, want), [len(r) * P for r in s.o.rows])
             s.set_len(np.where(rng.random(nslots) < 0.8, grown, -1).tolist())
         elif kind == 1:
@@ -585,6 +618,104 @@ def test_prompts_then_tokens(ctx):
     s.compact()
     s.check()
     g.destroy()
+
+
+def test_captured_step(ctx):
+    """A whole step captured -- pages taken and copied, append, attention, lengths
+    advanced -- and replayed at lengths that grow over page ends, a fork among
+    them, with eager work between: every replay as the oracle has it."""
+    say("captured step")
+    rng = np.random.default_rng(60)
+    nh, nkv, hd, P, ns, maxpages, npages = 4, 2, 64, 16, 3, 6, 30
+    pb, ld = bo.page_bytes(P, nkv, hd), (nh + 2 * nkv) * hd
+    o, c = bo.Pages(ns, maxpages, npages, P), bo.Cache(npages, P, nkv, hd)
+    pool, _ = dev(ctx, c.to_bytes())
+    st = o.arrays()
+    names = ["cu", "table", "len", "held", "ref", "want", "source"]
+    ix, off = dev(ctx, np.arange(ns + 1, dtype=np.int32), *st.values(), np.zeros(ns, np.int32),
+                  np.full(ns, -1, np.int32))
+    at = {n: x // 4 for n, x in zip(names, off)}
+    oinv, oy = ns * ld, ns * ld + 32
+    a = ctx.alloc(4 * (oy + ns * nh * hd))
+    a.upload(inv_freq(hd), 4 * oinv)
+    state = (ix, at["table"], at["len"], at["held"], at["ref"])
+
+    def issue():
+        where = (pool, 0, npages, P, ix, at["cu"], at["len"], at["table"], ns, ns, maxpages)
+        q8hip.pages_reserve(ctx, *state, at["want"], ns, maxpages, npages, P, pool, 0, pb)
+        q8hip.kv8_append(ctx, a, 0, nh * hd, (nh + nkv) * hd, oinv, 0, *where, nh, nkv, hd, ld=ld)
+        q8hip.kv8_attention(ctx, a, 0, oy, *where, nh, nkv, hd, ldq=ld)
+        q8hip.pages_set_len(ctx, *state, at["want"], ns, maxpages, npages, P)
+
+    ctx.graph_begin()
+    issue()
+    g = ctx.graph_end()
+    for t in range(40):
+        if t == 21:                                  # slots 0 and 2 continue slot 1
+            ix.upload(np.array([1, -1, 1], np.int32), 4 * at["source"])
+            q8hip.pages_fork(ctx, *state, at["source"], ns, maxpages, npages)
+            o.fork([1, -1, 1])
+        want = [n + 1 for n in o.len]
+        ix.upload(np.array(want, np.int32), 4 * at["want"])
+        x = rng.standard_normal((ns, ld)).astype(np.float32) * (1 + t % 3)
+        a.upload(x)
+        if t % 5 == 4:
+            issue()                                  # eager between replays
+        else:
+            g.launch()
+        for f, to in o.reserve(want):
+            c.k[to], c.v[to], c.s[to] = c.k[f], c.v[f], c.s[f]
+        table, length = o.arrays()["table"], np.array(o.len)
+        q, k, v = (y.reshape(ns, -1, hd) for y in np.split(x, [nh * hd, (nh + nkv) * hd], 1))
+        qr, _ = c.append(q, k, v, inv_freq(hd), [0, 1, 2, 3], length, table)
+        y = a.download((ns, nh, hd), np.float32, 4 * oy)
+        assert max_rel_err(y, c.attention(qr, [0, 1, 2, 3], length, table)) <= 1e-5, t
+        o.set_len(want)
+        for name, ref in o.arrays().items():
+            assert np.array_equal(ix.download(ref.shape, np.int32, 4 * at[name]), ref), (t, name)
+        assert np.array_equal(pool.download((npages, pb), np.uint8), c.to_bytes()), t
+    g.destroy()
+
+
+def test_far_pages(ctx):
+    """Pages beyond 4 GiB: append, attention and compaction at 64-bit offsets."""
+    say("far pages")
+    rng = np.random.default_rng(61)
+    P, nkv, hd, nh = 128, 8, 128, 8
+    pb = bo.page_bytes(P, nkv, hd)
+    npages = (5 << 30) // pb
+    p = Paged(ctx, rng, [3, 1], [200, 500], P, nkv, hd)
+    near = p.c.npages
+    far = npages - near + np.arange(near)
+    p.pool.free()
+    p.pool = ctx.alloc(npages * pb)
+    p.pool.upload(p.c.to_bytes(), int(far[0]) * pb)
+    local = p.table.copy()
+    p.table = np.where(local >= 0, local + far[0], -1).astype(np.int32)
+    p.upload()
+    where = (p.pool, 0, npages, P, p.ix, *p.at, 2, 4, p.maxpages)
+    ld = (nh + 2 * nkv) * hd
+    x = rng.standard_normal((4, ld)).astype(np.float32)
+    a, (_, oinv, oy) = dev(ctx, x, inv_freq(hd), np.zeros((4, nh * hd), np.float32))
+    q8hip.kv8_append(ctx, a, 0, nh * hd, (nh + nkv) * hd, oinv // 4, 0, *where, nh, nkv, hd, ld=ld)
+    q8hip.kv8_attention(ctx, a, 0, oy // 4, *where, nh, nkv, hd, ldq=ld)
+    q, k, v = (y.reshape(4, -1, hd) for y in np.split(x, [nh * hd, (nh + nkv) * hd], 1))
+    qr, _ = p.c.append(q, k, v, inv_freq(hd), p.cu, p.old, local)
+    ref = p.c.attention(qr, p.cu, p.old, local)
+    assert max_rel_err(a.download((4, nh, hd), np.float32, oy), ref) <= 1e-5
+    assert np.array_equal(p.pool.download((near, pb), np.uint8, int(far[0]) * pb), p.c.to_bytes())
+    held = (local >= 0).sum(1).astype(np.int32)
+    ref_counts = np.zeros(npages, np.int32)
+    ref_counts[p.table[p.table >= 0]] = 1
+    ix, off = dev(ctx, p.table, held, ref_counts, np.zeros(1, np.int32))
+    q8hip.pages_compact(ctx, ix, *(x // 4 for x in off), 2, p.maxpages, npages, p.pool, 0, pb)
+    n = int(held.sum())
+    moved = ix.download(p.table.shape, np.int32)
+    order = np.argsort(np.argsort(local[local >= 0]))
+    assert np.array_equal(moved[moved >= 0], order)
+    assert ix.download((1,), np.int32, off[3])[0] == n
+    assert np.array_equal(p.pool.download((n, pb), np.uint8), p.c.to_bytes()[np.sort(local[local >= 0])])
+    p.pool.free()
 
 
 def test_graphs_share_scratch(ctx):

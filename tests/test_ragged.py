@@ -57,3 +57,13 @@ def test_oracle_pages():
     assert p.compact() == (3, [(4, 1)]) and p.rows[1] == [0, 1]
     # too few pages: the slots from the first that does not fit on get nothing
     assert p.reserve([64, 64, 64]) == [] and [len(r) for r in p.rows] == [4, 2, 1]
+    # pages reserved ahead that a fork shares: replaced when their slots write to them
+    p = bo.Pages(2, 6, 12, 16)
+    p.reserve([60, 0])
+    p.set_len([0, -1])
+    p.reserve([60, 0])
+    p.len[0] = 20
+    p.fork([-1, 0])
+    assert p.rows == [[0, 1, 2, 3]] * 2
+    assert p.reserve([33, 20]) == [(1, 4)] and p.rows == [[0, 4, 5, 3], [0, 1, 2, 3]]
+    assert p.reserve([33, 70]) == [] and p.rows[1] == [0, 1, 2, 6, 7]
