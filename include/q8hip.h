@@ -485,7 +485,9 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
  * want-1 go to, the partly filled one with its contents copied in every layer.
  * (Slots that share a page and grow in the same call each get one.)  Where the
  * free pages do not reach, the slots from the first that does not fit on get
- * nothing: held and table stay.  Up to about 5.5 million pages. */
+ * nothing: held and table stay.  (Such a slot has held*page < want, or still a
+ * page with ref > 1 among those it would write to: do not append to it.)  Up to
+ * about 5.5 million pages. */
 int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
                      uint64_t oheld_i32, uint64_t oref_i32, uint64_t owant_i32, int64_t nslots,
                      int64_t maxpages, int64_t npages, int page, q8_buf *pages, uint64_t opages,

@@ -45,6 +45,7 @@ class Pages:
         self.ix = Buffer.alloc(ctx, 4 * top)
         self.ix.upload(start)
         self.length = [0] * slots              # the lengths, as the host knows them
+        self.forked = set()                    # slots that may share pages
 
     def _state(self):
         return (self.ix, *(self.at[n] for n in ("table", "len", "held", "ref")))
@@ -61,23 +62,41 @@ class Pages:
         took) when the free pages do not reach."""
         shape = (self.slots, self.maxpages, self.npages)
         q8hip.pages_reserve(self.ctx, *self._state(), self._arg(want), *shape, self.page, *self._pool())
-        held = self.ix.download((self.slots,), np.int32, 4 * self.at["held"])
-        if any(w > int(h) * self.page for w, h in zip(want, held)):
+        if self._short(want):
             self.set_len(self.length)
             raise RuntimeError("KV pages full")
+
+    def _short(self, want) -> bool:
+        """Whether a slot lacks pages for want tokens, or is to write to a page that
+        another slot names: one that found no free page for its copy keeps it, with
+        its held pages as they were."""
+        held = self.ix.download((self.slots,), np.int32, 4 * self.at["held"])
+        if any(w > int(h) * self.page for w, h in zip(want, held)):
+            return True
+        grow = [s for s in self.forked if want[s] > self.length[s]]
+        if not grow:
+            return False
+        table = self.ix.download((self.slots, self.maxpages), np.int32, 4 * self.at["table"])
+        ref = self.ix.download((self.npages,), np.int32, 4 * self.at["ref"])
+        return any((ref[table[s, self.length[s] // self.page:-(-want[s] // self.page)]] > 1).any()
+                   for s in grow)
 
     def set_len(self, new: Sequence[int]) -> None:
         """The slots' lengths; pages behind them are released."""
         q8hip.pages_set_len(self.ctx, *self._state(), self._arg(new), self.slots, self.maxpages,
                             self.npages, self.page)
         self.length = [int(n) if n >= 0 else old for n, old in zip(new, self.length)]
+        self.forked -= {s for s in self.forked if self.length[s] == 0}
 
     def fork(self, source: Sequence[int]) -> None:
         """Slot s continues slot source[s] (-1: unchanged)."""
         q8hip.pages_fork(self.ctx, *self._state(), self._arg(source), self.slots, self.maxpages,
                          self.npages)
-        self.length = [self.length[f] if 0 <= f < self.slots else n
-                       for f, n in zip(source, self.length)]
+        pairs = [(s, f) for s, f in enumerate(source) if 0 <= f < self.slots and f != s]
+        old = list(self.length)
+        for s, f in pairs:
+            self.length[s] = old[f]
+            self.forked |= {s, f}
 
     def compact(self) -> int:
         """The pages in use moved to the lowest ids; how many there are."""
@@ -236,12 +255,15 @@ class Q8Batch:
 
     def truncate(self, lengths: Mapping[int, int]) -> None:
         """Shortens slots (rejected drafts); 0 ends a sequence."""
-        if any(not 0 <= n <= self.pages.length[s] for s, n in lengths.items()):
-            raise ValueError("truncate: a length past the slot's tokens")
+        if any(not 0 <= s < self.slots or not 0 <= n <= self.pages.length[s]
+               for s, n in lengths.items()):
+            raise ValueError("truncate: no such slot, or a length past its tokens")
         self.pages.set_len([lengths.get(s, -1) for s in range(self.slots)])
 
     def fork(self, source: Mapping[int, int]) -> None:
         """Slot s continues slot source[s], sharing its pages."""
+        if any(not 0 <= x < self.slots for pair in source.items() for x in pair):
+            raise ValueError("fork: no such slot")
         self.pages.fork([source.get(s, -1) for s in range(self.slots)])
 
     def compact(self) -> int:

@@ -45,9 +45,9 @@ __device__ __forceinline__ SeqAt find_seq(const int *__restrict__ cu, const int 
 }
 
 // cos and sin of pos * inv to f64 accuracy: the angle as an exact f64
-// product (24 x 31 bits), less the nearest multiple of pi / 2 (pi / 2 in three
-// parts, the first two of 33 bits, so that their products with the count are
-// exact), then the Taylor series on [-pi/4, pi/4], whose first left-out terms
+// product (24 x 29 bits), less the nearest multiple of pi / 2 (pi / 2 in three
+// parts, the first two of 33 bits, so that their products with counts below 2^20
+// are exact), then the Taylor series on [-pi/4, pi/4], whose first left-out terms
 // are below 2^-54.  f32 angles of far positions are off by up to 2^-8 rad at
 // 10^5 tokens; here the rotated key is rounded once, so equal inputs give
 // equal codes on every path.

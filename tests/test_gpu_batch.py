@@ -901,3 +901,36 @@ def test_packed_long(ctx, act):
             bar = 1e-5 * np.abs(ref).max() if act == "f32" else \
                 2.0 ** -8 * np.abs(ref) + 2.0 ** -11 * np.abs(v.astype(np.float64)).max() + 1e-5
             assert (np.abs(y[r] - ref) <= bar).all(), r
+
+
+def test_pages_full_beside_shared(ctx):
+    """A fork that would grow inside a shared page needs one of its own: with none
+    free the reservation is refused, though the slot's held pages would do.  With
+    one of the two slots released the other grows in place."""
+    from lama32_mojo_amd.batch import Pages
+    say("pages full beside shared")
+    p = Pages(ctx, 2, 1, 1, 16, 1, 1, 64)
+    p.reserve([10, 0])
+    p.set_len([10, 0])
+    p.fork([-1, 0])
+    for want in ([11, 10], [10, 11], [11, 11]):
+        with pytest.raises(RuntimeError, match="pages full"):
+            p.reserve(want)
+        assert p.length == [10, 10]
+        assert p.ix.download((2,), np.int32, 4 * p.at["table"]).tolist() == [0, 0]
+    p.reserve([10, 10])                                      # nothing grows
+    p.set_len([0, -1])
+    p.reserve([0, 16])
+    p.set_len([-1, 16])
+    assert p.ix.download((2,), np.int32, 4 * p.at["table"]).tolist() == [-1, 0]
+    # room for one copy: slot 0 gets it, slot 1 then has the old page alone
+    p2 = Pages(ctx, 2, 2, 2, 16, 1, 1, 64)
+    p2.reserve([10, 0])
+    p2.set_len([10, 0])
+    p2.fork([-1, 0])
+    p2.reserve([11, 10])
+    p2.set_len([11, 10])
+    p2.reserve([11, 11])
+    assert sorted(p2.ix.download((2, 2), np.int32, 4 * p2.at["table"])[:, 0].tolist()) == [0, 1]
+    p2.close()
+    p.close()
