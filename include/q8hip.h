@@ -442,7 +442,8 @@ uint64_t q8_kv8_page_bytes(int page, int nkv, int head_dim);
  * as binary16 rows [rows, nkv*head_dim] at okc and ovc of kv (the prompt rows
  * that q8_attention_packed reads).
  * Angles are formed to 64 bits and a rotated key is rounded to f32 once.  A
- * page's scale of a head is s = max(s_old, max |x| / 127) over the new rows x
+ * page's scale of a head is s = max(s_old, max |x| * (1/127)) over the new rows x,
+ * an f32 product with the f32 nearest to 1/127
  * (s_old counts where the page holds older tokens of the sequence), codes are
  * the quotients x / s rounded to the nearest, ties to even; where the scale
  * grows, the older tokens' codes become code * s_old / s rounded likewise.  A

@@ -85,8 +85,9 @@ __device__ __forceinline__ void sincos_pos(int pos, float inv, double &sn, doubl
 // One block of 256 threads per (page that a sequence's new rows touch, KV
 // head), grid (seq_blocks(rows, nseq, page, 2), nkv).  It rotates the head's
 // keys and its query heads, takes the largest |k| and |v| of the new rows,
-// settles the page's two scales (s1 = max(s0, amax / 127); s0 counts where old
-// tokens lie in the page), re-rounds the old tokens' codes where the scale
+// settles the page's two scales (s1 = max(s0, amax * f32(1 / 127)), a product by
+// definition: the quotient is another number in 1 of 20 cases, and codes beside a
+// border with it; s0 counts where old tokens lie in the page), re-rounds the old tokens' codes where the scale
 // grew, and writes the new codes.  A thread holds (token, dims 4j .. 4j+3 and
 // their partners half a head on) items, so the rotation needs no exchange and
 // the values stay in registers between the two passes.
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const uint32_t mx = max(max(red[x][0], red[x][1]), max(red[x][2], red[x][3]));
-    const float am = __builtin_bit_cast(float, mx) / 127.0f;
+    const float am = __builtin_bit_cast(float, mx) * (1.0f / 127.0f);
     s0[x] = e > 0 ? (x ? old1 : old0) : 0.0f;
     s1[x] = am > s0[x] || am != am ? am : s0[x];          // (a NaN s0 stays)
     fine[x] = __builtin_isfinite(s1[x]);

@@ -7,7 +7,7 @@ Formulas (rows of sequence i: cu[i] .. cu[i+1]-1, at positions len[i] + j):
              over the t that row r sees
   rotation   (a, b) -> (a cos - b sin, b cos + a sin), angle position * inv_freq,
              keys rounded to f32 once
-  codes      s = max(s_old, f32(max |x| / 127)); rint(x / s), half to even, in
+  codes      s = max(s_old, f32(max |x| * f32(1 / 127))); rint(x / s), half to even, in
              [-127, 127]; older codes rint(c s_old / s) where s grew
 """
 
@@ -127,7 +127,7 @@ class Cache:
         """New codes of one head in one page; returns the scale."""
         s0 = np.float32(s_old) if old else np.float32(0)
         top = np.abs(x).max()
-        s1 = np.float32(top) / np.float32(127)
+        s1 = np.float32(top) * (np.float32(1) / np.float32(127))
         if np.isfinite(s1) and not s1 > s0:
             s1 = s0
         if not (np.isfinite(s1) and np.isfinite(s0)):

@@ -903,6 +903,27 @@ def test_packed_long(ctx, act):
             assert (np.abs(y[r] - ref) <= bar).all(), r
 
 
+def test_append_scale_rounding(ctx):
+    """The scale is the f32 product of the largest value and f32(1 / 127), whose last
+    bit differs from the quotient's for the values taken here: scales and codes equal
+    the oracle's, codes beside a border of either among them."""
+    say("append scale rounding")
+    rng = np.random.default_rng(77)
+    one = np.float32(1) / np.float32(127)
+    top = rng.uniform(1, 8, 4000).astype(np.float32)
+    top = top[top * one != top / np.float32(127)][:32]
+    assert top.size == 32
+    p = Paged(ctx, rng, [16] * 32, [0] * 32, 16, 1, 64)
+    q, k, v = (rng.standard_normal((p.rows, 1, 64)).astype(np.float32) for _ in range(3))
+    for i, t in enumerate(top):
+        x = v[16 * i:16 * i + 16]
+        s = t * one
+        x[:] = ((rng.integers(-126, 126, x.shape) + 0.5) * float(s)).astype(np.float32)
+        x[np.abs(x) > t] = 0
+        x[0, 0, 0] = t
+    check_append(p, q, k, v)
+
+
 def test_pages_full_beside_shared(ctx):
     """A fork that would grow inside a shared page needs one of its own: with none
     free the reservation is refused, though the slot's held pages would do.  With
