@@ -71,7 +71,8 @@ Q8_HD int kv8_units_of(const Kv8Seq &s) {
   const int64_t u = (int64_t)s.row_tiles * s.key_units;
   return u < kKv8MaxUnits ? (int)u : kKv8MaxUnits;
 }
-Q8_HD int kv8_add(int a, int b) { return a + b < kKv8MaxUnits ? a + b : kKv8MaxUnits; }
+// (of counts from 0 to the limit; two at the limit would not fit an int32)
+Q8_HD int kv8_add(int a, int b) { return a < kKv8MaxUnits - b ? a + b : kKv8MaxUnits; }
 // Units per block of nblocks; at least `least` (a block's waves take a unit
 // each), so a small call uses fewer blocks.
 Q8_HD int kv8_units_per_block(int64_t units, int nblocks, int least) {
