@@ -462,7 +462,8 @@ int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint
  * (row stride ldq, 0: dense) over the 8-bit cache: row j of sequence i attends
  * its cached tokens 0 .. len[i] + j (those of this call's rows included, so
  * q8_kv8_append comes first), one row a sequence or several (drafted tokens, a
- * prompt's next chunk).  Within 1e-5 of float64 over the stored values.  A row
+ * prompt's next chunk).  Within 1e-5 of float64 over the stored values, every
+ * dimension of q carried as f32 carries it (f32 scores of size S add S 2^-22).  A row
  * that sees a missing page is NaN.  Up to 512 KV heads and 2^22 rows.  The split
  * records live in the context's scratch (q8_set_stream). */
 int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,

@@ -348,7 +348,14 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
 // Scores: S^T = K Q^T on v_mfma_i32_16x16x64_i8 with the codes as they are and
 // q as four signed base-256 digits of 2^30 q / 2^e (2^e the power of two above
 // the column's largest |q|): exact integer sums, joined in f32, so q is carried
-// to 2^-31 of the column's largest and nothing is lost in the sum.  Outputs:
+// to 2^-31 of the column's largest and nothing is lost in the sum.  That is an
+// error of the score: the dims' roundings add up to at most sqrt(HD) 2^(e-31) of
+// the largest |k|, and to 2^(e-31) / sqrt(3) of it in the mean square (6 times
+// that is 6.6e-6 where 2^e |k| reaches 2^12).  Beyond 2^12, where dims that are
+// many times the others meet codes near 0, a unit's scores are formed with q as
+// three bf16 terms, which carry every dim as f32 does (beside dims 2^14 to 2^126
+// times the others 3e-5 to 1 -> 6e-7 of float64; all units formed so: 64 sequences
+// 67 -> 85 us, 4 contexts of up to 131000 tokens 122 -> 152).  Outputs:
 // O^T += V^T P^T on v_mfma_f32_16x16x32_bf16, the codes as bf16 (exact) and
 // p vs as three bf16 terms whose sum is the f32 value, whatever the scales.
 // (Codes as bf16 in both products cost 192 more conversions of a unit's 700
@@ -395,6 +402,12 @@ __device__ __forceinline__ void digits4(const float (&x)[4], uint32_t (&o)[4]) {
   o[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
   o[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
   o[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// The scale of a unit's integer scores, 2^(e - 30) ks log2(e) / sqrt(HD), up to
+// which 2^e 127 ks <= 2^12.
+template <int HD> __device__ __forceinline__ float kv8_exact_up_to() {
+  return 1.44269504088896341f / sqrtf((float)HD) * (0x1p-18f / 127.0f);
 }
 
 // The plan of a call in LDS: the prefix sums of the sequences' units (WHOLE: row
@@ -601,6 +614,12 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     const int u = nx.u + (nx.t1 - nx.t0);
     if (u < uend) nx = place(u, nx.i);
   };
+  // q of this lane's column of a row tile (one that does not exist: the first
+  // row's), from dim 16 g4 on
+  auto q_at = [&](const Kv8Place &p, int row0, int n) {
+    const int lin = p.rt * NC + cc, j = lin / grp;
+    return a.q + (int64_t)(row0 + (j < n ? j : 0)) * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
+  };
   load_ids();
   load_k();
   load_v();
@@ -622,8 +641,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
       float x[HH][16];
 #pragma unroll
       for (int h = 0; h < HH; ++h) {
-        const float *q = a.q + (int64_t)(row0 + (j < n ? j : 0)) * a.ldq +
-                         (int64_t)(g * grp + lin % grp) * HD + 64 * h + 16 * g4;
+        const float *q = q_at(cu, row0, n) + 64 * h;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const f32x4 y = *reinterpret_cast<const f32x4_u *>(q + 4 * v);
@@ -664,24 +682,53 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int kt = WHOLE ? w : cu.t0; kt < cu.t1; kt += step) {
       f32x4 s[4];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        i32x4 d[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          d[k] = i32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int h = 0; h < HH; ++h)
-            d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[tt][h]),
-                                                         __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0,
-                                                         0, 0);
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v)       // (|d| < 2^21 each: the pairs fit)
-          s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
-                                    (float)((d[1][v] << 8) + d[0][v]));
-      }
       const float sc = qs * ks, vsc = vs;
+      if (__builtin_amdgcn_ballot_w64(fabsf(sc) > kv8_exact_up_to<HD>()) == 0) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          i32x4 d[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            d[k] = i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int h = 0; h < HH; ++h)
+              d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[tt][h]),
+                                                           __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0,
+                                                           0, 0);
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v)     // (|d| < 2^21 each: the pairs fit)
+            s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
+                                      (float)((d[1][v] << 8) + d[0][v]));
+        }
+      } else {
+        // step 2 h + x: dims 64 h + 16 g4 + 8 x .. of both operands; q at the integer
+        // scores' scale (2^30 / 2^e, exactly), so that no product overflows
+        const float up = qscale / qs;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const float *q = q_at(cu, row0, n);
+#pragma unroll
+        for (int z = 0; z < 2 * HH; ++z) {
+          float y[8];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const f32x4 a = *reinterpret_cast<const f32x4_u *>(q + 64 * (z >> 1) + 8 * (z & 1) + 4 * v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[4 * v + i] = a[i] * up;
+          }
+          u32x4 qf[3];
+          split3x8(y, qf);
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            const bf16x8_t kb = codes_to_bf16(kr[tt][z >> 1][2 * (z & 1)], kr[tt][z >> 1][2 * (z & 1) + 1]);
+#pragma unroll
+            for (int k = 2; k >= 0; --k)
+              s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, __builtin_bit_cast(bf16x8_t, qf[k]),
+                                                              s[tt], 0, 0, 0);
+          }
+        }
+      }
       load_k();
       const int key0 = kt * kKv8Unit + 16 * g4;
       const bool masked = kt * kKv8Unit + kKv8Unit > kmin;

@@ -35,3 +35,36 @@ def test_cache_nonsense_offsets(ctx):
         run_append(p, q, k, v)
         for b in (p.pool, p.ix):
             b.free()
+
+
+@pytest.mark.parametrize("large", [2.0 ** 14, 2.0 ** 20, 2.0 ** 23, 2.0 ** 34, 2.0 ** 60, 2.0 ** 126])
+@pytest.mark.parametrize("nh,nkv,hd,P,lens,old", [
+    (8, 2, 128, 64, [1, 1], [500, 90]),                # whole row tiles
+    (6, 2, 64, 16, [2, 1, 3], [40, 300, 0]),
+    (8, 2, 128, 64, [1, 2, 1], [1500, 700, 64 * 20]),  # runs of split contexts
+    (5, 1, 64, 128, [1, 1], [3000, 1000]),
+    (20, 1, 128, 32, [1, 1], [1500, 900]),             # 32 columns
+    (40, 1, 64, 128, [2, 2], [1100, 1500]),            # 64 columns
+])
+def test_cache_carries_q_beside_a_large_dim(ctx, nh, nkv, hd, P, lens, old, large):
+    """q counts as f32: beside dims many times the others, whose K codes are 0, the
+    scores of the others stay within 1e-5 (every second row; the others ordinary)."""
+    say("cache large q", nh, hd, P, lens, large)
+    rng = np.random.default_rng(nh + hd)
+    p = Paged(ctx, rng, lens, old, P, nkv, hd)
+    p.c.k[..., 5] = 0
+    p.c.k[..., hd - 3] = 0
+    p.pool.upload(p.c.to_bytes())
+    q = rng.standard_normal((p.rows, nh, hd)).astype(np.float32)
+    q[::2, :, 5] = large
+    q[::2, 1::2, hd - 3] = -large / 3
+    y, ref = run_cache(p, q), p.c.attention(q, p.cu, p.old, p.table)
+    for r in range(p.rows):
+        assert max_rel_err(y[r], ref[r]) <= 1e-5, r
+    # K that sees them: the scores' own size decides, here one key takes all
+    p.c.k[..., 5] = rng.integers(-127, 128, p.c.k.shape[:-1])
+    p.pool.upload(p.c.to_bytes())
+    y = run_cache(p, q)
+    assert np.isfinite(y).all()
+    for b in (p.pool, p.ix):
+        b.free()
