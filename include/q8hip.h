@@ -421,8 +421,9 @@ int q8_token_begin(q8_ctx *ctx, q8_buf *ids, uint64_t oid_i32, int32_t id, q8_bu
  * or bf16 (act_dtype Q8_SRC_F32 / Q8_SRC_BF16; offsets oq and oy in elements of
  * that type), row r of q at oq + r*ldq (ldq = 0: nheads*head_dim, dense), out
  * dense; K and V are binary16 rows [rows, nkv*head_dim] at okc and ovc of kv, as
- * q8_rope_kv and q8_kv8_append write them.  f32 q keeps f32 accuracy (<= 1e-5),
- * bf16 q rounds the probabilities to binary16.  head_dim 64 or 128, nheads / nkv
+ * q8_rope_kv and q8_kv8_append write them.  f32 q keeps f32 accuracy (<= 1e-5;
+ * f32 scores of size S add S 2^-22), bf16 q rounds the probabilities to binary16;
+ * both carry every dimension of q as it stands.  head_dim 64 or 128, nheads / nkv
  * up to 128, rows up to 2^24 (row tiles times KV heads below 2^24); q, out, K and V rows start 16-byte aligned
  * (Q8_ERR_UNSUPPORTED otherwise).  Values that a row does not see, infinities
  * and NaN included, do not reach it. */

@@ -15,7 +15,8 @@
 // largest; K and V are binary16 already, so products are exact and the sums,
 // f32, have f32-level error.  bf16 q fits one binary16 after the scaling, and
 // p is rounded to one (2^-12 of itself, a sixteenth of the bf16 output's own
-// rounding): half the matrix work.
+// rounding): half the matrix work.  Columns where those terms hold too little of
+// the small dims of q (kFarDim) are formed in f32.
 // Bound: MFMA (4 hd flops per (row, head, key seen), twice issued for f32) with
 // the softmax's VALU work and the LDS traffic beside it; of 16001 rows in bf16
 // (2.1 ms, 1000 TFLOP/s) the staging of the tiles costs 0.5 ms and the LDS reads of
@@ -47,6 +48,18 @@ constexpr int kWideRows = 4096;
 // Sequences up to which the row tiles are served longest first.
 constexpr int kSorted = 16;
 
+// Small dims of q: the terms' 2^-25 (at largest values in [2^14, 2^15)) is up to 2^-19
+// of a dim 20 binary exponents below its column's largest, and bf16 (8 bits) is
+// exact in them down to 31 below.  Dims that lie further below (one f32 column of
+// normal values in 4000) make an error of the score of at most sqrt(HD) 2^-40
+// max|q| max|k|, and of 6.6e-6, counting 6 times the mean square, where max|q|
+// max|k| (max|q| as its power of two) reaches 2^20: no binary16 k takes a
+// largest q below 32 there.  From 32 on a wave with such a column looks its keys
+// through, and columns past 2^20 are formed in f32: beside dims that are 2^23 to
+// 2^126 times the others, and 0 in K, 1e-5 to 1 -> 6e-7 of float64.  (If every
+// wave looked: 8088 ragged f32 rows 357 -> 452 us; none does for ordinary q.)
+template <bool BF16> constexpr int kFarDim = BF16 ? 31 : 20;
+
 // Rows of a block of nw waves, 32 columns each.
 __host__ __device__ inline int rows_per_block(int grp, int nw) { return 32 * nw / grp; }
 
@@ -74,6 +87,24 @@ __device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f3
 __device__ __forceinline__ void store4(__bf16 *p, f32x4 v) {
   *reinterpret_cast<u32x2 *>(p) =
       u32x2{bf16_rne(v.x) | bf16_rne(v.y) << 16, bf16_rne(v.z) | bf16_rne(v.w) << 16};
+}
+
+// The largest |k| of the keys 0 .. nk-1, by one wave.
+template <int HD>
+__device__ __forceinline__ float largest(const __half *__restrict__ kc, int64_t kvdim, int nk, int lane) {
+  constexpr int LPK = HD / 8, KPW = 64 / LPK;            // lanes of a key, keys of a load
+  uint32_t mx = 0;
+  for (int j0 = lane / LPK; j0 < nk; j0 += 8 * KPW) {
+    u32x4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      x[u] = *reinterpret_cast<const u32x4 *>(kc + (int64_t)min(j0 + u * KPW, nk - 1) * kvdim + lane % LPK * 8);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) mx = max(mx, max(x[u][v] & 0x7fffu, x[u][v] >> 16 & 0x7fffu));
+  }
+  return wave_max((float)__builtin_bit_cast(_Float16, (uint16_t)mx));
 }
 
 // One (row, head) over its keys 0 .. nk-1 by one wave in f32, reading no other
@@ -216,18 +247,24 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedAttnArgs 
   const bool wlive = w * 32 / grp < PB && row0 + w * 32 / grp < n;
 
   half8 qf[NT][KS];
-  float cs;
+  float cs, klim;                                // |k| up to which the terms of q do
   {
     const T *qr = static_cast<const T *>(a.q) + (int64_t)(r0 + i) * a.ldq + (int64_t)head * HD + 8 * hf;
     float qv[KS][8], mx = 0.0f;
+    uint32_t mn = ~0u;                           // (2 |q| as bits) - 1: zeros are largest
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       load8(qr + 16 * k, qv[k]);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) mx = fmaxf(mx, fabsf(qv[k][c]));
+      for (int c = 0; c < 8; ++c) {
+        mx = fmaxf(mx, fabsf(qv[k][c]));
+        mn = min(mn, (__builtin_bit_cast(uint32_t, qv[k][c]) << 1) - 1u);
+      }
     }
     mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mn = min(mn, (uint32_t)__shfl_xor((int)mn, 32));
     const int ex = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255u) - 127;
+    klim = (int)(mn >> 24) + kFarDim<BF16> < ex + 127 ? __builtin_ldexpf(1.0f, 20 - ex) : INFINITY;
     const int e = min(max(14 - ex, -126), 126);
     const float qsc = __builtin_ldexpf(1.0f, e);
     cs = __builtin_ldexpf(1.44269504088896341f / sqrtf((float)HD), -e);
@@ -401,7 +438,8 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_attn_kernel(PackedAttnArgs 
 #pragma unroll
     for (int v = 0; v < 16; ++v) chk = __builtin_fmaf(o[t][v], 0.0f, chk);
   chk += __shfl_xor(chk, 32);
-  const bool bad = chk != 0.0f;
+  bool bad = chk != 0.0f;
+  if (__builtin_amdgcn_ballot_w64(live && klim < 65536.0f)) bad |= largest<HD>(kc, kvdim, wlast, lane) > klim;
   T *out = static_cast<T *>(a.out);
   const int64_t qdim = (int64_t)a.nheads * HD;
   if (live && !bad) {

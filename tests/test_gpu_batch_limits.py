@@ -7,7 +7,8 @@ import pytest
 from lama32_mojo_amd import q8hip
 from oracle import batch_oracle as bo
 from oracle.q8_oracle import max_rel_err
-from test_gpu_batch import Paged, inv_freq, run_append, run_cache, say
+from test_gpu_batch import (Paged, bf16_bits, bf16_to_f32, offsets, packed_inputs, run_append,
+                            run_cache, run_packed, say)
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +69,36 @@ def test_cache_carries_q_beside_a_large_dim(ctx, nh, nkv, hd, P, lens, old, larg
     assert np.isfinite(y).all()
     for b in (p.pool, p.ix):
         b.free()
+
+
+def bf16_bar(ref, v):
+    """Half a bf16 step of the output, half a binary16 step of the largest |v| for the
+    probabilities, the f32 bar."""
+    return 2.0 ** -8 * np.abs(ref) + 2.0 ** -11 * np.abs(v.astype(np.float64)).max() + 1e-5
+
+
+@pytest.mark.parametrize("large", [2.0 ** 14, 2.0 ** 20, 2.0 ** 23, 2.0 ** 34, 2.0 ** 43, 2.0 ** 60, 2.0 ** 126])
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,hd,lens", [(8, 2, 64, [1, 130, 7]), (8, 2, 128, [1, 130, 7]), (2, 1, 128, [4200])])
+def test_packed_carries_q_beside_a_large_dim(ctx, nh, nkv, hd, lens, act, large):
+    """q counts as it stands: beside dims many times the others, which K does not
+    have, the scores of the others stay as exact (every second row; the others
+    ordinary)."""
+    say("packed large q", nh, hd, lens, act, large)
+    rng = np.random.default_rng(nh + hd)
+    q, k, v = packed_inputs(rng, lens, nh, nkv, hd)
+    k[..., 5] = 0
+    k[..., hd - 3] = 0
+    q[::2, :, 5] = large
+    q[::2, 1::2, hd - 3] = -large / 3
+    if act == "bf16":
+        q = bf16_to_f32(bf16_bits(q))
+    y = run_packed(ctx, q, k, v, offsets(lens), act)
+    cu = offsets(lens)
+    rows = range(len(q)) if len(q) < 500 else [0, 1, 2, 63, 64, 255, 256, 2047, 2048, 4198, 4199]
+    for r in rows:
+        a = cu[np.searchsorted(cu, r, "right") - 1]
+        ref = bo.attend(q[r:r + 1].astype(np.float64), k[a:r + 1].astype(np.float64),
+                        v[a:r + 1].astype(np.float64), r - a)[0]
+        bar = 1e-5 * np.abs(ref).max() if act == "f32" else bf16_bar(ref, v)
+        assert (np.abs(y[r] - ref) <= bar).all(), r
