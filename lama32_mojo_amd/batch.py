@@ -86,7 +86,7 @@ class Pages:
         q8hip.pages_set_len(self.ctx, *self._state(), self._arg(new), self.slots, self.maxpages,
                             self.npages, self.page)
         self.length = [int(n) if n >= 0 else old for n, old in zip(new, self.length)]
-        self.forked -= {s for s in self.forked if self.length[s] == 0}
+        self.forked -= {s for s, n in enumerate(new) if n == 0}    # (these hold no pages now)
 
     def fork(self, source: Sequence[int]) -> None:
         """Slot s continues slot source[s] (-1: unchanged)."""
