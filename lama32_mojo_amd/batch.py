@@ -42,9 +42,11 @@ class Pages:
             top += n
         start = np.zeros(top, np.int32)
         start[self.at["table"]:self.at["table"] + slots * maxpages] = -1
+        self.ints = top
         self.ix = Buffer.alloc(ctx, 4 * top)
         self.ix.upload(start)
         self.length = [0] * slots              # the lengths, as the host knows them
+        self.held = [0] * slots                # the pages held, likewise
         self.forked = set()                    # slots that may share pages
 
     def _state(self):
@@ -61,10 +63,22 @@ class Pages:
         """Pages for want[s] tokens in every slot; raises (and gives back what it
         took) when the free pages do not reach."""
         shape = (self.slots, self.maxpages, self.npages)
+        # a refused call's copies of shared pages cannot be told from the others, and
+        # pages held ahead not from what it took: then the state as it was goes back
+        keep = any(h > self._pages_of(n) for h, n in zip(self.held, self.length)) or \
+            any(want[s] > self.length[s] for s in self.forked)
+        before = self.ix.download((self.ints,), np.int32) if keep else None
         q8hip.pages_reserve(self.ctx, *self._state(), self._arg(want), *shape, self.page, *self._pool())
         if self._short(want):
-            self.set_len(self.length)
+            if keep:
+                self.ix.upload(before)
+            else:
+                self.set_len(self.length)
             raise RuntimeError("KV pages full")
+        self.held = [max(h, self._pages_of(w)) for h, w in zip(self.held, want)]
+
+    def _pages_of(self, n: int) -> int:
+        return -(-int(n) // self.page)
 
     def _short(self, want) -> bool:
         """Whether a slot lacks pages for want tokens, or is to write to a page that
@@ -86,6 +100,7 @@ class Pages:
         q8hip.pages_set_len(self.ctx, *self._state(), self._arg(new), self.slots, self.maxpages,
                             self.npages, self.page)
         self.length = [int(n) if n >= 0 else old for n, old in zip(new, self.length)]
+        self.held = [self._pages_of(n) if n >= 0 else h for n, h in zip(new, self.held)]
         self.forked -= {s for s, n in enumerate(new) if n == 0}    # (these hold no pages now)
 
     def fork(self, source: Sequence[int]) -> None:
@@ -93,9 +108,9 @@ class Pages:
         q8hip.pages_fork(self.ctx, *self._state(), self._arg(source), self.slots, self.maxpages,
                          self.npages)
         pairs = [(s, f) for s, f in enumerate(source) if 0 <= f < self.slots and f != s]
-        old = list(self.length)
+        old = list(zip(self.length, self.held))
         for s, f in pairs:
-            self.length[s] = old[f]
+            self.length[s], self.held[s] = old[f]
             self.forked |= {s, f}
 
     def compact(self) -> int:

@@ -102,3 +102,43 @@ def test_fork_of_reserved_pages(pages):
     with pytest.raises(RuntimeError, match="pages full"):
         p.reserve([10, 0, 19])
     assert p.length == [0, 0, 19]
+
+
+def test_refusal_leaves_the_state(pages):
+    """A refused reservation leaves what was there, pages held ahead and shared ones
+    among them: what an earlier reservation promised is still there."""
+    p = pages(3, 6, 5)
+    p.reserve([40, 0, 20])
+    p.set_len([-1, -1, 20])                                   # slot 0 holds 3 pages ahead
+    before = state(p)
+    for want in ([40, 32, 20], [70, 0, 64], [40, 0, 1000]):
+        with pytest.raises(RuntimeError, match="pages full"):
+            p.reserve(want)
+        assert state(p) == before and p.length == [0, 0, 20]
+    p.fork([-1, 0, -1])
+    before = state(p)
+    with pytest.raises(RuntimeError, match="pages full"):
+        p.reserve([40, 40, 20])                               # each sharer lacks three
+    assert state(p) == before
+    p.set_len([0, -1, -1])                                    # slot 1 has them alone
+    p.reserve([0, 48, 20])
+    assert state(p)[0][1][:3] == before[0][0][:3]
+    # nothing held ahead: the pages that slots got before the refused one are free again
+    q = pages(3, 4, 4)
+    q.reserve([16, 16, 0])
+    q.set_len([16, 16, 0])
+    before = state(q)
+    with pytest.raises(RuntimeError, match="pages full"):
+        q.reserve([32, 16, 64])
+    assert state(q) == before
+    # a copy of a shared page is given back too
+    q = pages(3, 3, 2)
+    q.reserve([10, 0, 0])
+    q.set_len([10, 0, 0])
+    q.fork([-1, 0, -1])
+    before = state(q)
+    with pytest.raises(RuntimeError, match="pages full"):
+        q.reserve([11, 10, 32])
+    assert state(q) == before
+    q.reserve([10, 10, 32])
+    assert state(q)[3] == [2, 1, 1]
