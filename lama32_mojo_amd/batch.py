@@ -96,7 +96,11 @@ class Pages:
                    for s in grow)
 
     def set_len(self, new: Sequence[int]) -> None:
-        """The slots' lengths; pages behind them are released."""
+        """The slots' lengths (-1: unchanged; at most what the slot's pages hold); pages
+        behind them are released."""
+        for s, (n, h) in enumerate(zip(new, self.held)):
+            if n > h * self.page:
+                raise ValueError(f"set_len: slot {s} holds pages for {h * self.page} tokens, not {n}")
         q8hip.pages_set_len(self.ctx, *self._state(), self._arg(new), self.slots, self.maxpages,
                             self.npages, self.page)
         self.length = [int(n) if n >= 0 else old for n, old in zip(new, self.length)]

@@ -142,3 +142,22 @@ def test_refusal_leaves_the_state(pages):
     assert state(q) == before
     q.reserve([10, 10, 32])
     assert state(q)[3] == [2, 1, 1]
+
+
+def test_length_past_the_held_pages(pages):
+    """A length that the slot's pages do not hold is refused: the host's lengths stay
+    those of the device."""
+    p = pages(3, 6, 4)
+    p.reserve([20, 0, 64])
+    p.set_len([20, -1, -1])
+    before = state(p)
+    for new in ([33, -1, -1], [-1, 1, -1], [20, 0, 65]):
+        with pytest.raises(ValueError, match="set_len"):
+            p.set_len(new)
+        assert state(p) == before and p.length == before[1] == [20, 0, 0]
+    p.set_len([32, -1, 50])
+    p.fork([-1, 2, -1])
+    with pytest.raises(ValueError, match="set_len"):
+        p.set_len([-1, 65, -1])
+    p.set_len([-1, 64, 0])
+    assert p.length == state(p)[1] == [32, 64, 0]
