@@ -53,6 +53,8 @@ class Pages:
         return (self.ix, *(self.at[n] for n in ("table", "len", "held", "ref")))
 
     def _arg(self, values) -> int:
+        if len(values) != self.slots:
+            raise ValueError(f"{len(values)} values for {self.slots} slots")
         self.ix.upload(np.asarray(values, np.int32), 4 * self.at["arg"])
         return self.at["arg"]
 
@@ -66,7 +68,7 @@ class Pages:
         # a refused call's copies of shared pages cannot be told from the others, and
         # pages held ahead not from what it took: then the state as it was goes back
         keep = any(h > self._pages_of(n) for h, n in zip(self.held, self.length)) or \
-            any(want[s] > self.length[s] for s in self.forked)
+            any(w > n for s, (w, n) in enumerate(zip(want, self.length)) if s in self.forked)
         before = self.ix.download((self.ints,), np.int32) if keep else None
         q8hip.pages_reserve(self.ctx, *self._state(), self._arg(want), *shape, self.page, *self._pool())
         if self._short(want):

@@ -161,3 +161,17 @@ def test_length_past_the_held_pages(pages):
         p.set_len([-1, 65, -1])
     p.set_len([-1, 64, 0])
     assert p.length == state(p)[1] == [32, 64, 0]
+
+
+def test_one_value_per_slot(pages):
+    """Lists of another length than the slots (whose rest would be that of an earlier
+    call) are refused."""
+    p = pages(3, 6, 4)
+    p.reserve([20, 20, 20])
+    p.set_len([20, 20, 20])
+    before = state(p)
+    for call in (p.reserve, p.set_len, p.fork):
+        for values in ([16], [1] * 4, []):
+            with pytest.raises(ValueError, match="slot"):
+                call(values)
+            assert state(p) == before and p.length == [20, 20, 20]
