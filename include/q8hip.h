@@ -449,7 +449,8 @@ uint64_t q8_kv8_page_bytes(int page, int nkv, int head_dim);
  * the quotients x / s rounded to the nearest, ties to even; where the scale
  * grows, the older tokens' codes become code * s_old / s rounded likewise.  A
  * page that takes a NaN or an infinity gets the scale NaN: every row that sees
- * one of its tokens is NaN from then on.  Rows whose page is missing (an id
+ * one of its tokens is NaN from then on.  (Until it holds no older token when
+ * rows are appended; tokens returned by q8_pages_set_len count until then.)  Rows whose page is missing (an id
  * outside [0, npages), positions from maxpages*page on) are not stored.  Pages
  * that are written must belong to one sequence alone (q8_pages_reserve). */
 int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint64_t ov_f32,
@@ -498,7 +499,11 @@ int q8_pages_reserve(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i
 
 /* len[s] = new[s] (at most what the held pages hold; new[s] < 0 leaves the slot
  * alone), and the pages behind it are released: the advance after a step, the
- * return of rejected tokens and, with 0, the end of a sequence. */
+ * return of rejected tokens and, with 0, the end of a sequence.  Contents of
+ * pages stay as they are: in the 8-bit cache a page that keeps older tokens also
+ * keeps the scale that the returned ones had raised (or made NaN), and the older
+ * codes as rounded to it.  A slot forked before such tokens keeps the page free of
+ * them: they go to a copy, and the slot continues from its fork. */
 int q8_pages_set_len(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t olen_i32,
                      uint64_t oheld_i32, uint64_t oref_i32, uint64_t onew_i32, int64_t nslots,
                      int64_t maxpages, int64_t npages, int page);

@@ -275,7 +275,9 @@ class Q8Batch:
         return dict(zip(slots, flat))
 
     def truncate(self, lengths: Mapping[int, int]) -> None:
-        """Shortens slots (rejected drafts); 0 ends a sequence."""
+        """Shortens slots (rejected drafts); 0 ends a sequence.  The page that a slot's
+        end falls into keeps the scale that the dropped tokens gave it: fork the slot
+        before a draft, and back if it is rejected, to be without it."""
         if any(not 0 <= s < self.slots or not 0 <= n <= self.pages.length[s]
                for s, n in lengths.items()):
             raise ValueError("truncate: no such slot, or a length past its tokens")
