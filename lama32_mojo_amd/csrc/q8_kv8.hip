@@ -464,13 +464,14 @@ __device__ __forceinline__ int kv8_seq_of(const int *pre, int nseq, int u) {
   return lo;
 }
 
-// Tables of up to this many units, and no more blocks of 8 waves than about one
-// per CU, take a block per row tile: the merge launch costs 4 us, a second
-// round of blocks more (heads of 128 in groups of 4, us whole / split: 1 sequence
-// of 500 tokens 11.4 / 13.3, of 900 15.4 / 13.5; 32 of 500 12.9 / 16.2; 64 of
-// 500 23.6 / 18.1).
+// Tables of up to this many units, and no more blocks of 8 waves than CUs (one fits a
+// CU), take a block per row tile: the merge launch costs 4 us, a second round of
+// blocks more (us whole / split: 1 sequence of 500 tokens, heads of 128 in groups
+// of 4, 11.4 / 13.3, of 900 15.4 / 13.5; 32 of 700, 256 blocks, 14.7 / 22.8, 34 of
+// 700, 272 blocks, 26.1 / 23.5; heads of 64 in groups of 16, 32 of 250 7.7 / 13.1,
+// 48 17.1 / 14.4).
 constexpr int kKv8WholeUnits = 12;
-constexpr int kKv8WholeBlocks = 384;
+constexpr int kKv8WholeBlocks = 256;
 constexpr int kKv8Waves = 4;              // waves of a block (WHOLE: 8)
 constexpr int kKv8PlanSeq = 1024;         // sequences of a launch (16 KB of LDS for the plan)
 
@@ -928,7 +929,9 @@ hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
   const Kv8Args &c = a.c;
   const int grp = c.nheads / c.nkv;
   const size_t plan = (size_t)(4 * c.nseq + 1) * 4;
-  const int64_t tiles = c.rows * grp / NC + c.nseq;
+  // a sequence of n rows has ceil(n grp / NC) row tiles: no more than each row alone
+  // would, nor than n grp / NC and one
+  const int64_t tiles = std::min(c.rows * ((grp + NC - 1) / NC), c.rows * grp / NC + c.nseq);
   const int64_t key_units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit;
   if (key_units <= kKv8WholeUnits && tiles * c.nkv <= kKv8WholeBlocks) {
     const size_t lds = (size_t)(8 / MT / 2) * NC * (HD + 4) * 4 + plan;

@@ -102,3 +102,20 @@ def test_packed_carries_q_beside_a_large_dim(ctx, nh, nkv, hd, lens, act, large)
                         v[a:r + 1].astype(np.float64), r - a)[0]
         bar = 1e-5 * np.abs(ref).max() if act == "f32" else bf16_bar(ref, v)
         assert (np.abs(y[r] - ref) <= bar).all(), r
+
+
+@pytest.mark.parametrize("nh,nkv,hd,nseq,most", [
+    (8, 2, 64, 128, 1), (8, 2, 64, 129, 1),       # 256 and 258 row tiles over the KV heads
+    (32, 2, 128, 65, 1), (40, 1, 64, 100, 3), (6, 2, 128, 40, 9), (20, 4, 64, 66, 2)])
+def test_cache_tiles_of_many_sequences(ctx, nh, nkv, hd, nseq, most):
+    """Every row tile has its block, whole or split, where tiles are about as many as
+    the card has CUs: sequences of one row, of none, and of several that end inside
+    a tile."""
+    say("cache tiles", nh, nkv, hd, nseq, most)
+    rng = np.random.default_rng(nseq)
+    lens = [1] * nseq if most == 1 else rng.integers(0, most + 1, nseq).tolist()
+    p = Paged(ctx, rng, lens, rng.integers(0, 120, nseq).tolist(), 32, nkv, hd)
+    q = rng.standard_normal((p.rows, nh, hd)).astype(np.float32)
+    assert max_rel_err(run_cache(p, q), p.c.attention(q, p.cu, p.old, p.table)) <= 1e-5
+    for b in (p.pool, p.ix):
+        b.free()
