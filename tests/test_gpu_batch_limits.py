@@ -4,10 +4,9 @@
 import numpy as np
 import pytest
 
-from lama32_mojo_amd import q8hip
 from oracle import batch_oracle as bo
 from oracle.q8_oracle import max_rel_err
-from test_gpu_batch import (Paged, bf16_bits, bf16_to_f32, offsets, packed_inputs, run_append,
+from test_gpu_batch import (PageState, Paged, bf16_bits, bf16_to_f32, offsets, packed_inputs, run_append,
                             run_cache, run_packed, say)
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +118,96 @@ def test_cache_tiles_of_many_sequences(ctx, nh, nkv, hd, nseq, most):
     assert max_rel_err(run_cache(p, q), p.c.attention(q, p.cu, p.old, p.table)) <= 1e-5
     for b in (p.pool, p.ix):
         b.free()
+
+
+def packed_errors(ctx, lens, nh, nkv, hd, act, seed, rows=None):
+    """Rows of a packed call against float64; the bars of test_gpu_batch.py."""
+    rng = np.random.default_rng(seed)
+    q, k, v = packed_inputs(rng, lens, nh, nkv, hd)
+    if act == "bf16":
+        q = bf16_to_f32(bf16_bits(q))
+    cu = offsets(lens)
+    y = run_packed(ctx, q, k, v, cu, act, dead=2)
+    for r in range(len(q)) if rows is None else rows:
+        a = cu[np.searchsorted(cu, r, "right") - 1]
+        ref = bo.attend(q[r:r + 1].astype(np.float64), k[a:r + 1].astype(np.float64),
+                        v[a:r + 1].astype(np.float64), r - a)[0]
+        bar = 1e-5 * np.abs(ref).max() if act == "f32" else bf16_bar(ref, v)
+        assert (np.abs(y[r] - ref) <= bar).all(), r
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,nkv,hd", [(33, 1, 64), (66, 2, 128), (100, 1, 128), (128, 1, 64), (128, 1, 128)])
+def test_packed_wide_groups(ctx, nh, nkv, hd, act):
+    """Groups whose heads take several waves, with columns left over in one."""
+    say("packed groups", nh, nkv, hd, act)
+    packed_errors(ctx, [1, 0, 5, 70], nh, nkv, hd, act, nh)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("grp", [3, 5, 7])
+def test_packed_long_odd_groups(ctx, grp, act):
+    """The 8-wave blocks of long prompts, at groups that leave columns over."""
+    say("packed long groups", grp, act)
+    n = 4097 + 4200
+    rows = np.unique(np.r_[0:3, 36:38, 84:87, 4094:4099, 4180:4184, n - 90:n - 86, n - 3:n])
+    packed_errors(ctx, [4097, 4200], grp, 1, 128, act, grp, rows)
+
+
+@pytest.mark.parametrize("nseq", [15, 16, 17])
+def test_packed_sequence_counts(ctx, nseq):
+    """Either side of the count up to which tiles go longest first."""
+    say("packed sequences", nseq)
+    lens = [(37 * i * i + 11 * i) % 150 for i in range(nseq)]
+    packed_errors(ctx, lens, 4, 2, 64, "f32", nseq)
+    packed_errors(ctx, lens[::-1], 6, 2, 128, "bf16", nseq)
+
+
+def test_reserve_over_many_pages(ctx):
+    """Pools of more pages than one go of the search: free pages that begin behind the
+    first go, runs that cross from one to the next, and too few of them."""
+    say("pages 60000")
+    s = PageState(ctx, 24, 3000, 60000, 16, layers=1, pb=16)
+    s.reserve([16 * (1500 + 37 * i % 200) for i in range(22)] + [0, 0])    # past 32768
+    s.set_len([16 * len(r) for r in s.o.rows])
+    s.check()
+    s.set_len([-1, 160, -1, 0] + [-1] * 20)                                 # holes in the first go
+    s.fork([-1, -1, -1, 4] + [-1] * 20)
+    s.reserve([n + (16 * 2900 - n if 12 < i < 24 else i % 3) for i, n in enumerate(s.o.len)])
+    s.check()
+    s.set_len([16 * len(r) if i % 2 else -1 for i, r in enumerate(s.o.rows)])
+    s.reserve([16 * 3000] * 24)                                             # 72000: the pool ends
+    s.check()
+    s.reserve([16 * 3000 if i % 5 == 0 else n for i, n in enumerate(s.o.len)])
+    s.compact()
+    s.check()
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_greedy_ids_are_the_largest_logits(ctx, kind):
+    """forward's ids, one a slot and one a row, are the argmax of the logits that the
+    same calls return."""
+    from lama32_mojo_amd import batch, model as gm
+    from test_model_oracle import qwen_tiny, tiny_model
+    say("greedy ids", kind)
+    spec, t, inv = tiny_model() if kind == "llama" else qwen_tiny()
+    cfg = gm.Config(spec.hidden, spec.layers, spec.n_heads, spec.n_kv, spec.head_dim, spec.inter,
+                    spec.vocab, spec.eps, 500000.0 if kind == "llama" else 1000000.0, 32.0, 1.0, 4.0,
+                    8192.0, tied=spec.tied, qk_norm=spec.qk_norm,
+                    rope="llama3" if kind == "llama" else "plain")
+    m = gm.Q8Llama(ctx, cfg, 16, weights=t)
+    two = [batch.Q8Batch(m, slots=4, npages=24, maxlen=160, page=16, max_rows=128) for _ in range(2)]
+    rng = np.random.default_rng(2)
+    draw = lambda n: rng.integers(0, spec.vocab, n).tolist()
+    for tokens, every in (({0: draw(37), 1: draw(5), 3: draw(20)}, False), ({0: draw(1), 1: draw(1), 3: draw(1)}, False),
+                          ({0: draw(4), 3: draw(3)}, True), ({2: draw(7)}, True), ({1: draw(33), 2: draw(1)}, False),
+                          ({2: draw(1)}, False)):
+        lg, ids = two[0].forward(tokens, every=every, logits=True), two[1].forward(tokens, every=every)
+        assert set(ids) == set(lg) == set(tokens)
+        for s in tokens:
+            want = np.argmax(lg[s], -1)
+            assert ids[s] == (want.tolist() if every else int(want)), (s, tokens)
+            assert not every or len(ids[s]) == len(tokens[s])
+    for b in two:
+        b.close()
+    m.close()
