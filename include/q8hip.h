@@ -75,9 +75,9 @@ void q8_destroy(q8_ctx *ctx);
  * streams are not ordered, except that one that uses the context's scratch
  * (q8_linear of more than 4 rows or of unaligned ones, q8_linear_bf16act, _swiglu
  * and _rmsnorm, q8_head_argmax, q8_decode_attention, q8_attention from 16
- * rows on, q8_kv8_attention, q8_pages_reserve and _compact, q8_graph_launch) starts behind the last such call on another
- * stream; for that, a stream stays valid until another one is set, or
- * until q8_sync has returned on it.  A graph that the caller captured and
+ * rows on, q8_kv8_attention, q8_pages_reserve and _compact, q8_graph_launch)
+ * starts behind the last such call on another stream; for that, a stream stays
+ * valid until another one is set, or until q8_sync has returned on it.  A graph that the caller captured and
  * launches by itself is not seen by this. */
 int q8_set_stream(q8_ctx *ctx, void *hip_stream);
 void *q8_get_stream(q8_ctx *ctx);
@@ -424,8 +424,8 @@ int q8_token_begin(q8_ctx *ctx, q8_buf *ids, uint64_t oid_i32, int32_t id, q8_bu
  * q8_rope_kv and q8_kv8_append write them.  f32 q keeps f32 accuracy (<= 1e-5;
  * f32 scores of size S add S 2^-22), bf16 q rounds the probabilities to binary16;
  * both carry every dimension of q as it stands.  head_dim 64 or 128, nheads / nkv
- * up to 128, rows up to 2^24 (row tiles times KV heads below 2^24); q, out, K and V rows start 16-byte aligned
- * (Q8_ERR_UNSUPPORTED otherwise).  Values that a row does not see, infinities
+ * up to 128, rows up to 2^24 (row tiles times KV heads below 2^24); q, out, K and V
+ * rows start 16-byte aligned (Q8_ERR_UNSUPPORTED otherwise).  Values that a row does not see, infinities
  * and NaN included, do not reach it. */
 int q8_attention_packed(q8_ctx *ctx, q8_buf *q, uint64_t oq, int act_dtype, int64_t ldq, q8_buf *kv,
                         uint64_t okc_f16, uint64_t ovc_f16, q8_buf *out, uint64_t oy, q8_buf *ix,
@@ -449,10 +449,11 @@ uint64_t q8_kv8_page_bytes(int page, int nkv, int head_dim);
  * the quotients x / s rounded to the nearest, ties to even; where the scale
  * grows, the older tokens' codes become code * s_old / s rounded likewise.  A
  * page that takes a NaN or an infinity gets the scale NaN: every row that sees
- * one of its tokens is NaN from then on.  (Until it holds no older token when
- * rows are appended; tokens returned by q8_pages_set_len count until then.)  Rows whose page is missing (an id
- * outside [0, npages), positions from maxpages*page on) are not stored.  Pages
- * that are written must belong to one sequence alone (q8_pages_reserve). */
+ * one of its tokens is NaN from then on (until rows are appended to it while it
+ * holds no older token; tokens returned by q8_pages_set_len count until then).
+ * Rows whose page is missing (an id outside [0, npages), positions from
+ * maxpages*page on) are not stored.  Pages that are written must belong to one
+ * sequence alone (q8_pages_reserve). */
 int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint64_t ov_f32,
                   uint64_t oinv_f32, uint64_t oqr_f32, int64_t ld, int64_t ldr, q8_buf *kv,
                   uint64_t okc_f16, uint64_t ovc_f16, q8_buf *pages, uint64_t opages,
@@ -465,8 +466,9 @@ int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint
  * its cached tokens 0 .. len[i] + j (those of this call's rows included, so
  * q8_kv8_append comes first), one row a sequence or several (drafted tokens, a
  * prompt's next chunk).  Within 1e-5 of float64 over the stored values, every
- * dimension of q carried as f32 carries it (f32 scores of size S add S 2^-22).  A row
- * that sees a missing page is NaN.  Up to 512 KV heads and 2^22 rows.  The split
+ * dimension of q carried as f32 carries it (f32 scores of size S add S 2^-22).  A
+ * row that sees a missing page (an id outside [0, npages)) is NaN; rows at
+ * positions from maxpages*page on see the tokens before them that the table has.  Up to 512 KV heads and 2^22 rows.  The split
  * records live in the context's scratch (q8_set_stream). */
 int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
                      q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,

@@ -307,7 +307,8 @@ struct PagePool {
   int64_t page_bytes, layers, stride;
 };
 constexpr int kPagesMaxSlots = 4096;   // lengths and tables of a column in LDS
-// ws: 2 * nslots + 1 + 3 * npages ints (the copies to make, the pages replaced).
+// ws: 2 * nslots + 1 + 3 * npages ints: the copies to make, at most one a slot, and
+// the pages replaced, three ints each, at most as many as there are free pages.
 hipError_t launch_pages_reserve(const PagesArgs &a, const int *want, const PagePool &pool, int *ws,
                                 hipStream_t st);
 hipError_t launch_pages_set_len(const PagesArgs &a, const int *new_len, hipStream_t st);

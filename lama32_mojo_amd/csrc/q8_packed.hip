@@ -15,7 +15,9 @@
 // largest; K and V are binary16 already, so products are exact and the sums,
 // f32, have f32-level error.  bf16 q fits one binary16 after the scaling, and
 // p is rounded to one (2^-12 of itself, a sixteenth of the bf16 output's own
-// rounding): half the matrix work.  Columns where those terms hold too little of
+// rounding): half the matrix work.  (Of 16282 rows the error is 1.66e-3 of float64,
+// with f32 probabilities 1.65e-3; one output in ten is the neighbouring bf16 value
+// of the one that those give.)  Columns where those terms hold too little of
 // the small dims of q (kFarDim) are formed in f32.
 // Bound: MFMA (4 hd flops per (row, head, key seen), twice issued for f32) with
 // the softmax's VALU work and the LDS traffic beside it; of 16001 rows in bf16

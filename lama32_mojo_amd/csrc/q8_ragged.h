@@ -49,7 +49,8 @@ Q8_HD int64_t kv8_page_bytes(int page, int nkv, int hd) {
 
 // The work of a cache attention call: units of 64 keys, counted over
 // sequences and, within one, over its row tiles of `cols` (row, query head)
-// columns.  Block b serves the units [b * per, (b + 1) * per).
+// columns.  Run r of the call (a wave's, or of as many waves as a row tile has
+// 16-column parts) serves the units [r * per, (r + 1) * per).
 constexpr int kKv8Unit = 64;
 struct Kv8Seq {
   int n, old, row_tiles, key_units;
@@ -73,10 +74,10 @@ Q8_HD int kv8_units_of(const Kv8Seq &s) {
 }
 // (of counts from 0 to the limit; two at the limit would not fit an int32)
 Q8_HD int kv8_add(int a, int b) { return a < kKv8MaxUnits - b ? a + b : kKv8MaxUnits; }
-// Units per block of nblocks; at least `least` (a block's waves take a unit
-// each), so a small call uses fewer blocks.
-Q8_HD int kv8_units_per_block(int64_t units, int nblocks, int least) {
-  const int64_t per = ((int64_t)units + nblocks - 1) / nblocks;
+// Units of each of nruns runs; at least `least` (the kernels': 1), so a small call
+// uses fewer of them.
+Q8_HD int kv8_units_per_block(int64_t units, int nruns, int least) {
+  const int64_t per = ((int64_t)units + nruns - 1) / nruns;
   return (int)(per < least ? least : per);
 }
 
