@@ -91,9 +91,9 @@ __device__ __forceinline__ void sincos_pos(int pos, float inv, double &sn, doubl
 // the old tokens' codes where the scale grew, and writes the new codes.  Keys,
 // whose codes must not depend on the path, are rotated in f64 and rounded once;
 // q takes cos and sin rounded to f32 and f32 products (3.5e-8 of float64; rounded
-// once 2.5e-8, for f64 products of every head of the group).  A thread holds (token, dims 4j .. 4j+3 and their partners half a head
-// on) items, so the rotation needs no exchange and the values stay in registers
-// between the two passes.
+// once 2.5e-8, for f64 products of every head of the group).  A thread holds
+// (token, dims 4j .. 4j+3 and their partners half a head on) items, so the
+// rotation needs no exchange and the values stay in registers between the passes.
 // Bound: HBM for prompts (q read and written, k and v read, codes written),
 // the chain of dependent loads for a token per sequence.
 

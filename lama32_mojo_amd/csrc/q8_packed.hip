@@ -53,13 +53,13 @@ constexpr int kSorted = 16;
 // Small dims of q: the terms' 2^-25 (at largest values in [2^14, 2^15)) is up to 2^-19
 // of a dim 20 binary exponents below its column's largest, and bf16 (8 bits) is
 // exact in them down to 31 below.  Dims that lie further below (one f32 column of
-// normal values in 4000) make an error of the score of at most sqrt(HD) 2^-40
-// max|q| max|k|, and of 6.6e-6, counting 6 times the mean square, where max|q|
-// max|k| (max|q| as its power of two) reaches 2^20: no binary16 k takes a
-// largest q below 32 there.  From 32 on a wave with such a column looks its keys
-// through, and columns past 2^20 are formed in f32: beside dims that are 2^23 to
-// 2^126 times the others, and 0 in K, 1e-5 to 1 -> 6e-7 of float64.  (If every
-// wave looked: 8088 ragged f32 rows 357 -> 452 us; none does for ordinary q.)
+// normal values in 4000) make an error of the score of at most sqrt(HD) 2^-39
+// max|q| max|k| (max|q| as the power of two below it), and of 6.6e-6, 6 times the
+// mean square, where that product reaches 2^20: no binary16 k takes a largest q
+// below 32 there.  From 32 on a wave with such a column looks its keys through, and
+// columns past 2^20 are formed in f32: beside dims that are 2^23 to 2^126 times
+// the others, and 0 in K, 1e-5 to 1 -> 8e-7 of float64.  (If every wave looked:
+// 8088 ragged f32 rows 357 -> 452 us; with largest q below 32 none does.)
 template <bool BF16> constexpr int kFarDim = BF16 ? 31 : 20;
 
 // Rows of a block of nw waves, 32 columns each.

@@ -1,8 +1,9 @@
-// Host check of the unit sums of csrc/q8_ragged.h where the offsets hold
-// nonsense: the prefix sums of a cache attention call (the block's scan, step by
-// step), the search for a unit's sequence and the place within it, for offsets
-// out of order whose sums pass 2^30.  Every row tile, column and row that a block
-// would serve has to lie inside its sequence.
+// Host check of the units of work of csrc/q8_ragged.h.  Well-formed calls: every
+// unit in one run at each column count, and the records that runs leave.  Offsets
+// that hold nonsense: the prefix sums of a cache attention call (the block's scan,
+// step by step), the search for a unit's sequence and the place within it, with
+// offsets out of order whose sums pass 2^30; every row tile, column and row that a
+// block would serve has to lie inside its sequence.
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -85,8 +86,56 @@ static void call(const std::vector<int> &cu, const std::vector<int> &len, int64_
   }
 }
 
+// A well-formed call: every (row tile, 64 keys) in one run, records where the merge
+// looks for them, none written twice.
+static void cover(const std::vector<int> &cu, const std::vector<int> &len, int64_t rows, int64_t cap,
+                  int grp, int cols, int runs) {
+  const int nseq = (int)len.size();
+  std::vector<Kv8Seq> sq;
+  std::vector<int> pre(1, 0);
+  int64_t tiles = 0;
+  for (int i = 0; i < nseq; ++i) {
+    sq.push_back(kv8_seq(cu[i], cu[i + 1], len[i], rows, cap, grp, cols));
+    pre.push_back(kv8_add(pre.back(), kv8_units_of(sq[i])));
+    tiles += sq[i].row_tiles;
+  }
+  // the bounds that launches are sized by
+  CHECK(tiles <= rows * ((grp + cols - 1) / cols) && tiles <= rows * grp / cols + nseq);
+  const int units = pre.back(), per = kv8_units_per_block(units, runs, 1);
+  std::vector<int> seen(units, 0);
+  for (int r = 0; r < runs; ++r) {
+    int slots[2] = {0, 0}, i = 0;
+    for (int64_t u = (int64_t)r * per, uend = u + per < units ? u + per : units; u < uend;) {
+      while (pre[i + 1] <= u) ++i;
+      const int ku = sq[i].key_units, rt = ((int)u - pre[i]) / ku, t0 = ((int)u - pre[i]) % ku;
+      const int t1 = ku < t0 + uend - u ? ku : (int)(t0 + uend - u);
+      CHECK(rt < sq[i].row_tiles && t1 > t0);
+      for (int t = t0; t < t1; ++t) ++seen[u + t - t0];
+      const int ua = pre[i] + rt * ku, b0 = ua / per, b1 = (ua + ku - 1) / per;
+      CHECK((t0 == 0 && t1 == ku) == (b0 == b1));
+      if (b0 != b1) {
+        CHECK((t0 == 0) == (r == b0));
+        CHECK(++slots[t0 == 0] == 1);
+      }
+      u += t1 - t0;
+    }
+  }
+  for (int v : seen) CHECK(v == 1);
+}
+
 int main() {
   std::mt19937 rng(11);
+  for (int round = 0; round < 200; ++round) {
+    std::vector<int> cu(1, 0), len;
+    for (int i = 0, nseq = 1 + (int)(rng() % 90u), most = 1 + (int)(rng() % 40u); i < nseq; ++i) {
+      cu.push_back(cu.back() + (rng() % 5u ? (int)(rng() % (unsigned)most) : 0));
+      len.push_back((int)(rng() % 900u));
+    }
+    for (int cols : {16, 32, 64})
+      for (int runs : {1, 5, 64, 2048})
+        cover(cu, len, cu.back() + (int)(rng() % 9u), 16 * (1 + (int)(rng() % 64u)), 1 + (int)(rng() % 70u),
+              cols, runs);
+  }
   for (int a : {0, 1, kKv8MaxUnits / 2, kKv8MaxUnits - 1, kKv8MaxUnits})
     for (int b : {0, 1, kKv8MaxUnits / 2, kKv8MaxUnits - 1, kKv8MaxUnits}) {
       const int64_t s = (int64_t)a + b;

@@ -1,6 +1,7 @@
-"""Unit sums of the cache attention (csrc/q8_ragged.h) for offsets that hold
-nonsense, on the CPU under the sanitizers: sums that pass 2^30 stay at it, and
-every row tile, column and row found from them lies inside its sequence."""
+"""Units of work of the cache attention (csrc/q8_ragged.h) on the CPU under the
+sanitizers: runs and records of well-formed calls, and offsets that hold nonsense,
+whose sums stay at 2^30 and whose row tiles, columns and rows lie inside their
+sequences."""
 
 import os
 import shutil
@@ -9,7 +10,7 @@ import subprocess
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-def test_unit_sums_saturate(tmp_path):
+def test_units_and_sums(tmp_path):
     gxx = shutil.which("g++")
     assert gxx, "g++ is needed"
     out = str(tmp_path / "sums")
