@@ -526,6 +526,30 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
                      int64_t npages, q8_buf *pages, uint64_t opages, uint64_t page_bytes,
                      int64_t layers, uint64_t layer_stride);
 
+/* ---- drawing tokens ----------------------------------------------------------- */
+
+/* ids [rows] = a token drawn from each row of n f32 logits at ox + r*ldx (ldx = 0:
+ * dense), by the row's temperature T, top_p, min_p and random number u -- four arrays
+ * of `rows` f32 one after the other at oparam of `a` -- and k, int32 [rows] at otopk
+ * of `ids`.  (The reference decodes greedily, q8_argmax.)  With w_i = exp((x_i -
+ * max) / T) and the tokens in the order of x descending, then index ascending:
+ *   k      keeps the first k tokens (k <= 0: all);
+ *   top_p  keeps, of those, each one before which less than top_p of their sum of w
+ *          lies, the first one always (top_p >= 1: all);
+ *   min_p  keeps, of those, the ones with w_i >= min_p (1 at most; the largest w is 1);
+ *   the id is the first token whose running sum of w exceeds u times the sum of all
+ *   kept (u in [0, 1); values outside are taken to its ends).
+ * T <= 0 takes the first token of the order.  Settings that are NaN are off (u: 0, T:
+ * the first token).  With lp non-null, lp[r] at olp is the log of the id's w over
+ * the kept sum (f32).  Logits that are -inf or NaN are never drawn; of a row with
+ * +inf, only those are; a row without any token gives id -1 and -inf.  Weights and
+ * sums are held to 2^-40 and f64, in an order that depends on the inputs alone, so
+ * equal inputs give equal ids.  1 <= n <= 2^22.  The context's scratch is used
+ * (q8_set_stream). */
+int q8_sample(q8_ctx *ctx, q8_buf *a, uint64_t ox_f32, int64_t ldx, int64_t rows, int64_t n,
+              uint64_t oparam_f32, q8_buf *ids, uint64_t otopk_i32, uint64_t oid_i32, q8_buf *lp,
+              uint64_t olp_f32);
+
 /* ---- HIP graphs ------------------------------------------------------------ */
 
 /* Capture every call issued on the context's stream between begin and end

@@ -317,4 +317,16 @@ hipError_t launch_pages_fork(const PagesArgs &a, const int *source, hipStream_t 
 hipError_t launch_pages_compact(const PagesArgs &a, int *live, const PagePool &pool, int *ws,
                                 hipStream_t st);
 
+// ---- drawing tokens (q8_sample.hip) ------------------------------------------------
+struct SampleArgs {
+  const float *x;          // logits of row r at x + r * ldx
+  int64_t ldx, rows, n;
+  const float *param;      // [4][rows]: temperature, top_p, min_p, u
+  const int *topk;         // [rows]
+  int *ids;                // [rows]
+  float *logp;             // [rows] or null
+  uint8_t *ws;             // the slices' histograms, 16-byte aligned
+};
+hipError_t launch_sample(const SampleArgs &a, int64_t ws_bytes, hipStream_t st);
+
 }  // namespace q8

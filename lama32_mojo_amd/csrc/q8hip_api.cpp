@@ -2073,6 +2073,54 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
 
 // ---- HIP graphs -------------------------------------------------------------------
 
+// ---- drawing tokens -----------------------------------------------------------------
+
+int q8_sample(q8_ctx *ctx, q8_buf *a, uint64_t ox_f32, int64_t ldx, int64_t rows, int64_t n,
+              uint64_t oparam_f32, q8_buf *ids, uint64_t otopk_i32, uint64_t oid_i32, q8_buf *lp,
+              uint64_t olp_f32) {
+  const char *what = "q8_sample";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!a || !ids) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (rows < 0 || rows > ((int64_t)1 << 24) || n <= 0 || n > ((int64_t)1 << 22))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: rows=%lld, n=%lld (0 .. 2^24 rows of 1 .. 2^22 logits)", what,
+                (long long)rows, (long long)n);
+  if (ldx != 0 && (ldx < n || ldx > INT32_MAX))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: row stride %lld (0, or at least %lld)", what, (long long)ldx,
+                (long long)n);
+  if (ldx == 0) ldx = n;
+  const uint64_t R = (uint64_t)rows, xn = rows_span(rows, ldx, (uint64_t)n);
+  if (int rc = check_f32(ctx, a, ox_f32, xn, what, "logits")) return rc;
+  if (int rc = check_f32(ctx, a, oparam_f32, 4 * R, what, "settings")) return rc;
+  const Ints v[] = {{"k", otopk_i32, R, false}, {"ids", oid_i32, R, true}};
+  if (int rc = check_ints(ctx, ids, v, 2, what)) return rc;
+  if (lp && !fits(olp_f32, R, 4, lp->size))
+    return fail(ctx, Q8_ERR_RANGE, "%s: the log-probabilities exceed their buffer", what);
+  if (share(ids, oid_i32 * 4, R * 4, a, ox_f32 * 4, xn * 4) ||
+      share(ids, oid_i32 * 4, R * 4, a, oparam_f32 * 4, 16 * R) ||
+      (lp && (share(lp, olp_f32 * 4, R * 4, a, ox_f32 * 4, xn * 4) ||
+              share(lp, olp_f32 * 4, R * 4, a, oparam_f32 * 4, 16 * R) ||
+              share(lp, olp_f32 * 4, R * 4, ids, otopk_i32 * 4, R * 4) ||
+              share(lp, olp_f32 * 4, R * 4, ids, oid_i32 * 4, R * 4))))
+    return fail(ctx, Q8_ERR_ARG, "%s: an output overlaps another array", what);
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  q8::SampleArgs p;
+  p.x = fptr(a, ox_f32);
+  p.ldx = ldx;
+  p.rows = rows;
+  p.n = n;
+  p.param = fptr(a, oparam_f32);
+  p.topk = iptr(ids, otopk_i32);
+  p.ids = iptr(ids, oid_i32);
+  p.logp = lp ? fptr(lp, olp_f32) : nullptr;
+  p.ws = static_cast<uint8_t *>(ctx->act16);
+  const hipError_t e =
+      with_scratch(ctx, [&] { return q8::launch_sample(p, kAct16Bytes, ctx->stream); });
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_sample launch");
+  return ok(ctx);
+}
+
 struct q8_graph {
   hipGraph_t graph = nullptr;
   hipGraphExec_t exec = nullptr;

@@ -130,6 +130,7 @@ SIGNATURES = {
     "q8_pages_fork": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64]),
     "q8_pages_compact": (_I, [_P, _P, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _P, _U64, _U64,
                               _I64, _U64]),
+    "q8_sample": (_I, [_P, _P, _U64, _I64, _I64, _I64, _U64, _P, _U64, _U64, _P, _U64]),
     "q8_graph_begin": (_I, [_P]),
     "q8_graph_end": (_I, [_P, ctypes.POINTER(_P)]),
     "q8_graph_launch": (_I, [_P, _P]),
@@ -586,3 +587,14 @@ def pages_compact(ctx: Context, ix: Buffer, otab: int, oheld: int, oref: int, ol
     ctx.check(ctx._lib.q8_pages_compact(
         ctx.h, ix.h, int(otab), int(oheld), int(oref), int(olive), int(nslots), int(maxpages),
         int(npages), pages.h, int(opages), int(page_bytes), int(layers), int(layer_stride)))
+
+
+# ---- drawing tokens ---------------------------------------------------------------------
+
+def sample(ctx: Context, a: Buffer, ox: int, rows: int, n: int, oparam: int, ids: Buffer, otopk: int,
+           oid: int, lp: Buffer | None = None, olp: int = 0, ldx: int = 0) -> None:
+    """A token id from each row of logits by the row's temperature, top_p, min_p and
+    random number (f32 [4][rows] at oparam of a) and k (int32 [rows] at otopk of ids);
+    with lp, the log-probabilities: q8_sample."""
+    ctx.check(ctx._lib.q8_sample(ctx.h, a.h, int(ox), int(ldx), int(rows), int(n), int(oparam), ids.h,
+                                 int(otopk), int(oid), _h(lp), int(olp)))

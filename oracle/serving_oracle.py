@@ -1,0 +1,44 @@
+"""Float64 restatement of the calls for requests that differ: drawing tokens,
+low-rank adapters, attention after a shared prefix.
+
+  sample   w_i = exp((x_i - max) / T); order x descending, index ascending; kept: the
+           first k, of these the ones with less than top_p of the sum before them, of
+           these the ones with w_i >= min_p; drawn: the first whose running sum exceeds
+           u times the kept sum
+  lora     y = base + scale B (A x), an A per part of the columns
+  share    sequences whose tables begin with the same page: the lowest leads; tokens
+           shared: the whole cached pages p that maximise (members with p pages in
+           common with it - 1) * p, the longest of equal ones
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+
+def sample_row(x, temp=1.0, k=0, top_p=1.0, min_p=0.0, u=0.0):
+    """(id, log-probability) of one row of logits."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    order = np.argsort(-x, kind="stable")
+    order = order[x[order] > -np.inf]
+    if len(order) == 0:
+        return -1, -np.inf
+    temp, top_p, min_p, u = (np.float64(np.float32(v)) for v in (temp, top_p, min_p, u))
+    if not temp > 0:
+        return int(order[0]), 0.0
+    v = x[order]
+    if v[0] == np.inf:
+        w = (v == np.inf).astype(np.float64)
+    else:
+        with np.errstate(under="ignore"):
+            w = np.exp((v - v[0]) / temp)
+    n = k if 0 < k < len(w) else len(w)
+    w = w[:n]
+    if top_p < 1:
+        w = w[:max(1, int((np.cumsum(w) - w < top_p * w.sum()).sum()))]
+    if min_p > 0:
+        w = w[:max(1, int((w >= min(min_p, 1.0)).sum()))]
+    c = np.cumsum(w)
+    u = min(u, 1 - 2.0 ** -24) if u > 0 else 0.0
+    at = min(int((c <= u * c[-1]).sum()), int((w > 0).sum()) - 1)
+    return int(order[at]), float(np.log(w[at] / c[-1]))
