@@ -526,6 +526,34 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
                      int64_t npages, q8_buf *pages, uint64_t opages, uint64_t page_bytes,
                      int64_t layers, uint64_t layer_stride);
 
+/* ---- adapters of several requests --------------------------------------------- */
+
+/* y[r] = base[r] + scale[i] B_i (A_i x[r]) for the rows r of every sequence whose
+ * adapter is i: low-rank adapters beside a projection that all requests share (base
+ * is its output).  (The reference has one set of weights.)  Rows and sequences as
+ * above: sequence s has the rows cu[s] .. cu[s+1]-1; its adapter is id[s], int32
+ * [nseq], and one outside [0, nadapters) is none: y = base.  Rows from cu[nseq] on are
+ * left as they are.
+ *
+ * n0, n1, n2: the columns of up to three stacked projections that share x (q|k|v:
+ * all; gate|up: n2 = 0; one: n1 = n2 = 0); each has an A of its own.  Adapter i of rank
+ * rank[i] (int32 [nadapters], on the device; at most max_rank; 0: as none), with
+ * p = rank[i] rounded up to a multiple of 8: its A's lie one after the other, each
+ * [p][m], from element oa + i*a_stride of w on; its B, [n0 + n1 + n2][p], from ob +
+ * i*b_stride on.  Elements behind the rank are zeros.  w_dtype Q8_SRC_BF16 or
+ * Q8_SRC_F32; A, B and the strides 16-byte aligned (Q8_ERR_UNSUPPORTED otherwise).
+ * x [rows, m] at ox (row stride ldx, 0: dense), base and y [rows, n0 + n1 + n2]
+ * (row stride ldy, 0: dense), y = base in place allowed; scale f32 [nadapters].
+ * m a multiple of 8; ranks up to 256, up to 4096 adapters and 4096 sequences, more
+ * than one with the same adapter.  f32 accuracy: x, A x and f32 weights enter as they
+ * are, sums are f32.  A row with infinities or NaN in x has NaN in its y and leaves
+ * others as they are.  The context's scratch is used (q8_set_stream). */
+int q8_lora(q8_ctx *ctx, q8_buf *w, int w_dtype, uint64_t oa, int64_t a_stride, uint64_t ob,
+            int64_t b_stride, int64_t nadapters, int max_rank, q8_buf *a, uint64_t ox_f32, int64_t ldx,
+            uint64_t obase_f32, uint64_t oy_f32, int64_t ldy, uint64_t oscale_f32, q8_buf *ix,
+            uint64_t ocu_i32, uint64_t oid_i32, uint64_t orank_i32, int64_t nseq, int64_t rows, int64_t m,
+            int64_t n0, int64_t n1, int64_t n2);
+
 /* ---- drawing tokens ----------------------------------------------------------- */
 
 /* ids [rows] = a token drawn from each row of n f32 logits at ox + r*ldx (ldx = 0:

@@ -317,6 +317,29 @@ hipError_t launch_pages_fork(const PagesArgs &a, const int *source, hipStream_t 
 hipError_t launch_pages_compact(const PagesArgs &a, int *live, const PagePool &pool, int *ws,
                                 hipStream_t st);
 
+// ---- adapters of several requests (q8_lora.hip) ----------------------------------
+// Sequence i's rows cu[i] .. cu[i+1]-1 take the adapter id[i] (outside [0,
+// nadapters): none).
+struct LoraArgs {
+  const uint8_t *A, *B;    // adapter i at i * a_stride, i * b_stride elements
+  bool f32;                // type of A and B: f32 or bf16
+  int64_t a_stride, b_stride, nadapters;
+  int max_rank;            // a multiple of 8
+  const float *x, *base;   // rows at x + r * ldx, base + r * ldy
+  float *y;
+  int64_t ldx, ldy;
+  bool in_place;           // y is base
+  const float *scale;      // [nadapters]
+  const int *cu, *id, *rank;
+  int64_t nseq, rows, m;
+  int parts, width[3];     // stacked projections and their columns
+  float *ws;               // 16-byte aligned
+  int ranks, splits, tiles, tile0;   // set by the launch
+};
+constexpr int kLoraMaxRank = 256;
+constexpr int kLoraMaxAdapters = 4096;
+hipError_t launch_lora(const LoraArgs &a, int64_t ws_floats, hipStream_t st);
+
 // ---- drawing tokens (q8_sample.hip) ------------------------------------------------
 struct SampleArgs {
   const float *x;          // logits of row r at x + r * ldx

@@ -2073,6 +2073,100 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
 
 // ---- HIP graphs -------------------------------------------------------------------
 
+// ---- adapters of several requests ------------------------------------------------------
+
+int q8_lora(q8_ctx *ctx, q8_buf *w, int w_dtype, uint64_t oa, int64_t a_stride, uint64_t ob,
+            int64_t b_stride, int64_t nadapters, int max_rank, q8_buf *a, uint64_t ox_f32, int64_t ldx,
+            uint64_t obase_f32, uint64_t oy_f32, int64_t ldy, uint64_t oscale_f32, q8_buf *ix,
+            uint64_t ocu_i32, uint64_t oid_i32, uint64_t orank_i32, int64_t nseq, int64_t rows, int64_t m,
+            int64_t n0, int64_t n1, int64_t n2) {
+  const char *what = "q8_lora";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!w || !a || !ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (w_dtype != Q8_SRC_F32 && w_dtype != Q8_SRC_BF16)
+    return fail(ctx, Q8_ERR_ARG, "%s: w_dtype=%d (Q8_SRC_F32 or Q8_SRC_BF16)", what, w_dtype);
+  if (int rc = check_seqs(ctx, nseq, rows, what)) return rc;
+  const int64_t most = (int64_t)1 << 24;
+  if (nseq > q8::kKv8MaxSeq || nadapters > q8::kLoraMaxAdapters || max_rank > q8::kLoraMaxRank)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nseq=%lld, nadapters=%lld, max_rank=%d (at most %d, %d, %d)",
+                what, (long long)nseq, (long long)nadapters, max_rank, q8::kKv8MaxSeq, q8::kLoraMaxAdapters,
+                q8::kLoraMaxRank);
+  if (nadapters <= 0 || max_rank <= 0 || m <= 0 || m % 8 != 0 || m > most || n0 <= 0 || n1 < 0 || n2 < 0 ||
+      n0 > most || n1 > most || n2 > most || (n2 > 0 && n1 == 0))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: nadapters=%lld, max_rank=%d, m=%lld (a positive multiple of 8), widths "
+                "%lld, %lld, %lld (the first ones positive; all at most 2^24)", what, (long long)nadapters,
+                max_rank, (long long)m, (long long)n0, (long long)n1, (long long)n2);
+  const int64_t R = (max_rank + 7) / 8 * 8, n = n0 + n1 + n2;
+  const int parts = n2 ? 3 : n1 ? 2 : 1;
+  if (a_stride < parts * R * m || b_stride < n * R || a_stride > ((int64_t)1 << 40) ||
+      b_stride > ((int64_t)1 << 40))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: an adapter's A of %lld elements or B of %lld does not fit its stride "
+                "(%lld, %lld)", what, (long long)(parts * R * m), (long long)(n * R), (long long)a_stride,
+                (long long)b_stride);
+  if ((ldx != 0 && (ldx < m || ldx > INT32_MAX)) || (ldy != 0 && (ldy < n || ldy > INT32_MAX)))
+    return fail(ctx, Q8_ERR_SHAPE, "%s: row strides %lld, %lld (0, or at least %lld, %lld)", what,
+                (long long)ldx, (long long)ldy, (long long)m, (long long)n);
+  if (ldx == 0) ldx = m;
+  if (ldy == 0) ldy = n;
+  const uint64_t es = w_dtype == Q8_SRC_F32 ? 4 : 2, na = (uint64_t)nadapters;
+  const uint64_t an = (na - 1) * (uint64_t)a_stride + (uint64_t)(parts * R * m);
+  const uint64_t bn = (na - 1) * (uint64_t)b_stride + (uint64_t)(n * R);
+  if (!fits(oa, an, es, w->size) || !fits(ob, bn, es, w->size))
+    return fail(ctx, Q8_ERR_RANGE, "%s: the adapters exceed their buffer", what);
+  const uint64_t xn = rows_span(rows, ldx, (uint64_t)m), yn = rows_span(rows, ldy, (uint64_t)n);
+  if (int rc = check_f32(ctx, a, ox_f32, xn, what, "x")) return rc;
+  if (int rc = check_f32(ctx, a, obase_f32, yn, what, "base")) return rc;
+  if (int rc = check_f32(ctx, a, oy_f32, yn, what, "y")) return rc;
+  if (int rc = check_f32(ctx, a, oscale_f32, na, what, "scale")) return rc;
+  const Ints v[] = {{"cu", ocu_i32, (uint64_t)nseq + 1, false},
+                    {"id", oid_i32, (uint64_t)nseq, false},
+                    {"rank", orank_i32, na, false}};
+  if (int rc = check_ints(ctx, ix, v, 3, what)) return rc;
+  bool clash = overlaps(oy_f32, oy_f32 + yn, ox_f32, ox_f32 + xn) ||
+               overlaps(oy_f32, oy_f32 + yn, oscale_f32, oscale_f32 + na) ||
+               (oy_f32 != obase_f32 && overlaps(oy_f32, oy_f32 + yn, obase_f32, obase_f32 + yn)) ||
+               share(a, oy_f32 * 4, yn * 4, w, oa * es, an * es) ||
+               share(a, oy_f32 * 4, yn * 4, w, ob * es, bn * es);
+  for (const Ints &i : v) clash = clash || share(a, oy_f32 * 4, yn * 4, ix, i.off * 4, i.count * 4);
+  if (clash) return fail(ctx, Q8_ERR_ARG, "%s: y overlaps an input (base at y itself excepted)", what);
+  if (at(w, oa * es) % 16 != 0 || at(w, ob * es) % 16 != 0 || (uint64_t)a_stride * es % 16 != 0 ||
+      (uint64_t)b_stride * es % 16 != 0)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: the adapters must start 16-byte aligned", what);
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0 || nseq == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  q8::LoraArgs p;
+  p.A = bytes(w, oa * es);
+  p.B = bytes(w, ob * es);
+  p.f32 = w_dtype == Q8_SRC_F32;
+  p.a_stride = a_stride;
+  p.b_stride = b_stride;
+  p.nadapters = nadapters;
+  p.max_rank = (int)R;
+  p.x = fptr(a, ox_f32);
+  p.base = fptr(a, obase_f32);
+  p.y = fptr(a, oy_f32);
+  p.ldx = ldx;
+  p.ldy = ldy;
+  p.in_place = oy_f32 == obase_f32;
+  p.scale = fptr(a, oscale_f32);
+  p.cu = iptr(ix, ocu_i32);
+  p.id = iptr(ix, oid_i32);
+  p.rank = iptr(ix, orank_i32);
+  p.nseq = nseq;
+  p.rows = rows;
+  p.m = m;
+  p.parts = parts;
+  p.width[0] = (int)n0;
+  p.width[1] = (int)n1;
+  p.width[2] = (int)n2;
+  p.ws = static_cast<float *>(ctx->act16);
+  const hipError_t e =
+      with_scratch(ctx, [&] { return q8::launch_lora(p, kAct16Bytes / 4, ctx->stream); });
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_lora launch");
+  return ok(ctx);
+}
+
 // ---- drawing tokens -----------------------------------------------------------------
 
 int q8_sample(q8_ctx *ctx, q8_buf *a, uint64_t ox_f32, int64_t ldx, int64_t rows, int64_t n,

@@ -130,6 +130,8 @@ SIGNATURES = {
     "q8_pages_fork": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64]),
     "q8_pages_compact": (_I, [_P, _P, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _P, _U64, _U64,
                               _I64, _U64]),
+    "q8_lora": (_I, [_P, _P, _I, _U64, _I64, _U64, _I64, _I64, _I, _P, _U64, _I64, _U64, _U64, _I64, _U64,
+                     _P, _U64, _U64, _U64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "q8_sample": (_I, [_P, _P, _U64, _I64, _I64, _I64, _U64, _P, _U64, _U64, _P, _U64]),
     "q8_graph_begin": (_I, [_P]),
     "q8_graph_end": (_I, [_P, ctypes.POINTER(_P)]),
@@ -587,6 +589,23 @@ def pages_compact(ctx: Context, ix: Buffer, otab: int, oheld: int, oref: int, ol
     ctx.check(ctx._lib.q8_pages_compact(
         ctx.h, ix.h, int(otab), int(oheld), int(oref), int(olive), int(nslots), int(maxpages),
         int(npages), pages.h, int(opages), int(page_bytes), int(layers), int(layer_stride)))
+
+
+# ---- adapters of several requests ---------------------------------------------------------
+
+def lora(ctx: Context, w: Buffer, oa: int, a_stride: int, ob: int, b_stride: int, nadapters: int,
+         max_rank: int, a: Buffer, ox: int, obase: int, oy: int, oscale: int, ix: Buffer, ocu: int,
+         oid: int, orank: int, nseq: int, rows: int, m: int, widths, dtype="bf16", ldx: int = 0,
+         ldy: int = 0) -> None:
+    """y = base + scale B (A x) with the adapter of each row's sequence; widths: the
+    columns of one to three stacked projections; adapters "bf16" or "f32": q8_lora."""
+    if not 1 <= len(widths) <= 3:
+        raise ValueError(f"lora: {len(widths)} stacked projections (1 to 3)")
+    n = [int(v) for v in widths] + [0] * (3 - len(widths))
+    ctx.check(ctx._lib.q8_lora(
+        ctx.h, w.h, dtype if isinstance(dtype, int) else ACT[dtype], int(oa), int(a_stride), int(ob),
+        int(b_stride), int(nadapters), int(max_rank), a.h, int(ox), int(ldx), int(obase), int(oy), int(ldy),
+        int(oscale), ix.h, int(ocu), int(oid), int(orank), int(nseq), int(rows), int(m), *n))
 
 
 # ---- drawing tokens ---------------------------------------------------------------------

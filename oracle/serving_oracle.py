@@ -42,3 +42,23 @@ def sample_row(x, temp=1.0, k=0, top_p=1.0, min_p=0.0, u=0.0):
     u = min(u, 1 - 2.0 ** -24) if u > 0 else 0.0
     at = min(int((c <= u * c[-1]).sum()), int((w > 0).sum()) - 1)
     return int(order[at]), float(np.log(w[at] / c[-1]))
+
+
+def lora(x, base, cu, ids, A, B, scale, widths):
+    """A[i]: the parts' [rank, m] matrices one under the other, B[i] [n, rank] (lists, by
+    adapter; None: rank 0).  (y, the sum of magnitudes behind each of its elements)."""
+    x, y = x.astype(np.float64), base.astype(np.float64).copy()
+    size = np.abs(y)
+    first = np.concatenate([[0], np.cumsum(widths)])
+    for s, i in enumerate(ids):
+        rows = slice(cu[s], cu[s + 1])
+        if not 0 <= i < len(A) or A[i] is None or cu[s + 1] <= cu[s]:
+            continue
+        a, b, r = A[i].astype(np.float64), B[i].astype(np.float64), B[i].shape[1]
+        for p in range(len(widths)):
+            ap, bp = a[p * r:(p + 1) * r], b[first[p]:first[p + 1]]
+            cols = slice(first[p], first[p + 1])
+            with np.errstate(invalid="ignore", over="ignore"):
+                y[rows, cols] += float(scale[i]) * (x[rows] @ ap.T) @ bp.T
+                size[rows, cols] += abs(float(scale[i])) * (np.abs(x[rows]) @ np.abs(ap).T) @ np.abs(bp).T
+    return y, size

@@ -4,7 +4,8 @@ what each refuses and with which status; valid calls reach the device step."""
 import pytest
 
 from lama32_mojo_amd import q8hip
-from lama32_mojo_amd.q8hip import (Q8_ERR_ARG, Q8_ERR_NODEVICE, Q8_ERR_RANGE, Q8_ERR_SHAPE, Q8Error)
+from lama32_mojo_amd.q8hip import (Q8_ERR_ARG, Q8_ERR_NODEVICE, Q8_ERR_RANGE, Q8_ERR_SHAPE,
+                                   Q8_ERR_UNSUPPORTED, Q8Error)
 
 
 @pytest.fixture
@@ -40,3 +41,31 @@ def test_sample(hctx):
     rc = hctx._lib.q8_sample(hctx.h, None, 0, 0, R, n, 0, ids.h, 0, R, None, 0)
     assert rc == Q8_ERR_ARG
     assert hctx._lib.q8_sample(None, a.h, 0, 0, R, n, R * n, ids.h, 0, R, None, 0) == Q8_ERR_ARG
+
+
+def test_lora(hctx):
+    T, m, na, R, widths = 9, 64, 3, 16, [40, 8]
+    n = sum(widths)
+    sa, sb = 2 * R * m, n * R
+    a, w, ix = hctx.alloc(4 * (T * (m + 2 * n) + na)), hctx.alloc(2 * na * (sa + sb)), hctx.alloc(4 * (4 + 3 + na))
+
+    def call(oa=0, sa=sa, ob=na * sa, sb=sb, na=na, R=R, ox=0, obase=T * m, oy=T * (m + n), osc=T * (m + 2 * n),
+             ocu=0, oid=4, orank=7, nseq=3, rows=T, m=m, widths=widths, dtype="bf16", ldx=0, ldy=0, w=w, a=a):
+        return code(q8hip.lora, hctx, w, oa, sa, ob, sb, na, R, a, ox, obase, oy, osc, ix, ocu, oid, orank, nseq, rows,
+                    m, widths, dtype, ldx, ldy)
+    assert call() == call(obase=T * (m + n)) == call(rows=0) == call(nseq=0) == call(R=13) == Q8_ERR_NODEVICE
+    assert call(dtype=3) == Q8_ERR_ARG
+    assert call(m=60) == call(m=0) == call(na=0) == call(R=0) == call(widths=[0]) == Q8_ERR_SHAPE
+    assert call(widths=[40, 0, 8]) == call(sa=sa - 8) == call(sb=sb - 8) == call(rows=-1) == Q8_ERR_SHAPE
+    assert call(R=24) == call(ldx=m - 1) == call(ldy=n - 1) == call(widths=[40, 16]) == Q8_ERR_SHAPE
+    assert call(R=257) == call(na=4097) == call(nseq=4097) == Q8_ERR_UNSUPPORTED
+    assert call(dtype="f32") == call(na=4) == call(ob=na * sa + 8) == call(oa=1 << 62) == Q8_ERR_RANGE
+    assert call(osc=T * (m + 2 * n) + 1) == call(rows=10) == call(ldx=m + 300) == call(ldy=n + 9) == Q8_ERR_RANGE
+    assert call(orank=8) == call(nseq=7) == call(ocu=9) == Q8_ERR_RANGE
+    assert call(oy=0) == call(ldx=m + 100) == call(oy=T * m + 1) == call(oy=T * (m + n) - n) == Q8_ERR_ARG
+    small = hctx.alloc(2 * na * (sa + sb) + 4)
+    assert call(oa=1, w=small, ob=na * sa + 2) == call(ob=na * sa + 1, w=small) == Q8_ERR_UNSUPPORTED
+    with pytest.raises(ValueError):
+        call(widths=[8, 8, 8, 8])
+    with pytest.raises(ValueError):
+        call(widths=[])
