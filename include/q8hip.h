@@ -475,6 +475,35 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
                      uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
                      int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim);
 
+/* Sequences that name the same pages for their first tokens (forks of one prompt):
+ * q8_kv8_share finds them from the tables, once a step, and q8_kv8_attention_shared
+ * reads those tokens once for all of them, in every layer.  (No counterpart in the
+ * reference.)
+ *
+ * q8_kv8_share_ints: the int32 that what is shared takes (0 for sizes that are not
+ * supported: up to 1024 sequences, 2^22 rows).
+ * q8_kv8_share: sequences with rows whose tables begin with the same page are led by
+ * the first of them; of the counts p of whole pages of cached tokens, the one that
+ * saves the most reads, (members with p such pages in common with the leader - 1) * p,
+ * is shared by those members, the longest of equal ones (of at most 64 groups, the ones
+ * with the lowest leaders).  Written at oshare of ix: the
+ * number of groups; group [nseq] of each sequence (numbered by leader, -1: none);
+ * tokens [nseq] that it shares; and lists for the attention.  What is shared belongs
+ * to the cu, len and table that it was found from: find it again when they change.
+ * q8_kv8_attention_shared: as q8_kv8_attention of the same arrays, within the same
+ * bounds.  Sequences without a group are served as there.  The context's scratch
+ * is used; where the rows of a call leave no room for the groups' records
+ * there (some 1500 rows of 32 heads of 128), each sequence reads its own tokens. */
+uint64_t q8_kv8_share_ints(int64_t nseq, int64_t rows);
+int q8_kv8_share(q8_ctx *ctx, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32,
+                 int64_t nseq, int64_t rows, int64_t maxpages, int64_t npages, int page,
+                 uint64_t oshare_i32);
+int q8_kv8_attention_shared(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
+                            q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+                            uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
+                            int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim,
+                            uint64_t oshare_i32);
+
 /* Pages.  The state of nslots slots (sequences) over a pool of npages pages is
  * four int32 arrays of `ix`: table [nslots][maxpages], -1 behind the held pages;
  * len [nslots] tokens; held [nslots] pages; ref [npages], the table entries that

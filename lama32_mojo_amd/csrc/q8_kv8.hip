@@ -417,10 +417,38 @@ template <int HD> __device__ __forceinline__ float kv8_exact_up_to() {
 // tiles), pre[0] = 0 .. pre[nseq], and their first rows, row counts and cached
 // tokens; all NT threads.
 struct Kv8Plan {
-  int *pre, *row0, *n, *old;
+  int *pre, *row0, *n, *old, *k0;
 };
-template <bool WHOLE, int NT>
-__device__ __forceinline__ int kv8_plan(const Kv8Args &c, int cols, const Kv8Plan &pl, int *wsum) {
+
+// What q8_kv8_share found: the group of each sequence (-1: none), the tokens that it
+// takes from the group, the place of its first row in the list of rows; the groups'
+// leaders and the places of their rows; the list.  Read as if it could hold anything.
+struct Kv8ShareAt {
+  const int *group, *tok, *pos, *lead, *gcu, *row;
+  int groups;
+};
+Q8_HD int kv8_most_groups(int64_t nseq, int64_t rows) {
+  const int64_t n = (nseq < rows ? nseq : rows) / 2;
+  return (int)(n < kKv8ShareGroups ? n : kKv8ShareGroups);
+}
+__device__ __forceinline__ Kv8ShareAt kv8_share_at(const Kv8Args &c, const int *p) {
+  const int nseq = (int)c.nseq;
+  return {p + 1,         p + 1 + nseq,          p + 1 + 2 * nseq,     p + 1 + 3 * nseq,
+          p + 1 + 4 * nseq, p + 2 + 5 * (int64_t)nseq, clamp_i(p[0], 0, kv8_most_groups(c.nseq, c.rows))};
+}
+// Tokens of sequence i that its group's part of the attention covers, whole pages.
+__device__ __forceinline__ int kv8_shared_tokens(const Kv8Args &c, const Kv8ShareAt &sh, int i) {
+  const int g = sh.group[i];
+  return g >= 0 && g < sh.groups ? clamp_i(sh.tok[i], 0, c.maxpages * c.page) & ~(c.page - 1) : 0;
+}
+
+// What of a sequence a launch goes through: all its keys, the ones behind the shared
+// tokens, or (a group's rows) the shared ones.
+enum { KV8_ALL = 0, KV8_OWN = 1, KV8_SHARED = 2 };
+
+template <bool WHOLE, int NT, int PART>
+__device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, int cols, const Kv8Plan &pl,
+                                        int *wsum) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, nseq = (int)c.nseq;
   const int grp = c.nheads / c.nkv;
   int base = 0;
@@ -430,7 +458,12 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &c, int cols, const Kv8Pla
     int u = 0;
     if (i < nseq) {
       const int a = c.cu[i];
-      const Kv8Seq s = kv8_seq(a, c.cu[i + 1], c.len[i], c.rows, c.maxpages * c.page, grp, cols);
+      Kv8Seq s = kv8_seq(a, c.cu[i + 1], c.len[i], c.rows, c.maxpages * c.page, grp, cols);
+      if (PART == KV8_OWN) {
+        const int k0 = kv8_shared_tokens(c, kv8_share_at(c, share), i);
+        kv8_from(s, k0, c.maxpages * c.page);
+        pl.k0[i] = k0;
+      }
       u = WHOLE ? s.row_tiles : kv8_units_of(s);
       pl.row0[i] = clamp_i(a, 0, c.rows);
       pl.n[i] = s.n;
@@ -493,14 +526,71 @@ __device__ __forceinline__ int *kv8_plan_at(const Kv8AttnArgs &a, int runs) {
 struct Kv8Place {
   int u, i, rt, kt, t0, t1, units;       // units: the row tile's
   int ctx;                               // keys its last row sees
+  int k0;                                // the first unit's first key
 };
+
+// The groups' part: a block goes through `per` units at most of one row tile of a
+// group, cut so that about a.shared_target blocks have work.  base[g] .. base[g+1]:
+// the blocks of group g, its tiles' cuts one after the other; base has groups + 1
+// entries in LDS.  Returns per.
+__device__ __forceinline__ void kv8_group(const Kv8Args &c, const Kv8ShareAt &sh, int g, int cols, int *n,
+                                          int *tiles, int *units) {
+  const int lead = clamp_i(sh.lead[g], 0, c.nseq - 1);
+  const int a = clamp_i(sh.gcu[g], 0, c.rows), b = clamp_i(sh.gcu[g + 1], 0, c.rows);
+  *n = b > a ? b - a : 0;
+  *tiles = (int)(((int64_t)*n * (c.nheads / c.nkv) + cols - 1) / cols);
+  *units = (kv8_shared_tokens(c, sh, lead) + kKv8Unit - 1) / kKv8Unit;
+}
+template <int NT>
+__device__ __forceinline__ int kv8_group_plan(const Kv8Args &c, const Kv8ShareAt &sh, int cols, int target,
+                                              int *base, int *wsum) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  int per = 1;
+  if (t == 0) base[0] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {   // the units of all, then the blocks of each
+    int sum = 0;
+    for (int g0 = 0; g0 < sh.groups; g0 += NT) {
+      const int g = g0 + t;
+      int u = 0;
+      if (g < sh.groups) {
+        int n, tiles, units;
+        kv8_group(c, sh, g, cols, &n, &tiles, &units);
+        const int64_t v = (int64_t)tiles * (pass ? (units + per - 1) / per : units);
+        u = v < kKv8MaxUnits ? (int)v : kKv8MaxUnits;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(u, d);
+        if (lane >= d) u = kv8_add(u, o);
+      }
+      if (lane == 63) wsum[w] = u;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int x = 0; x < NT / 64; ++x) {
+        u = kv8_add(u, x < w ? wsum[x] : 0);
+        all = kv8_add(all, wsum[x]);
+      }
+      if (pass && g < sh.groups) base[g + 1] = kv8_add(sum, u);
+      sum = kv8_add(sum, all);
+      __syncthreads();
+    }
+    if (pass == 0) per = kv8_units_per_block(sum, target, 1);
+  }
+  __syncthreads();                        // (base, also where there are no groups)
+  return per;
+}
+constexpr int kKv8SharedCols = 64;       // columns of a group's row tile
 
 //
 // WIDE (pages of 128 tokens, runs): a V column of a page is one 128-byte line,
 // of which a unit takes half.  The even unit's load brings the odd unit's half
 // into registers too; fetched a unit later, the line had left the L2 by then
 // (4 contexts of up to 131000 tokens 142 -> 128 us).
-template <int HD, int MT, bool WHOLE, bool WIDE>
+// PART: see above.  KV8_SHARED's columns are (row of the group, query head), its rows
+// from the list, and all see all keys; it leaves one record a block.
+template <int HD, int MT, bool WHOLE, bool WIDE, int PART>
 __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kernel(Kv8AttnArgs a) {
   constexpr int DT = HD / 16, HH = HD / 64, NC = 16 * MT, NW = WHOLE ? 8 : kKv8Waves;
   constexpr int RW = NW / MT;             // runs of a block
@@ -527,12 +617,25 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   pl.row0 = pl.pre + nseq + 1;
   pl.n = pl.row0 + nseq;
   pl.old = pl.n + nseq;
+  pl.k0 = pl.old + nseq;
 
-  const int units = kv8_plan<WHOLE, 64 * NW>(c, NC, pl, wsum);
+  Kv8ShareAt sh;
+  if constexpr (PART != KV8_ALL) sh = kv8_share_at(c, a.share);
+  int units, shared_per = 0;
+  if constexpr (PART == KV8_SHARED) {
+    shared_per = kv8_group_plan<64 * NW>(c, sh, NC, a.shared_target, pl.pre, wsum);
+    units = pl.pre[sh.groups];
+    if (blockIdx.x == 0 && g == 0) {       // the join reads the plan
+      for (int i = t; i <= sh.groups; i += 64 * NW) a.shared_plan[1 + i] = pl.pre[i];
+      if (t == 0) a.shared_plan[0] = shared_per;
+    }
+  } else {
+    units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, NC, pl, wsum);
+  }
   const int runs = gridDim.x * RW, run = blockIdx.x * RW + w;
-  const int per = WHOLE ? 1 : kv8_units_per_block(units, runs, 1);
+  const int per = WHOLE || PART == KV8_SHARED ? 1 : kv8_units_per_block(units, runs, 1);
   // the merge reads the plan behind the records
-  if (!WHOLE && blockIdx.x == 0 && g == 0)
+  if (!WHOLE && PART != KV8_SHARED && blockIdx.x == 0 && g == 0)
     for (int i = t; i <= nseq; i += 64 * NW) kv8_plan_at<HD, NC>(a, runs)[i] = pl.pre[i];
   const int u0 = WHOLE ? (int)blockIdx.x : run * per;
   const int uend = WHOLE ? min((int)blockIdx.x + 1, units) : min(u0 + per, units);
@@ -541,9 +644,23 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   // the place of unit u, in sequence i or behind it
   auto place = [&](int u, int i) {
     Kv8Place p;
+    if constexpr (PART == KV8_SHARED) {
+      int n, tiles;
+      kv8_group(c, sh, i, NC, &n, &tiles, &p.units);
+      const int cuts = max(1, (p.units + shared_per - 1) / shared_per);
+      p.u = u;
+      p.i = i;
+      p.k0 = 0;
+      p.ctx = kv8_shared_tokens(c, sh, clamp_i(sh.lead[i], 0, nseq - 1));
+      p.rt = (u - pl.pre[i]) / cuts;
+      p.t0 = p.kt = (u - pl.pre[i]) % cuts * shared_per;
+      p.t1 = min(p.units, p.t0 + shared_per);
+      return p;
+    }
     while (pl.pre[i + 1] <= u) ++i;
     const int local = u - pl.pre[i], ctx = min(pl.old[i] + pl.n[i], cap);
-    p.units = (ctx + kKv8Unit - 1) / kKv8Unit;
+    p.k0 = PART == KV8_OWN ? pl.k0[i] : 0;
+    p.units = (ctx - p.k0 + kKv8Unit - 1) / kKv8Unit;
     p.u = u;
     p.i = i;
     p.ctx = ctx;
@@ -561,14 +678,15 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   int idk = 0, idv = 0;
   bool second = false;                    // vr2 holds the V of the unit loaded next
   const int step = WHOLE ? RW : 1;
-  Kv8Place nx = place(u0, kv8_seq_of(pl.pre, nseq, u0));
+  Kv8Place nx = place(u0, kv8_seq_of(pl.pre, PART == KV8_SHARED ? sh.groups : nseq, u0));
   Kv8Place cu = nx;
   if (WHOLE) nx.kt = w;
   auto have = [&]() { return nx.kt < nx.t1; };
   auto load_ids = [&]() {
     if (!have()) return;
-    const int *tab = c.tab + (int64_t)nx.i * c.maxpages;
-    const int kk = nx.kt * kKv8Unit + 16 * (col >> 2), kv = nx.kt * kKv8Unit + 16 * g4;
+    const int *tab =
+        c.tab + (int64_t)(PART == KV8_SHARED ? clamp_i(sh.lead[nx.i], 0, nseq - 1) : nx.i) * c.maxpages;
+    const int kk = nx.k0 + nx.kt * kKv8Unit + 16 * (col >> 2), kv = nx.k0 + nx.kt * kKv8Unit + 16 * g4;
     idk = kk < nx.ctx ? tab[kk >> psh] : 0;
     idv = kv < nx.ctx ? tab[kv >> psh] : 0;
   };
@@ -576,7 +694,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     if (!have()) return;
     const int id = page_or_none(idk, (int)c.npages);
     const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
-                       (int64_t)(((nx.kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD +
+                       (int64_t)(((nx.k0 + nx.kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD +
                        16 * g4;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
@@ -597,7 +715,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     const float *sc = reinterpret_cast<const float *>(base + scales_at);
     ks = id < 0 ? __builtin_nanf("") : sc[g];
     vs = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
-    const uint8_t *p = base + v_at + (int64_t)col * P + ((nx.kt * kKv8Unit + 16 * g4) & (P - 1));
+    const uint8_t *p = base + v_at + (int64_t)col * P + ((nx.k0 + nx.kt * kKv8Unit + 16 * g4) & (P - 1));
     // non-temporal where a load takes whole lines (64 sequences, pages of 64
     // tokens, 71 -> 67 us; with WIDE's two loads a line 124 -> 132)
 #pragma unroll
@@ -614,7 +732,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   };
   auto advance = [&]() {
     nx.kt += step;
-    if (WHOLE || nx.kt < nx.t1) return;
+    if (WHOLE || PART == KV8_SHARED || nx.kt < nx.t1) return;
     const int u = nx.u + (nx.t1 - nx.t0);
     if (u < uend) nx = place(u, nx.i);
   };
@@ -622,7 +740,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   // row's), from dim 16 g4 on
   auto q_at = [&](const Kv8Place &p, int row0, int n) {
     const int lin = p.rt * NC + cc, j = lin / grp;
-    return a.q + (int64_t)(row0 + (j < n ? j : 0)) * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
+    int64_t row = row0 + (j < n ? j : 0);
+    if constexpr (PART == KV8_SHARED) row = clamp_i(sh.row[row], 0, c.rows - 1);
+    return a.q + row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
   };
   load_ids();
   load_k();
@@ -631,11 +751,18 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   load_ids();
 
   for (;;) {                              // row tiles of the run
-    const int row0 = pl.row0[cu.i], n = pl.n[cu.i], old = pl.old[cu.i];
+    int row0, n, old = 0;
+    if constexpr (PART == KV8_SHARED) {
+      int tiles, units;
+      kv8_group(c, sh, cu.i, NC, &n, &tiles, &units);
+      row0 = clamp_i(sh.gcu[cu.i], 0, c.rows);
+    } else {
+      row0 = pl.row0[cu.i], n = pl.n[cu.i], old = pl.old[cu.i];
+    }
     // ---- this lane's digits of q: column col, dims 64 h + 16 g4 ..; the keys
     // its columns see: 0 .. kend-1 (0: no such column)
     const int lin = cu.rt * NC + cc, j = lin / grp;
-    const int kend = j < n ? min(old + j + 1, cap) : 0;
+    const int kend = j < n ? (PART == KV8_SHARED ? cu.ctx : min(old + j + 1, cap)) : 0;
     int kmin = j < n ? kend : INT32_MAX;
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) kmin = min(kmin, __shfl_xor(kmin, d));
@@ -734,8 +861,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
         }
       }
       load_k();
-      const int key0 = kt * kKv8Unit + 16 * g4;
-      const bool masked = kt * kKv8Unit + kKv8Unit > kmin;
+      const int key0 = cu.k0 + kt * kKv8Unit + 16 * g4;
+      const bool masked = cu.k0 + kt * kKv8Unit + kKv8Unit > kmin;
       float tmax = -INFINITY;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
@@ -826,6 +953,18 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
       }
       if (w != 0) return;
     }
+    if constexpr (PART == KV8_SHARED) {
+      if (j < n) {
+        float *rec = a.shared_rec + ((int64_t)blockIdx.x * c.nkv + g) * kv8_record<HD, NC>();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(rec + cc * HD + 16 * d + 4 * g4) = o[d];
+        if (g4 == 0) {
+          rec[NC * HD + cc] = m;
+          rec[NC * HD + NC + cc] = l;
+        }
+      }
+      return;
+    }
     if (j < n) {
       const bool whole = WHOLE || (cu.t0 == 0 && cu.t1 == cu.units);
       float *rec = a.ws + (((int64_t)run * c.nkv + g) * 2 + (cu.t0 == 0)) * kv8_record<HD, NC>();
@@ -838,6 +977,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
         rec[NC * HD + cc] = m;
         rec[NC * HD + NC + cc] = l;
       }
+      if (PART == KV8_OWN && whole && g4 == 0) {      // (for the join with the group's part)
+        float *ml = a.ml + 2 * ((int64_t)(row0 + j) * c.nheads + g * grp + lin % grp);
+        ml[0] = m;
+        ml[1] = l;
+      }
     }
     const int u = cu.u + (cu.t1 - cu.t0);
     if (WHOLE || u >= uend) return;
@@ -848,7 +992,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
 // Joins the records of the row tiles that several runs served: grid
 // (rows, nkv, heads of a group / hb).  The block's threads are groups over hb
 // heads x HD / 4 dims; the groups take the records in turn and meet in LDS.
-template <int HD, int MT>
+// PART KV8_OWN: also joins the group's records (and the output as it stands, where
+// one run served the row).
+template <int HD, int MT, int PART>
 __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs, int hb) {
   constexpr int NC = 16 * MT, NT = 512;
   __shared__ __attribute__((aligned(16))) float so[NT * 4];
@@ -861,7 +1007,25 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   // the sequence of this row: the last one that begins at it or before
   const SeqAt at = find_seq(c.cu, c.len, nseq, c.rows, row, 1, 0);
   const int lo = at.i, j = row - at.r0;
-  const Kv8Seq sq = kv8_seq(at.r0, at.r1, at.len, c.rows, c.maxpages * c.page, grp, NC);
+  Kv8Seq sq = kv8_seq(at.r0, at.r1, at.len, c.rows, c.maxpages * c.page, grp, NC);
+  // the group's records of this row: cuts of them, from block `cut0` on
+  Kv8ShareAt sh;
+  int group = -1, cuts = 0, cut0 = 0, place = 0;
+  if constexpr (PART == KV8_OWN) {
+    sh = kv8_share_at(c, a.share);
+    const int k0 = kv8_shared_tokens(c, sh, lo);
+    kv8_from(sq, k0, c.maxpages * c.page);
+    group = sh.group[lo];
+    if (group < 0 || group >= sh.groups) group = -1;
+    if (group >= 0) {
+      int n, tiles, units;
+      kv8_group(c, sh, group, kKv8SharedCols, &n, &tiles, &units);
+      const int sper = max(1, a.shared_plan[0]);
+      cuts = (units + sper - 1) / sper;
+      cut0 = a.shared_plan[1 + group];
+      place = clamp_i((int64_t)sh.pos[lo] + j - clamp_i(sh.gcu[group], 0, c.rows), 0, max(0, n - 1));
+    }
+  }
   if (j < 0 || j >= sq.n) return;             // behind the last sequence
   constexpr int IPH = HD / 4;
   const int sg = NT / (hb * IPH);             // groups of threads
@@ -874,8 +1038,40 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
     const int b1 = clamp_i((ua + sq.key_units - 1) / per, 0, runs - 1);
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool on = grp_id < sg && hh < grp && b0 != b1;   // (b0 == b1: written whole)
-    for (int z0 = b0 + grp_id; on && z0 <= b1; z0 += 4 * sg) {
+    // (b0 == b1: written whole)
+    const bool on = grp_id < sg && hh < grp && (b0 != b1 || (PART == KV8_OWN && group >= 0));
+    if constexpr (PART == KV8_OWN) {
+      if (on && group >= 0) {
+        // the group's cuts, then the row's own run where it has one
+        const int slin = place * grp + hh, cols = kKv8SharedCols;
+        const int64_t first = (int64_t)cut0 + (int64_t)(slin / cols) * cuts;
+        const int all = cuts + (b0 == b1 && sq.key_units > 0);
+        for (int z = grp_id; z < all; z += sg) {
+          float zm, zl, w = 1.0f;
+          const float *src;
+          if (z < cuts) {
+            const int64_t b = min(first + z, (int64_t)a.shared_blocks - 1);
+            const float *r = a.shared_rec + (b * c.nkv + g) * kv8_record<HD, kKv8SharedCols>();
+            zm = r[cols * HD + slin % cols];
+            zl = r[cols * HD + cols + slin % cols];
+            src = r + slin % cols * HD + d;
+          } else {
+            const int64_t h = (int64_t)row * c.nheads + g * grp + hh;
+            zm = a.ml[2 * h];
+            w = zl = a.ml[2 * h + 1];
+            src = a.out + h * HD + d;
+          }
+          const f32x4 zo = *reinterpret_cast<const f32x4_u *>(src);
+          const float mx = fmaxf(m, zm), ms = mx == -INFINITY ? 0.0f : mx;
+          const float f0 = __builtin_amdgcn_exp2f(m - ms), f = __builtin_amdgcn_exp2f(zm - ms);
+          l = __builtin_fmaf(f, zl, l * f0);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(f * w, zo[v], o[v] * f0);
+          m = mx;
+        }
+      }
+    }
+    for (int z0 = b0 + grp_id; on && b0 != b1 && z0 <= b1; z0 += 4 * sg) {
       float zm[4], zl[4];
       f32x4 zo[4];
 #pragma unroll
@@ -926,19 +1122,19 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   }
 }
 
-template <int HD, int MT>
+template <int HD, int MT, int PART>
 hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
   constexpr int NC = 16 * MT, RW = kKv8Waves / MT;
   const Kv8Args &c = a.c;
   const int grp = c.nheads / c.nkv;
-  const size_t plan = (size_t)(4 * c.nseq + 1) * 4;
+  const size_t plan = (size_t)((PART == KV8_OWN ? 5 : 4) * c.nseq + 1) * 4;
   // a sequence of n rows has ceil(n grp / NC) row tiles: no more than each row alone
   // would, nor than n grp / NC and one
   const int64_t tiles = std::min(c.rows * ((grp + NC - 1) / NC), c.rows * grp / NC + c.nseq);
   const int64_t key_units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit;
-  if (key_units <= kKv8WholeUnits && tiles * c.nkv <= kKv8WholeBlocks) {
+  if (PART == KV8_ALL && key_units <= kKv8WholeUnits && tiles * c.nkv <= kKv8WholeBlocks) {
     const size_t lds = (size_t)(8 / MT / 2) * NC * (HD + 4) * 4 + plan;
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, true, false>), dim3((unsigned)tiles, (unsigned)c.nkv),
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, true, false, KV8_ALL>), dim3((unsigned)tiles, (unsigned)c.nkv),
                        dim3(512), lds, st, a);
     return hipGetLastError();
   }
@@ -950,15 +1146,15 @@ hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
   if (nb < 1) return hipErrorInvalidValue;
   const dim3 grid((unsigned)nb, (unsigned)c.nkv), block(64 * kKv8Waves);
   if (c.page == 128)
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, true>), grid, block, plan, st, a);
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, true, PART>), grid, block, plan, st, a);
   else
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, false>), grid, block, plan, st, a);
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, false, PART>), grid, block, plan, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   // few rows: more blocks, with more groups of threads over a row's records
   int hb = std::min(grp, 512 / (HD / 4));
   while (hb > 1 && c.rows * c.nkv * ((grp + hb - 1) / hb) < 256) hb = (hb + 1) / 2;
-  hipLaunchKernelGGL((kv8_merge_kernel<HD, MT>),
+  hipLaunchKernelGGL((kv8_merge_kernel<HD, MT, PART>),
                      dim3((unsigned)c.rows, (unsigned)c.nkv, (unsigned)((grp + hb - 1) / hb)),
                      dim3(512), 0, st, a, (int)(nb * RW), hb);
   return hipGetLastError();
@@ -984,7 +1180,8 @@ hipError_t launch_kv8_append(const Kv8AppendArgs &a, hipStream_t st) {
 
 template <int MT>
 static hipError_t launch_kv8_cols(const Kv8AttnArgs &a, hipStream_t st) {
-  return a.c.head_dim == 64 ? launch_kv8_attn_t<64, MT>(a, st) : launch_kv8_attn_t<128, MT>(a, st);
+  return a.c.head_dim == 64 ? launch_kv8_attn_t<64, MT, KV8_ALL>(a, st)
+                            : launch_kv8_attn_t<128, MT, KV8_ALL>(a, st);
 }
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
@@ -1003,6 +1200,46 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+// The groups' part (a row tile of 64 columns cut over blocks), each sequence's own
+// part, and the merge that joins them.
+template <int HD>
+static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
+  const Kv8Args &c = a.c;
+  const int64_t grp = c.nheads / c.nkv, cols = c.rows * grp;
+  const int64_t groups = kv8_most_groups(c.nseq, c.rows);
+  const int64_t tiles = cols / kKv8SharedCols + groups, rec = c.nkv * kv8_record<HD, kKv8SharedCols>();
+  // maxima and sums per (row, head), the groups' plan and records (three quarters of
+  // the space at most), then what the sequences' own parts leave
+  const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4, plan = (groups + 5) / 4 * 4;
+  const int64_t room = (a.ws_floats / 4 * 3 - ml - plan) / rec;
+  const int64_t want = (512 + c.nkv - 1) / c.nkv;
+  a.shared_target = (int)std::min(want, room - tiles);
+  // (more rows than there is room for: every sequence for itself)
+  if (a.shared_target < std::min<int64_t>(want, 8) || groups == 0) return launch_kv8_attention(a, st);
+  const int64_t blocks = a.shared_target + tiles, recs = blocks * rec;
+  a.ml = a.ws;
+  a.shared_plan = reinterpret_cast<int *>(a.ws + ml);
+  a.shared_rec = a.ws + ml + plan;
+  a.shared_blocks = (int)blocks;
+  a.ws += ml + plan + recs;
+  a.ws_floats -= ml + plan + recs;
+  const dim3 grid((unsigned)blocks, (unsigned)c.nkv), block(64 * kKv8Waves);
+  const size_t lds = (size_t)(groups + 1) * 4;
+  if (c.page == 128)
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, 4, false, true, KV8_SHARED>), grid, block, lds, st, a);
+  else
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, 4, false, false, KV8_SHARED>), grid, block, lds, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  return cols <= 16 * c.nseq   ? launch_kv8_attn_t<HD, 1, KV8_OWN>(a, st)
+         : cols <= 32 * c.nseq ? launch_kv8_attn_t<HD, 2, KV8_OWN>(a, st)
+                               : launch_kv8_attn_t<HD, 4, KV8_OWN>(a, st);
+}
+
+hipError_t launch_kv8_attention_shared(const Kv8AttnArgs &a, hipStream_t st) {
+  return a.c.head_dim == 64 ? launch_kv8_shared_t<64>(a, st) : launch_kv8_shared_t<128>(a, st);
 }
 
 }  // namespace q8

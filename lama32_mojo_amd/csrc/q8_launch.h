@@ -291,10 +291,23 @@ struct Kv8AttnArgs {
   float *out;              // [rows, nheads * head_dim]
   float *ws;               // split records, 16-byte aligned
   int64_t ws_floats;
+  // shared prefixes: what q8_kv8_share wrote; the others are set by the launch
+  const int *share;
+  float *ml, *shared_rec;
+  int *shared_plan;
+  int shared_target, shared_blocks;
 };
 // Sequences of one call: their unit counts are summed in LDS.
 constexpr int kKv8MaxSeq = 4096;
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st);
+// Sequences of a call that shares prefixes (the plan of a call in LDS).
+constexpr int kKv8ShareSeq = 1024;
+// Groups of a call: their row tiles need records, whose number the host bounds.
+constexpr int kKv8ShareGroups = 64;
+inline int64_t kv8_share_ints(int64_t nseq, int64_t rows) { return 5 * nseq + 2 + rows; }
+hipError_t launch_kv8_attention_shared(const Kv8AttnArgs &a, hipStream_t st);
+// (of c: the int32 arrays, their sizes, npages and page)
+hipError_t launch_kv8_share(const Kv8Args &c, int *share, hipStream_t st);
 
 struct PagesArgs {
   int *tab, *len, *held, *ref;   // [nslots][maxpages], [nslots], [nslots], [npages]

@@ -65,6 +65,11 @@ Q8_HD Kv8Seq kv8_seq(int cu0, int cu1, int len, int64_t rows, int64_t cap, int g
   s.key_units = s.n ? (int)((ctx + kKv8Unit - 1) / kKv8Unit) : 0;
   return s;
 }
+// The same for the keys from k0 on.
+Q8_HD void kv8_from(Kv8Seq &s, int k0, int64_t cap) {
+  const int64_t ctx = (int64_t)s.old + s.n < cap ? (int64_t)s.old + s.n : cap;
+  s.key_units = s.n && ctx > k0 ? (int)((ctx - k0 + kKv8Unit - 1) / kKv8Unit) : 0;
+}
 // The unit counts are summed up to this (arrays that hold nonsense cannot make
 // them overflow; a call that could reach it is refused).
 constexpr int kKv8MaxUnits = 1 << 30;

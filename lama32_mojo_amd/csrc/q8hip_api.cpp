@@ -1865,11 +1865,14 @@ int q8_kv8_append(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, uint64_t ok_f32, uint
   return ok(ctx);
 }
 
-int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
-                     q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
-                     uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
-                     int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim) {
-  const char *what = "q8_kv8_attention";
+namespace {
+
+// q8_kv8_attention and, with `shared`, q8_kv8_attention_shared.
+int run_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32, q8_buf *pages,
+                      uint64_t opages, int64_t npages, int page, q8_buf *ix, uint64_t ocu_i32,
+                      uint64_t olen_i32, uint64_t otab_i32, int64_t nseq, int64_t rows, int64_t maxpages,
+                      int nheads, int nkv, int head_dim, bool shared, uint64_t oshare_i32,
+                      const char *what) {
   if (int rc = check_ctx(ctx)) return rc;
   if (!a) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
   q8::Kv8AttnArgs p;
@@ -1892,6 +1895,14 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
     return fail(ctx, Q8_ERR_SHAPE, "%s: %lld rows over %lld pages each are too many for one call", what,
                 (long long)rows, (long long)maxpages);
   const uint64_t qspan = rows_span(rows, ldq, (uint64_t)qdim), on = (uint64_t)rows * (uint64_t)qdim;
+  const uint64_t sn = shared ? (uint64_t)q8::kv8_share_ints(nseq, rows) : 0;
+  if (shared) {
+    if (nseq > q8::kKv8ShareSeq)
+      return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nseq=%lld (at most %d sequences that share)", what,
+                  (long long)nseq, q8::kKv8ShareSeq);
+    const Ints v[] = {{"what is shared", oshare_i32, sn, false}};
+    if (int rc = check_ints(ctx, ix, v, 1, what)) return rc;
+  }
   if (int rc = check_f32(ctx, a, oq_f32, qspan, what, "q")) return rc;
   if (int rc = check_f32(ctx, a, oy_f32, on, what, "out")) return rc;
   const uint64_t pn = (uint64_t)npages * (uint64_t)q8::kv8_page_bytes(page, nkv, head_dim);
@@ -1899,7 +1910,8 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
       share(a, oy_f32 * 4, on * 4, pages, opages, pn) ||
       share(a, oy_f32 * 4, on * 4, ix, ocu_i32 * 4, ((uint64_t)nseq + 1) * 4) ||
       share(a, oy_f32 * 4, on * 4, ix, olen_i32 * 4, (uint64_t)nseq * 4) ||
-      share(a, oy_f32 * 4, on * 4, ix, otab_i32 * 4, (uint64_t)nseq * (uint64_t)maxpages * 4))
+      share(a, oy_f32 * 4, on * 4, ix, otab_i32 * 4, (uint64_t)nseq * (uint64_t)maxpages * 4) ||
+      share(a, oy_f32 * 4, on * 4, ix, oshare_i32 * 4, sn * 4))
     return fail(ctx, Q8_ERR_ARG, "%s: out overlaps an input", what);
   if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
   if (rows == 0 || nseq == 0) return ok(ctx);
@@ -1909,10 +1921,79 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
   p.out = fptr(a, oy_f32);
   p.ws = static_cast<float *>(ctx->act16);
   p.ws_floats = kAct16Bytes / 4;
-  const hipError_t e = with_scratch(ctx, [&] { return q8::launch_kv8_attention(p, ctx->stream); });
-  if (e != hipSuccess) return hip_fail(ctx, e, "q8_kv8_attention launch");
+  p.share = shared ? iptr(ix, oshare_i32) : nullptr;
+  const hipError_t e = with_scratch(ctx, [&] {
+    return shared ? q8::launch_kv8_attention_shared(p, ctx->stream)
+                  : q8::launch_kv8_attention(p, ctx->stream);
+  });
+  if (e != hipSuccess) return hip_fail(ctx, e, what);
   return ok(ctx);
 }
+
+}  // namespace
+
+int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
+                     q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+                     uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
+                     int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim) {
+  return run_kv8_attention(ctx, a, oq_f32, ldq, oy_f32, pages, opages, npages, page, ix, ocu_i32,
+                           olen_i32, otab_i32, nseq, rows, maxpages, nheads, nkv, head_dim, false, 0,
+                           "q8_kv8_attention");
+}
+
+uint64_t q8_kv8_share_ints(int64_t nseq, int64_t rows) {
+  if (nseq < 0 || nseq > q8::kKv8ShareSeq || rows < 0 || rows > (1 << 22)) return 0;
+  return (uint64_t)q8::kv8_share_ints(nseq, rows);
+}
+
+int q8_kv8_share(q8_ctx *ctx, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32,
+                 int64_t nseq, int64_t rows, int64_t maxpages, int64_t npages, int page,
+                 uint64_t oshare_i32) {
+  const char *what = "q8_kv8_share";
+  if (int rc = check_ctx(ctx)) return rc;
+  if (!ix) return fail(ctx, Q8_ERR_ARG, "%s: null buffer", what);
+  if (int rc = check_seqs(ctx, nseq, rows, what)) return rc;
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: page=%d tokens (supported: 16, 32, 64 or 128)", what, page);
+  if (nseq > q8::kKv8ShareSeq)
+    return fail(ctx, Q8_ERR_UNSUPPORTED, "%s: nseq=%lld (at most %d sequences that share)", what,
+                (long long)nseq, q8::kKv8ShareSeq);
+  if (rows > (1 << 22) || npages <= 0 || npages > INT32_MAX || maxpages <= 0 ||
+      maxpages > ((int64_t)1 << 30) / page)
+    return fail(ctx, Q8_ERR_SHAPE, "%s: rows=%lld, npages=%lld, maxpages=%lld (at most 2^22 rows; at least 1, "
+                "maxpages * page at most 2^30)", what, (long long)rows, (long long)npages, (long long)maxpages);
+  const Ints v[] = {{"cu", ocu_i32, (uint64_t)nseq + 1, false},
+                    {"len", olen_i32, (uint64_t)nseq, false},
+                    {"table", otab_i32, (uint64_t)nseq * (uint64_t)maxpages, false},
+                    {"what is shared", oshare_i32, (uint64_t)q8::kv8_share_ints(nseq, rows), true}};
+  if (int rc = check_ints(ctx, ix, v, 4, what)) return rc;
+  if (ctx->host_only) return fail(ctx, Q8_ERR_NODEVICE, "%s: host-only context", what);
+  if (rows == 0 || nseq == 0) return ok(ctx);
+  if (int rc = set_device(ctx)) return rc;
+  q8::Kv8Args c = {};
+  c.npages = npages;
+  c.page = page;
+  c.cu = iptr(ix, ocu_i32);
+  c.len = iptr(ix, olen_i32);
+  c.tab = iptr(ix, otab_i32);
+  c.nseq = nseq;
+  c.rows = rows;
+  c.maxpages = maxpages;
+  const hipError_t e = q8::launch_kv8_share(c, iptr(ix, oshare_i32), ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "q8_kv8_share launch");
+  return ok(ctx);
+}
+
+int q8_kv8_attention_shared(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint64_t oy_f32,
+                            q8_buf *pages, uint64_t opages, int64_t npages, int page, q8_buf *ix,
+                            uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32, int64_t nseq,
+                            int64_t rows, int64_t maxpages, int nheads, int nkv, int head_dim,
+                            uint64_t oshare_i32) {
+  return run_kv8_attention(ctx, a, oq_f32, ldq, oy_f32, pages, opages, npages, page, ix, ocu_i32,
+                           olen_i32, otab_i32, nseq, rows, maxpages, nheads, nkv, head_dim, true,
+                           oshare_i32, "q8_kv8_attention_shared");
+}
+
 
 namespace {
 

@@ -124,6 +124,10 @@ SIGNATURES = {
                            _U64, _I64, _I, _P, _U64, _U64, _U64, _I64, _I64, _I64, _I, _I, _I]),
     "q8_kv8_attention": (_I, [_P, _P, _U64, _I64, _U64, _P, _U64, _I64, _I, _P, _U64, _U64, _U64,
                               _I64, _I64, _I64, _I, _I, _I]),
+    "q8_kv8_share_ints": (_U64, [_I64, _I64]),
+    "q8_kv8_share": (_I, [_P, _P, _U64, _U64, _U64, _I64, _I64, _I64, _I64, _I, _U64]),
+    "q8_kv8_attention_shared": (_I, [_P, _P, _U64, _I64, _U64, _P, _U64, _I64, _I, _P, _U64, _U64, _U64,
+                                     _I64, _I64, _I64, _I, _I, _I, _U64]),
     "q8_pages_reserve": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _I, _P, _U64,
                               _U64, _I64, _U64]),
     "q8_pages_set_len": (_I, [_P, _P, _U64, _U64, _U64, _U64, _U64, _I64, _I64, _I64, _I]),
@@ -554,6 +558,33 @@ def kv8_attention(ctx: Context, a: Buffer, oq: int, oy: int, pages: Buffer, opag
         ctx.h, a.h, int(oq), int(ldq), int(oy), pages.h, int(opages), int(npages), int(page), ix.h,
         int(ocu), int(olen), int(otab), int(nseq), int(rows), int(maxpages), int(nheads),
         int(nkv), int(head_dim)))
+
+
+def kv8_share_ints(nseq: int, rows: int) -> int:
+    """int32 that what sequences share takes: q8_kv8_share_ints."""
+    n = int(lib().q8_kv8_share_ints(int(nseq), int(rows)))
+    if n == 0:
+        raise Q8Error(Q8_ERR_UNSUPPORTED, f"no sharing among nseq={nseq} sequences of rows={rows}")
+    return n
+
+
+def kv8_share(ctx: Context, ix: Buffer, ocu: int, olen: int, otab: int, nseq: int, rows: int,
+              maxpages: int, npages: int, page: int, oshare: int) -> None:
+    """Which sequences share the pages of their first tokens: q8_kv8_share."""
+    ctx.check(ctx._lib.q8_kv8_share(ctx.h, ix.h, int(ocu), int(olen), int(otab), int(nseq), int(rows),
+                                    int(maxpages), int(npages), int(page), int(oshare)))
+
+
+def kv8_attention_shared(ctx: Context, a: Buffer, oq: int, oy: int, pages: Buffer, opages: int,
+                         npages: int, page: int, ix: Buffer, ocu: int, olen: int, otab: int,
+                         nseq: int, rows: int, maxpages: int, nheads: int, nkv: int, head_dim: int,
+                         oshare: int, ldq: int = 0) -> None:
+    """kv8_attention with the tokens that kv8_share found read once per group:
+    q8_kv8_attention_shared."""
+    ctx.check(ctx._lib.q8_kv8_attention_shared(
+        ctx.h, a.h, int(oq), int(ldq), int(oy), pages.h, int(opages), int(npages), int(page), ix.h,
+        int(ocu), int(olen), int(otab), int(nseq), int(rows), int(maxpages), int(nheads), int(nkv),
+        int(head_dim), int(oshare)))
 
 
 def pages_reserve(ctx: Context, ix: Buffer, otab: int, olen: int, oheld: int, oref: int,

@@ -62,3 +62,32 @@ def lora(x, base, cu, ids, A, B, scale, widths):
                 y[rows, cols] += float(scale[i]) * (x[rows] @ ap.T) @ bp.T
                 size[rows, cols] += abs(float(scale[i])) * (np.abs(x[rows]) @ np.abs(ap).T) @ np.abs(bp).T
     return y, size
+
+
+def share(cu, length, table, page, npages, most_groups=64):
+    """(group, tokens) of every sequence."""
+    ns = len(length)
+    whole = [min(length[i], table.shape[1] * page) // page if cu[i + 1] > cu[i] else 0 for i in range(ns)]
+
+    def common(i, j):
+        n = 0
+        while n < min(whole[i], whole[j]) and table[i][n] == table[j][n] and 0 <= table[i][n] < npages:
+            n += 1
+        return n
+    lead = [next((j for j in range(i + 1) if whole[j] and table[j][0] == table[i][0]), -1)
+            if whole[i] and 0 <= table[i][0] < npages else -1 for i in range(ns)]
+    group, tokens, count = [-1] * ns, [0] * ns, 0
+    for f in range(ns):
+        member = {i: common(i, f) for i in range(ns) if lead[i] == f}
+        if lead[f] != f or count == most_groups:
+            continue
+        saves = {p: (sum(c >= p for c in member.values()) - 1) * p for p in member.values()}
+        saved = max(saves.values())
+        take = max(p for p, v in saves.items() if v == saved)
+        if saved <= 0:
+            continue
+        for i, c in member.items():
+            if c >= take:
+                group[i], tokens[i] = count, take * page
+        count += 1
+    return group, tokens

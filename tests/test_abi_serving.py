@@ -69,3 +69,35 @@ def test_lora(hctx):
         call(widths=[8, 8, 8, 8])
     with pytest.raises(ValueError):
         call(widths=[])
+
+
+def test_share(hctx):
+    ns, T, maxpages, npages, page, nh, nkv, hd = 3, 9, 4, 5, 16, 4, 2, 64
+    n = q8hip.kv8_share_ints(ns, T)
+    assert q8hip.kv8_share_ints(1024, 1 << 22) > 1 << 22
+    for bad in ((1025, 1), (-1, 1), (1, -1), (1, (1 << 22) + 1)):
+        with pytest.raises(Q8Error):
+            q8hip.kv8_share_ints(*bad)
+    at = 2 * ns + 1 + ns * maxpages
+    ix, a = hctx.alloc(4 * (at + n)), hctx.alloc(4 * 2 * T * nh * hd)
+    pages = hctx.alloc(npages * q8hip.kv8_page_bytes(page, nkv, hd))
+
+    def find(ocu=0, olen=ns + 1, otab=2 * ns + 1, ns=ns, rows=T, maxpages=maxpages, npages=npages, page=page, at=at):
+        return code(q8hip.kv8_share, hctx, ix, ocu, olen, otab, ns, rows, maxpages, npages, page, at)
+    assert find() == find(rows=0) == find(ns=0) == Q8_ERR_NODEVICE
+    assert find(page=24) == find(ns=1025) == Q8_ERR_UNSUPPORTED
+    assert find(ns=-1) == find(rows=-1) == find(maxpages=0) == find(npages=0) == Q8_ERR_SHAPE
+    assert find(rows=(1 << 22) + 1) == find(maxpages=1 << 27) == Q8_ERR_SHAPE
+    assert find(at=at + 1) == find(rows=T + 1) == find(otab=at + n) == Q8_ERR_RANGE
+    assert find(at=at - 1) == find(at=0) == find(ocu=at + 2) == Q8_ERR_ARG
+
+    def call(oy=T * nh * hd, ns=ns, at=at, rows=T, a=a, hd=hd, ix=ix):
+        return code(q8hip.kv8_attention_shared, hctx, a, 0, oy, pages, 0, npages, page, ix, 0, ns + 1, 2 * ns + 1, ns,
+                    rows, maxpages, nh, nkv, hd, at)
+    assert call() == call(rows=0) == Q8_ERR_NODEVICE
+    assert call(at=at + 1) == call(at=1 << 62) == Q8_ERR_RANGE
+    assert call(oy=0) == Q8_ERR_ARG
+    assert call(hd=96) == Q8_ERR_UNSUPPORTED
+    many = hctx.alloc(1 << 24)
+    assert call(ns=1025, ix=many, at=100000) == Q8_ERR_UNSUPPORTED and call(ns=1024, ix=many, at=100000) == Q8_ERR_NODEVICE
+    assert call(a=many, ix=many, oy=(1 << 20), at=(1 << 20) + 5) == Q8_ERR_ARG
