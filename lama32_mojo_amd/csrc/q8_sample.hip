@@ -8,7 +8,7 @@
 // width 1 / 16 gives the running sums at bin borders, and only the bins that the
 // three borders (k-th token, top_p of the mass, u W) fall into are looked into.
 //
-// Weights are held relative to their bin's lower edge, in [1, e^(1/16)), as whole
+// Weights are held relative to their bin's middle, within 1 / 32 of 1, as whole
 // numbers of 2^-40: integer sums, so the order of the atomics does not matter and
 // equal inputs give equal ids; over bins they are summed in f64 in a fixed order.
 // Bins reach 64 below the maximum (e^-64 of the largest weight: 2^22 such tokens
@@ -29,19 +29,27 @@ constexpr double kBinsPerUnit = 16.0;
 constexpr int kHistThreads = 512;
 constexpr int kPerThread = 16;                        // logits a thread holds
 constexpr int kChunk = kHistThreads * kPerThread;
-constexpr int kList = 4096;                           // members of a bin kept in LDS
+constexpr int kList = 8192;                           // members of a bin kept in LDS
+// A sum that meets a border exactly (equal logits, a power of two of the mass) has met
+// it, whatever the last bits of the f64 sums say.
+constexpr double kTie = 0x1p-45;
+constexpr int kMaxSlices = 64;
+constexpr int kTop = 256;                             // tokens of a slice that are listed
 
 // A slice's part of its row: sums and counts of the bins below its own maximum.
+// Behind them its largest tokens: all those of its first `upto` bins.
 struct SampleSlice {
   uint64_t mass[kBins];
   uint32_t count[kBins];
   double top;                                         // bin number of the maximum
   float max;                                          // -inf: no token
   int index;                                          // its lowest index
+  int upto, listed;
+  uint64_t list[kTop];
 };
 
-// y = x / T and the bin that holds it, as whole numbers in f64 (floor(16 y), exact);
-// infinities have a bin of their own.
+// y = x / T and the bin that holds it, as whole numbers in f64 (16 y to the nearest,
+// exact); infinities have a bin of their own.
 struct BinOf {
   double y, a;
 };
@@ -49,7 +57,7 @@ __device__ __forceinline__ BinOf bin_of(float x, double inv_t) {
   BinOf b;
   b.y = (double)x * inv_t;
   if (x == INFINITY) b.y = INFINITY;                  // (T = inf: inf * 0)
-  b.a = __builtin_floor(b.y * kBinsPerUnit);
+  b.a = __builtin_rint(b.y * kBinsPerUnit);
   return b;
 }
 // Bins below the one of the maximum; kBins: out of reach.
@@ -57,22 +65,99 @@ __device__ __forceinline__ int below(double top, double a) {
   const double d = top - a;
   return top == a ? 0 : d < (double)kBins ? (int)d : kBins;
 }
-// exp(y - edge) 2^40 as a whole number.  The argument is in [0, 1/16): the series
-// to the 8th power is below 2^-54 off.  Adding 2^52 leaves the integer in the low
-// bits.
-__device__ __forceinline__ uint64_t weight(const BinOf &b) {
-  const double r = __builtin_isinf(b.y) ? 0.0 : __builtin_fma(b.a, -1.0 / kBinsPerUnit, b.y);
-  double p = 1.0 / 40320.0;
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
+// exp(y - middle of the bin) 2^40 as a whole number, from 16 times that difference, at
+// most 1 / 2: the series to the 5th power is 2^-39 off at most.  Adding 2^52 leaves the
+// integer in the low bits.
+__device__ __forceinline__ uint64_t weight16(double z) {
+  constexpr double h = 1.0 / kBinsPerUnit;
+  double p = h * h * h * h * h / 120.0;
+  p = __builtin_fma(p, z, h * h * h * h / 24.0);
+  p = __builtin_fma(p, z, h * h * h / 6.0);
+  p = __builtin_fma(p, z, h * h / 2.0);
+  p = __builtin_fma(p, z, h);
+  p = __builtin_fma(p, z, 1.0);
   const double w = __builtin_fma(p, 0x1p40, 0x1p52);
   return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ uint64_t weight(const BinOf &b) {
+  return weight16(__builtin_isinf(b.y) ? 0.0 : b.y * kBinsPerUnit - b.a);
+}
+
+// A token's place in the order, ascending: larger values first, then lower indices.
+__device__ __forceinline__ uint64_t place(float x, int i) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);           // (-0 as 0)
+  const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;         // ascending with x
+  return (uint64_t)~key << 32 | (uint32_t)i;
+}
+
+// Inclusive sums over a wave's lanes (rows of 16, then the rows' last lanes into the
+// rows behind), in one fixed order.
+template <int CTRL, int ROWS, class T> __device__ __forceinline__ T from_lanes(T v) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    int w[W];
+  } x = __builtin_bit_cast(Words, v), y;
+#pragma unroll
+  for (int i = 0; i < W; ++i) y.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(T, y);                    // (0 where there is no such lane)
+}
+template <class T> __device__ __forceinline__ T wave_sums(T v) {
+  v += from_lanes<0x111, 0xf>(v);                     // row_shr 1, 2, 4, 8
+  v += from_lanes<0x112, 0xf>(v);
+  v += from_lanes<0x114, 0xf>(v);
+  v += from_lanes<0x118, 0xf>(v);
+  v += from_lanes<0x142, 0xa>(v);                     // row_bcast 15 to rows 1, 3
+  v += from_lanes<0x143, 0xc>(v);                     // row_bcast 31 to rows 2, 3
+  return v;
+}
+// Over the block's threads; *all: the last one's.  wsum: a value a wave; the caller
+// waits before it writes there again.
+template <int NT, class T> __device__ __forceinline__ T block_sums(T v, T *wsum, T *all) {
+  static_assert(NT / 64 <= 16, "the waves' sums are a row of lanes");
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  v = wave_sums(v);
+  if (lane == 63) wsum[w] = v;
+  __syncthreads();
+  T s = wave_sums((lane & 15) < NT / 64 ? wsum[lane & 15] : (T)0);     // (the first row of lanes)
+  struct Words {
+    int w[sizeof(T) / 4];
+  } x = __builtin_bit_cast(Words, s), y, z;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) {
+    y.w[i] = w > 0 ? __builtin_amdgcn_readlane(x.w[i], w > 0 ? w - 1 : 0) : 0;
+    z.w[i] = __builtin_amdgcn_readlane(x.w[i], NT / 64 - 1);
+  }
+  *all = __builtin_bit_cast(T, z);
+  return __builtin_bit_cast(T, y) + v;
+}
+
+// Four times 4 logits of a row, the u-th at i + u * step, -inf from `end` on.  The loads
+// are not in a branch (those of a place behind the end take the row's start), so they
+// all go out together.
+template <int STEP>
+__device__ __forceinline__ void load16(const float *x, int64_t i, int64_t end, float (&v)[16]) {
+  if (end < 4) {                                      // (uniform: a row of 1 to 3 logits)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = e < 4 && i + e < end ? x[i + e] : -INFINITY;
+    return;
+  }
+  f32x4 y[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t at = i + u * STEP;
+    y[u] = *reinterpret_cast<const f32x4_u *>(x + (at + 4 <= end ? at : 0));
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t at = i + u * STEP;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * u + e] = at + 4 <= end ? y[u][e] : -INFINITY;
+    if (at < end && at + 4 > end) {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (at + e < end) v[4 * u + e] = x[at + e];
+    }
+  }
 }
 
 struct RowSettings {
@@ -101,19 +186,24 @@ __device__ __forceinline__ RowSettings settings(const SampleArgs &a, int64_t row
 // a logit.  A block walks its slice in chunks that it holds in registers; the
 // bins are a ring whose head is the slice's largest value so far, so the row's
 // maximum need not be known first.
-__global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(SampleArgs a, int64_t row0,
-                                                                   int64_t slice_len) {
+__global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs a, int64_t row0,
+                                                                      int64_t slice_len) {
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ float wmax[kHistThreads / 64];
-  __shared__ int best;
+  __shared__ uint64_t wsum[kHistThreads / 64], wsum2[kHistThreads / 64];
+  __shared__ int best, upto, listed;
   const int t = threadIdx.x;
   const int64_t row = row0 + blockIdx.y;
   const float *x = a.x + row * a.ldx;
   SampleSlice *out = reinterpret_cast<SampleSlice *>(a.ws) + (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t i0 = blockIdx.x * slice_len, i1 = min(i0 + slice_len, a.n);
+  float v[kPerThread];
+  static_assert(kPerThread == 16, "load16");
+  auto load = [&](int64_t c) { load16<4 * kHistThreads>(x, c + 4 * t, i1, v); };
+  load(i0);
   const RowSettings s = settings(a, row);
   const bool counts = s.k < a.n;
-  const int64_t i0 = blockIdx.x * slice_len, i1 = min(i0 + slice_len, a.n);
   for (int b = t; b < kBins; b += kHistThreads) {
     mass[b] = 0;
     count[b] = 0;
@@ -122,22 +212,10 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(SampleArgs a,
   double top_bin = -INFINITY;
   int head = 0, index = INT32_MAX;
   for (int64_t c = i0; c < i1; c += kChunk) {
-    float v[kPerThread];
+    if (c > i0) load(c);
     float m = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < kPerThread / 4; ++q) {
-      const int64_t i = c + 4 * (q * kHistThreads + t);
-      if (i + 4 <= i1) {
-        const f32x4 y = *reinterpret_cast<const f32x4_u *>(x + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = y[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < i1 ? x[i + e] : -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, v[4 * q + e]);          // (NaN: not taken)
-    }
+    for (int e = 0; e < kPerThread; ++e) m = fmaxf(m, v[e]);            // (NaN: not taken)
     m = wave_max(m);
     if ((t & 63) == 0) wmax[t >> 6] = m;
     if (t == 0) best = INT32_MAX;
@@ -169,66 +247,107 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(SampleArgs a,
       index = best;
     }
     if (!s.greedy) {
+      // (adding 1.5 2^52 rounds to a whole number, whose low bits are the bin's; further
+      // from 0 than that allows, the plain way)
+      const double scale = s.inv_t * kBinsPerUnit, least = top_bin - kBins + 0.5;
+      const bool near = __builtin_fabs(top_bin) < 0x1p30;
 #pragma unroll
       for (int e = 0; e < kPerThread; ++e) {
-        if (!(v[e] > -INFINITY)) continue;
-        const BinOf b = bin_of(v[e], s.inv_t);
-        const int d = below(top_bin, b.a);
-        if (d >= kBins) continue;
+        int d;
+        uint64_t w;
+        if (near) {
+          const double z = (double)v[e] * scale;
+          if (!(z > least) || v[e] == -INFINITY) continue;              // (and NaN)
+          const double whole = z + 0x1.8p52;
+          d = (int)top_bin - (int)(uint32_t)__builtin_bit_cast(uint64_t, whole);
+          w = weight16(z - (whole - 0x1.8p52));
+        } else {
+          if (!(v[e] > -INFINITY)) continue;
+          const BinOf b = bin_of(v[e], s.inv_t);
+          d = below(top_bin, b.a);
+          if (d >= kBins) continue;
+          w = weight(b);
+        }
         const int at = (head + d) & (kBins - 1);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&mass[at]), (unsigned long long)weight(b));
+        atomicAdd(reinterpret_cast<unsigned long long *>(&mass[at]), (unsigned long long)w);
         if (counts) atomicAdd(&count[at], 1u);
       }
     }
     __syncthreads();                                  // wmax, best, the ring's head
   }
+  // A slice of one chunk lists its largest tokens from the registers: those of as many
+  // bins as hold kTop (weights are within 1 / 32 of 2^40, so sums bound the counts).
+  const bool lists = i1 - i0 <= kChunk && !s.greedy && top > -INFINITY &&
+                     (counts || s.top_p < 1.0 || s.min_p > 0.0);
+  if (t == 0) upto = listed = 0;
+  if (lists) {
+    const int b0 = (head + 2 * t) & (kBins - 1), b1 = (head + 2 * t + 1) & (kBins - 1);
+    const uint64_t m0 = mass[b0], m1 = mass[b1];
+    uint64_t every;
+    const uint64_t all = block_sums<kHistThreads>(m0 + m1, wsum, &every);
+    constexpr uint64_t kMost = (uint64_t)(kTop * 15 / 16) << 40;
+    // (0 and set before the barrier in the sums; the bins that fit are the first ones)
+    if (all <= kMost) atomicMax(&upto, 2 * t + 2);
+    else if (all - m1 <= kMost) atomicMax(&upto, 2 * t + 1);
+    __syncthreads();
+    // by value, from a little below the bins on: more do no harm as far as there is room
+    float lo = INFINITY;
+    if (upto > 0) {
+      const double at = (top_bin - (double)upto + 0.5) / kBinsPerUnit / s.inv_t;
+      lo = __builtin_isinf(top_bin) ? INFINITY
+           : at == at               ? (float)(at - __builtin_fabs(at) * 0x1p-22 - 0x1p-140)
+                                    : -INFINITY;
+    }
+    uint32_t mine = 0;                                // which of v
+#pragma unroll
+    for (int e = 0; e < kPerThread; ++e) mine |= (uint32_t)(v[e] >= lo && v[e] > -INFINITY) << e;
+    const uint64_t have = __builtin_popcount(mine);
+    uint64_t n;
+    const uint64_t to = block_sums<kHistThreads>(have, wsum2, &n);
+    const bool fits = n <= kTop;                      // (the whole block)
+    if (t == 0) {
+      listed = fits ? (int)n : 0;
+      if (!fits) upto = 0;
+    }
+    uint64_t *at = out->list + (to - have);
+#pragma unroll
+    for (int q = 0; q < kPerThread / 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (fits && mine >> (4 * q + e) & 1)
+          *at++ = place(v[4 * q + e], (int)(i0 + 4 * (q * kHistThreads + t) + e));
+  }
+  __syncthreads();
   if (t == 0) {
     out->top = top_bin;
     out->max = top;
     out->index = index;
+    out->upto = upto;
+    out->listed = listed;
   }
   if (s.greedy) return;
   for (int b = t; b < kBins; b += kHistThreads) {
     const int at = (head + b) & (kBins - 1);
     out->mass[b] = mass[at];
-    out->count[b] = count[at];
+    if (counts) out->count[b] = count[at];
   }
 }
 
 // ---- pass 2: one block of kBins threads per row --------------------------------
-// A token's place in the order, ascending: larger values first, then lower indices.
-__device__ __forceinline__ uint64_t place(float x, int i) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);           // (-0 as 0)
-  const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;         // ascending with x
-  return (uint64_t)~key << 32 | (uint32_t)i;
-}
-
-// Inclusive sums over the block's threads, in one fixed order.
-template <class T> __device__ __forceinline__ T block_sums(T v, T *wsum) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  if (lane == 63) wsum[w] = v;
-  __syncthreads();
-  T base = 0;
-  for (int x = 0; x < w; ++x) base += wsum[x];
-  __syncthreads();
-  return base + v;
-}
+// The slices' bins are added up; where the kept tokens are few they are sorted and
+// the filters and the draw are one running sum, else each border's bin is looked into.
+// Bound: the chain of dependent reads and block-wide sums, 10 us of it, and for rows
+// whose kept tokens are many the second read of the logits.
 
 struct SelectLds {
-  uint64_t mass[kBins];
+  uint64_t mass[kBins];                               // (sorting: places; sums as f64)
   uint32_t count[kBins];
-  uint64_t list[kList];                               // places of a bin's members
+  uint64_t list[kList];                               // places of the members
   uint64_t wsum64[kBins / 64];
-  double wsumd[kBins / 64];
+  double wsumd[2][kBins / 64];
   uint32_t wsum32[kBins / 64];
-  uint64_t lo, hi, found;
+  uint64_t found;
   uint64_t before;                                    // sum before what was found
-  double dsum;
   uint32_t n, where;
 };
 
@@ -237,94 +356,240 @@ __device__ __forceinline__ float value_of(uint64_t place) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// The row's members of the bin `bin`: visit(place) for each.  From the list where
-// they fit, else from the row.
-template <class F>
-__device__ __forceinline__ void members(const SampleArgs &a, const float *x, double inv_t, double bin,
-                                        const SelectLds &l, bool listed, F visit) {
-  if (listed) {
-    for (uint32_t i = threadIdx.x; i < l.n; i += kBins) visit(l.list[i]);
-    return;
-  }
-  for (int64_t i0 = 0; i0 < a.n; i0 += 4 * kBins) {
-    const int64_t i = i0 + 4 * threadIdx.x;
-    float v[4];
-    if (i + 4 <= a.n) {
-      const f32x4 y = *reinterpret_cast<const f32x4_u *>(x + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = y[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = i + e < a.n ? x[i + e] : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (v[e] > -INFINITY && bin_of(v[e], inv_t).a == bin) visit(place(v[e], (int)(i + e)));
+// The row and its slices, whose heads are one a lane.
+struct RowAt {
+  const float *x;
+  int64_t n;
+  double inv_t;
+  const SampleSlice *slices;
+  int nslices;
+  double top;                                         // lane's slice: see SampleSlice
+  float max;
+  int upto, listed;
+};
+
+// Values of a bin: from lo to hi.  (bin_of is monotone, so floats say exactly what f64
+// would.)
+struct Values {
+  float lo, hi;
+  __device__ __forceinline__ bool has(float x) const { return x >= lo && x <= hi; }
+};
+// The first float, in ascending order, of a bin from `bin` on (past: behind it); NaN-free.
+// The wave halves the 2^32 patterns six times in 64 parts.
+__device__ __forceinline__ uint32_t first_key(double bin, bool past, double inv_t) {
+  const uint32_t least = 0x007fffffu + 1, most = 0xff800000u;          // keys of -FLT_MAX, +inf
+  uint32_t at = least;                                // (the answer lies from at on)
+#pragma unroll 1
+  for (int sh = 26; ; sh = sh > 6 ? sh - 6 : 0) {
+    const uint64_t k = (uint64_t)at + ((uint64_t)(threadIdx.x & 63) << sh);
+    const uint32_t key = k < most ? (uint32_t)k : most;
+    const float x = __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    const double a = bin_of(x, inv_t).a;
+    // lanes are ascending: the last one before the bin
+    const uint64_t before = __builtin_amdgcn_ballot_w64(past ? a <= bin : a < bin);
+    if (before == 0) return at;
+    const uint64_t n = (uint64_t)at + ((uint64_t)(63 - __builtin_clzll(before)) << sh);
+    if (n >= most) return most + 1;                   // (none)
+    at = (uint32_t)n;
+    if (sh == 0) return at + 1;
   }
 }
+__device__ __forceinline__ float float_of(uint32_t key) {
+  return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ Values values_of(double from, double to, double inv_t) {
+  const uint32_t a = first_key(from, false, inv_t);
+  const uint32_t b = to == INFINITY ? 0xff800001u : first_key(to, true, inv_t);
+  if (a >= b) return {INFINITY, -INFINITY};           // (no float)
+  return {float_of(a), float_of(b - 1)};
+}
 
-// Puts the members of `bin` into the list; whether they fit.
-__device__ __forceinline__ bool gather(const SampleArgs &a, const float *x, double inv_t, double bin,
-                                       SelectLds &l) {
+// Puts the tokens of the bins from `from` up to `to`, and of `also`, into LDS as far as they
+// fit; their number is l.n.  From the slices' lists where those hold them all, else
+// from the row.
+__device__ __forceinline__ void gather(const RowAt &r, double from, double to, double also, SelectLds &l) {
   __syncthreads();
   if (threadIdx.x == 0) l.n = 0;
   __syncthreads();
-  members(a, x, inv_t, bin, l, false, [&](uint64_t p) {
-    const uint32_t i = atomicAdd(&l.n, 1u);
-    if (i < kList) l.list[i] = p;
-  });
-  __syncthreads();
-  return l.n <= kList;
-}
-
-// The first member of the bin, in the order, up to which the sum of weights (or,
-// BY_COUNT, the number) satisfies `reached`; the last one where none does.  *upto:
-// the sum of weights up to it, itself included.  Each step narrows the places to one
-// of kBins parts.
-template <bool BY_COUNT, class F>
-__device__ __forceinline__ uint64_t select(const SampleArgs &a, const float *x, double inv_t, double bin,
-                                           SelectLds &l, bool listed, F reached, uint64_t *upto) {
-  const int t = threadIdx.x;
-  if (t == 0) {
-    l.lo = UINT64_MAX;
-    l.hi = 0;
+  const double least = __builtin_fmin(from, also);
+  const int lane = threadIdx.x & 63;
+  const bool all = __builtin_amdgcn_ballot_w64(lane < r.nslices && r.max > -INFINITY && least <= r.top &&
+                                               below(r.top, least) >= r.upto) == 0;
+  const Values one = values_of(from, to, r.inv_t);
+  const Values two = also == from ? one : values_of(also, also, r.inv_t);
+  // a wave's candidates take their places together: `n` of this lane's
+  auto places = [&](uint32_t n) {
+    const uint32_t upto = wave_sums(n);
+    const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
+    uint32_t at = 0;
+    if (sum) {
+      if (lane == 0) at = atomicAdd(&l.n, sum);
+      at = __builtin_amdgcn_readfirstlane(at);
+    }
+    return at + upto - n;
+  };
+  if (all) {
+    constexpr int kU = 4;
+    for (int e0 = 0; e0 < r.nslices * kTop; e0 += kU * kBins) {
+      uint64_t p[kU];
+      uint32_t mask = 0;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        // (kTop is four waves: a slice is one for the whole wave)
+        const int e = e0 + u * kBins + threadIdx.x;
+        const int i = min(__builtin_amdgcn_readfirstlane(e / kTop), r.nslices - 1);
+        const bool on = e < r.nslices * kTop && e % kTop < __builtin_amdgcn_readlane(r.listed, i);
+        p[u] = on ? r.slices[i].list[e % kTop] : UINT64_MAX;
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const float x = value_of(p[u]);
+        mask |= (uint32_t)(p[u] != UINT64_MAX && (one.has(x) || two.has(x))) << u;
+      }
+      uint32_t at = places(__builtin_popcount(mask));
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (mask >> u & 1) {
+          if (at < kList) l.list[at] = p[u];
+          ++at;
+        }
+    }
+    __syncthreads();
+    return;
   }
-  __syncthreads();
-  {
-    uint64_t lo = UINT64_MAX, hi = 0;
-    members(a, x, inv_t, bin, l, listed, [&](uint64_t p) {
-      lo = min(lo, p);
-      hi = max(hi, p);
-    });
-    if (lo <= hi) {
-      atomicMin(reinterpret_cast<unsigned long long *>(&l.lo), (unsigned long long)lo);
-      atomicMax(reinterpret_cast<unsigned long long *>(&l.hi), (unsigned long long)hi);
+  // indices first (a lane's candidates are few of its 16), then their values
+  for (int64_t i0 = 4 * threadIdx.x; i0 - 4 * threadIdx.x < r.n; i0 += 16 * kBins) {
+    float v[16];
+    load16<4 * kBins>(r.x, i0, r.n, v);
+    uint32_t mask = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mask |= (uint32_t)(one.has(v[e]) || two.has(v[e])) << e;
+    if (__builtin_amdgcn_ballot_w64(mask != 0) == 0) continue;
+    uint32_t at = places(__builtin_popcount(mask));
+    while (mask) {
+      const int e = __builtin_ctz(mask);
+      mask &= mask - 1;
+      if (at < kList) l.list[at] = (uint64_t)(i0 + 4 * (e / 4) * kBins + e % 4);
+      ++at;
     }
   }
   __syncthreads();
-  uint64_t lo = l.lo, hi = l.hi, mass0 = 0;
-  uint32_t count0 = 0;
+  const uint32_t n = min(l.n, (uint32_t)kList);
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kBins) {
+    int j[4];
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) j[u] = i0 + u * kBins < n ? (int)l.list[i0 + u * kBins] : 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = r.x[j[u]];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i0 + u * kBins < n) l.list[i0 + u * kBins] = place(v[u], j[u]);
+  }
+  __syncthreads();
+}
+
+// The members of a bin: visit(place) for each, from LDS where all that was gathered fits,
+// else from the row.
+template <class F>
+__device__ __forceinline__ void members(const RowAt &r, const Values &bin, const SelectLds &l, F visit) {
+  if (l.n <= kList) {
+    for (uint32_t i = threadIdx.x; i < l.n; i += kBins)
+      if (bin.has(value_of(l.list[i]))) visit(l.list[i]);
+    return;
+  }
+  for (int64_t i = threadIdx.x; i < r.n; i += kBins) {
+    const float z = r.x[i];
+    if (bin.has(z)) visit(place(z, (int)i));
+  }
+}
+
+// What a border asks for: the number `want`, or the weights' sum `rel`, reached or passed.
+struct Border {
+  bool by_count, passed;
+  uint64_t want;
+  double rel;
+  __device__ __forceinline__ bool operator()(uint64_t mass, uint32_t count) const {
+    return by_count ? count >= want : passed ? (double)mass > rel : (double)mass >= rel;
+  }
+};
+
+// The first member of the bin, in the order, up to which the members satisfy `reached`;
+// the last one where none does.  *upto: the sum of weights up to it, itself included.
+// Each step narrows the places to one of kBins parts; few members of LDS are compared
+// with each other.
+__device__ __forceinline__ uint64_t select(const RowAt &r, const Values &bin, SelectLds &l, const Border &reached,
+                                           uint64_t *upto) {
+  const int t = threadIdx.x;
+  // (an upper bound of the members left; where others were gathered too, or all do
+  // not fit, it is not known)
+  uint64_t lo = place(bin.hi, 0), hi = place(bin.lo, -1), mass0 = 0;
+  uint32_t count0 = 0, left = l.n;
+  __syncthreads();
   while (lo < hi) {
+    if (l.n <= kList && left <= kBins / 4) {
+      // a thread a member, against all: places in l.mass, weights behind them
+      __syncthreads();
+      if (t == 0) l.where = 0;
+      __syncthreads();
+      members(r, bin, l, [&](uint64_t p) {
+        if (p < lo || p > hi) return;
+        const uint32_t i = atomicAdd(&l.where, 1u);
+        l.mass[i] = p;
+        l.mass[kBins / 2 + i] = weight(bin_of(value_of(p), r.inv_t));
+      });
+      __syncthreads();
+      left = l.where;
+      bool is = false;
+      uint64_t p = 0, m = mass0;
+      if (t < (int)left) {
+        p = l.mass[t];
+        const uint64_t w = l.mass[kBins / 2 + t];
+        uint32_t c = count0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < left; ++j) {
+          const bool first = l.mass[j] < p;
+          m += first ? l.mass[kBins / 2 + j] : 0;
+          c += first;
+        }
+        is = reached(m + w, c + 1) && !reached(m, c);
+        if (c - count0 == left - 1) {                 // the last one, unless another is it
+          l.found = p;
+          l.before = m;
+        }
+      }
+      __syncthreads();
+      if (is) {
+        l.found = p;
+        l.before = m;
+      }
+      __syncthreads();
+      lo = hi = l.found;
+      mass0 = l.before;
+      break;
+    }
     const int bits = 64 - __builtin_clzll(hi - lo);   // places lo .. lo + 2^bits - 1
     const int sh = bits > 10 ? bits - 10 : 0;
     l.mass[t] = 0;
     l.count[t] = 0;
     if (t == 0) l.where = 0;
     __syncthreads();
-    members(a, x, inv_t, bin, l, listed, [&](uint64_t p) {
+    members(r, bin, l, [&](uint64_t p) {
       if (p < lo || p > hi) return;
       const uint32_t s = (uint32_t)((p - lo) >> sh);
       atomicAdd(reinterpret_cast<unsigned long long *>(&l.mass[s]),
-                (unsigned long long)weight(bin_of(value_of(p), inv_t)));
+                (unsigned long long)weight(bin_of(value_of(p), r.inv_t)));
       atomicAdd(&l.count[s], 1u);
     });
     __syncthreads();
     const uint64_t m = l.mass[t];
     const uint32_t c = l.count[t];
-    const uint64_t mi = mass0 + block_sums(m, l.wsum64);
-    const uint32_t ci = count0 + block_sums(c, l.wsum32);
-    const bool on = c > 0 && reached(BY_COUNT ? (uint64_t)ci : mi);
-    const bool on_before = c > 0 && reached(BY_COUNT ? (uint64_t)(ci - c) : mi - m);
+    uint64_t every;
+    uint32_t number;
+    const uint64_t mi = mass0 + block_sums<kBins>(m, l.wsum64, &every);
+    const uint32_t ci = count0 + block_sums<kBins>(c, l.wsum32, &number);
+    const bool on = c > 0 && reached(mi, ci);
+    const bool on_before = c > 0 && reached(mi - m, ci - c);
     // the first part that reaches it; the last one that holds anything otherwise
     const bool any = __syncthreads_or(on);
     if (any ? on && !on_before : c > 0) atomicMax(&l.where, (uint32_t)t);
@@ -337,176 +602,258 @@ __device__ __forceinline__ uint64_t select(const SampleArgs &a, const float *x, 
     __syncthreads();
     mass0 = l.found;
     count0 = (uint32_t)l.before;
+    left = l.count[at];
     const uint64_t nlo = lo + ((uint64_t)at << sh);
     hi = min(hi, nlo + (((uint64_t)1 << sh) - 1));
     lo = nlo;
-    if (sh > 0 && l.count[at] == 1) {                 // one member: find it
-      __syncthreads();
-      members(a, x, inv_t, bin, l, listed, [&](uint64_t p) {
+    __syncthreads();
+    if (sh > 0 && left == 1) {                        // one member: find it
+      members(r, bin, l, [&](uint64_t p) {
         if (p >= lo && p <= hi) l.found = p;
       });
       __syncthreads();
       lo = hi = l.found;
+      __syncthreads();
     }
-    __syncthreads();
   }
-  *upto = mass0 + weight(bin_of(value_of(lo), inv_t));
+  *upto = mass0 + weight(bin_of(value_of(lo), r.inv_t));
   return lo;
+}
+
+// The block's values, one a thread, in ascending order.  (Lanes of a wave exchange
+// in registers, waves through `via`.)
+__device__ __forceinline__ uint64_t sorted(uint64_t v, uint32_t n, uint64_t *via) {
+  const int t = threadIdx.x;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t & ~63);
+  for (uint32_t k = 2; k < 2 * n; k *= 2) {           // (places are not equal; pads are)
+    for (uint32_t j = k / 2; j > 0; j /= 2) {
+      uint64_t o;
+      if (wave >= 2 * n) {                            // (pads alone)
+        if (j >= 64) {
+          __syncthreads();
+          __syncthreads();
+        }
+        continue;
+      }
+      if (j < 64) {
+        o = __shfl_xor(v, (int)j);
+      } else {
+        __syncthreads();
+        via[t] = v;
+        __syncthreads();
+        o = via[t ^ j];
+      }
+      const bool up = (t & k) == 0, low = (t & j) == 0;
+      v = up == low ? min(v, o) : max(v, o);
+    }
+  }
+  __syncthreads();
+  return v;
 }
 
 __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_t row0, int slices) {
   __shared__ SelectLds l;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, lane = t & 63;
   const int64_t row = row0 + blockIdx.x;
-  const float *x = a.x + row * a.ldx;
   const SampleSlice *sl = reinterpret_cast<const SampleSlice *>(a.ws) + (int64_t)blockIdx.x * slices;
+  static_assert(kMaxSlices <= 64, "a slice a lane");
+  const SampleSlice &mine = sl[min(lane, slices - 1)];
   const RowSettings s = settings(a, row);
-  // the row's maximum
-  float top = -INFINITY;
-  double top_bin = -INFINITY;
-  int index = INT32_MAX;
-  for (int i = 0; i < slices; ++i) {
-    if (sl[i].max > top) {
-      top = sl[i].max;
-      top_bin = sl[i].top;
-      index = sl[i].index;
-    } else if (sl[i].max == top) {
-      index = min(index, sl[i].index);
-    }
-  }
+  const RowAt r = {a.x + row * a.ldx, a.n, s.inv_t, sl, slices, mine.top, mine.max, mine.upto, mine.listed};
+  int index = mine.index;
+  const float top = wave_max(r.max);                  // the row's maximum
+  const uint64_t tops = __builtin_amdgcn_ballot_w64(r.max == top);
+  const double top_bin = __shfl(r.top, __builtin_ctzll(tops));
   if (top == -INFINITY || s.greedy) {                 // (the whole block)
+    if (r.max != top) index = INT32_MAX;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) index = min(index, __shfl_xor(index, d));
     if (t == 0) {
       a.ids[row] = top == -INFINITY ? -1 : index;
       if (a.logp) a.logp[row] = top == -INFINITY ? -INFINITY : 0.0f;
     }
     return;
   }
+  const bool counts = s.k < a.n;
   // this thread's bin, t below the maximum's
   uint64_t m = 0;
   uint32_t c = 0;
-  for (int i = 0; i < slices; ++i) {
-    if (sl[i].max == -INFINITY) continue;
-    const int shift = below(top_bin, sl[i].top);
-    if (t >= shift) {
-      m += sl[i].mass[t - shift];
-      c += sl[i].count[t - shift];
+  const int down = r.max == -INFINITY ? kBins : below(top_bin, r.top);
+  for (int i0 = 0; i0 < slices; i0 += 8) {
+    uint64_t mi[8];
+    uint32_t ci[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = min(i0 + u, slices - 1), shift = __builtin_amdgcn_readlane(down, i);
+      const bool on = i0 + u < slices && t >= shift;
+      mi[u] = on ? sl[i].mass[t - shift] : 0;
+      ci[u] = on && counts ? sl[i].count[t - shift] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      m += mi[u];
+      c += ci[u];
     }
   }
+  // (without a count: about as many, weights are within 1 / 32 of 2^40)
+  if (!counts) c = (uint32_t)((m + ((uint64_t)1 << 39)) >> 40);
   const double ymax = bin_of(top, s.inv_t).y;
-  const double rest = __builtin_isinf(ymax) ? 0.0 : ymax - top_bin / kBinsPerUnit;    // exact
+  // (y of the maximum from its bin's middle on, exact)
+  const double rest = __builtin_isinf(ymax) ? 0.0 : ymax - top_bin / kBinsPerUnit;
   const double unit = exp(-(double)t / kBinsPerUnit - rest) * 0x1p-40;  // weight of 1 in this bin
-  const double mine = (double)m * unit;
-  const double upto = block_sums(mine, l.wsumd);      // this bin included
-  const uint32_t cupto = block_sums(c, l.wsum32);
-  // the bin that a border falls into: the first one that reaches it, `upto` and
-  // `unit` of which go around; the last one with tokens where rounding leaves none
+  const double here = (double)m * unit;
+  double total;
+  uint32_t tokens;
+  const double upto = block_sums<kBins>(here, l.wsumd[0], &total);     // this bin included
+  const uint32_t cupto = block_sums<kBins>(c, l.wsum32, &tokens);
+  // the bin that a border falls into: the first one that reaches it, what is before it
+  // and its unit; the last one with tokens where rounding leaves none
   __shared__ double e_before, e_unit;
+  __shared__ uint32_t e_count;
   auto border = [&](bool on) {
     const bool any = __syncthreads_or(on && m > 0);
     if (t == 0) l.where = any ? kBins : 0;
     __syncthreads();
-    if (m > 0) {
-      if (any) {
-        if (on) atomicMin(&l.where, (uint32_t)t);
-      } else {
-        atomicMax(&l.where, (uint32_t)t);
-      }
+    const uint64_t who = __builtin_amdgcn_ballot_w64(m > 0 && (on || !any));
+    if (who && lane == 0) {
+      if (any) atomicMin(&l.where, (uint32_t)(t + __builtin_ctzll(who)));
+      else atomicMax(&l.where, (uint32_t)(t + 63 - __builtin_clzll(who)));
     }
     __syncthreads();
     const int b = (int)l.where;
     if (t == b) {
-      e_before = upto - mine;
+      e_before = upto - here;
       e_unit = unit;
+      e_count = cupto;
     }
     __syncthreads();
     return b;
   };
   auto bin_at = [&](int b) { return b == 0 ? top_bin : top_bin - (double)b; };
+  const bool by_k = counts && s.k < (int64_t)tokens;
+  // the last bin of min_p: weights from min_p on
+  int last = kBins - 1;
+  if (s.min_p > 0.0 && !__builtin_isinf(ymax))
+    last = min(last, below(top_bin, __builtin_rint((ymax + log(s.min_p)) * kBinsPerUnit)));
 
-  if (t == kBins - 1) {
-    l.dsum = upto;
-    l.found = cupto;
-  }
+  // Few kept tokens: gathered and sorted.  Many: the bin of the k-th token, of top_p, of
+  // min_p and of the draw in turn, each where its setting is on.
+  enum { FEW, BY_K, BY_MASS, BY_WEIGHT, DRAW };
+  int b = last;
+  if (by_k) b = border((int64_t)cupto >= s.k);        // (top_p goes by the sum of all k)
+  else if (s.top_p < 1.0) b = min(b, border(upto >= fmax(s.top_p, 0.0) * total * (1.0 - kTie)));
+  if (t == b) e_count = cupto;
   __syncthreads();
-  double W = l.dsum;
-  const uint32_t tokens = (uint32_t)l.found;
-  __syncthreads();
-  int have = -1;                                      // the bin in the list
-  bool listed = false;
-  auto look = [&](int b) {
-    if (have != b) listed = gather(a, x, s.inv_t, bin_at(b), l);
-    have = b;
-  };
-  uint64_t J;
-  if (s.k < (int64_t)tokens) {
-    const int b = border((int64_t)cupto >= s.k);
-    if (t == b) l.before = cupto - c;
-    __syncthreads();
-    const uint64_t want = (uint64_t)s.k - l.before;
-    const double before = e_before, u = e_unit;
-    look(b);
-    select<true>(a, x, s.inv_t, bin_at(b), l, listed, [&](uint64_t n) { return n >= want; }, &J);
-    W = before + (double)J * u;
-  }
-  if (s.top_p < 1.0) {
-    const double want = fmax(s.top_p, 0.0) * W;
-    const int b = border(upto >= want);
-    const double before = e_before, u = e_unit, rel = (want - before) / u;
-    look(b);
-    select<false>(a, x, s.inv_t, bin_at(b), l, listed, [&](uint64_t n) { return (double)n >= rel; }, &J);
-    W = fmin(W, before + (double)J * u);
-  }
-  if (s.min_p > 0.0) {
-    // tokens of weight min_p and more: whole bins above the border's
-    const double z = log(s.min_p);                    // y - ymax from which on
-    const double edge = __builtin_isinf(ymax) ? top_bin : __builtin_floor((ymax + z) * kBinsPerUnit);
-    const int d = below(top_bin, edge);
-    if (d < kBins) {
-      if (t == d) {
-        e_before = upto - mine;
-        e_unit = unit;
-        l.dsum = (double)m;
+  double W = total;
+  double have = NAN, also = NAN;                      // the bins in LDS
+  // (estimates of counts are within 1 / 32)
+  for (int stage = e_count <= kBins * 15 / 16 ? FEW : BY_K; stage <= DRAW; ++stage) {
+    if ((stage == BY_K && !by_k) || (stage == BY_MASS && !(s.top_p < 1.0)) ||
+        (stage == BY_WEIGHT && !(s.min_p > 0.0 && last < kBins - 1)))
+      continue;
+    double want = 0.0, more = NAN;
+    if (stage == BY_K) {
+      b = border((int64_t)cupto >= s.k);
+    } else if (stage == BY_MASS) {
+      want = fmax(s.top_p, 0.0) * W * (1.0 - kTie);
+      b = border(upto >= want);
+    } else if (stage == BY_WEIGHT) {
+      b = border(t == last);
+      if (b != last) {                                // (no token there)
+        if (t == last) e_before = upto;
+        __syncthreads();
+        if (e_before > 0.0) W = fmin(W, e_before);
+        __syncthreads();
+        continue;
       }
+    } else if (stage == DRAW) {
+      want = s.u * W * (1.0 + kTie);
+      b = border(upto > want);
+    }
+    const double before = e_before, u = e_unit;
+    if (stage == BY_MASS) {
+      // with it the bin that the draw falls into, by what is kept at least, where
+      // both fit into LDS
+      const int draw = border(upto > s.u * before * (1.0 + kTie));
+      if (t == 0) l.where = 0;
       __syncthreads();
-      const double before = e_before, u = e_unit;
-      if (l.dsum > 0.0) look(d);
+      if (t == b || t == draw) atomicAdd(&l.where, (uint32_t)((m >> 40) + (m >> 45)));
       __syncthreads();
+      if (l.where <= kList) more = bin_at(draw);
+      __syncthreads();
+    }
+    const double bin = bin_at(b);
+    if (stage == FEW || !(bin == have || bin == also)) {
+      gather(r, bin, stage == FEW ? INFINITY : bin, stage == FEW || more != more ? bin : more, l);
+      have = stage == FEW ? NAN : bin;
+      also = more;
+    }
+    if (stage == FEW) {
+      const uint32_t n = l.n;                         // (1 at least: the maximum)
+      if (n > kBins) continue;
+      const uint64_t p = sorted((uint32_t)t < n ? l.list[t] : UINT64_MAX, n, l.mass);
+      const bool in = (uint32_t)t < n;
+      double y = 0.0, w = 0.0;
+      if (in) {
+        y = bin_of(value_of(p), s.inv_t).y;
+        w = __builtin_isinf(ymax) ? 1.0 : exp(y - ymax);
+      }
+      double every;
+      const double sum = block_sums<kBins>(w, l.wsumd[1], &every);
+      double *sums = reinterpret_cast<double *>(l.mass);
+      sums[t] = sum;
+      __syncthreads();
+      const double S = by_k ? sums[min((int64_t)n, s.k) - 1] : total;
+      const bool keep = in && t < s.k && (t == 0 || ((s.top_p >= 1.0 || sum - w < s.top_p * S * (1.0 - kTie)) &&
+                                                     w >= s.min_p));
+      const int kept = __syncthreads_count(keep);     // (a head of the order)
+      W = sums[kept - 1];
+      const int at = min(__syncthreads_count(in && sum <= s.u * W * (1.0 + kTie)), kept - 1);
+      if (t == at) {
+        a.ids[row] = (int)(uint32_t)p;
+        if (a.logp) a.logp[row] = (float)((__builtin_isinf(ymax) ? 0.0 : y - ymax) - log(W));
+      }
+      return;
+    }
+    const Values in_bin = values_of(bin, bin, s.inv_t);
+    if (stage == BY_WEIGHT) {
       if (t == 0) l.found = 0;
       __syncthreads();
-      if (l.dsum > 0.0) {
-        uint64_t part = 0;
-        members(a, x, s.inv_t, bin_at(d), l, listed, [&](uint64_t p) {
-          const BinOf q = bin_of(value_of(p), s.inv_t);
-          if (__builtin_isinf(ymax) || exp(q.y - ymax) >= s.min_p) part += weight(q);
-        });
-        if (part) atomicAdd(reinterpret_cast<unsigned long long *>(&l.found), (unsigned long long)part);
-      }
+      uint64_t part = 0;
+      members(r, in_bin, l, [&](uint64_t p) {
+        const BinOf q = bin_of(value_of(p), s.inv_t);
+        if (exp(q.y - ymax) >= s.min_p) part += weight(q);
+      });
+      if (part) atomicAdd(reinterpret_cast<unsigned long long *>(&l.found), (unsigned long long)part);
       __syncthreads();
       const double kept = before + (double)l.found * u;
       if (kept > 0.0) W = fmin(W, kept);
       __syncthreads();
+      continue;
     }
-  }
-  const double want = s.u * W;
-  const int b = border(upto > want);
-  const double before = e_before, u = e_unit, rel = (want - before) / u;
-  look(b);
-  const uint64_t p = select<false>(a, x, s.inv_t, bin_at(b), l, listed,
-                                   [&](uint64_t n) { return (double)n > rel; }, &J);
-  if (t == 0) {
-    a.ids[row] = (int)(uint32_t)p;
-    const double y = bin_of(value_of(p), s.inv_t).y;
-    if (a.logp) a.logp[row] = (float)((__builtin_isinf(ymax) ? 0.0 : y - ymax) - log(W));
+    if (t == b) l.before = cupto - c;
+    __syncthreads();
+    const Border reached = {stage == BY_K, stage == DRAW, (uint64_t)s.k - l.before, (want - before) / u};
+    uint64_t J;
+    const uint64_t p = select(r, in_bin, l, reached, &J);
+    if (stage != DRAW) {
+      W = fmin(W, before + (double)J * u);
+    } else if (t == 0) {
+      a.ids[row] = (int)(uint32_t)p;
+      const double y = bin_of(value_of(p), s.inv_t).y;
+      if (a.logp) a.logp[row] = (float)((__builtin_isinf(ymax) ? 0.0 : y - ymax) - log(W));
+    }
   }
 }
 
 }  // namespace
 
-// Slices of a row: enough blocks for the chip (two of 512 threads a CU), none
+// Slices of a row: enough blocks for the chip (four of 512 threads a CU), none
 // shorter than a chunk.
+constexpr int64_t kBlocks = 1024;
 static int64_t sample_slices(int64_t rows, int64_t n) {
-  const int64_t most = (n + kChunk - 1) / kChunk;
-  return std::max<int64_t>(1, std::min(most, (512 + rows - 1) / rows));
+  const int64_t most = std::min<int64_t>(kMaxSlices, (n + kChunk - 1) / kChunk);
+  return std::max<int64_t>(1, std::min(most, (kBlocks + rows - 1) / rows));
 }
 
 hipError_t launch_sample(const SampleArgs &a, int64_t ws_bytes, hipStream_t st) {
