@@ -413,6 +413,38 @@ template <int HD> __device__ __forceinline__ float kv8_exact_up_to() {
   return 1.44269504088896341f / sqrtf((float)HD) * (0x1p-18f / 127.0f);
 }
 
+// The four digits of a column's q (this lane's dims of it, x); returns the scale of the
+// integer scores, 2^(e - 30) qscale, or NaN where q is not finite.
+template <int HD>
+__device__ __forceinline__ float kv8_digits(const float (&x)[HD / 64][16], float qscale,
+                                            u32x4 (&qd)[4][HD / 64]) {
+  constexpr int HH = HD / 64;
+  uint32_t bits = 0;                      // |q| as bits: NaN and infinity above all
+#pragma unroll
+  for (int h = 0; h < HH; ++h)
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+      bits = max(bits, __builtin_bit_cast(uint32_t, x[h][v]) & 0x7fffffffu);
+  bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16));
+  bits = max(bits, (uint32_t)__shfl_xor((int)bits, 32));
+  const bool fine = bits < 0x7f800000u;
+  const int e = max((int)(bits >> 23) - 126, -90);     // |q| < 2^e
+  const float up = __builtin_ldexpf(1.0f, 30 - e);
+#pragma unroll
+  for (int h = 0; h < HH; ++h)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      float y[4];
+      uint32_t d[4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) y[z] = fine ? x[h][4 * v + z] * up : 0.0f;
+      digits4(y, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) qd[k][h][v] = d[k];
+    }
+  return fine ? __builtin_ldexpf(qscale, e - 30) : __builtin_nanf("");
+}
+
 // The plan of a call in LDS: the prefix sums of the sequences' units (WHOLE: row
 // tiles), pre[0] = 0 .. pre[nseq], and their first rows, row counts and cached
 // tokens; all NT threads.
@@ -442,9 +474,9 @@ __device__ __forceinline__ int kv8_shared_tokens(const Kv8Args &c, const Kv8Shar
   return g >= 0 && g < sh.groups ? clamp_i(sh.tok[i], 0, c.maxpages * c.page) & ~(c.page - 1) : 0;
 }
 
-// What of a sequence a launch goes through: all its keys, the ones behind the shared
-// tokens, or (a group's rows) the shared ones.
-enum { KV8_ALL = 0, KV8_OWN = 1, KV8_SHARED = 2 };
+// What of a sequence a launch goes through: all its keys, or the ones behind the
+// shared tokens.
+enum { KV8_ALL = 0, KV8_OWN = 1 };
 
 template <bool WHOLE, int NT, int PART>
 __device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, int cols, const Kv8Plan &pl,
@@ -582,14 +614,14 @@ __device__ __forceinline__ int kv8_group_plan(const Kv8Args &c, const Kv8ShareAt
   return per;
 }
 constexpr int kKv8SharedCols = 64;       // columns of a group's row tile
+constexpr int kKv8SharedBlocks = 768;    // three a CU
 
 //
 // WIDE (pages of 128 tokens, runs): a V column of a page is one 128-byte line,
 // of which a unit takes half.  The even unit's load brings the odd unit's half
 // into registers too; fetched a unit later, the line had left the L2 by then
 // (4 contexts of up to 131000 tokens 142 -> 128 us).
-// PART: see above.  KV8_SHARED's columns are (row of the group, query head), its rows
-// from the list, and all see all keys; it leaves one record a block.
+// PART: see above.
 template <int HD, int MT, bool WHOLE, bool WIDE, int PART>
 __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kernel(Kv8AttnArgs a) {
   constexpr int DT = HD / 16, HH = HD / 64, NC = 16 * MT, NW = WHOLE ? 8 : kKv8Waves;
@@ -619,23 +651,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   pl.old = pl.n + nseq;
   pl.k0 = pl.old + nseq;
 
-  Kv8ShareAt sh;
-  if constexpr (PART != KV8_ALL) sh = kv8_share_at(c, a.share);
-  int units, shared_per = 0;
-  if constexpr (PART == KV8_SHARED) {
-    shared_per = kv8_group_plan<64 * NW>(c, sh, NC, a.shared_target, pl.pre, wsum);
-    units = pl.pre[sh.groups];
-    if (blockIdx.x == 0 && g == 0) {       // the join reads the plan
-      for (int i = t; i <= sh.groups; i += 64 * NW) a.shared_plan[1 + i] = pl.pre[i];
-      if (t == 0) a.shared_plan[0] = shared_per;
-    }
-  } else {
-    units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, NC, pl, wsum);
-  }
+  const int units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, NC, pl, wsum);
   const int runs = gridDim.x * RW, run = blockIdx.x * RW + w;
-  const int per = WHOLE || PART == KV8_SHARED ? 1 : kv8_units_per_block(units, runs, 1);
+  const int per = WHOLE ? 1 : kv8_units_per_block(units, runs, 1);
   // the merge reads the plan behind the records
-  if (!WHOLE && PART != KV8_SHARED && blockIdx.x == 0 && g == 0)
+  if (!WHOLE && blockIdx.x == 0 && g == 0)
     for (int i = t; i <= nseq; i += 64 * NW) kv8_plan_at<HD, NC>(a, runs)[i] = pl.pre[i];
   const int u0 = WHOLE ? (int)blockIdx.x : run * per;
   const int uend = WHOLE ? min((int)blockIdx.x + 1, units) : min(u0 + per, units);
@@ -644,19 +664,6 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   // the place of unit u, in sequence i or behind it
   auto place = [&](int u, int i) {
     Kv8Place p;
-    if constexpr (PART == KV8_SHARED) {
-      int n, tiles;
-      kv8_group(c, sh, i, NC, &n, &tiles, &p.units);
-      const int cuts = max(1, (p.units + shared_per - 1) / shared_per);
-      p.u = u;
-      p.i = i;
-      p.k0 = 0;
-      p.ctx = kv8_shared_tokens(c, sh, clamp_i(sh.lead[i], 0, nseq - 1));
-      p.rt = (u - pl.pre[i]) / cuts;
-      p.t0 = p.kt = (u - pl.pre[i]) % cuts * shared_per;
-      p.t1 = min(p.units, p.t0 + shared_per);
-      return p;
-    }
     while (pl.pre[i + 1] <= u) ++i;
     const int local = u - pl.pre[i], ctx = min(pl.old[i] + pl.n[i], cap);
     p.k0 = PART == KV8_OWN ? pl.k0[i] : 0;
@@ -678,14 +685,13 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   int idk = 0, idv = 0;
   bool second = false;                    // vr2 holds the V of the unit loaded next
   const int step = WHOLE ? RW : 1;
-  Kv8Place nx = place(u0, kv8_seq_of(pl.pre, PART == KV8_SHARED ? sh.groups : nseq, u0));
+  Kv8Place nx = place(u0, kv8_seq_of(pl.pre, nseq, u0));
   Kv8Place cu = nx;
   if (WHOLE) nx.kt = w;
   auto have = [&]() { return nx.kt < nx.t1; };
   auto load_ids = [&]() {
     if (!have()) return;
-    const int *tab =
-        c.tab + (int64_t)(PART == KV8_SHARED ? clamp_i(sh.lead[nx.i], 0, nseq - 1) : nx.i) * c.maxpages;
+    const int *tab = c.tab + (int64_t)nx.i * c.maxpages;
     const int kk = nx.k0 + nx.kt * kKv8Unit + 16 * (col >> 2), kv = nx.k0 + nx.kt * kKv8Unit + 16 * g4;
     idk = kk < nx.ctx ? tab[kk >> psh] : 0;
     idv = kv < nx.ctx ? tab[kv >> psh] : 0;
@@ -732,7 +738,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   };
   auto advance = [&]() {
     nx.kt += step;
-    if (WHOLE || PART == KV8_SHARED || nx.kt < nx.t1) return;
+    if (WHOLE || nx.kt < nx.t1) return;
     const int u = nx.u + (nx.t1 - nx.t0);
     if (u < uend) nx = place(u, nx.i);
   };
@@ -740,9 +746,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   // row's), from dim 16 g4 on
   auto q_at = [&](const Kv8Place &p, int row0, int n) {
     const int lin = p.rt * NC + cc, j = lin / grp;
-    int64_t row = row0 + (j < n ? j : 0);
-    if constexpr (PART == KV8_SHARED) row = clamp_i(sh.row[row], 0, c.rows - 1);
-    return a.q + row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
+    return a.q + (int64_t)(row0 + (j < n ? j : 0)) * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
   };
   load_ids();
   load_k();
@@ -751,18 +755,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   load_ids();
 
   for (;;) {                              // row tiles of the run
-    int row0, n, old = 0;
-    if constexpr (PART == KV8_SHARED) {
-      int tiles, units;
-      kv8_group(c, sh, cu.i, NC, &n, &tiles, &units);
-      row0 = clamp_i(sh.gcu[cu.i], 0, c.rows);
-    } else {
-      row0 = pl.row0[cu.i], n = pl.n[cu.i], old = pl.old[cu.i];
-    }
+    const int row0 = pl.row0[cu.i], n = pl.n[cu.i], old = pl.old[cu.i];
     // ---- this lane's digits of q: column col, dims 64 h + 16 g4 ..; the keys
     // its columns see: 0 .. kend-1 (0: no such column)
     const int lin = cu.rt * NC + cc, j = lin / grp;
-    const int kend = j < n ? (PART == KV8_SHARED ? cu.ctx : min(old + j + 1, cap)) : 0;
+    const int kend = j < n ? min(old + j + 1, cap) : 0;
     int kmin = j < n ? kend : INT32_MAX;
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) kmin = min(kmin, __shfl_xor(kmin, d));
@@ -780,30 +777,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
           for (int z = 0; z < 4; ++z) x[h][4 * v + z] = y[z];
         }
       }
-      uint32_t bits = 0;                  // |q| as bits: NaN and infinity above all
-#pragma unroll
-      for (int h = 0; h < HH; ++h)
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          bits = max(bits, __builtin_bit_cast(uint32_t, x[h][v]) & 0x7fffffffu);
-      bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16));
-      bits = max(bits, (uint32_t)__shfl_xor((int)bits, 32));
-      const bool fine = bits < 0x7f800000u;
-      const int e = max((int)(bits >> 23) - 126, -90);     // |q| < 2^e
-      const float up = __builtin_ldexpf(1.0f, 30 - e);
-      qs = fine ? __builtin_ldexpf(qscale, e - 30) : __builtin_nanf("");
-#pragma unroll
-      for (int h = 0; h < HH; ++h)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          float y[4];
-          uint32_t d[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) y[z] = fine ? x[h][4 * v + z] * up : 0.0f;
-          digits4(y, d);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) qd[k][h][v] = d[k];
-        }
+      qs = kv8_digits<HD>(x, qscale, qd);
     }
 
     // ---- the wave's units
@@ -953,18 +927,6 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
       }
       if (w != 0) return;
     }
-    if constexpr (PART == KV8_SHARED) {
-      if (j < n) {
-        float *rec = a.shared_rec + ((int64_t)blockIdx.x * c.nkv + g) * kv8_record<HD, NC>();
-#pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(rec + cc * HD + 16 * d + 4 * g4) = o[d];
-        if (g4 == 0) {
-          rec[NC * HD + cc] = m;
-          rec[NC * HD + NC + cc] = l;
-        }
-      }
-      return;
-    }
     if (j < n) {
       const bool whole = WHOLE || (cu.t0 == 0 && cu.t1 == cu.units);
       float *rec = a.ws + (((int64_t)run * c.nkv + g) * 2 + (cu.t0 == 0)) * kv8_record<HD, NC>();
@@ -986,6 +948,234 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     const int u = cu.u + (cu.t1 - cu.t0);
     if (WHOLE || u >= uend) return;
     cu = place(u, cu.i);
+  }
+}
+
+// ---- the shared tokens of groups ------------------------------------------------------
+// A block of 4 waves takes a row tile of 64 columns (row of the group, query head), 16 a
+// wave, over a cut of the group's shared tokens; all columns see all of them.  A unit's K
+// codes and its V, as bf16 once for all waves, go through LDS in the layout of the MFMA
+// operands (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in
+// flight beside this one's products.  Scores, probabilities and products are those of
+// kv8_attn_kernel.  Bound: VALU (the joins of the digits, exp, p in three terms: 340
+// operations a unit and 16 columns, 190 of them for codes -> bf16 if every wave did that
+// for itself).
+template <int HD>
+__global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
+  constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8SharedCols, NW = 4;
+  constexpr int KF = 4 * HH / NW, VF = DT / NW;        // fragments that a wave stages
+  extern __shared__ int base[];                        // the blocks of the groups
+  __shared__ int wsum[NW];
+  __shared__ __attribute__((aligned(16))) u32x4 kbuf[2][4 * HH][64], vbuf[2][2 * DT][64];
+  const Kv8Args &c = a.c;
+  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6), cc = 16 * w + col;
+  const int g = blockIdx.y, grp = c.nheads / c.nkv, P = c.page;
+  const int psh = 31 - __builtin_clz(P);
+  const int64_t pbytes = kv8_page_bytes(P, c.nkv, HD);
+  const int64_t scales_at = kv8_scales_at(P, c.nkv, HD);
+  const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
+  const float qscale = 1.44269504088896341f / sqrtf((float)HD);
+  const Kv8ShareAt sh = kv8_share_at(c, a.share);
+  const int per = kv8_group_plan<64 * NW>(c, sh, NC, a.shared_target, base, wsum);
+  if (blockIdx.x == 0 && g == 0) {        // the join reads the plan
+    for (int i = t; i <= sh.groups; i += 64 * NW) a.shared_plan[1 + i] = base[i];
+    if (t == 0) a.shared_plan[0] = per;
+  }
+  const int b = blockIdx.x;
+  if (b >= base[sh.groups]) return;       // (the whole block)
+  const int i = kv8_seq_of(base, sh.groups, b);
+  int n, tiles, units;
+  kv8_group(c, sh, i, NC, &n, &tiles, &units);
+  const int cuts = max(1, (units + per - 1) / per);
+  const int lead = clamp_i(sh.lead[i], 0, c.nseq - 1), tokens = kv8_shared_tokens(c, sh, lead);
+  const int rt = (b - base[i]) / cuts, t0 = (b - base[i]) % cuts * per, t1 = min(units, t0 + per);
+  const int *tab = c.tab + (int64_t)lead * c.maxpages;
+
+  // what a wave stages: K fragments KF w .. (tt = f / HH, dims 64 (f % HH) + 16 g4 ..) and
+  // V fragments VF w .. (dims 16 f + col, keys 16 g4 ..); the lane's pages of both
+  int idk, idv;
+  u32x4 kr[KF], vr[VF];
+  float ks = 0.0f, vs = 0.0f, ks1, vs1;
+  auto load_ids = [&](int kt) {
+    const int kk = kt * kKv8Unit + 16 * (col >> 2), kv = kt * kKv8Unit + 16 * g4;
+    idk = kt < t1 && kk < tokens ? tab[kk >> psh] : 0;
+    idv = kt < t1 && kv < tokens ? tab[kv >> psh] : 0;
+  };
+  auto load = [&](int kt) {
+    int id = page_or_none(idk, (int)c.npages);
+    const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
+                       (int64_t)(((kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD + 16 * g4;
+#pragma unroll
+    for (int f = 0; f < KF; ++f)
+      kr[f] = *reinterpret_cast<const u32x4 *>(p + 4 * ((KF * w + f) / HH) * HD + 64 * ((KF * w + f) % HH));
+    id = page_or_none(idv, (int)c.npages);
+    p = c.pages + (id < 0 ? 0 : id) * pbytes;
+    const float *sc = reinterpret_cast<const float *>(p + scales_at);
+    ks1 = id < 0 ? __builtin_nanf("") : sc[g];
+    vs1 = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
+    p += v_at + (int64_t)col * P + ((kt * kKv8Unit + 16 * g4) & (P - 1));
+#pragma unroll
+    for (int f = 0; f < VF; ++f) vr[f] = *reinterpret_cast<const u32x4 *>(p + (int64_t)16 * (VF * w + f) * P);
+  };
+  auto store = [&](int to) {
+#pragma unroll
+    for (int f = 0; f < KF; ++f) kbuf[to][KF * w + f][lane] = kr[f];
+#pragma unroll
+    for (int f = 0; f < VF; ++f)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        vbuf[to][2 * (VF * w + f) + e][lane] =
+            __builtin_bit_cast(u32x4, codes_to_bf16(vr[f][2 * e], vr[f][2 * e + 1]));
+    ks = ks1;
+    vs = vs1;
+  };
+  load_ids(t0);
+  load(t0);
+  load_ids(t0 + 1);
+
+  // this lane's digits of q
+  const int lin = rt * NC + cc, j = lin / grp;
+  const int row = clamp_i(sh.row[clamp_i(sh.gcu[i], 0, c.rows) + (j < n ? j : 0)], 0, c.rows - 1);
+  const float *q = a.q + (int64_t)row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
+  u32x4 qd[4][HH];
+  float qs;
+  {
+    float x[HH][16];
+#pragma unroll
+    for (int h = 0; h < HH; ++h)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const f32x4 y = *reinterpret_cast<const f32x4_u *>(q + 64 * h + 4 * v);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) x[h][4 * v + z] = y[z];
+      }
+    qs = kv8_digits<HD>(x, qscale, qd);
+  }
+  store(0);
+  __syncthreads();
+
+  f32x4 o[DT];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int kt = t0; kt < t1; ++kt) {
+    const int at = (kt - t0) & 1;
+    if (kt + 1 < t1) {
+      load(kt + 1);
+      load_ids(kt + 2);
+    }
+    f32x4 s[4];
+    const float sc = qs * ks, vsc = vs;
+    if (__builtin_amdgcn_ballot_w64(fabsf(sc) > kv8_exact_up_to<HD>()) == 0) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        i32x4 d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[k] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < HH; ++h) {
+          const i32x4 kf = __builtin_bit_cast(i32x4, kbuf[at][tt * HH + h][lane]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0, 0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v)       // (|d| < 2^21 each: the pairs fit)
+          s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
+                                    (float)((d[1][v] << 8) + d[0][v]));
+      }
+    } else {
+      // q as three bf16 terms (see kv8_attn_kernel)
+      const float up = qscale / qs;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int z = 0; z < 2 * HH; ++z) {
+        float y[8];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const f32x4 x = *reinterpret_cast<const f32x4_u *>(q + 64 * (z >> 1) + 8 * (z & 1) + 4 * v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[4 * v + e] = x[e] * up;
+        }
+        u32x4 qf[3];
+        split3x8(y, qf);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u32x4 kf = kbuf[at][tt * HH + (z >> 1)][lane];
+          const bf16x8_t kb = codes_to_bf16(kf[2 * (z & 1)], kf[2 * (z & 1) + 1]);
+#pragma unroll
+          for (int k = 2; k >= 0; --k)
+            s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, __builtin_bit_cast(bf16x8_t, qf[k]), s[tt], 0, 0, 0);
+        }
+      }
+    }
+    // (the last unit's keys behind the shared tokens: a page of 16 or 32 may end there)
+    const int key0 = kt * kKv8Unit + 16 * g4;
+    const bool masked = kt * kKv8Unit + kKv8Unit > tokens;
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float x = s[tt][v] * sc;
+        if (masked) x = key0 + 4 * tt + v < tokens ? x : -INFINITY;
+        s[tt][v] = x;
+        tmax = fmaxf(tmax, x);
+      }
+    tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
+    tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+    const float mnew = fmaxf(m, __builtin_rintf(tmax));
+    const float ms = mnew == -INFINITY ? 0.0f : mnew;
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mnew;
+    float ps = 0.0f;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float p = __builtin_amdgcn_exp2f(s[tt][v] - ms);
+        ps += p;
+        float x = p * vsc;
+        if (masked) x = key0 + 4 * tt + v < tokens ? x : 0.0f;
+        s[tt][v] = x;
+      }
+    l = __builtin_fmaf(l, alpha, ps);
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u32x4 pf[3];
+      float x[8];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3];
+      split3x8(x, pf);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, vbuf[at][2 * d + e][lane]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, pf[k]), o[d], 0, 0, 0);
+      }
+    }
+    // (the other buffer's last readers are behind the barrier before this unit)
+    if (kt + 1 < t1) {
+      store(at ^ 1);
+      __syncthreads();
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (j >= n) return;
+  float *rec = a.shared_rec + ((int64_t)b * c.nkv + g) * kv8_record<HD, NC>();
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(rec + cc * HD + 16 * d + 4 * g4) = o[d];
+  if (g4 == 0) {
+    rec[NC * HD + cc] = m;
+    rec[NC * HD + NC + cc] = l;
   }
 }
 
@@ -1214,7 +1404,7 @@ static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
   // the space at most), then what the sequences' own parts leave
   const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4, plan = (groups + 5) / 4 * 4;
   const int64_t room = (a.ws_floats / 4 * 3 - ml - plan) / rec;
-  const int64_t want = (512 + c.nkv - 1) / c.nkv;
+  const int64_t want = (kKv8SharedBlocks + c.nkv - 1) / c.nkv;
   a.shared_target = (int)std::min(want, room - tiles);
   // (more rows than there is room for: every sequence for itself)
   if (a.shared_target < std::min<int64_t>(want, 8) || groups == 0) return launch_kv8_attention(a, st);
@@ -1225,12 +1415,8 @@ static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
   a.shared_blocks = (int)blocks;
   a.ws += ml + plan + recs;
   a.ws_floats -= ml + plan + recs;
-  const dim3 grid((unsigned)blocks, (unsigned)c.nkv), block(64 * kKv8Waves);
-  const size_t lds = (size_t)(groups + 1) * 4;
-  if (c.page == 128)
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, 4, false, true, KV8_SHARED>), grid, block, lds, st, a);
-  else
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, 4, false, false, KV8_SHARED>), grid, block, lds, st, a);
+  hipLaunchKernelGGL((kv8_shared_kernel<HD>), dim3((unsigned)blocks, (unsigned)c.nkv), dim3(256),
+                     (size_t)(groups + 1) * 4, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   return cols <= 16 * c.nseq   ? launch_kv8_attn_t<HD, 1, KV8_OWN>(a, st)

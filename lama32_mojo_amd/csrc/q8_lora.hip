@@ -25,6 +25,7 @@ namespace {
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // any f32 address
 
 constexpr int kThreads = 256;
+constexpr int kCols = 512;                            // columns of a block, 64-row tiles
 constexpr int kRankTiles = 4;                         // 16-rank tiles of a shrink block
 
 // x as three bf16 terms (truncations, exact), eight values.
@@ -50,36 +51,40 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                  __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Eight weights as terms; c += W x over them, the smallest products first.
+// Eight weights as loaded, and their terms; times(): c += W x, the smallest products
+// first.
 template <bool F32> struct Weights8 {
-  u32x4 t[F32 ? 3 : 1];
+  u32x4 raw[F32 ? 2 : 1];
   __device__ __forceinline__ void load(const uint8_t *w, int64_t elem) {
+    const u32x4 *p = reinterpret_cast<const u32x4 *>(w + (F32 ? 4 : 2) * elem);
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) raw[i] = p[i];
+  }
+  __device__ __forceinline__ void terms(bool in, u32x4 (&t)[F32 ? 3 : 1]) const {
     if constexpr (F32) {
-      const float *p = reinterpret_cast<const float *>(w) + elem;
-      const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
-      const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      const f32x4 a = __builtin_bit_cast(f32x4, raw[0]), b = __builtin_bit_cast(f32x4, raw[1]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = !in ? 0.0f : e < 4 ? a[e] : b[e - 4];
       split3x8(x, t);
     } else {
-      t[0] = *reinterpret_cast<const u32x4 *>(w + 2 * elem);
+      t[0] = in ? raw[0] : u32x4{0, 0, 0, 0};
     }
   }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int k = 0; k < (F32 ? 3 : 1); ++k) t[k] = u32x4{0, 0, 0, 0};
-  }
-  __device__ __forceinline__ f32x4 times(const u32x4 (&x)[3], f32x4 c) const {
+  __device__ __forceinline__ f32x4 times(bool in, const u32x4 (&x)[3], f32x4 c) const {
+    u32x4 t[F32 ? 3 : 1];
+    terms(in, t);
     if constexpr (F32) {
       c = mfma(t[2], x[0], c);
       c = mfma(t[0], x[2], c);
       c = mfma(t[1], x[1], c);
       c = mfma(t[1], x[0], c);
       c = mfma(t[0], x[1], c);
-      return mfma(t[0], x[0], c);
     } else {
       c = mfma(t[0], x[2], c);
       c = mfma(t[0], x[1], c);
-      return mfma(t[0], x[0], c);
     }
+    return mfma(t[0], x[0], c);
   }
 };
 
@@ -125,12 +130,20 @@ __device__ __forceinline__ bool lora_tile(const LoraArgs &a, uint32_t tile, uint
   };
   auto who = [&](int i) {
     const int id = a.id[i];
-    return id >= 0 && id < na && a.rank[id] > 0 ? id : na;
+    return id >= 0 && id < na ? id : na;
   };
+  const int rank0 = t < na ? a.rank[t] : 0;           // (in flight beside the search)
+  // (this thread's first sequence stays in registers)
+  int first0 = 0, who0 = -1;
+  uint32_t n0 = 0;
+  if (t < nseq) {
+    who0 = who(t);
+    n0 = of(t, &first0);
+  }
   for (int i = t; i < nseq; i += kThreads) {
-    int first;
-    const uint32_t n = of(i, &first);
-    if (n) atomicAdd(&count[who(i)], n);
+    int first = first0;
+    const uint32_t n = i == t ? n0 : of(i, &first);
+    if (n) atomicAdd(&count[i == t ? who0 : who(i)], n);
   }
   __syncthreads();
   // the adapter that holds the tile
@@ -157,13 +170,20 @@ __device__ __forceinline__ bool lora_tile(const LoraArgs &a, uint32_t tile, uint
   if (t < TR) rows[t] = 0;
   __syncthreads();
   if (found[0] < 0) return false;
+  if (t == found[0]) found[3] = rank0;
+  else if (t == 0 && found[0] >= kThreads && found[0] < na) found[3] = a.rank[found[0]];
   const uint32_t p0 = (uint32_t)found[1];
   uint32_t base = 0;
   for (int i0 = 0; i0 < nseq; i0 += kThreads) {
     const int i = i0 + t;
     int first = 0;
     uint32_t n = 0;
-    if (i < nseq && who(i) == found[0]) n = of(i, &first);
+    if (i0 == 0) {
+      first = first0;
+      n = who0 == found[0] ? n0 : 0;
+    } else if (i < nseq && who(i) == found[0]) {
+      n = of(i, &first);
+    }
     const uint32_t end = base + block_scan(n, wsum, &all), from = end - n;
     if (n)
       for (int k = 0; k < TR; ++k)
@@ -175,7 +195,7 @@ __device__ __forceinline__ bool lora_tile(const LoraArgs &a, uint32_t tile, uint
   return true;
 }
 
-// A tile's record: adapter, number of rows, the rows; behind the records of all
+// A tile's record: adapter, number of rows, rank, the rows; behind the records of all
 // tiles the parts of A x, [tile][part of K][row][rank].
 template <int TR> constexpr int record_ints() { return TR + 4; }
 template <int TR> __device__ __forceinline__ int *record_at(const LoraArgs &a, int tile) {
@@ -195,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   constexpr int TR = 16 * RT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ uint32_t wsum[kThreads / 64];
-  __shared__ int found[3], rows[TR];
+  __shared__ int found[4], rows[TR];
   __shared__ f32x4 meet[RT == 1 ? 3 : 1][kRankTiles][64];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int col = lane & 15, g4 = lane >> 4;
@@ -204,17 +224,18 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
     if (t == 0 && split == 0 && blockIdx.z == 0) record_at<TR>(a, blockIdx.x)[1] = 0;
     return;
   }
-  const int ad = found[0], n = found[2];
+  const int ad = found[0], n = found[2], rank = ad < a.nadapters ? found[3] : 0;
   if (split == 0 && blockIdx.z == 0) {
     int *rec = record_at<TR>(a, blockIdx.x);
     if (t == 0) {
       rec[0] = ad;
       rec[1] = n;
+      rec[2] = rank;
     }
     if (t < TR) rec[4 + t] = rows[t];
   }
-  if (ad == a.nadapters) return;
-  const int rp = rank8(a.rank[ad], a.max_rank), ranks = a.parts * rp;
+  if (rank <= 0) return;
+  const int rp = rank8(rank, a.max_rank), ranks = a.parts * rp;
   const int q0 = blockIdx.z * kRankTiles;             // this block's first rank tile
   const int nq = min(kRankTiles, (ranks + 15) / 16 - q0);
   if (nq <= 0) return;
@@ -230,27 +251,37 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   f32x4 acc[kRankTiles];
 #pragma unroll
   for (int q = 0; q < kRankTiles; ++q) acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // U steps of 32 at a time, all their loads first
+  constexpr int U = F32 ? 1 : 4, STEP = RT == 1 ? 128 : 32;
   if (RT == 1 || 16 * w < n) {
-    for (int64_t k = k0 + (RT == 1 ? 32 * w : 0); k < k1; k += RT == 1 ? 128 : 32) {
-      const bool in = k + 8 * g4 < k1;                // (m is a multiple of 8)
-      const int64_t kk = in ? k : -8 * g4;            // (row's start: any valid one)
-      const f32x4 xa = *reinterpret_cast<const f32x4_u *>(x + kk);
-      const f32x4 xb = *reinterpret_cast<const f32x4_u *>(x + kk + 4);
-      float xs[8];
+    for (int64_t k = k0 + (RT == 1 ? 32 * w : 0); k < k1; k += U * STEP) {
+      f32x4 xa[U], xb[U];
+      Weights8<F32> wt[U][kRankTiles];
+      bool in[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        xs[e] = in ? xa[e] : 0.0f;
-        xs[4 + e] = in ? xb[e] : 0.0f;
+      for (int u = 0; u < U; ++u) {
+        const int64_t ku = k + u * STEP;
+        in[u] = ku + 8 * g4 < k1;                     // (m is a multiple of 8)
+        const int64_t kk = in[u] ? ku : -8 * g4;      // (row's start: any valid one)
+        xa[u] = *reinterpret_cast<const f32x4_u *>(x + kk);
+        xb[u] = *reinterpret_cast<const f32x4_u *>(x + kk + 4);
+#pragma unroll
+        for (int q = 0; q < kRankTiles; ++q)
+          if (q < nq) wt[u][q].load(A, wrow[q] + kk);
       }
-      u32x4 xt[3];
-      split3x8(xs, xt);
 #pragma unroll
-      for (int q = 0; q < kRankTiles; ++q) {
-        if (q >= nq) continue;
-        Weights8<F32> wt;
-        wt.load(A, wrow[q] + kk);
-        if (!in) wt.zero();
-        acc[q] = wt.times(xt, acc[q]);
+      for (int u = 0; u < U; ++u) {
+        float xs[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          xs[e] = in[u] ? xa[u][e] : 0.0f;
+          xs[4 + e] = in[u] ? xb[u][e] : 0.0f;
+        }
+        u32x4 xt[3];
+        split3x8(xs, xt);
+#pragma unroll
+        for (int q = 0; q < kRankTiles; ++q)
+          if (q < nq) acc[q] = wt[u][q].times(in[u], xt, acc[q]);
       }
     }
   }
@@ -277,17 +308,26 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
 
 // y = base + B (s A x) of a tile and up to `cols` columns of one of the stacked
 // projections: grid (tiles, column blocks).  The block adds the parts of A x and keeps
-// them in LDS as three bf16 terms; an MFMA step takes four (term, eight ranks) pairs, so
-// ranks of 8 and 16 fill it too.  16 columns at a time, four of a row in a lane.
+// them in LDS as three bf16 terms.  A lane loads the weights of eight ranks of a column
+// once for all products of terms; ranks of 8 and 16 leave room in an MFMA step (32
+// ranks), which then takes four or two products.  A wave takes 32 columns at a time;
+// base and the first weights are loaded ahead of the LDS work.  The accumulators hold
+// 16 rows x 64 B; they are turned in LDS to 8 rows x 128 B, whole lines (4126 rows x 28672
+// columns read and written 233 -> 195 us by that alone).
+// Rows lie a multiple of 4 KB apart, as a rule, which is one channel of the L2 for all
+// of them: blocks begin at different columns, so that they do not go from channel to
+// channel together.
 template <bool F32, int RT>
-__global__ __launch_bounds__(kThreads) void lora_expand_kernel(LoraArgs a, int cols) {
-  constexpr int TR = 16 * RT;
+__global__ __launch_bounds__(kThreads, 3) void lora_expand_kernel(LoraArgs a, int cols) {
+  constexpr int TR = 16 * RT, CT = 2, WC = 16 * CT, BC = WC * (kThreads / 64);
+  constexpr int KINDS = F32 ? 6 : 3;                  // products of terms
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ __attribute__((aligned(16))) float turn[kThreads / 64][16][WC + 4];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int col = lane & 15, g4 = lane >> 4;
   const int *rec = record_at<TR>(a, blockIdx.x);
-  const int ad = rec[0], n = rec[1];
-  if (n <= 0) return;
+  const int ad = rec[0], n = rec[1], rp = rank8(rec[2], a.max_rank);
+  if (n <= 0 || (rp == 0 && a.in_place)) return;
   // the part and its columns
   int p = 0, b = blockIdx.y, first = 0;
   while (p < a.parts - 1 && b >= (a.width[p] + cols - 1) / cols) {
@@ -295,31 +335,95 @@ __global__ __launch_bounds__(kThreads) void lora_expand_kernel(LoraArgs a, int c
     first += a.width[p++];
   }
   const int c0 = b * cols, c1 = min(c0 + cols, a.width[p]);
-  if (ad == a.nadapters) {                            // no adapter: base as it is
-    for (int r = 0; r < n; ++r) {
-      const int64_t o = (int64_t)rec[4 + r] * a.ldy + first;
-      for (int c = c0 + t; c < c1; c += kThreads) a.y[o + c] = a.base[o + c];
+  if (rp == 0) {                                      // no adapter: base as it is
+    const int q = (c1 - c0 + 3) / 4, all = n * q;
+    for (int i0 = t; i0 < all; i0 += 4 * kThreads) {
+      f32x4 v[4];
+      int64_t o[4];
+      int left[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * kThreads, all - 1), r = i / q, c = c0 + 4 * (i - r * q);
+        left[u] = i0 + u * kThreads < all ? c1 - c : 0;
+        o[u] = (int64_t)rec[4 + r] * a.ldy + first + c;
+        if (left[u] >= 4) v[u] = *reinterpret_cast<const f32x4_u *>(a.base + o[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (left[u] >= 4) *reinterpret_cast<f32x4_u *>(a.y + o[u]) = v[u];
+        else
+          for (int e = 0; e < left[u]; ++e) a.y[o[u] + e] = a.base[o[u] + e];
+      }
     }
     return;
   }
-  const int rp = rank8(a.rank[ad], a.max_rank);
   const int ld = rp + 8;                              // bf16 of an LDS row
   uint16_t *xs = reinterpret_cast<uint16_t *>(lds);   // [3][TR][ld]
+  const uint8_t *B = a.B + (int64_t)ad * a.b_stride * (F32 ? 4 : 2);
+  // eights of ranks, groups of four of them (a lane's: 4 q + g4 % side), products a step
+  const int chunks = rp / 8, groups = (chunks + 3) / 4;
+  const int shift = chunks > 2 ? 2 : chunks - 1, side = 1 << shift;    // 1, 2 or 4
+  const int steps = ((KINDS << shift) + 3) / 4;
+  // this lane's rows, 8 h + lane / 8 of each 16, and columns 4 (lane % 8) .. of each 32
+  const int rl = lane >> 3, cl = 4 * (lane & 7);
+  int yrow[RT][2];
+#pragma unroll
+  for (int u = 0; u < RT; ++u)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) yrow[u][h] = rec[4 + 16 * u + 8 * h + rl];
+  auto row_at = [&](int u, int h) { return (int64_t)yrow[u][h] * a.ldy + first; };
+
+  f32x4 base[RT][2];
+  Weights8<F32> wt[CT];
+  auto load_weights = [&](int c, int q) {
+    const int j = 8 * min(4 * q + (g4 & (side - 1)), chunks - 1);
+#pragma unroll
+    for (int v = 0; v < CT; ++v) wt[v].load(B, (int64_t)(first + min(c + 16 * v + col, c1 - 1)) * rp + j);
+  };
+  auto load = [&](int c) {
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int left = c1 - c - cl;
+        base[u][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (16 * u + 8 * h + rl < n) {
+          const float *q = a.base + row_at(u, h) + c + cl;
+          if (left >= 4) base[u][h] = *reinterpret_cast<const f32x4_u *>(q);
+          else
+            for (int e = 0; e < 3; ++e)
+              if (e < left) base[u][h][e] = q[e];
+        }
+      }
+    load_weights(c, 0);
+  };
+  const int its = (c1 - c0 + BC - 1) / BC;
+  int it = (int)((blockIdx.x + blockIdx.y) % (unsigned)its);
+  auto column = [&](int i) { return c0 + BC * i + WC * w; };
+  load(column(it));
+
   const float s = a.scale[ad];
-  for (int i = t; i < TR * (rp / 8); i += kThreads) {
-    const int r = i / (rp / 8), j = 8 * (i % (rp / 8));
+  for (int i = t; i < TR * chunks; i += kThreads) {
+    const int r = i / chunks, j = 8 * (i - r * chunks);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
     if (r < n) {
-      for (int z = 0; z < a.splits; ++z) {
-        const float *q = part_at<TR>(a, blockIdx.x, z) + (int64_t)r * a.ranks + p * rp + j;
-        const f32x4 u0 = *reinterpret_cast<const f32x4 *>(q), u1 = *reinterpret_cast<const f32x4 *>(q + 4);
+      const float *q = part_at<TR>(a, blockIdx.x, 0) + (int64_t)r * a.ranks + p * rp + j;
+      const int64_t next = (int64_t)TR * a.ranks;
+      for (int z0 = 0; z0 < a.splits; z0 += 4) {
+        f32x4 u[4][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] += u0[e];
-          v[4 + e] += u1[e];
-        }
+        for (int z = 0; z < 4; ++z)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            u[z][h] = *reinterpret_cast<const f32x4 *>(q + min(z0 + z, a.splits - 1) * next + 4 * h);
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (z0 + z < a.splits) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += u[z][e / 4][e % 4];
+          }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= s;
@@ -330,62 +434,70 @@ __global__ __launch_bounds__(kThreads) void lora_expand_kernel(LoraArgs a, int c
     for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4 *>(xs + ((int64_t)k * TR + r) * ld + j) = o[k];
   }
   __syncthreads();
-  const uint8_t *B = a.B + (int64_t)ad * a.b_stride * (F32 ? 4 : 2);
-  const int chunks = rp / 8;
-  const int pairs = (F32 ? 6 : 3) * chunks, steps = (pairs + 3) / 4;
-  int64_t yrow[RT];
+
+  for (int done = 0; done < its; ++done) {
+    const int c = column(it);
+    f32x4 d[RT][CT];
 #pragma unroll
-  for (int u = 0; u < RT; ++u) yrow[u] = (int64_t)rec[4 + 16 * u + col] * a.ldy + first;
-  for (int c = c0 + 16 * w; c < c1; c += 16 * (kThreads / 64)) {
-    const int64_t brow = (int64_t)(first + min(c + col, c1 - 1)) * rp;
-    const int cc = c + 4 * g4, left = c1 - cc;        // this lane's columns
-    f32x4 acc[RT];
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int v = 0; v < CT; ++v) d[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < groups; ++q) {
+      const int chunk = 4 * q + (g4 & (side - 1));
+      u32x4 tm[CT][F32 ? 3 : 1];
+#pragma unroll
+      for (int v = 0; v < CT; ++v) wt[v].terms(chunk < chunks, tm[v]);
+      if (q + 1 < groups) load_weights(c, q + 1);
+      // terms of x and of the weights, the smallest products first; f32:
+      // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+#pragma unroll
+      for (int z = 0; z < KINDS; ++z) {
+        if (z >= steps) continue;
+        const int kind = (z << (2 - shift)) + (g4 >> shift);
+        const bool in = kind < KINDS && chunk < chunks;
+        const int xt = !in ? 0 : F32 ? 0x021010 >> (4 * (5 - kind)) & 3 : 2 - kind;
+        const int wk = in && F32 ? 0x201100 >> (4 * (5 - kind)) & 3 : 0;
+        u32x4 wv[CT];
+#pragma unroll
+        for (int v = 0; v < CT; ++v) {
+          wv[v] = tm[v][0];
+          if constexpr (F32) wv[v] = wk == 0 ? tm[v][0] : wk == 1 ? tm[v][1] : tm[v][2];
+        }
+#pragma unroll
+        for (int u = 0; u < RT; ++u) {
+          u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + (xt * TR + 16 * u + col) * ld + 8 * (in ? chunk : 0));
+          if (!in) xv = u32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int v = 0; v < CT; ++v) d[u][v] = mfma(wv[v], xv, d[u][v]);
+        }
+      }
+    }
+    f32x4 out[RT][2];
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (16 * u + col < n) {
-        const float *q = a.base + yrow[u] + cc;
-        if (left >= 4) acc[u] = *reinterpret_cast<const f32x4_u *>(q);
+      // (one wave's own LDS, whose operations go in order)
+#pragma unroll
+      for (int v = 0; v < CT; ++v) *reinterpret_cast<f32x4 *>(&turn[w][col][16 * v + 4 * g4]) = d[u][v];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        out[u][h] = *reinterpret_cast<const f32x4 *>(&turn[w][8 * h + rl][cl]) + base[u][h];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    it = it + 1 < its ? it + 1 : 0;
+    if (done + 1 < its) load(column(it));
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int left = c1 - c - cl;
+        if (16 * u + 8 * h + rl >= n) continue;
+        float *q = a.y + row_at(u, h) + c + cl;
+        if (left >= 4) *reinterpret_cast<f32x4_u *>(q) = out[u][h];
         else
           for (int e = 0; e < 3; ++e)
-            if (e < left) acc[u][e] = q[e];
+            if (e < left) q[e] = out[u][h][e];
       }
-    }
-    f32x4 d[RT];
-#pragma unroll
-    for (int u = 0; u < RT; ++u) d[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int z = 0; z < steps; ++z) {
-      // pair: the smallest products first
-      const int pair = 4 * z + g4;
-      const bool in = pair < pairs;
-      const int kind = in ? pair / chunks : 0, j = in ? 8 * (pair % chunks) : 0;
-      // terms of x and of the weights: f32 (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-      const int xt = F32 ? (0x021010 >> (4 * (5 - kind))) & 3 : 2 - kind;
-      Weights8<F32> wt;
-      wt.load(B, brow + j);
-      u32x4 wv = wt.t[0];
-      if constexpr (F32) {
-        const int wk = (0x201100 >> (4 * (5 - kind))) & 3;
-        wv = wk == 0 ? wt.t[0] : wk == 1 ? wt.t[1] : wt.t[2];
-      }
-      if (!in) wv = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int u = 0; u < RT; ++u) {
-        u32x4 xv = *reinterpret_cast<const u32x4 *>(xs + ((int64_t)xt * TR + 16 * u + col) * ld + j);
-        if (!in) xv = u32x4{0, 0, 0, 0};
-        d[u] = mfma(wv, xv, d[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < RT; ++u) {
-      if (16 * u + col >= n) continue;
-      acc[u] += d[u];
-      float *q = a.y + yrow[u] + cc;
-      if (left >= 4) *reinterpret_cast<f32x4_u *>(q) = acc[u];
-      else
-        for (int e = 0; e < 3; ++e)
-          if (e < left) q[e] = acc[u][e];
-    }
   }
 }
 
@@ -403,7 +515,7 @@ hipError_t launch_lora_t(LoraArgs a, int64_t ws_floats, hipStream_t st) {
   const int64_t per = record_ints<TR>() + (int64_t)a.splits * TR * a.ranks;
   const int64_t most = std::min<int64_t>(ws_floats / per, 65535);
   if (most < 1) return hipErrorInvalidValue;
-  const int cols = RT == 1 ? 512 : 2048;
+  const int cols = RT == 1 ? 128 : kCols;
   int blocks = 0;
   for (int p = 0; p < a.parts; ++p) blocks += (a.width[p] + cols - 1) / cols;
   const size_t lds0 = (size_t)(a.nadapters + 1) * 4, lds1 = (size_t)3 * TR * (a.max_rank + 8) * 2;

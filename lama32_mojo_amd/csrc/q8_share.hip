@@ -87,6 +87,7 @@ __global__ __launch_bounds__(kKv8ShareSeq) void share_group_kernel(Kv8Args c, in
   const int me = who[t], p = pages[t];
   if (me >= 0) {
     int members = 0;
+#pragma unroll 8
     for (int j = 0; j < nseq; ++j) members += who[j] == me && pages[j] >= p;
     // (members below 2^10, pages at most 2^26: 36 bits and 28; the longest of equal ones)
     atomicMax(&best[me], (unsigned long long)(members - 1) * p << 28 | (unsigned)p);
@@ -103,20 +104,22 @@ __global__ __launch_bounds__(kKv8ShareSeq) void share_group_kernel(Kv8Args c, in
   __syncthreads();
   int g = 0;
   uint32_t at = 0;                                    // (unsigned: nonsense in cu may wrap)
-  for (int j = 0; j < nseq; ++j)
-    if (in && j < me) g += index[j];
+#pragma unroll 8
+  for (int j = 0; j < nseq; ++j) g += j < me ? index[j] : 0;
+  g = in ? g : 0;
   in = in && g < kKv8ShareGroups;
   __syncthreads();
   if (!in) who[t] = -1;
   __syncthreads();
-  for (int j = 0; j < nseq; ++j) {
-    at += in && who[j] == me && j < t ? (uint32_t)rows[j] : 0;
-  }
-  // the rows of the groups before
+  // and the rows of the groups before
   uint32_t before = 0, all = 0;
+#pragma unroll 8
   for (int j = 0; j < nseq; ++j) {
-    if (in && who[j] >= 0 && who[j] < me) before += (uint32_t)rows[j];
-    if (who[j] >= 0) all += (uint32_t)rows[j];
+    const int wj = who[j];
+    const uint32_t n = (uint32_t)rows[j];
+    at += wj == me && j < t ? n : 0;
+    before += wj >= 0 && wj < me ? n : 0;
+    all += wj >= 0 ? n : 0;
   }
   if (t == 0) groups = 0;
   __syncthreads();
@@ -145,7 +148,7 @@ hipError_t launch_kv8_share(const Kv8Args &c, int *share, hipStream_t st) {
   hipLaunchKernelGGL(share_find_kernel, dim3((unsigned)c.nseq), dim3(kThreads), 0, st, c, share);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(share_group_kernel, dim3(1), dim3(kKv8ShareSeq), 0, st, c, share);
+  hipLaunchKernelGGL(share_group_kernel, dim3(1), dim3((unsigned)((c.nseq + 63) / 64 * 64)), 0, st, c, share);
   return hipGetLastError();
 }
 
