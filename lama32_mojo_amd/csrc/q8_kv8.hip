@@ -453,10 +453,10 @@ struct Kv8Plan {
 };
 
 // What q8_kv8_share found: the group of each sequence (-1: none), the tokens that it
-// takes from the group, the place of its first row in the list of rows; the groups'
-// leaders and the places of their rows; the list.  Read as if it could hold anything.
+// takes from the group and the place of its first row in the list of rows; the groups'
+// leaders, tokens and places of their rows; the list.  Read as if it could hold anything.
 struct Kv8ShareAt {
-  const int *group, *tok, *pos, *lead, *gcu, *row;
+  const int *group, *tok, *pos, *lead, *gtok, *gcu, *row;
   int groups;
 };
 Q8_HD int kv8_most_groups(int64_t nseq, int64_t rows) {
@@ -464,14 +464,18 @@ Q8_HD int kv8_most_groups(int64_t nseq, int64_t rows) {
   return (int)(n < kKv8ShareGroups ? n : kKv8ShareGroups);
 }
 __device__ __forceinline__ Kv8ShareAt kv8_share_at(const Kv8Args &c, const int *p) {
-  const int nseq = (int)c.nseq;
-  return {p + 1,         p + 1 + nseq,          p + 1 + 2 * nseq,     p + 1 + 3 * nseq,
-          p + 1 + 4 * nseq, p + 2 + 5 * (int64_t)nseq, clamp_i(p[0], 0, kv8_most_groups(c.nseq, c.rows))};
+  const int64_t n = c.nseq;
+  return {p + 1,         p + 1 + n,     p + 1 + 2 * n, p + 1 + 3 * n,
+          p + 1 + 4 * n, p + 1 + 5 * n, p + 2 + 6 * n, clamp_i(p[0], 0, kv8_most_groups(n, c.rows))};
 }
-// Tokens of sequence i that its group's part of the attention covers, whole pages.
+// Shared tokens as read: whole pages of what the table can hold.
+__device__ __forceinline__ int kv8_tokens(const Kv8Args &c, int tok) {
+  return clamp_i(tok, 0, c.maxpages * c.page) & ~(c.page - 1);
+}
+// Tokens of sequence i that its group's part of the attention covers.
 __device__ __forceinline__ int kv8_shared_tokens(const Kv8Args &c, const Kv8ShareAt &sh, int i) {
-  const int g = sh.group[i];
-  return g >= 0 && g < sh.groups ? clamp_i(sh.tok[i], 0, c.maxpages * c.page) & ~(c.page - 1) : 0;
+  const int g = sh.group[i], tok = sh.tok[i];
+  return g >= 0 && g < sh.groups ? kv8_tokens(c, tok) : 0;
 }
 
 // What of a sequence a launch goes through: all its keys, or the ones behind the
@@ -541,6 +545,7 @@ __device__ __forceinline__ int kv8_seq_of(const int *pre, int nseq, int u) {
 constexpr int kKv8WholeUnits = 12;
 constexpr int kKv8WholeBlocks = 256;
 constexpr int kKv8Waves = 4;              // waves of a block (WHOLE: 8)
+constexpr int kKv8ShareCols = 16 * kKv8Waves;   // columns of a row tile of the shared tokens
 constexpr int kKv8PlanSeq = 1024;         // sequences of a launch (16 KB of LDS for the plan)
 
 // Record of a run and KV head: o[NC][HD] unnormalised, m[NC], l[NC] (of the
@@ -561,61 +566,41 @@ struct Kv8Place {
   int k0;                                // the first unit's first key
 };
 
-// The groups' part: a block goes through `per` units at most of one row tile of a
-// group, cut so that about a.shared_target blocks have work.  base[g] .. base[g+1]:
-// the blocks of group g, its tiles' cuts one after the other; base has groups + 1
-// entries in LDS.  Returns per.
-__device__ __forceinline__ void kv8_group(const Kv8Args &c, const Kv8ShareAt &sh, int g, int cols, int *n,
-                                          int *tiles, int *units) {
-  const int lead = clamp_i(sh.lead[g], 0, c.nseq - 1);
-  const int a = clamp_i(sh.gcu[g], 0, c.rows), b = clamp_i(sh.gcu[g + 1], 0, c.rows);
-  *n = b > a ? b - a : 0;
-  *tiles = (int)(((int64_t)*n * (c.nheads / c.nkv) + cols - 1) / cols);
-  *units = (kv8_shared_tokens(c, sh, lead) + kKv8Unit - 1) / kKv8Unit;
-}
-template <int NT>
-__device__ __forceinline__ int kv8_group_plan(const Kv8Args &c, const Kv8ShareAt &sh, int cols, int target,
-                                              int *base, int *wsum) {
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  int per = 1;
-  if (t == 0) base[0] = 0;
+// The groups' part, a group a lane (whole waves): a block goes through `per` units at most
+// of one row tile of a group, cut so that about `target` blocks have work.  The blocks of
+// group g are base .. base + tiles * cuts - 1, its tiles' cuts one after the other.
+struct Kv8Groups {
+  int lead, tokens, row0, n, units, cuts, base;
+  int per, blocks;                       // the same in all lanes
+};
+__device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8ShareAt &sh, int target) {
+  const int lane = threadIdx.x & 63, at = clamp_i(lane, 0, c.nseq - 1);
+  Kv8Groups g;
+  g.lead = clamp_i(sh.lead[at], 0, c.nseq - 1);
+  g.tokens = kv8_tokens(c, sh.gtok[at]);
+  g.row0 = clamp_i(sh.gcu[at], 0, c.rows);
+  const int end = clamp_i(sh.gcu[at + 1], 0, c.rows);
+  g.n = lane < sh.groups && end > g.row0 ? end - g.row0 : 0;
+  g.units = (g.tokens + kKv8Unit - 1) / kKv8Unit;
+  const int64_t tiles = ((int64_t)g.n * (c.nheads / c.nkv) + kKv8ShareCols - 1) / kKv8ShareCols;
+  const int64_t work = tiles * g.units;
+  int u = work < kKv8MaxUnits ? (int)work : kKv8MaxUnits;
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {   // the units of all, then the blocks of each
-    int sum = 0;
-    for (int g0 = 0; g0 < sh.groups; g0 += NT) {
-      const int g = g0 + t;
-      int u = 0;
-      if (g < sh.groups) {
-        int n, tiles, units;
-        kv8_group(c, sh, g, cols, &n, &tiles, &units);
-        const int64_t v = (int64_t)tiles * (pass ? (units + per - 1) / per : units);
-        u = v < kKv8MaxUnits ? (int)v : kKv8MaxUnits;
-      }
+  for (int d = 1; d < 64; d <<= 1) u = kv8_add(u, __shfl_xor(u, d));
+  g.per = kv8_units_per_block(u, target, 1);
+  g.cuts = (g.units + g.per - 1) / g.per;
+  const int64_t blocks = tiles * g.cuts;
+  const int mine = blocks < kKv8MaxUnits ? (int)blocks : kKv8MaxUnits;
+  u = mine;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(u, d);
-        if (lane >= d) u = kv8_add(u, o);
-      }
-      if (lane == 63) wsum[w] = u;
-      __syncthreads();
-      int all = 0;
-#pragma unroll
-      for (int x = 0; x < NT / 64; ++x) {
-        u = kv8_add(u, x < w ? wsum[x] : 0);
-        all = kv8_add(all, wsum[x]);
-      }
-      if (pass && g < sh.groups) base[g + 1] = kv8_add(sum, u);
-      sum = kv8_add(sum, all);
-      __syncthreads();
-    }
-    if (pass == 0) per = kv8_units_per_block(sum, target, 1);
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(u, d);
+    if (lane >= d) u = kv8_add(u, o);
   }
-  __syncthreads();                        // (base, also where there are no groups)
-  return per;
+  g.base = u - mine;
+  g.blocks = __builtin_amdgcn_readlane(u, 63);
+  return g;
 }
-constexpr int kKv8SharedCols = 64;       // columns of a group's row tile
-constexpr int kKv8SharedBlocks = 768;    // three a CU
-
 //
 // WIDE (pages of 128 tokens, runs): a V column of a page is one 128-byte line,
 // of which a unit takes half.  The even unit's load brings the odd unit's half
@@ -952,8 +937,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
 }
 
 // ---- the shared tokens of groups ------------------------------------------------------
-// A block of 4 waves takes a row tile of 64 columns (row of the group, query head), 16 a
-// wave, over a cut of the group's shared tokens; all columns see all of them.  A unit's K
+// A block takes a row tile of 64 columns (row of the group, query head), 16 a wave, over a cut of the group's shared tokens; all columns see all of them.  A unit's K
 // codes and its V, as bf16 once for all waves, go through LDS in the layout of the MFMA
 // operands (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in
 // flight beside this one's products.  Scores, probabilities and products are those of
@@ -961,11 +945,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
 // operations a unit and 16 columns, 190 of them for codes -> bf16 if every wave did that
 // for itself).
 template <int HD>
-__global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
-  constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8SharedCols, NW = 4;
-  constexpr int KF = 4 * HH / NW, VF = DT / NW;        // fragments that a wave stages
-  extern __shared__ int base[];                        // the blocks of the groups
-  __shared__ int wsum[NW];
+__global__ __launch_bounds__(64 * kKv8Waves, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
+  constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8ShareCols;
+  constexpr int KF = 4 * HH / kKv8Waves, VF = DT / kKv8Waves;   // fragments that a wave stages
   __shared__ __attribute__((aligned(16))) u32x4 kbuf[2][4 * HH][64], vbuf[2][2 * DT][64];
   const Kv8Args &c = a.c;
   const int t = threadIdx.x, lane = t & 63, col = lane & 15, g4 = lane >> 4;
@@ -977,19 +959,16 @@ __global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
   const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
   const float qscale = 1.44269504088896341f / sqrtf((float)HD);
   const Kv8ShareAt sh = kv8_share_at(c, a.share);
-  const int per = kv8_group_plan<64 * NW>(c, sh, NC, a.shared_target, base, wsum);
-  if (blockIdx.x == 0 && g == 0) {        // the join reads the plan
-    for (int i = t; i <= sh.groups; i += 64 * NW) a.shared_plan[1 + i] = base[i];
-    if (t == 0) a.shared_plan[0] = per;
-  }
+  const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
   const int b = blockIdx.x;
-  if (b >= base[sh.groups]) return;       // (the whole block)
-  const int i = kv8_seq_of(base, sh.groups, b);
-  int n, tiles, units;
-  kv8_group(c, sh, i, NC, &n, &tiles, &units);
-  const int cuts = max(1, (units + per - 1) / per);
-  const int lead = clamp_i(sh.lead[i], 0, c.nseq - 1), tokens = kv8_shared_tokens(c, sh, lead);
-  const int rt = (b - base[i]) / cuts, t0 = (b - base[i]) % cuts * per, t1 = min(units, t0 + per);
+  if (b >= gs.blocks) return;             // (the whole block)
+  // the last group that begins at this block or before and has any
+  const int i = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(gs.n > 0 && gs.cuts > 0 && gs.base <= b));
+  const int lead = __builtin_amdgcn_readlane(gs.lead, i), tokens = __builtin_amdgcn_readlane(gs.tokens, i);
+  const int n = __builtin_amdgcn_readlane(gs.n, i), row0 = __builtin_amdgcn_readlane(gs.row0, i);
+  const int cuts = __builtin_amdgcn_readlane(gs.cuts, i), local = b - __builtin_amdgcn_readlane(gs.base, i);
+  const int units = __builtin_amdgcn_readlane(gs.units, i);
+  const int rt = local / cuts, t0 = local % cuts * gs.per, t1 = min(units, t0 + gs.per);
   const int *tab = c.tab + (int64_t)lead * c.maxpages;
 
   // what a wave stages: K fragments KF w .. (tt = f / HH, dims 64 (f % HH) + 16 g4 ..) and
@@ -1036,7 +1015,7 @@ __global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
 
   // this lane's digits of q
   const int lin = rt * NC + cc, j = lin / grp;
-  const int row = clamp_i(sh.row[clamp_i(sh.gcu[i], 0, c.rows) + (j < n ? j : 0)], 0, c.rows - 1);
+  const int row = clamp_i(sh.row[row0 + (j < n ? j : 0)], 0, c.rows - 1);
   const float *q = a.q + (int64_t)row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
   u32x4 qd[4][HH];
   float qs;
@@ -1066,7 +1045,8 @@ __global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
       load_ids(kt + 2);
     }
     f32x4 s[4];
-    const float sc = qs * ks, vsc = vs;
+    const float sc = qs * ks;
+    __builtin_amdgcn_s_setprio(1);        // the matrix cores' work first, VALU beside it
     if (__builtin_amdgcn_ballot_w64(fabsf(sc) > kv8_exact_up_to<HD>()) == 0) {
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
@@ -1111,36 +1091,49 @@ __global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
         }
       }
     }
-    // (the last unit's keys behind the shared tokens: a page of 16 or 32 may end there)
-    const int key0 = kt * kKv8Unit + 16 * g4;
+    __builtin_amdgcn_s_setprio(0);
+    // A lane's 16 keys are of one page, so its scores have one scale.  The last unit's keys
+    // behind the shared tokens (a page of 16 or 32 may end there) are a path of their own.
+    const int left = tokens - (kt * kKv8Unit + 16 * g4);        // this lane's keys, at most 16
     const bool masked = kt * kKv8Unit + kKv8Unit > tokens;
-    float tmax = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        float x = s[tt][v] * sc;
-        if (masked) x = key0 + 4 * tt + v < tokens ? x : -INFINITY;
-        s[tt][v] = x;
-        tmax = fmaxf(tmax, x);
-      }
+      for (int v = 0; v < 4; ++v) top = fmaxf(top, s[tt][v]);
+    if (masked) {
+      top = -INFINITY;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, 4 * tt + v < left ? s[tt][v] : -INFINITY);
+    }
+    float tmax = top == -INFINITY ? top : top * sc;
     tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
     tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+    // (the maximum rounded to an integer, see kv8_attn_kernel)
     const float mnew = fmaxf(m, __builtin_rintf(tmax));
     const float ms = mnew == -INFINITY ? 0.0f : mnew;
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
     m = mnew;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) s[tt][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][v], sc, -ms));
+    float vsc = vs;
+    if (masked) {
+      // (a page of NaN scale counts for the rows that see one of its keys)
+      if (left <= 0) vsc = 0.0f;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[tt][v] = 4 * tt + v < left ? s[tt][v] : 0.0f;
+    }
     float ps = 0.0f;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float p = __builtin_amdgcn_exp2f(s[tt][v] - ms);
-        ps += p;
-        float x = p * vsc;
-        if (masked) x = key0 + 4 * tt + v < tokens ? x : 0.0f;
-        s[tt][v] = x;
-      }
+      for (int v = 0; v < 4; ++v) ps += s[tt][v];
     l = __builtin_fmaf(l, alpha, ps);
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
 #pragma unroll
@@ -1151,16 +1144,24 @@ __global__ __launch_bounds__(256, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
       u32x4 pf[3];
       float x[8];
 #pragma unroll
-      for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3];
+      for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3] * vsc;
       split3x8(x, pf);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, vbuf[at][2 * d + e][lane]);
+      for (int d0 = 0; d0 < DT; d0 += 4) {
+        u32x4 va[4];
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, pf[k]), o[d], 0, 0, 0);
+        for (int d = 0; d < 4; ++d) va[d] = vbuf[at][2 * (d0 + d) + e][lane];
+#pragma unroll
+        for (int k = 2; k >= 0; --k)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, va[d]),
+                                                                __builtin_bit_cast(bf16x8_t, pf[k]), o[d0 + d],
+                                                                0, 0, 0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     // (the other buffer's last readers are behind the barrier before this unit)
     if (kt + 1 < t1) {
       store(at ^ 1);
@@ -1199,21 +1200,19 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   const int lo = at.i, j = row - at.r0;
   Kv8Seq sq = kv8_seq(at.r0, at.r1, at.len, c.rows, c.maxpages * c.page, grp, NC);
   // the group's records of this row: cuts of them, from block `cut0` on
-  Kv8ShareAt sh;
   int group = -1, cuts = 0, cut0 = 0, place = 0;
   if constexpr (PART == KV8_OWN) {
-    sh = kv8_share_at(c, a.share);
-    const int k0 = kv8_shared_tokens(c, sh, lo);
-    kv8_from(sq, k0, c.maxpages * c.page);
-    group = sh.group[lo];
+    const Kv8ShareAt sh = kv8_share_at(c, a.share);
+    const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
+    const int pos = sh.pos[lo];
+    kv8_from(sq, kv8_shared_tokens(c, sh, lo), c.maxpages * c.page);
+    group = __builtin_amdgcn_readfirstlane(sh.group[lo]);
     if (group < 0 || group >= sh.groups) group = -1;
     if (group >= 0) {
-      int n, tiles, units;
-      kv8_group(c, sh, group, kKv8SharedCols, &n, &tiles, &units);
-      const int sper = max(1, a.shared_plan[0]);
-      cuts = (units + sper - 1) / sper;
-      cut0 = a.shared_plan[1 + group];
-      place = clamp_i((int64_t)sh.pos[lo] + j - clamp_i(sh.gcu[group], 0, c.rows), 0, max(0, n - 1));
+      cuts = __builtin_amdgcn_readlane(gs.cuts, group);
+      cut0 = __builtin_amdgcn_readlane(gs.base, group);
+      place = clamp_i((int64_t)pos + j - __builtin_amdgcn_readlane(gs.row0, group), 0,
+                      max(0, __builtin_amdgcn_readlane(gs.n, group) - 1));
     }
   }
   if (j < 0 || j >= sq.n) return;             // behind the last sequence
@@ -1233,30 +1232,40 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
     if constexpr (PART == KV8_OWN) {
       if (on && group >= 0) {
         // the group's cuts, then the row's own run where it has one
-        const int slin = place * grp + hh, cols = kKv8SharedCols;
+        const int slin = place * grp + hh;
+        constexpr int cols = kKv8ShareCols;
         const int64_t first = (int64_t)cut0 + (int64_t)(slin / cols) * cuts;
         const int all = cuts + (b0 == b1 && sq.key_units > 0);
-        for (int z = grp_id; z < all; z += sg) {
-          float zm, zl, w = 1.0f;
-          const float *src;
-          if (z < cuts) {
-            const int64_t b = min(first + z, (int64_t)a.shared_blocks - 1);
-            const float *r = a.shared_rec + (b * c.nkv + g) * kv8_record<HD, kKv8SharedCols>();
-            zm = r[cols * HD + slin % cols];
-            zl = r[cols * HD + cols + slin % cols];
-            src = r + slin % cols * HD + d;
-          } else {
-            const int64_t h = (int64_t)row * c.nheads + g * grp + hh;
-            zm = a.ml[2 * h];
-            w = zl = a.ml[2 * h + 1];
-            src = a.out + h * HD + d;
-          }
-          const f32x4 zo = *reinterpret_cast<const f32x4_u *>(src);
-          const float mx = fmaxf(m, zm), ms = mx == -INFINITY ? 0.0f : mx;
-          const float f0 = __builtin_amdgcn_exp2f(m - ms), f = __builtin_amdgcn_exp2f(zm - ms);
-          l = __builtin_fmaf(f, zl, l * f0);
+        const int64_t h = (int64_t)row * c.nheads + g * grp + hh;
+        for (int z0 = grp_id; z0 < all; z0 += 4 * sg) {
+          float zm[4], zl[4], zw[4];
+          f32x4 zo[4];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(f * w, zo[v], o[v] * f0);
+          for (int x = 0; x < 4; ++x) {
+            const int z = z0 + x * sg < all ? z0 + x * sg : z0;
+            const int64_t rb = min(first + z, (int64_t)a.shared_blocks - 1);
+            const float *r = a.shared_rec + (rb * c.nkv + g) * kv8_record<HD, cols>();
+            const bool rec = z < cuts;
+            zm[x] = rec ? r[cols * HD + slin % cols] : a.ml[2 * h];
+            zl[x] = rec ? r[cols * HD + cols + slin % cols] : a.ml[2 * h + 1];
+            zw[x] = rec ? 1.0f : zl[x];
+            zo[x] = *reinterpret_cast<const f32x4_u *>(rec ? r + slin % cols * HD + d : a.out + h * HD + d);
+          }
+          float mx = m;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx = fmaxf(mx, zm[x]);
+          const float ms = mx == -INFINITY ? 0.0f : mx;
+          const float f0 = __builtin_amdgcn_exp2f(m - ms);
+          l *= f0;
+          o *= f0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (z0 + x * sg >= all) continue;
+            const float f = __builtin_amdgcn_exp2f(zm[x] - ms), fw = f * zw[x];
+            l = __builtin_fmaf(f, zl[x], l);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(fw, zo[x][v], o[v]);
+          }
           m = mx;
         }
       }
@@ -1394,29 +1403,29 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
 
 // The groups' part (a row tile of 64 columns cut over blocks), each sequence's own
 // part, and the merge that joins them.
-template <int HD>
-static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
+template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
   const Kv8Args &c = a.c;
+  constexpr int NC = kKv8ShareCols;
   const int64_t grp = c.nheads / c.nkv, cols = c.rows * grp;
   const int64_t groups = kv8_most_groups(c.nseq, c.rows);
-  const int64_t tiles = cols / kKv8SharedCols + groups, rec = c.nkv * kv8_record<HD, kKv8SharedCols>();
-  // maxima and sums per (row, head), the groups' plan and records (three quarters of
-  // the space at most), then what the sequences' own parts leave
-  const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4, plan = (groups + 5) / 4 * 4;
-  const int64_t room = (a.ws_floats / 4 * 3 - ml - plan) / rec;
-  const int64_t want = (kKv8SharedBlocks + c.nkv - 1) / c.nkv;
+  const int64_t tiles = cols / NC + groups, rec = c.nkv * kv8_record<HD, NC>();
+  // maxima and sums per (row, head), the groups' records (three quarters of the space
+  // at most), then what the sequences' own parts leave
+  const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4;
+  const int64_t room = (a.ws_floats / 4 * 3 - ml) / rec;
+  // as many blocks as are resident: three a compute unit
+  const int64_t want = (768 + c.nkv - 1) / c.nkv;
   a.shared_target = (int)std::min(want, room - tiles);
   // (more rows than there is room for: every sequence for itself)
   if (a.shared_target < std::min<int64_t>(want, 8) || groups == 0) return launch_kv8_attention(a, st);
   const int64_t blocks = a.shared_target + tiles, recs = blocks * rec;
   a.ml = a.ws;
-  a.shared_plan = reinterpret_cast<int *>(a.ws + ml);
-  a.shared_rec = a.ws + ml + plan;
+  a.shared_rec = a.ws + ml;
   a.shared_blocks = (int)blocks;
-  a.ws += ml + plan + recs;
-  a.ws_floats -= ml + plan + recs;
-  hipLaunchKernelGGL((kv8_shared_kernel<HD>), dim3((unsigned)blocks, (unsigned)c.nkv), dim3(256),
-                     (size_t)(groups + 1) * 4, st, a);
+  a.ws += ml + recs;
+  a.ws_floats -= ml + recs;
+  hipLaunchKernelGGL(kv8_shared_kernel<HD>, dim3((unsigned)blocks, (unsigned)c.nkv), dim3(64 * kKv8Waves), 0, st,
+                     a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   return cols <= 16 * c.nseq   ? launch_kv8_attn_t<HD, 1, KV8_OWN>(a, st)

@@ -294,7 +294,6 @@ struct Kv8AttnArgs {
   // shared prefixes: what q8_kv8_share wrote; the others are set by the launch
   const int *share;
   float *ml, *shared_rec;
-  int *shared_plan;
   int shared_target, shared_blocks;
 };
 // Sequences of one call: their unit counts are summed in LDS.
@@ -304,7 +303,7 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st);
 constexpr int kKv8ShareSeq = 1024;
 // Groups of a call: their row tiles need records, whose number the host bounds.
 constexpr int kKv8ShareGroups = 64;
-inline int64_t kv8_share_ints(int64_t nseq, int64_t rows) { return 5 * nseq + 2 + rows; }
+inline int64_t kv8_share_ints(int64_t nseq, int64_t rows) { return 6 * nseq + 2 + rows; }
 hipError_t launch_kv8_attention_shared(const Kv8AttnArgs &a, hipStream_t st);
 // (of c: the int32 arrays, their sizes, npages and page)
 hipError_t launch_kv8_share(const Kv8Args &c, int *share, hipStream_t st);

@@ -2,9 +2,9 @@
 // tokens: what q8_kv8_attention_shared reads once for all of them.
 //
 // Written, int32: the number of groups G; group[nseq]; tokens[nseq]; pos[nseq], the
-// place of the sequence's first row in the list of rows; lead[nseq], of group g at g;
-// gcu[nseq + 1], group g's rows being the places gcu[g] .. gcu[g+1]-1; row[rows], the
-// list.  Bound: two launches and their chains of dependent reads (tables of 8000 pages
+// place of the sequence's first row in the list of rows; lead[nseq] and gtokens[nseq],
+// of group g at g; gcu[nseq + 1], group g's rows being the places gcu[g] .. gcu[g+1]-1;
+// row[rows], the list.  Bound: two launches and their chains of dependent reads (tables of 8000 pages
 // a sequence are 2 MB for 64).
 #include "q8_launch.h"
 #include "q8_ragged.h"
@@ -66,29 +66,37 @@ __global__ __launch_bounds__(kThreads) void share_find_kernel(Kv8Args c, int *sh
 // save the most reads, (members with p pages and more in common - 1) * p, are the
 // group's.
 __global__ __launch_bounds__(kKv8ShareSeq) void share_group_kernel(Kv8Args c, int *share) {
-  __shared__ int who[kKv8ShareSeq], pages[kKv8ShareSeq], rows[kKv8ShareSeq], index[kKv8ShareSeq];
+  // (read four at a time; behind nseq: no sequence)
+  __shared__ __attribute__((aligned(16))) int who[kKv8ShareSeq], pages[kKv8ShareSeq], rows[kKv8ShareSeq],
+      index[kKv8ShareSeq];
   __shared__ unsigned long long best[kKv8ShareSeq];
   __shared__ int groups;
   const int t = threadIdx.x, nseq = (int)c.nseq;
   int *group = share + 1, *tok = share + 1 + nseq, *pos = share + 1 + 2 * nseq, *lead = share + 1 + 3 * nseq;
-  int *gcu = share + 1 + 4 * nseq, *list = share + 2 + 5 * nseq;
-  int r0 = 0, n = 0;
-  best[t] = 0;
-  who[t] = -1;
-  pages[t] = rows[t] = 0;
+  int *gtok = share + 1 + 4 * nseq, *gcu = share + 1 + 5 * nseq, *list = share + 2 + 6 * nseq;
+  int r0 = 0, n = 0, me = -1, p = 0;
   if (t < nseq) {
     r0 = clamp_i(c.cu[t], 0, c.rows);
     n = max(clamp_i(c.cu[t + 1], 0, c.rows) - r0, 0);
-    who[t] = lead[t];
-    pages[t] = pos[t];
-    rows[t] = n;
+    me = lead[t];
+    p = pos[t];
   }
+  best[t] = 0;
+  who[t] = me;
+  pages[t] = p;
+  rows[t] = n;
   __syncthreads();
-  const int me = who[t], p = pages[t];
+  const int4 *who4 = reinterpret_cast<const int4 *>(who), *pages4 = reinterpret_cast<const int4 *>(pages);
+  const int4 *rows4 = reinterpret_cast<const int4 *>(rows), *index4 = reinterpret_cast<const int4 *>(index);
+  const int quads = (nseq + 3) / 4;
   if (me >= 0) {
     int members = 0;
-#pragma unroll 8
-    for (int j = 0; j < nseq; ++j) members += who[j] == me && pages[j] >= p;
+#pragma unroll 4
+    for (int j = 0; j < quads; ++j) {
+      const int4 w = who4[j], g = pages4[j];
+      members += ((w.x == me) & (g.x >= p)) + ((w.y == me) & (g.y >= p)) + ((w.z == me) & (g.z >= p)) +
+                 ((w.w == me) & (g.w >= p));
+    }
     // (members below 2^10, pages at most 2^26: 36 bits and 28; the longest of equal ones)
     atomicMax(&best[me], (unsigned long long)(members - 1) * p << 28 | (unsigned)p);
   }
@@ -96,36 +104,40 @@ __global__ __launch_bounds__(kKv8ShareSeq) void share_group_kernel(Kv8Args c, in
   const unsigned long long b = me >= 0 ? best[me] : 0;
   const int take = b >> 28 ? (int)(b & 0xfffffffu) : 0;
   bool in = take > 0 && p >= take;
-  __syncthreads();
-  if (!in) who[t] = -1;
   // groups in the order of their leaders, which are their first members
   const bool leads = in && me == t;
+  if (!in) who[t] = -1;
   index[t] = leads;
+  if (t == 0) groups = 0;
   __syncthreads();
   int g = 0;
-  uint32_t at = 0;                                    // (unsigned: nonsense in cu may wrap)
-#pragma unroll 8
-  for (int j = 0; j < nseq; ++j) g += j < me ? index[j] : 0;
-  g = in ? g : 0;
+#pragma unroll 4
+  for (int j = 0; j < quads; ++j) {
+    const int4 x = index4[j];
+    g += (4 * j < me ? x.x : 0) + (4 * j + 1 < me ? x.y : 0) + (4 * j + 2 < me ? x.z : 0) + (4 * j + 3 < me ? x.w : 0);
+  }
   in = in && g < kKv8ShareGroups;
   __syncthreads();
   if (!in) who[t] = -1;
   __syncthreads();
-  // and the rows of the groups before
-  uint32_t before = 0, all = 0;
-#pragma unroll 8
-  for (int j = 0; j < nseq; ++j) {
-    const int wj = who[j];
-    const uint32_t n = (uint32_t)rows[j];
-    at += wj == me && j < t ? n : 0;
-    before += wj >= 0 && wj < me ? n : 0;
-    all += wj >= 0 ? n : 0;
+  // the rows of the groups before, of the group's members before, of all
+  // (unsigned: nonsense in cu may wrap)
+  uint32_t before = 0, at = 0, all = 0;
+#pragma unroll 4
+  for (int j = 0; j < quads; ++j) {
+    const int4 w = who4[j], x = rows4[j];
+    const int wj[4] = {w.x, w.y, w.z, w.w}, xj[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      at += wj[u] == me && 4 * j + u < t ? (uint32_t)xj[u] : 0;
+      before += wj[u] >= 0 && wj[u] < me ? (uint32_t)xj[u] : 0;
+      all += wj[u] >= 0 ? (uint32_t)xj[u] : 0;
+    }
   }
-  if (t == 0) groups = 0;
-  __syncthreads();
   if (leads && in) {
     atomicAdd(&groups, 1);
     lead[g] = t;
+    gtok[g] = take * c.page;
     gcu[g] = (int)before;
   }
   __syncthreads();
