@@ -601,7 +601,253 @@ __device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8Share
   g.blocks = __builtin_amdgcn_readlane(u, 63);
   return g;
 }
-//
+
+// ---- the shared tokens of groups ------------------------------------------------------
+// A block takes a row tile of 64 columns (row of the group, query head), 16 a wave, over
+// a cut of the group's shared tokens; all columns see all of them.  A unit's K codes and
+// its V, as bf16 once for all waves, go through LDS in the layout of the MFMA operands (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in
+// flight beside this one's products.  Scores, probabilities and products are those of
+// kv8_attn_kernel.  Bound: VALU (the joins of the digits, exp, p in three terms: 340
+// operations a unit and 16 columns, 190 of them for codes -> bf16 if every wave did that
+// for itself).
+template <int HD> __device__ __forceinline__ void kv8_shared_block(const Kv8AttnArgs &a) {
+  constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8ShareCols;
+  constexpr int KF = 4 * HH / kKv8Waves, VF = DT / kKv8Waves;   // fragments that a wave stages
+  __shared__ __attribute__((aligned(16))) u32x4 kbuf[2][4 * HH][64], vbuf[2][2 * DT][64];
+  const Kv8Args &c = a.c;
+  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6), cc = 16 * w + col;
+  const int g = blockIdx.y, grp = c.nheads / c.nkv, P = c.page;
+  const int psh = 31 - __builtin_clz(P);
+  const int64_t pbytes = kv8_page_bytes(P, c.nkv, HD);
+  const int64_t scales_at = kv8_scales_at(P, c.nkv, HD);
+  const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
+  const float qscale = 1.44269504088896341f / sqrtf((float)HD);
+  const Kv8ShareAt sh = kv8_share_at(c, a.share);
+  const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
+  const int b = blockIdx.x;
+  if (b >= gs.blocks) return;             // (the whole block)
+  // the last group that begins at this block or before and has any
+  const int i = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(gs.n > 0 && gs.cuts > 0 && gs.base <= b));
+  const int lead = __builtin_amdgcn_readlane(gs.lead, i), tokens = __builtin_amdgcn_readlane(gs.tokens, i);
+  const int n = __builtin_amdgcn_readlane(gs.n, i), row0 = __builtin_amdgcn_readlane(gs.row0, i);
+  const int cuts = __builtin_amdgcn_readlane(gs.cuts, i), local = b - __builtin_amdgcn_readlane(gs.base, i);
+  const int units = __builtin_amdgcn_readlane(gs.units, i);
+  const int rt = local / cuts, t0 = local % cuts * gs.per, t1 = min(units, t0 + gs.per);
+  const int *tab = c.tab + (int64_t)lead * c.maxpages;
+
+  // what a wave stages: K fragments KF w .. (tt = f / HH, dims 64 (f % HH) + 16 g4 ..) and
+  // V fragments VF w .. (dims 16 f + col, keys 16 g4 ..); the lane's pages of both
+  int idk, idv;
+  u32x4 kr[KF], vr[VF];
+  float ks = 0.0f, vs = 0.0f, ks1, vs1;
+  auto load_ids = [&](int kt) {
+    const int kk = kt * kKv8Unit + 16 * (col >> 2), kv = kt * kKv8Unit + 16 * g4;
+    idk = kt < t1 && kk < tokens ? tab[kk >> psh] : 0;
+    idv = kt < t1 && kv < tokens ? tab[kv >> psh] : 0;
+  };
+  auto load = [&](int kt) {
+    int id = page_or_none(idk, (int)c.npages);
+    const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
+                       (int64_t)(((kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD + 16 * g4;
+#pragma unroll
+    for (int f = 0; f < KF; ++f)
+      kr[f] = *reinterpret_cast<const u32x4 *>(p + 4 * ((KF * w + f) / HH) * HD + 64 * ((KF * w + f) % HH));
+    id = page_or_none(idv, (int)c.npages);
+    p = c.pages + (id < 0 ? 0 : id) * pbytes;
+    const float *sc = reinterpret_cast<const float *>(p + scales_at);
+    ks1 = id < 0 ? __builtin_nanf("") : sc[g];
+    vs1 = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
+    p += v_at + (int64_t)col * P + ((kt * kKv8Unit + 16 * g4) & (P - 1));
+#pragma unroll
+    for (int f = 0; f < VF; ++f) vr[f] = *reinterpret_cast<const u32x4 *>(p + (int64_t)16 * (VF * w + f) * P);
+  };
+  auto store = [&](int to) {
+#pragma unroll
+    for (int f = 0; f < KF; ++f) kbuf[to][KF * w + f][lane] = kr[f];
+#pragma unroll
+    for (int f = 0; f < VF; ++f)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        vbuf[to][2 * (VF * w + f) + e][lane] =
+            __builtin_bit_cast(u32x4, codes_to_bf16(vr[f][2 * e], vr[f][2 * e + 1]));
+    ks = ks1;
+    vs = vs1;
+  };
+  load_ids(t0);
+  load(t0);
+  load_ids(t0 + 1);
+
+  // this lane's digits of q
+  const int lin = rt * NC + cc, j = lin / grp;
+  const int row = clamp_i(sh.row[row0 + (j < n ? j : 0)], 0, c.rows - 1);
+  const float *q = a.q + (int64_t)row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
+  u32x4 qd[4][HH];
+  float qs;
+  {
+    float x[HH][16];
+#pragma unroll
+    for (int h = 0; h < HH; ++h)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const f32x4 y = *reinterpret_cast<const f32x4_u *>(q + 64 * h + 4 * v);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) x[h][4 * v + z] = y[z];
+      }
+    qs = kv8_digits<HD>(x, qscale, qd);
+  }
+  store(0);
+  __syncthreads();
+
+  f32x4 o[DT];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int kt = t0; kt < t1; ++kt) {
+    const int at = (kt - t0) & 1;
+    if (kt + 1 < t1) {
+      load(kt + 1);
+      load_ids(kt + 2);
+    }
+    f32x4 s[4];
+    const float sc = qs * ks;
+    __builtin_amdgcn_s_setprio(1);        // the matrix cores' work first, VALU beside it
+    if (__builtin_amdgcn_ballot_w64(fabsf(sc) > kv8_exact_up_to<HD>()) == 0) {
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        i32x4 d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[k] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < HH; ++h) {
+          const i32x4 kf = __builtin_bit_cast(i32x4, kbuf[at][tt * HH + h][lane]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0, 0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v)       // (|d| < 2^21 each: the pairs fit)
+          s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
+                                    (float)((d[1][v] << 8) + d[0][v]));
+      }
+    } else {
+      // q as three bf16 terms (see kv8_attn_kernel)
+      const float up = qscale / qs;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int z = 0; z < 2 * HH; ++z) {
+        float y[8];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const f32x4 x = *reinterpret_cast<const f32x4_u *>(q + 64 * (z >> 1) + 8 * (z & 1) + 4 * v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[4 * v + e] = x[e] * up;
+        }
+        u32x4 qf[3];
+        split3x8(y, qf);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u32x4 kf = kbuf[at][tt * HH + (z >> 1)][lane];
+          const bf16x8_t kb = codes_to_bf16(kf[2 * (z & 1)], kf[2 * (z & 1) + 1]);
+#pragma unroll
+          for (int k = 2; k >= 0; --k)
+            s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, __builtin_bit_cast(bf16x8_t, qf[k]), s[tt], 0, 0, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    // A lane's 16 keys are of one page, so its scores have one scale.  The last unit's keys
+    // behind the shared tokens (a page of 16 or 32 may end there) are a path of their own.
+    const int left = tokens - (kt * kKv8Unit + 16 * g4);        // this lane's keys, at most 16
+    const bool masked = kt * kKv8Unit + kKv8Unit > tokens;
+    float top = -INFINITY;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) top = fmaxf(top, s[tt][v]);
+    if (masked) {
+      top = -INFINITY;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, 4 * tt + v < left ? s[tt][v] : -INFINITY);
+    }
+    float tmax = top == -INFINITY ? top : top * sc;
+    tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
+    tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
+    // (the maximum rounded to an integer, see kv8_attn_kernel)
+    const float mnew = fmaxf(m, __builtin_rintf(tmax));
+    const float ms = mnew == -INFINITY ? 0.0f : mnew;
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mnew;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) s[tt][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][v], sc, -ms));
+    float vsc = vs;
+    if (masked) {
+      // (a page of NaN scale counts for the rows that see one of its keys)
+      if (left <= 0) vsc = 0.0f;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[tt][v] = 4 * tt + v < left ? s[tt][v] : 0.0f;
+    }
+    float ps = 0.0f;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) ps += s[tt][v];
+    l = __builtin_fmaf(l, alpha, ps);
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u32x4 pf[3];
+      float x[8];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3] * vsc;
+      split3x8(x, pf);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int d0 = 0; d0 < DT; d0 += 4) {
+        u32x4 va[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) va[d] = vbuf[at][2 * (d0 + d) + e][lane];
+#pragma unroll
+        for (int k = 2; k >= 0; --k)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, va[d]),
+                                                                __builtin_bit_cast(bf16x8_t, pf[k]), o[d0 + d],
+                                                                0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    // (the other buffer's last readers are behind the barrier before this unit)
+    if (kt + 1 < t1) {
+      store(at ^ 1);
+      __syncthreads();
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (j >= n) return;
+  float *rec = a.shared_rec + ((int64_t)b * c.nkv + g) * kv8_record<HD, NC>();
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(rec + cc * HD + 16 * d + 4 * g4) = o[d];
+  if (g4 == 0) {
+    rec[NC * HD + cc] = m;
+    rec[NC * HD + NC + cc] = l;
+  }
+}
+template <int HD> __global__ __launch_bounds__(64 * kKv8Waves, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
+  kv8_shared_block<HD>(a);
+}
+
 // WIDE (pages of 128 tokens, runs): a V column of a page is one 128-byte line,
 // of which a unit takes half.  The even unit's load brings the odd unit's half
 // into registers too; fetched a unit later, the line had left the L2 by then
@@ -609,6 +855,14 @@ __device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8Share
 // PART: see above.
 template <int HD, int MT, bool WHOLE, bool WIDE, int PART>
 __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kernel(Kv8AttnArgs a) {
+  // the first blocks: the groups' part, if it has no launch of its own
+  const int first = PART == KV8_OWN ? a.shared_first : 0, bx = (int)blockIdx.x - first;
+  if constexpr (PART == KV8_OWN) {
+    if (bx < 0) {
+      kv8_shared_block<HD>(a);
+      return;
+    }
+  }
   constexpr int DT = HD / 16, HH = HD / 64, NC = 16 * MT, NW = WHOLE ? 8 : kKv8Waves;
   constexpr int RW = NW / MT;             // runs of a block
   constexpr int OST = HD + 4;             // floats of a column's sums in LDS
@@ -637,13 +891,13 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   pl.k0 = pl.old + nseq;
 
   const int units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, NC, pl, wsum);
-  const int runs = gridDim.x * RW, run = blockIdx.x * RW + w;
+  const int runs = ((int)gridDim.x - first) * RW, run = bx * RW + w;
   const int per = WHOLE ? 1 : kv8_units_per_block(units, runs, 1);
   // the merge reads the plan behind the records
-  if (!WHOLE && blockIdx.x == 0 && g == 0)
+  if (!WHOLE && bx == 0 && g == 0)
     for (int i = t; i <= nseq; i += 64 * NW) kv8_plan_at<HD, NC>(a, runs)[i] = pl.pre[i];
-  const int u0 = WHOLE ? (int)blockIdx.x : run * per;
-  const int uend = WHOLE ? min((int)blockIdx.x + 1, units) : min(u0 + per, units);
+  const int u0 = WHOLE ? bx : run * per;
+  const int uend = WHOLE ? min(bx + 1, units) : min(u0 + per, units);
   if (u0 >= uend) return;                 // (WHOLE: the whole block)
 
   // the place of unit u, in sequence i or behind it
@@ -936,250 +1190,6 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   }
 }
 
-// ---- the shared tokens of groups ------------------------------------------------------
-// A block takes a row tile of 64 columns (row of the group, query head), 16 a wave, over a cut of the group's shared tokens; all columns see all of them.  A unit's K
-// codes and its V, as bf16 once for all waves, go through LDS in the layout of the MFMA
-// operands (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in
-// flight beside this one's products.  Scores, probabilities and products are those of
-// kv8_attn_kernel.  Bound: VALU (the joins of the digits, exp, p in three terms: 340
-// operations a unit and 16 columns, 190 of them for codes -> bf16 if every wave did that
-// for itself).
-template <int HD>
-__global__ __launch_bounds__(64 * kKv8Waves, 3) void kv8_shared_kernel(Kv8AttnArgs a) {
-  constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8ShareCols;
-  constexpr int KF = 4 * HH / kKv8Waves, VF = DT / kKv8Waves;   // fragments that a wave stages
-  __shared__ __attribute__((aligned(16))) u32x4 kbuf[2][4 * HH][64], vbuf[2][2 * DT][64];
-  const Kv8Args &c = a.c;
-  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g4 = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(t >> 6), cc = 16 * w + col;
-  const int g = blockIdx.y, grp = c.nheads / c.nkv, P = c.page;
-  const int psh = 31 - __builtin_clz(P);
-  const int64_t pbytes = kv8_page_bytes(P, c.nkv, HD);
-  const int64_t scales_at = kv8_scales_at(P, c.nkv, HD);
-  const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
-  const float qscale = 1.44269504088896341f / sqrtf((float)HD);
-  const Kv8ShareAt sh = kv8_share_at(c, a.share);
-  const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
-  const int b = blockIdx.x;
-  if (b >= gs.blocks) return;             // (the whole block)
-  // the last group that begins at this block or before and has any
-  const int i = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(gs.n > 0 && gs.cuts > 0 && gs.base <= b));
-  const int lead = __builtin_amdgcn_readlane(gs.lead, i), tokens = __builtin_amdgcn_readlane(gs.tokens, i);
-  const int n = __builtin_amdgcn_readlane(gs.n, i), row0 = __builtin_amdgcn_readlane(gs.row0, i);
-  const int cuts = __builtin_amdgcn_readlane(gs.cuts, i), local = b - __builtin_amdgcn_readlane(gs.base, i);
-  const int units = __builtin_amdgcn_readlane(gs.units, i);
-  const int rt = local / cuts, t0 = local % cuts * gs.per, t1 = min(units, t0 + gs.per);
-  const int *tab = c.tab + (int64_t)lead * c.maxpages;
-
-  // what a wave stages: K fragments KF w .. (tt = f / HH, dims 64 (f % HH) + 16 g4 ..) and
-  // V fragments VF w .. (dims 16 f + col, keys 16 g4 ..); the lane's pages of both
-  int idk, idv;
-  u32x4 kr[KF], vr[VF];
-  float ks = 0.0f, vs = 0.0f, ks1, vs1;
-  auto load_ids = [&](int kt) {
-    const int kk = kt * kKv8Unit + 16 * (col >> 2), kv = kt * kKv8Unit + 16 * g4;
-    idk = kt < t1 && kk < tokens ? tab[kk >> psh] : 0;
-    idv = kt < t1 && kv < tokens ? tab[kv >> psh] : 0;
-  };
-  auto load = [&](int kt) {
-    int id = page_or_none(idk, (int)c.npages);
-    const uint8_t *p = c.pages + (id < 0 ? 0 : id) * pbytes + k_at +
-                       (int64_t)(((kt * kKv8Unit + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * HD + 16 * g4;
-#pragma unroll
-    for (int f = 0; f < KF; ++f)
-      kr[f] = *reinterpret_cast<const u32x4 *>(p + 4 * ((KF * w + f) / HH) * HD + 64 * ((KF * w + f) % HH));
-    id = page_or_none(idv, (int)c.npages);
-    p = c.pages + (id < 0 ? 0 : id) * pbytes;
-    const float *sc = reinterpret_cast<const float *>(p + scales_at);
-    ks1 = id < 0 ? __builtin_nanf("") : sc[g];
-    vs1 = id < 0 ? __builtin_nanf("") : sc[c.nkv + g];
-    p += v_at + (int64_t)col * P + ((kt * kKv8Unit + 16 * g4) & (P - 1));
-#pragma unroll
-    for (int f = 0; f < VF; ++f) vr[f] = *reinterpret_cast<const u32x4 *>(p + (int64_t)16 * (VF * w + f) * P);
-  };
-  auto store = [&](int to) {
-#pragma unroll
-    for (int f = 0; f < KF; ++f) kbuf[to][KF * w + f][lane] = kr[f];
-#pragma unroll
-    for (int f = 0; f < VF; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        vbuf[to][2 * (VF * w + f) + e][lane] =
-            __builtin_bit_cast(u32x4, codes_to_bf16(vr[f][2 * e], vr[f][2 * e + 1]));
-    ks = ks1;
-    vs = vs1;
-  };
-  load_ids(t0);
-  load(t0);
-  load_ids(t0 + 1);
-
-  // this lane's digits of q
-  const int lin = rt * NC + cc, j = lin / grp;
-  const int row = clamp_i(sh.row[row0 + (j < n ? j : 0)], 0, c.rows - 1);
-  const float *q = a.q + (int64_t)row * a.ldq + (int64_t)(g * grp + lin % grp) * HD + 16 * g4;
-  u32x4 qd[4][HH];
-  float qs;
-  {
-    float x[HH][16];
-#pragma unroll
-    for (int h = 0; h < HH; ++h)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const f32x4 y = *reinterpret_cast<const f32x4_u *>(q + 64 * h + 4 * v);
-#pragma unroll
-        for (int z = 0; z < 4; ++z) x[h][4 * v + z] = y[z];
-      }
-    qs = kv8_digits<HD>(x, qscale, qd);
-  }
-  store(0);
-  __syncthreads();
-
-  f32x4 o[DT];
-  float m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kt = t0; kt < t1; ++kt) {
-    const int at = (kt - t0) & 1;
-    if (kt + 1 < t1) {
-      load(kt + 1);
-      load_ids(kt + 2);
-    }
-    f32x4 s[4];
-    const float sc = qs * ks;
-    __builtin_amdgcn_s_setprio(1);        // the matrix cores' work first, VALU beside it
-    if (__builtin_amdgcn_ballot_w64(fabsf(sc) > kv8_exact_up_to<HD>()) == 0) {
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        i32x4 d[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) d[k] = i32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; h < HH; ++h) {
-          const i32x4 kf = __builtin_bit_cast(i32x4, kbuf[at][tt * HH + h][lane]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            d[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, __builtin_bit_cast(i32x4, qd[k][h]), d[k], 0, 0, 0);
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v)       // (|d| < 2^21 each: the pairs fit)
-          s[tt][v] = __builtin_fmaf((float)((d[3][v] << 8) + d[2][v]), 65536.0f,
-                                    (float)((d[1][v] << 8) + d[0][v]));
-      }
-    } else {
-      // q as three bf16 terms (see kv8_attn_kernel)
-      const float up = qscale / qs;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int z = 0; z < 2 * HH; ++z) {
-        float y[8];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const f32x4 x = *reinterpret_cast<const f32x4_u *>(q + 64 * (z >> 1) + 8 * (z & 1) + 4 * v);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[4 * v + e] = x[e] * up;
-        }
-        u32x4 qf[3];
-        split3x8(y, qf);
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const u32x4 kf = kbuf[at][tt * HH + (z >> 1)][lane];
-          const bf16x8_t kb = codes_to_bf16(kf[2 * (z & 1)], kf[2 * (z & 1) + 1]);
-#pragma unroll
-          for (int k = 2; k >= 0; --k)
-            s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, __builtin_bit_cast(bf16x8_t, qf[k]), s[tt], 0, 0, 0);
-        }
-      }
-    }
-    __builtin_amdgcn_s_setprio(0);
-    // A lane's 16 keys are of one page, so its scores have one scale.  The last unit's keys
-    // behind the shared tokens (a page of 16 or 32 may end there) are a path of their own.
-    const int left = tokens - (kt * kKv8Unit + 16 * g4);        // this lane's keys, at most 16
-    const bool masked = kt * kKv8Unit + kKv8Unit > tokens;
-    float top = -INFINITY;
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) top = fmaxf(top, s[tt][v]);
-    if (masked) {
-      top = -INFINITY;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) top = fmaxf(top, 4 * tt + v < left ? s[tt][v] : -INFINITY);
-    }
-    float tmax = top == -INFINITY ? top : top * sc;
-    tmax = fmaxf(tmax, __shfl_xor(tmax, 16));
-    tmax = fmaxf(tmax, __shfl_xor(tmax, 32));
-    // (the maximum rounded to an integer, see kv8_attn_kernel)
-    const float mnew = fmaxf(m, __builtin_rintf(tmax));
-    const float ms = mnew == -INFINITY ? 0.0f : mnew;
-    const float alpha = __builtin_amdgcn_exp2f(m - ms);
-    m = mnew;
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) s[tt][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][v], sc, -ms));
-    float vsc = vs;
-    if (masked) {
-      // (a page of NaN scale counts for the rows that see one of its keys)
-      if (left <= 0) vsc = 0.0f;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) s[tt][v] = 4 * tt + v < left ? s[tt][v] : 0.0f;
-    }
-    float ps = 0.0f;
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) ps += s[tt][v];
-    l = __builtin_fmaf(l, alpha, ps);
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= alpha;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      u32x4 pf[3];
-      float x[8];
-#pragma unroll
-      for (int v = 0; v < 8; ++v) x[v] = s[2 * e + (v >> 2)][v & 3] * vsc;
-      split3x8(x, pf);
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int d0 = 0; d0 < DT; d0 += 4) {
-        u32x4 va[4];
-#pragma unroll
-        for (int d = 0; d < 4; ++d) va[d] = vbuf[at][2 * (d0 + d) + e][lane];
-#pragma unroll
-        for (int k = 2; k >= 0; --k)
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, va[d]),
-                                                                __builtin_bit_cast(bf16x8_t, pf[k]), o[d0 + d],
-                                                                0, 0, 0);
-      }
-    }
-    __builtin_amdgcn_s_setprio(0);
-    // (the other buffer's last readers are behind the barrier before this unit)
-    if (kt + 1 < t1) {
-      store(at ^ 1);
-      __syncthreads();
-    }
-  }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (j >= n) return;
-  float *rec = a.shared_rec + ((int64_t)b * c.nkv + g) * kv8_record<HD, NC>();
-#pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_u *>(rec + cc * HD + 16 * d + 4 * g4) = o[d];
-  if (g4 == 0) {
-    rec[NC * HD + cc] = m;
-    rec[NC * HD + NC + cc] = l;
-  }
-}
-
 // Joins the records of the row tiles that several runs served: grid
 // (rows, nkv, heads of a group / hb).  The block's threads are groups over hb
 // heads x HD / 4 dims; the groups take the records in turn and meet in LDS.
@@ -1337,13 +1347,14 @@ hipError_t launch_kv8_attn_t(const Kv8AttnArgs &a, hipStream_t st) {
                        dim3(512), lds, st, a);
     return hipGetLastError();
   }
-  // two blocks per CU over all KV heads, as far as the work (by its bound)
-  // and the records' space reach
-  int64_t nb = (512 + c.nkv - 1) / c.nkv;
+  // two blocks per CU over all KV heads (one beside the groups' blocks), as far as the
+  // work (by its bound) and the records' space reach
+  const int first = PART == KV8_OWN ? a.shared_first : 0;
+  int64_t nb = ((first ? 256 : 512) + c.nkv - 1) / c.nkv;
   nb = std::min(nb, (tiles * key_units + RW - 1) / RW);
   nb = std::min(nb, (a.ws_floats - c.nseq - 1) / (RW * 2 * (int64_t)c.nkv * kv8_record<HD, NC>()));
   if (nb < 1) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)nb, (unsigned)c.nkv), block(64 * kKv8Waves);
+  const dim3 grid((unsigned)(nb + first), (unsigned)c.nkv), block(64 * kKv8Waves);
   if (c.page == 128)
     hipLaunchKernelGGL((kv8_attn_kernel<HD, MT, false, true, PART>), grid, block, plan, st, a);
   else
@@ -1402,7 +1413,14 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
 }
 
 // The groups' part (a row tile of 64 columns cut over blocks), each sequence's own
-// part, and the merge that joins them.
+// part, and the merge that joins them.  Little work in the groups (by its bound, units of
+// row tiles and KV heads) takes one launch with the sequences' parts: a launch less,
+// but two blocks a CU where alone it has three (us together / apart, 8 KV heads: 64
+// sequences of 500 tokens behind 8000, heads of 128, 128 / 137; 64 behind 8000 with
+// pages of 128 73 / 72, behind 16000 98 / 90; 128 behind 32000 252 / 227; heads of 64:
+// 8 behind 1000, four layers, 70 / 97, 128 behind 8000 76 / 81, behind 16000 114 / 113,
+// behind 32000 188 / 177).
+template <int HD> constexpr int64_t kKv8TogetherUnits = HD == 64 ? 16000 : 6000;
 template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream_t st) {
   const Kv8Args &c = a.c;
   constexpr int NC = kKv8ShareCols;
@@ -1413,8 +1431,10 @@ template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream
   // at most), then what the sequences' own parts leave
   const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4;
   const int64_t room = (a.ws_floats / 4 * 3 - ml) / rec;
-  // as many blocks as are resident: three a compute unit
-  const int64_t want = (768 + c.nkv - 1) / c.nkv;
+  const int64_t units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit * ((cols + NC - 1) / NC) * c.nkv;
+  const bool together = units <= kKv8TogetherUnits<HD>;
+  // as many blocks as are resident
+  const int64_t want = ((together ? 512 : 768) + c.nkv - 1) / c.nkv;
   a.shared_target = (int)std::min(want, room - tiles);
   // (more rows than there is room for: every sequence for itself)
   if (a.shared_target < std::min<int64_t>(want, 8) || groups == 0) return launch_kv8_attention(a, st);
@@ -1422,12 +1442,15 @@ template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream
   a.ml = a.ws;
   a.shared_rec = a.ws + ml;
   a.shared_blocks = (int)blocks;
+  a.shared_first = together ? (int)blocks : 0;
   a.ws += ml + recs;
   a.ws_floats -= ml + recs;
-  hipLaunchKernelGGL(kv8_shared_kernel<HD>, dim3((unsigned)blocks, (unsigned)c.nkv), dim3(64 * kKv8Waves), 0, st,
-                     a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (!together) {
+    hipLaunchKernelGGL(kv8_shared_kernel<HD>, dim3((unsigned)blocks, (unsigned)c.nkv), dim3(64 * kKv8Waves), 0, st,
+                       a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   return cols <= 16 * c.nseq   ? launch_kv8_attn_t<HD, 1, KV8_OWN>(a, st)
          : cols <= 32 * c.nseq ? launch_kv8_attn_t<HD, 2, KV8_OWN>(a, st)
                                : launch_kv8_attn_t<HD, 4, KV8_OWN>(a, st);

@@ -135,6 +135,19 @@ def test_long_prefix(ctx):
         s.check(ctx, queries(rng, s.T, 4, 64))
 
 
+@pytest.mark.parametrize("P", [16, 128])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_wide_tables(ctx, P, hd):
+    """Tables with room for many more pages than are named, the groups' part a launch of its own."""
+    say("shared wide", P, hd)
+    rng = np.random.default_rng(P + hd)
+    s = Step(rng, [1, 3, 1, 0, 1, 2], [0, 1, 0, 0, 1, -1], [9, 300 // P + 1], [70, 0, 3, 5, 200, 90], P, 2, hd)
+    more = 64 * 9000 // P - s.maxpages
+    s.table = np.concatenate([s.table, np.full((s.ns, more), -1, np.int32)], axis=1)
+    s.maxpages += more
+    s.check(ctx, queries(rng, s.T, 8, hd), dead=1, off=3, extra=7)
+
+
 def test_drafts_in_wide_groups(ctx):
     """Row tiles of 32 and 64 columns for the sequences' own tokens."""
     say("shared drafts")
