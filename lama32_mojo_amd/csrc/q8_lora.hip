@@ -18,6 +18,7 @@
 #include "q8_ragged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace q8 {
 namespace {
@@ -251,39 +252,44 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   f32x4 acc[kRankTiles];
 #pragma unroll
   for (int q = 0; q < kRankTiles; ++q) acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  // U steps of 32 at a time, all their loads first
+  // U steps of 32 at a time, all their loads first; the last ones with a test for each
+  // lane's eight (m is a multiple of 8; those behind k1 load the row's start)
   constexpr int U = F32 ? 1 : 4, STEP = RT == 1 ? 128 : 32;
-  if (RT == 1 || 16 * w < n) {
-    for (int64_t k = k0 + (RT == 1 ? 32 * w : 0); k < k1; k += U * STEP) {
-      f32x4 xa[U], xb[U];
-      Weights8<F32> wt[U][kRankTiles];
-      bool in[U];
+  auto steps = [&](int64_t k, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    f32x4 xa[U], xb[U];
+    Weights8<F32> wt[U][kRankTiles];
+    bool in[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t ku = k + u * STEP;
-        in[u] = ku + 8 * g4 < k1;                     // (m is a multiple of 8)
-        const int64_t kk = in[u] ? ku : -8 * g4;      // (row's start: any valid one)
-        xa[u] = *reinterpret_cast<const f32x4_u *>(x + kk);
-        xb[u] = *reinterpret_cast<const f32x4_u *>(x + kk + 4);
+    for (int u = 0; u < U; ++u) {
+      const int64_t ku = k + u * STEP;
+      in[u] = WHOLE || ku + 8 * g4 < k1;
+      const int64_t kk = in[u] ? ku : -8 * g4;
+      xa[u] = *reinterpret_cast<const f32x4_u *>(x + kk);
+      xb[u] = *reinterpret_cast<const f32x4_u *>(x + kk + 4);
 #pragma unroll
-        for (int q = 0; q < kRankTiles; ++q)
-          if (q < nq) wt[u][q].load(A, wrow[q] + kk);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float xs[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          xs[e] = in[u] ? xa[u][e] : 0.0f;
-          xs[4 + e] = in[u] ? xb[u][e] : 0.0f;
-        }
-        u32x4 xt[3];
-        split3x8(xs, xt);
-#pragma unroll
-        for (int q = 0; q < kRankTiles; ++q)
-          if (q < nq) acc[q] = wt[u][q].times(in[u], xt, acc[q]);
-      }
+      for (int q = 0; q < kRankTiles; ++q)
+        if (q < nq) wt[u][q].load(A, wrow[q] + kk);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float xs[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        xs[e] = in[u] ? xa[u][e] : 0.0f;
+        xs[4 + e] = in[u] ? xb[u][e] : 0.0f;
+      }
+      u32x4 xt[3];
+      split3x8(xs, xt);
+#pragma unroll
+      for (int q = 0; q < kRankTiles; ++q)
+        if (q < nq) acc[q] = wt[u][q].times(in[u], xt, acc[q]);
+    }
+  };
+  if (RT == 1 || 16 * w < n) {
+    int64_t k = k0 + (RT == 1 ? 32 * w : 0);
+    for (; k + (U - 1) * STEP + 32 <= k1; k += U * STEP) steps(k, std::true_type{});
+    if (k < k1) steps(k, std::false_type{});
   }
   if (RT == 1) {
     if (w > 0) {
