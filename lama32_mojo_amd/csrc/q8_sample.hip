@@ -90,6 +90,17 @@ __device__ __forceinline__ uint64_t place(float x, int i) {
   return (uint64_t)~key << 32 | (uint32_t)i;
 }
 
+// A value that is the same in all lanes, in scalar registers.
+template <class T> __device__ __forceinline__ T uniform(T v) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    int w[W];
+  } x = __builtin_bit_cast(Words, v);
+#pragma unroll
+  for (int i = 0; i < W; ++i) x.w[i] = __builtin_amdgcn_readfirstlane(x.w[i]);
+  return __builtin_bit_cast(T, x);
+}
+
 // Inclusive sums over a wave's lanes (rows of 16, then the rows' last lanes into the
 // rows behind), in one fixed order.
 template <int CTRL, int ROWS, class T> __device__ __forceinline__ T from_lanes(T v) {
@@ -339,6 +350,14 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
 // Bound: the chain of dependent reads and block-wide sums, 10 us of it, and for rows
 // whose kept tokens are many the second read of the logits.
 
+// The bin that a border falls into, the sums before it and up to it, its own.
+struct BorderBin {
+  uint64_t mass;
+  double before, unit;                                // unit: weight of 1 in this bin
+  uint32_t count, upto;
+  int bin, pad;                                       // -1: none in this wave
+};
+
 struct SelectLds {
   uint64_t mass[kBins];                               // (sorting: places; sums as f64)
   uint32_t count[kBins];
@@ -346,9 +365,11 @@ struct SelectLds {
   uint64_t wsum64[kBins / 64];
   double wsumd[2][kBins / 64];
   uint32_t wsum32[kBins / 64];
+  BorderBin border[2][2][kBins / 64];
   uint64_t found;
   uint64_t before;                                    // sum before what was found
   uint32_t n, where;
+  uint32_t key[4];
 };
 
 __device__ __forceinline__ float value_of(uint64_t place) {
@@ -397,26 +418,35 @@ __device__ __forceinline__ uint32_t first_key(double bin, bool past, double inv_
 __device__ __forceinline__ float float_of(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
-__device__ __forceinline__ Values values_of(double from, double to, double inv_t) {
-  const uint32_t a = first_key(from, false, inv_t);
-  const uint32_t b = to == INFINITY ? 0xff800001u : first_key(to, true, inv_t);
-  if (a >= b) return {INFINITY, -INFINITY};           // (no float)
-  return {float_of(a), float_of(b - 1)};
+__device__ __forceinline__ Values values_of(uint32_t first, uint32_t behind) {
+  if (first >= behind) return {INFINITY, -INFINITY};  // (no float)
+  return {float_of(first), float_of(behind - 1)};
 }
 
 // Puts the tokens of the bins from `from` up to `to`, and of `also`, into LDS as far as they
 // fit; their number is l.n.  From the slices' lists where those hold them all, else
-// from the row.
-__device__ __forceinline__ void gather(const RowAt &r, double from, double to, double also, SelectLds &l) {
+// from the row.  *values1, *values2: the
+// values of both.
+__device__ __forceinline__ void gather(const RowAt &r, double from, double to, double also, SelectLds &l,
+                                       Values *values1, Values *values2) {
   __syncthreads();
   if (threadIdx.x == 0) l.n = 0;
+  // a border a wave
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave < (also == from ? 2 : 4)) {
+    const double bin = wave == 0 ? from : wave == 1 ? to : also;
+    const uint32_t k = bin == INFINITY && (wave & 1) ? 0xff800001u : first_key(bin, wave & 1, r.inv_t);
+    if ((threadIdx.x & 63) == 0) l.key[wave] = k;
+  }
   __syncthreads();
+  const Values one = values_of(uniform(l.key[0]), uniform(l.key[1]));
+  const Values two = also == from ? one : values_of(uniform(l.key[2]), uniform(l.key[3]));
+  *values1 = one;
+  *values2 = two;
   const double least = __builtin_fmin(from, also);
   const int lane = threadIdx.x & 63;
   const bool all = __builtin_amdgcn_ballot_w64(lane < r.nslices && r.max > -INFINITY && least <= r.top &&
                                                below(r.top, least) >= r.upto) == 0;
-  const Values one = values_of(from, to, r.inv_t);
-  const Values two = also == from ? one : values_of(also, also, r.inv_t);
   // a wave's candidates take their places together: `n` of this lane's
   auto places = [&](uint32_t n) {
     const uint32_t upto = wave_sums(n);
@@ -458,21 +488,43 @@ __device__ __forceinline__ void gather(const RowAt &r, double from, double to, d
     return;
   }
   // indices first (a lane's candidates are few of its 16), then their values
-  for (int64_t i0 = 4 * threadIdx.x; i0 - 4 * threadIdx.x < r.n; i0 += 16 * kBins) {
-    float v[16];
-    load16<4 * kBins>(r.x, i0, r.n, v);
-    uint32_t mask = 0;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mask |= (uint32_t)(one.has(v[e]) || two.has(v[e])) << e;
-    if (__builtin_amdgcn_ballot_w64(mask != 0) == 0) continue;
+  auto is = [&](float x) { return (uint32_t)(one.has(x) || two.has(x)); };
+  auto keep = [&](uint32_t i0, uint32_t mask) {
+    if (__builtin_amdgcn_ballot_w64(mask != 0) == 0) return;
     uint32_t at = places(__builtin_popcount(mask));
     while (mask) {
       const int e = __builtin_ctz(mask);
       mask &= mask - 1;
-      if (at < kList) l.list[at] = (uint64_t)(i0 + 4 * (e / 4) * kBins + e % 4);
+      if (at < kList) l.list[at] = i0 + 4 * (e / 4) * kBins + e % 4;
       ++at;
     }
+  };
+  // four loads are always in flight, each sent again for the next stride when it has been
+  // looked at; a place behind the end takes the row's start
+  const uint32_t fours = (uint32_t)r.n & ~3u, t4 = 4 * threadIdx.x;
+  if (fours > 0) {
+    f32x4 y[4];
+    auto load = [&](uint32_t i) {
+      return *reinterpret_cast<const f32x4_u *>(r.x + (i < fours ? i : 0));
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[u] = load(t4 + 4 * u * kBins);
+    for (uint32_t i0 = 0; i0 < fours; i0 += 16 * kBins) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t i = i0 + t4 + 4 * u * kBins;
+        uint32_t four = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four |= is(y[u][e]) << (4 * u + e);
+        mask |= i < fours ? four : 0;
+        y[u] = load(i + 16 * kBins);
+      }
+      keep(i0 + t4, mask);
+    }
   }
+  const uint32_t i = fours + threadIdx.x;
+  keep(i, i < (uint32_t)r.n ? is(r.x[i]) : 0);
   __syncthreads();
   const uint32_t n = min(l.n, (uint32_t)kList);
   for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * kBins) {
@@ -706,28 +758,35 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
   uint32_t tokens;
   const double upto = block_sums<kBins>(here, l.wsumd[0], &total);     // this bin included
   const uint32_t cupto = block_sums<kBins>(c, l.wsum32, &tokens);
-  // the bin that a border falls into: the first one that reaches it, what is before it
-  // and its unit; the last one with tokens where rounding leaves none
-  __shared__ double e_before, e_unit;
-  __shared__ uint32_t e_count;
+  // the bin that a border falls into: the first one that reaches it; the last one with
+  // tokens where rounding leaves none.  (Two places in turn: a barrier lies between two
+  // uses of the same.)
+  const uint64_t some = __builtin_amdgcn_ballot_w64(m > 0);
+  int turn = 0;
   auto border = [&](bool on) {
-    const bool any = __syncthreads_or(on && m > 0);
-    if (t == 0) l.where = any ? kBins : 0;
+    const uint64_t who = __builtin_amdgcn_ballot_w64(m > 0 && on);
+    const int first = who ? __builtin_ctzll(who) : -1, final = some ? 63 - __builtin_clzll(some) : -1;
+    BorderBin *to = l.border[turn][0] + (t >> 6);
+    if (lane == 0) to[0].bin = to[kBins / 64].bin = -1;
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+      if (lane == (z ? final : first)) {
+        BorderBin &o = to[z * (kBins / 64)];
+        o.mass = m;
+        o.before = upto - here;
+        o.unit = unit;
+        o.count = c;
+        o.upto = cupto;
+        o.bin = t;
+      }
     __syncthreads();
-    const uint64_t who = __builtin_amdgcn_ballot_w64(m > 0 && (on || !any));
-    if (who && lane == 0) {
-      if (any) atomicMin(&l.where, (uint32_t)(t + __builtin_ctzll(who)));
-      else atomicMax(&l.where, (uint32_t)(t + 63 - __builtin_clzll(who)));
-    }
-    __syncthreads();
-    const int b = (int)l.where;
-    if (t == b) {
-      e_before = upto - here;
-      e_unit = unit;
-      e_count = cupto;
-    }
-    __syncthreads();
-    return b;
+    // lane z: wave z's first, wave z - 16's last
+    const int has = lane < 2 * (kBins / 64) && l.border[turn][0][lane & 31].bin >= 0;
+    const uint64_t w = __builtin_amdgcn_ballot_w64(has);
+    const int at = (w & 0xffff) ? __builtin_ctzll(w) : 63 - __builtin_clzll(w);
+    const BorderBin f = uniform(l.border[turn][0][at]);
+    turn ^= 1;
+    return f;
   };
   auto bin_at = [&](int b) { return b == 0 ? top_bin : top_bin - (double)b; };
   const bool by_k = counts && s.k < (int64_t)tokens;
@@ -740,51 +799,50 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
   // min_p and of the draw in turn, each where its setting is on.
   enum { FEW, BY_K, BY_MASS, BY_WEIGHT, DRAW };
   int b = last;
-  if (by_k) b = border((int64_t)cupto >= s.k);        // (top_p goes by the sum of all k)
-  else if (s.top_p < 1.0) b = min(b, border(upto >= fmax(s.top_p, 0.0) * total * (1.0 - kTie)));
+  // (top_p goes by the sum of all k)
+  if (by_k || s.top_p < 1.0) {
+    const double least = fmax(s.top_p, 0.0) * total * (1.0 - kTie);
+    const int at = border(by_k ? (int64_t)cupto >= s.k : upto >= least).bin;
+    b = by_k ? at : min(b, at);
+  }
+  // a bin's running sums
+  __shared__ double e_upto;
+  __shared__ uint32_t e_count;
   if (t == b) e_count = cupto;
+  if (t == last) e_upto = upto;
   __syncthreads();
   double W = total;
   double have = NAN, also = NAN;                      // the bins in LDS
+  Values values1, values2;
   // (estimates of counts are within 1 / 32)
   for (int stage = e_count <= kBins * 15 / 16 ? FEW : BY_K; stage <= DRAW; ++stage) {
     if ((stage == BY_K && !by_k) || (stage == BY_MASS && !(s.top_p < 1.0)) ||
         (stage == BY_WEIGHT && !(s.min_p > 0.0 && last < kBins - 1)))
       continue;
-    double want = 0.0, more = NAN;
-    if (stage == BY_K) {
-      b = border((int64_t)cupto >= s.k);
-    } else if (stage == BY_MASS) {
-      want = fmax(s.top_p, 0.0) * W * (1.0 - kTie);
-      b = border(upto >= want);
-    } else if (stage == BY_WEIGHT) {
-      b = border(t == last);
-      if (b != last) {                                // (no token there)
-        if (t == last) e_before = upto;
-        __syncthreads();
-        if (e_before > 0.0) W = fmin(W, e_before);
-        __syncthreads();
-        continue;
-      }
-    } else if (stage == DRAW) {
-      want = s.u * W * (1.0 + kTie);
-      b = border(upto > want);
-    }
-    const double before = e_before, u = e_unit;
+    double more = NAN;
+    const double want = stage == BY_MASS ? fmax(s.top_p, 0.0) * W * (1.0 - kTie) : s.u * W * (1.0 + kTie);
+    BorderBin f = {};
+    if (stage != FEW)
+      f = border(stage == BY_K        ? (int64_t)cupto >= s.k
+                 : stage == BY_MASS   ? upto >= want
+                 : stage == BY_WEIGHT ? t == last
+                                      : upto > want);
     if (stage == BY_MASS) {
       // with it the bin that the draw falls into, by what is kept at least, where
       // both fit into LDS
-      const int draw = border(upto > s.u * before * (1.0 + kTie));
-      if (t == 0) l.where = 0;
-      __syncthreads();
-      if (t == b || t == draw) atomicAdd(&l.where, (uint32_t)((m >> 40) + (m >> 45)));
-      __syncthreads();
-      if (l.where <= kList) more = bin_at(draw);
-      __syncthreads();
+      const BorderBin draw = border(upto > s.u * f.before * (1.0 + kTie));
+      const uint64_t both = f.mass + (draw.bin == f.bin ? 0 : draw.mass);
+      if ((both >> 40) + (both >> 45) < kList) more = bin_at(draw.bin);
     }
-    const double bin = bin_at(b);
+    if (stage == BY_WEIGHT && f.bin != last) {        // (no token there)
+      if (e_upto > 0.0) W = fmin(W, e_upto);
+      continue;
+    }
+    const double before = f.before, u = f.unit;
+    const double bin = bin_at(stage == FEW ? b : f.bin);
     if (stage == FEW || !(bin == have || bin == also)) {
-      gather(r, bin, stage == FEW ? INFINITY : bin, stage == FEW || more != more ? bin : more, l);
+      gather(r, bin, stage == FEW ? INFINITY : bin, stage == FEW || more != more ? bin : more, l, &values1,
+             &values2);
       have = stage == FEW ? NAN : bin;
       also = more;
     }
@@ -815,7 +873,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
       }
       return;
     }
-    const Values in_bin = values_of(bin, bin, s.inv_t);
+    const Values in_bin = bin == have ? values1 : values2;
     if (stage == BY_WEIGHT) {
       if (t == 0) l.found = 0;
       __syncthreads();
@@ -831,9 +889,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
       __syncthreads();
       continue;
     }
-    if (t == b) l.before = cupto - c;
-    __syncthreads();
-    const Border reached = {stage == BY_K, stage == DRAW, (uint64_t)s.k - l.before, (want - before) / u};
+    const Border reached = {stage == BY_K, stage == DRAW, (uint64_t)s.k - (f.upto - f.count), (want - before) / u};
     uint64_t J;
     const uint64_t p = select(r, in_bin, l, reached, &J);
     if (stage != DRAW) {
