@@ -23,7 +23,7 @@ from typing import Mapping, Sequence
 import numpy as np
 
 from . import q8hip
-from .adapters import Adapters
+from .adapters import CALLS, Adapters
 from .model import Q8Llama, rope_inv_freq
 from .q8 import PAD, Acts, q8_rowstride
 from .q8hip import Buffer, Context
@@ -171,7 +171,7 @@ class Q8Batch:
         if share:
             extra["share"] = q8hip.kv8_share_ints(slots, self.max_rows)
         if adapters is not None:
-            extra |= dict(adapter=slots, rank=adapters.count)
+            extra |= dict(adapter=slots, rank=len(CALLS) * adapters.count)
         self.pages = Pages(self.ctx, slots, npages, -(-maxlen // page), page, cfg.layers, cfg.n_kv,
                            cfg.head_dim, extra)
         H, QD, KVD, I = cfg.hidden, cfg.q_dim(), cfg.kv_dim(), cfg.inter
@@ -202,7 +202,8 @@ class Q8Batch:
         m, widths = ad.shape[call]
         oa, sa, ob, sb = ad.at[L, call]
         q8hip.lora(self.ctx, ad.w, oa, sa, ob, sb, ad.count, ad.max_rank, self.a.buf, ox, oy, oy, self.oscale,
-                   p.ix, p.at["cu"], p.at["adapter"], p.at["rank"], self.slots, s, m, widths, dtype=ad.dtype)
+                   p.ix, p.at["cu"], p.at["adapter"], p.at["rank"] + list(CALLS).index(call) * ad.count, self.slots, s,
+                   m, widths, dtype=ad.dtype)
 
     def _layer(self, L: int, ox: int, s: int, packed: bool, lora: frozenset, shared: bool) -> None:
         """One block on the s rows at ox, in place.  (Adapters need the linears' inputs:
@@ -355,7 +356,9 @@ class Q8Batch:
         now = (ad.version, tuple(self.adapter))
         if now != self.loaded:
             self.pages.ix.upload(np.array(self.adapter, np.int32), 4 * self.pages.at["adapter"])
-            self.pages.ix.upload(np.array(ad.rank, np.int32), 4 * self.pages.at["rank"])
+            # (a call that an adapter does not change holds nothing of it: rank 0)
+            rank = [[r if c in has else 0 for r, has in zip(ad.rank, ad.has)] for c in CALLS]
+            self.pages.ix.upload(np.array(rank, np.int32).reshape(-1), 4 * self.pages.at["rank"])
             self.a.write(self.oscale, np.array(ad.scale, np.float32))
             self.loaded = now
         return frozenset().union(*(ad.has[i] for i in used))

@@ -118,6 +118,40 @@ def test_adapters(ctx, kind, dtype):
     m.close()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_adapters_of_other_linears(ctx, dtype):
+    """In one call with an adapter of all linears, one that changes few of them is the same
+    as alone, whatever its place held before.
+
+    The bits do not depend on the place.  Alone, the prompt takes calls of other row counts
+    (9 and 18), each within the bar of test_adapters (2 * 4.1e-4) of one float64 model, so
+    the two are within twice that; the token step reads 8-bit codes of which some may have
+    been rounded the other way, and is compared by its bits only."""
+    say("serving adapters of other linears", dtype)
+    spec, t, inv, cfg = tiny("llama")
+    rng = np.random.default_rng(9)
+    m = gm.Q8Llama(ctx, cfg, 16, weights=t)
+    ad = Adapters(ctx, cfg, 2, 16, dtype)
+    everything = [x for ls in CALLS.values() for x in ls]
+    few = matrices(rng, cfg, ad, 3, ["self_attn.o_proj"], dtype == "bf16")
+    ad.load(0, matrices(rng, cfg, ad, 16, everything, dtype == "bf16"), 16.0)
+    prompt = rng.integers(0, spec.vocab, 9).tolist()
+
+    def logits(both):
+        b = batch.Q8Batch(m, slots=2, npages=8, maxlen=64, page=16, max_rows=64, adapters=ad)
+        b.use({0: 0, 1: 1})
+        return [b.forward({s: prompt if len(x) else [7] for s in ((0, 1) if both else (1,))}, logits=True)[1]
+                for x in (prompt, [])]
+    ad.load(1, few, 3.0)
+    alone, both = logits(False), logits(True)
+    ad.load(1, {k: np.full_like(v, np.inf) for k, v in
+                matrices(rng, cfg, ad, 16, everything, dtype == "bf16").items()}, 1.0)
+    ad.load(1, few, 3.0)
+    again = logits(True)
+    assert np.array_equal(again[0], both[0]) and np.array_equal(again[1], both[1])
+    assert max_rel_err(both[0], alone[0]) <= 2 * 2 * 4.1e-4
+
+
 def test_without_adapters_in_use(ctx):
     """A batch that could have adapters, and one that draws, give the ids of one that
     cannot, bit for bit."""
