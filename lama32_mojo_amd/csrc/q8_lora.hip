@@ -521,9 +521,13 @@ hipError_t launch_lora_t(LoraArgs a, int64_t ws_floats, hipStream_t st) {
   const int64_t per = record_ints<TR>() + (int64_t)a.splits * TR * a.ranks;
   const int64_t most = std::min<int64_t>(ws_floats / per, 65535);
   if (most < 1) return hipErrorInvalidValue;
-  const int cols = RT == 1 ? 128 : kCols;
-  int blocks = 0;
-  for (int p = 0; p < a.parts; ++p) blocks += (a.width[p] + cols - 1) / cols;
+  // (blocks are a grid's y)
+  int cols = RT == 1 ? 128 : kCols, blocks = 0;
+  for (;; cols *= 2) {
+    blocks = 0;
+    for (int p = 0; p < a.parts; ++p) blocks += (a.width[p] + cols - 1) / cols;
+    if (blocks <= 65535) break;
+  }
   const size_t lds0 = (size_t)(a.nadapters + 1) * 4, lds1 = (size_t)3 * TR * (a.max_rank + 8) * 2;
   for (int64_t t0 = 0; t0 < all; t0 += most) {
     a.tile0 = (int)t0;

@@ -1994,7 +1994,6 @@ int q8_kv8_attention_shared(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq
                            oshare_i32, "q8_kv8_attention_shared");
 }
 
-
 namespace {
 
 int check_pages(q8_ctx *ctx, q8_buf *ix, int64_t nslots, int64_t maxpages, int64_t npages, int page,
@@ -2152,8 +2151,6 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
   return ok(ctx);
 }
 
-// ---- HIP graphs -------------------------------------------------------------------
-
 // ---- adapters of several requests ------------------------------------------------------
 
 int q8_lora(q8_ctx *ctx, q8_buf *w, int w_dtype, uint64_t oa, int64_t a_stride, uint64_t ob,
@@ -2295,6 +2292,8 @@ int q8_sample(q8_ctx *ctx, q8_buf *a, uint64_t ox_f32, int64_t ldx, int64_t rows
   if (e != hipSuccess) return hip_fail(ctx, e, "q8_sample launch");
   return ok(ctx);
 }
+
+// ---- HIP graphs -------------------------------------------------------------------
 
 struct q8_graph {
   hipGraph_t graph = nullptr;

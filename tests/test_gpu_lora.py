@@ -157,6 +157,13 @@ def test_many(ctx):
     Setup(rng, (rng.random(4096) < 0.7).astype(int).tolist(), ids.tolist(), [4] * 4096, 16, [8], "bf16").check(ctx)
 
 
+def test_more_columns_than_blocks(ctx):
+    """More blocks of 128 columns than a grid has places in y."""
+    say("lora wide")
+    rng = np.random.default_rng(11)
+    Setup(rng, [1], [0], [1], 8, [65535 * 128 + 130]).check(ctx)
+
+
 def test_scratch_in_parts(ctx):
     """More rows than the scratch holds parts of A x for: the tiles go in several runs."""
     say("lora scratch")
