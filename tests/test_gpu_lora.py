@@ -164,6 +164,26 @@ def test_more_columns_than_blocks(ctx):
     Setup(rng, [1], [0], [1], 8, [65535 * 128 + 130]).check(ctx)
 
 
+@pytest.mark.parametrize("rows", [1, 70])
+def test_far_adapters(ctx, rows):
+    """The second adapter's A and B begin more than 2^31 elements behind the first's."""
+    say("lora far", rows)
+    rng = np.random.default_rng(13)
+    s = Setup(rng, [rows], [0], [9], 64, [40])
+    y = s.check(ctx)
+    n, m, stride, ns = 40, 64, (1 << 31) + 64, 1
+    w, a, ix = ctx.alloc(2 * (4 * stride)), ctx.alloc(4 * (rows * (m + 2 * n) + 2)), ctx.alloc(4 * 5)
+    w.upload(s.w[:s.sa], 2 * stride)
+    w.upload(s.w[s.sa:], 2 * 3 * stride)
+    a.upload(np.concatenate([s.x.reshape(-1), s.base.reshape(-1), np.zeros(rows * n + 1, np.float32), s.scale]))
+    ix.upload(np.array([0, rows, 1, 0, 9], np.int32))
+    q8hip.lora(ctx, w, 0, stride, 2 * stride, stride, 2, 9, a, 0, rows * m, rows * (m + n), rows * (m + 2 * n), ix, 0, 2,
+               3, ns, rows, m, [n])
+    assert np.array_equal(a.download((rows, n), np.float32, 4 * rows * (m + n)), y)
+    for b in (w, a, ix):
+        b.free()
+
+
 def test_scratch_in_parts(ctx):
     """More rows than the scratch holds parts of A x for: the tiles go in several runs."""
     say("lora scratch")

@@ -217,6 +217,28 @@ def test_captured(ctx):
     ib.free()
 
 
+def test_far_rows(ctx):
+    """Rows whose bytes lie beyond 4 GiB: the ids of the same rows side by side."""
+    say("sample far")
+    rng = np.random.default_rng(14)
+    R, n, ld = 3, 20001, (1 << 29) + 3
+    x = (rng.standard_normal((R, n)) * 3).astype(np.float32)
+    par = np.array([[1.0, 0.7, 1.3], [0.9, 1.0, 0.95], [0, 0.01, 0], rng.random(R)], np.float32)
+    k = np.array([0, 0, 500], np.int32)
+    a, near, ids = ctx.alloc(4 * (2 * ld + n)), ctx.alloc(4 * (R * n + 4 * R)), ctx.alloc(4 * 3 * R)
+    near.upload(np.concatenate([x.reshape(-1), par.reshape(-1)]))
+    for r in range(R):
+        a.upload(x[r], 4 * r * ld)
+    a.upload(par.reshape(-1), 4 * (n + 5))                   # (between the rows)
+    ids.upload(k)
+    q8hip.sample(ctx, near, 0, R, n, R * n, ids, 0, R)
+    q8hip.sample(ctx, a, 0, R, n, n + 5, ids, 0, 2 * R, ldx=ld)
+    got = ids.download((3, R), np.int32)
+    assert np.array_equal(got[1], got[2]) and (got[1] >= 0).all()
+    for b in (a, near, ids):
+        b.free()
+
+
 def test_many_rows(ctx):
     """More rows than a launch's grid holds."""
     say("sample many rows")

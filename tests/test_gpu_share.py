@@ -46,20 +46,24 @@ class Step:
         n = q8hip.kv8_share_ints(self.ns, rows)
         return np.concatenate([self.cu, self.old, self.table.reshape(-1), np.full(n + 1, -77, np.int32)]).astype(np.int32)
 
-    def run(self, ctx, q, dead=0, off=0, extra=0, share=True, spoil=None):
+    def run(self, ctx, q, dead=0, off=0, extra=0, share=True, spoil=None, far=0):
+        """far: pages in front of the ones in use."""
         T, nh, hd = q.shape
         rows, ld, ns = T + dead, nh * hd + extra, self.ns
         arena = np.full(off + rows * (ld + nh * hd) + 4, 5, np.float32)
         arena[off:off + T * ld].reshape(T, ld)[:, :nh * hd] = q.reshape(T, -1)
         ints = self.ints(rows)
+        table = ints[2 * ns + 1:2 * ns + 1 + ns * self.maxpages]
+        table[table >= 0] += far
         at = 2 * ns + 1 + ns * self.maxpages
         a, ix, pool = ctx.alloc(arena.nbytes), ctx.alloc(ints.nbytes), self.c.to_bytes()
-        pages = ctx.alloc(pool.nbytes)
+        page_bytes, npages = pool.nbytes // self.c.npages, self.c.npages + far
+        pages = ctx.alloc(npages * page_bytes)
         a.upload(arena)
         ix.upload(ints)
-        pages.upload(pool)
+        pages.upload(pool, far * page_bytes)
         arrays = (ix, 0, ns + 1, 2 * ns + 1, ns, rows, self.maxpages)
-        q8hip.kv8_share(ctx, *arrays, self.c.npages, self.P, at)
+        q8hip.kv8_share(ctx, *arrays, npages, self.P, at)
         now = ix.download(ints.shape, np.int32)
         assert np.array_equal(now[:at], ints[:at]) and now[-1] == -77
         self.found = now[at + 1:at + 1 + ns].tolist(), now[at + 1 + ns:at + 1 + 2 * ns].tolist()
@@ -67,7 +71,7 @@ class Step:
         if spoil is not None:
             ix.upload(spoil(now[at:-1]).astype(np.int32), 4 * at)
         oy = off + rows * ld
-        args = (ctx, a, off, oy, pages, 0, self.c.npages, self.P, *arrays, nh, self.nkv, hd)
+        args = (ctx, a, off, oy, pages, 0, npages, self.P, *arrays, nh, self.nkv, hd)
         if share:
             q8hip.kv8_attention_shared(*args, at, ldq=ld if extra else 0)
         else:
@@ -146,6 +150,16 @@ def test_wide_tables(ctx, P, hd):
     s.table = np.concatenate([s.table, np.full((s.ns, more), -1, np.int32)], axis=1)
     s.maxpages += more
     s.check(ctx, queries(rng, s.T, 8, hd), dead=1, off=3, extra=7)
+
+
+def test_far_pages(ctx):
+    """Page ids whose bytes lie beyond 4 GiB: the bits of the same pages in front."""
+    say("shared far")
+    rng = np.random.default_rng(12)
+    s = Step(rng, [1, 2, 1, 1], [0, 0, -1, 0], [5], [70, 3, 90, 0], 64, 2, 128)
+    q = queries(rng, s.T, 8, 128)
+    far = (1 << 32) // q8hip.kv8_page_bytes(64, 2, 128) + 1
+    assert np.array_equal(s.run(ctx, q, far=far), s.check(ctx, q))
 
 
 def test_drafts_in_wide_groups(ctx):
