@@ -605,11 +605,15 @@ __device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8Share
 // ---- the shared tokens of groups ------------------------------------------------------
 // A block takes a row tile of 64 columns (row of the group, query head), 16 a wave, over
 // a cut of the group's shared tokens; all columns see all of them.  A unit's K codes and
-// its V, as bf16 once for all waves, go through LDS in the layout of the MFMA operands (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in
-// flight beside this one's products.  Scores, probabilities and products are those of
-// kv8_attn_kernel.  Bound: VALU (the joins of the digits, exp, p in three terms: 340
-// operations a unit and 16 columns, 190 of them for codes -> bf16 if every wave did that
-// for itself).
+// its V, as bf16 once for all waves, go through LDS in the layout of the MFMA operands
+// (a lane's 16 bytes side by side, no bank conflicts), the next unit's loads in flight
+// beside this one's products.  Scores, probabilities and products are those of
+// kv8_attn_kernel.
+// Bound: instruction issue; VALU (the joins of the digits, exp, p in three terms) and
+// MFMA (32 of int8, 48 of bf16 a unit and wave, heads of 128) take turns more than they
+// overlap: 128 sequences of 4 heads a KV head behind 32000 tokens 195 us, 105 of VALU
+// and 67-84 of MFMA by their counters, at 1.9 GHz.  (Eight waves over 128 columns, 4
+// waves a SIMD: 279 us.)
 template <int HD> __device__ __forceinline__ void kv8_shared_block(const Kv8AttnArgs &a) {
   constexpr int DT = HD / 16, HH = HD / 64, NC = kKv8ShareCols;
   constexpr int KF = 4 * HH / kKv8Waves, VF = DT / kKv8Waves;   // fragments that a wave stages

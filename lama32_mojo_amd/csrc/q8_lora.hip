@@ -26,7 +26,9 @@ namespace {
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // any f32 address
 
 constexpr int kThreads = 256;
-constexpr int kCols = 512;                            // columns of a block, 64-row tiles
+// Columns of a block, 64-row tiles (4130 rows x 28672 columns 261 us, 512 262, 128 284; 512
+// rows x 14336 columns 23.6, 512 25.9, 128 26.1).
+constexpr int kCols = 256;
 constexpr int kRankTiles = 4;                         // 16-rank tiles of a shrink block
 
 // x as three bf16 terms (truncations, exact), eight values.
@@ -208,19 +210,23 @@ __device__ __forceinline__ float *part_at(const LoraArgs &a, int tile, int split
          ((int64_t)tile * a.splits + split) * TR * a.ranks;
 }
 
-// A x of a tile over one part of K: grid (tiles, parts of K, groups of kRankTiles
-// rank tiles).  RT = 1: 16 rows, the waves take K steps in turn and meet in LDS; RT =
-// 4: 64 rows, 16 a wave.
+// A x of 16 rows of a tile over one part of K: grid (tiles, parts of K, groups of
+// kRankTiles rank tiles x the tile's 16-row parts).  The waves take K steps in turn and
+// meet in LDS.  (A wave to each 16 rows of 64 and all of its part of K took 51 us where
+// this takes 45: five adapters of rank 16 to 64 over 4130 rows of 4096, two projections.)
+// Bound: for prompts the matrix work and the weights' way through L1, 6 KB a wave and
+// step for 12 MFMAs; for token steps the chain cu -> adapter -> weights -> meeting (64
+// requests over 24 adapters 12 us, 1 request 5).
 template <bool F32, int RT>
 __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   constexpr int TR = 16 * RT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ uint32_t wsum[kThreads / 64];
   __shared__ int found[4], rows[TR];
-  __shared__ f32x4 meet[RT == 1 ? 3 : 1][kRankTiles][64];
+  __shared__ f32x4 meet[kThreads / 64 - 1][kRankTiles][64];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int col = lane & 15, g4 = lane >> 4;
-  const int split = blockIdx.y;
+  const int split = blockIdx.y, row0 = 16 * (blockIdx.z % RT);
   if (!lora_tile<TR>(a, a.tile0 + blockIdx.x, reinterpret_cast<uint32_t *>(lds), wsum, found, rows)) {
     if (t == 0 && split == 0 && blockIdx.z == 0) record_at<TR>(a, blockIdx.x)[1] = 0;
     return;
@@ -237,14 +243,14 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   }
   if (rank <= 0) return;
   const int rp = rank8(rank, a.max_rank), ranks = a.parts * rp;
-  const int q0 = blockIdx.z * kRankTiles;             // this block's first rank tile
+  const int q0 = blockIdx.z / RT * kRankTiles;        // this block's first rank tile
   const int nq = min(kRankTiles, (ranks + 15) / 16 - q0);
-  if (nq <= 0) return;
+  if (nq <= 0 || row0 >= n) return;
   const int64_t m = a.m;
   const int64_t per = ((m + a.splits - 1) / a.splits + 31) / 32 * 32;
   const int64_t k0 = split * per, k1 = min(k0 + per, m);
   const uint8_t *A = a.A + (int64_t)ad * a.a_stride * (F32 ? 4 : 2);
-  const float *x = a.x + (int64_t)rows[(RT == 1 ? 0 : 16 * w) + col] * a.ldx + 8 * g4;
+  const float *x = a.x + (int64_t)rows[row0 + col] * a.ldx + 8 * g4;
   int64_t wrow[kRankTiles];
 #pragma unroll
   for (int q = 0; q < kRankTiles; ++q)
@@ -254,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   for (int q = 0; q < kRankTiles; ++q) acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // U steps of 32 at a time, all their loads first; the last ones with a test for each
   // lane's eight (m is a multiple of 8; those behind k1 load the row's start)
-  constexpr int U = F32 ? 1 : 4, STEP = RT == 1 ? 128 : 32;
+  constexpr int U = F32 ? 1 : 4, STEP = 32 * (kThreads / 64);
   auto steps = [&](int64_t k, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     f32x4 xa[U], xb[U];
@@ -286,25 +292,21 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
         if (q < nq) acc[q] = wt[u][q].times(in[u], xt, acc[q]);
     }
   };
-  if (RT == 1 || 16 * w < n) {
-    int64_t k = k0 + (RT == 1 ? 32 * w : 0);
-    for (; k + (U - 1) * STEP + 32 <= k1; k += U * STEP) steps(k, std::true_type{});
-    if (k < k1) steps(k, std::false_type{});
+  int64_t k = k0 + 32 * w;
+  for (; k + (U - 1) * STEP + 32 <= k1; k += U * STEP) steps(k, std::true_type{});
+  if (k < k1) steps(k, std::false_type{});
+  if (w > 0) {
+#pragma unroll
+    for (int q = 0; q < kRankTiles; ++q) meet[w - 1][q][lane] = acc[q];
   }
-  if (RT == 1) {
-    if (w > 0) {
+  __syncthreads();
+  if (w > 0) return;
 #pragma unroll
-      for (int q = 0; q < kRankTiles; ++q) meet[w - 1][q][lane] = acc[q];
-    }
-    __syncthreads();
-    if (w > 0) return;
+  for (int z = 0; z < kThreads / 64 - 1; ++z)
 #pragma unroll
-    for (int z = 0; z < 3; ++z)
-#pragma unroll
-      for (int q = 0; q < kRankTiles; ++q) acc[q] += meet[z][q][lane];
-  }
+    for (int q = 0; q < kRankTiles; ++q) acc[q] += meet[z][q][lane];
   // lane: ranks 16 q + 4 g4 .. of row col
-  const int row = (RT == 1 ? 0 : 16 * w) + col;
+  const int row = row0 + col;
   if (row >= n) return;
   float *out = part_at<TR>(a, blockIdx.x, split) + (int64_t)row * a.ranks + 16 * q0 + 4 * g4;
 #pragma unroll
@@ -515,8 +517,8 @@ hipError_t launch_lora_t(LoraArgs a, int64_t ws_floats, hipStream_t st) {
   const int rank_groups = (a.ranks / 16 + kRankTiles - 1) / kRankTiles;
   // parts of K: two blocks a CU, each with four steps of 32 a wave at least; few
   // for large tiles, whose parts are added by every column block
-  const int64_t step = RT == 1 ? 512 : 1024;
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + all - 1) / all, (a.m + step - 1) / step));
+  const int64_t mine = all * RT;
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + mine - 1) / mine, (a.m + 511) / 512));
   if (RT > 1) a.splits = std::min(a.splits, 4);
   const int64_t per = record_ints<TR>() + (int64_t)a.splits * TR * a.ranks;
   const int64_t most = std::min<int64_t>(ws_floats / per, 65535);
@@ -533,7 +535,7 @@ hipError_t launch_lora_t(LoraArgs a, int64_t ws_floats, hipStream_t st) {
     a.tile0 = (int)t0;
     a.tiles = (int)std::min(most, all - t0);
     hipLaunchKernelGGL((lora_shrink_kernel<F32, RT>),
-                       dim3((unsigned)a.tiles, (unsigned)a.splits, (unsigned)rank_groups), dim3(kThreads), lds0,
+                       dim3((unsigned)a.tiles, (unsigned)a.splits, (unsigned)(rank_groups * RT)), dim3(kThreads), lds0,
                        st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -548,9 +550,13 @@ hipError_t launch_lora_t(LoraArgs a, int64_t ws_floats, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_lora(const LoraArgs &a, int64_t ws_floats, hipStream_t st) {
-  // tiles of 64 rows where an adapter has as many on average
+  // Tiles of 64 rows where an adapter has 256 on average (f32: 64): fewer reads of its
+  // weights and fewer terms of f32 ones, but fewer blocks (us in tiles of 64 / 16: four
+  // adapters of 4096 x 14336, rank 64, with 128 rows each 43 / 36, 192 43 / 45, 256 60
+  // / 63, 384 71 / 92; of 4096 x 4096, rank 16, 256 24 / 23, 512 31 / 34; f32, rank 64,
+  // 32 rows 46 / 43, 64 51 / 69, 256 118 / 212; rank 16, 64 23 / 21, 128 24 / 26).
   const int64_t groups = std::min(a.nseq, a.nadapters);
-  const bool wide = a.rows >= 64 * std::max<int64_t>(groups, 1) && a.max_rank <= 128;
+  const bool wide = a.rows >= (a.f32 ? 64 : 256) * std::max<int64_t>(groups, 1) && a.max_rank <= 128;
   if (a.f32) return wide ? launch_lora_t<true, 4>(a, ws_floats, st) : launch_lora_t<true, 1>(a, ws_floats, st);
   return wide ? launch_lora_t<false, 4>(a, ws_floats, st) : launch_lora_t<false, 1>(a, ws_floats, st);
 }

@@ -157,6 +157,16 @@ def test_many(ctx):
     Setup(rng, (rng.random(4096) < 0.7).astype(int).tolist(), ids.tolist(), [4] * 4096, 16, [8], "bf16").check(ctx)
 
 
+@pytest.mark.parametrize("rank", [1, 8, 9, 24, 40, 128])
+@pytest.mark.parametrize("lens", [[257], [500, 270, 0, 1, 63], [1024]])
+def test_tiles_of_64_rows(ctx, rank, lens):
+    say("lora tiles", rank, lens)
+    rng = np.random.default_rng(rank + lens[0])
+    s = Setup(rng, lens, [0, 1, 0, -1, 1][:len(lens)], [rank, 8][:len(lens)], 264, [300, 17], gap=1, dead=3)
+    y = s.check(ctx, pad=1, ex=5, ey=3)
+    assert np.array_equal(s.run(ctx, in_place=True), y)
+
+
 def test_more_columns_than_blocks(ctx):
     """More blocks of 128 columns than a grid has places in y."""
     say("lora wide")
