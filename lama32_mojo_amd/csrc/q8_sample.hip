@@ -193,9 +193,9 @@ __device__ __forceinline__ RowSettings settings(const SampleArgs &a, int64_t row
 }
 
 // ---- pass 1: the histogram of a slice, grid (slices, rows) ---------------------
-// Bound: 15 f64 operations and an LDS atomic a logit, beside one read of the logits
-// (256 rows of 151936, 156 MB, 50 us: 3.1 TB/s, half of what a plain read reaches; 64
-// rows of 128256 22 us; a row alone 10.5 us, its chain).  A block walks its slice in chunks that it holds in registers; the
+// Bound: VALU, 13 f64 operations and an LDS atomic a logit, beside one read of the logits
+// (256 rows of 151936, 156 MB, 43 us: 3.6 TB/s, half of what a plain read reaches; 64
+// rows of 128256 20.5 us; a row alone 9 us, its chain).  A block walks its slice in chunks that it holds in registers; the
 // bins are a ring whose head is the slice's largest value so far, so the row's
 // maximum need not be known first.
 __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs a, int64_t row0,
@@ -258,31 +258,31 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
       __syncthreads();
       index = best;
     }
-    if (!s.greedy) {
-      // (adding 1.5 2^52 rounds to a whole number, whose low bits are the bin's; further
-      // from 0 than that allows, the plain way)
+    auto add = [&](int at, uint64_t w) {
+      atomicAdd(reinterpret_cast<unsigned long long *>(&mass[at]), (unsigned long long)w);
+      if (counts) atomicAdd(&count[at], 1u);
+    };
+    // Adding 1.5 2^52 rounds to a whole number, whose low bits are the bin's; further
+    // from 0 than that allows, the plain way.
+    if (!s.greedy && __builtin_fabs(top_bin) < 0x1p30) {
       const double scale = s.inv_t * kBinsPerUnit, least = top_bin - kBins + 0.5;
-      const bool near = __builtin_fabs(top_bin) < 0x1p30;
+      const uint32_t from = (uint32_t)(head + (int)top_bin);
 #pragma unroll
       for (int e = 0; e < kPerThread; ++e) {
-        int d;
-        uint64_t w;
-        if (near) {
-          const double z = (double)v[e] * scale;
-          if (!(z > least) || v[e] == -INFINITY) continue;              // (and NaN)
-          const double whole = z + 0x1.8p52;
-          d = (int)top_bin - (int)(uint32_t)__builtin_bit_cast(uint64_t, whole);
-          w = weight16(z - (whole - 0x1.8p52));
-        } else {
-          if (!(v[e] > -INFINITY)) continue;
-          const BinOf b = bin_of(v[e], s.inv_t);
-          d = below(top_bin, b.a);
-          if (d >= kBins) continue;
-          w = weight(b);
-        }
-        const int at = (head + d) & (kBins - 1);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&mass[at]), (unsigned long long)w);
-        if (counts) atomicAdd(&count[at], 1u);
+        const double z = (double)v[e] * scale, whole = z + 0x1.8p52;
+        const uint64_t w = weight16(z - (whole - 0x1.8p52));
+        if (z > least)                                // (not NaN; of -inf it is that or -inf)
+          add((int)((from - (uint32_t)__builtin_bit_cast(uint64_t, whole)) & (kBins - 1)), w);
+      }
+    } else if (!s.greedy) {
+#pragma unroll 1
+      for (int e = 0; e < kPerThread; ++e) {
+        float x = v[0];
+#pragma unroll
+        for (int i = 1; i < kPerThread; ++i) x = i == e ? v[i] : x;
+        const BinOf b = bin_of(x, s.inv_t);
+        const int d = below(top_bin, b.a);
+        if (x > -INFINITY && d < kBins) add((head + d) & (kBins - 1), weight(b));
       }
     }
     __syncthreads();                                  // wmax, best, the ring's head
@@ -908,7 +908,8 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
 }  // namespace
 
 // Slices of a row: enough blocks for the chip (four of 512 threads a CU), none
-// shorter than a chunk.
+// shorter than a chunk (256 rows of 151936 with top-p: 127 us with 1024 blocks, 132 with
+// 512, 131 with 2048; 64 rows of 128256 73, 72, 73).
 constexpr int64_t kBlocks = 1024;
 static int64_t sample_slices(int64_t rows, int64_t n) {
   const int64_t most = std::min<int64_t>(kMaxSlices, (n + kChunk - 1) / kChunk);
