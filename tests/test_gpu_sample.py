@@ -217,6 +217,16 @@ def test_captured(ctx):
     ib.free()
 
 
+def test_largest_row(ctx):
+    """2^22 logits, spread and all alike."""
+    say("sample largest")
+    rng = np.random.default_rng(15)
+    x = (rng.standard_normal((2, 1 << 22)) * 3).astype(np.float32)
+    x[1] = 0.5
+    for kw in (dict(), dict(k=40, top_p=0.9), dict(top_p=0.95)):
+        check(ctx, x, u=np.array([0.3, 0.7], np.float32), **kw)
+
+
 def test_far_rows(ctx):
     """Rows whose bytes lie beyond 4 GiB: the ids of the same rows side by side."""
     say("sample far")
