@@ -158,6 +158,28 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(a, b), fmaxf(c, d));
 }
 
+// v of other lanes of the wave, 0 where there is none (all lanes active).
+template <int CTRL, int ROWS, class T> __device__ __forceinline__ T from_lanes(T v) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    int w[W];
+  } x = __builtin_bit_cast(Words, v), y;
+#pragma unroll
+  for (int i = 0; i < W; ++i) y.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(T, y);
+}
+
+// Inclusive sums by `add` (0: neutral) over a wave's lanes, in one fixed order: within
+// rows of 16, then the rows' last lanes into the rows behind.
+template <class T, class F> __device__ __forceinline__ T wave_scan(T v, F add) {
+  v = add(v, from_lanes<0x111, 0xf>(v));   // row_shr 1, 2, 4, 8
+  v = add(v, from_lanes<0x112, 0xf>(v));
+  v = add(v, from_lanes<0x114, 0xf>(v));
+  v = add(v, from_lanes<0x118, 0xf>(v));
+  v = add(v, from_lanes<0x142, 0xa>(v));   // row_bcast 15 to rows 1, 3
+  return add(v, from_lanes<0x143, 0xc>(v));   // row_bcast 31 to rows 2, 3
+}
+
 // Sum over a 256-thread block (4 waves), the same value in every thread:
 // wave sums, then (w0 + w1) + (w2 + w3).  red: 4 floats of LDS.
 __device__ __forceinline__ float block_sum256(float v, float *red) {

@@ -505,11 +505,7 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, int 
       pl.n[i] = s.n;
       pl.old[i] = s.old;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(u, d);
-      if (lane >= d) u = kv8_add(u, o);
-    }
+    u = wave_scan(u, [](int a, int b) { return kv8_add(a, b); });
     if (lane == 63) wsum[w] = u;
     __syncthreads();
     int all = 0;
@@ -584,19 +580,13 @@ __device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8Share
   g.units = (g.tokens + kKv8Unit - 1) / kKv8Unit;
   const int64_t tiles = ((int64_t)g.n * (c.nheads / c.nkv) + kKv8ShareCols - 1) / kKv8ShareCols;
   const int64_t work = tiles * g.units;
-  int u = work < kKv8MaxUnits ? (int)work : kKv8MaxUnits;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) u = kv8_add(u, __shfl_xor(u, d));
-  g.per = kv8_units_per_block(u, target, 1);
+  auto add = [](int a, int b) { return kv8_add(a, b); };
+  const int all = wave_scan(work < kKv8MaxUnits ? (int)work : kKv8MaxUnits, add);
+  g.per = kv8_units_per_block(__builtin_amdgcn_readlane(all, 63), target, 1);
   g.cuts = (g.units + g.per - 1) / g.per;
   const int64_t blocks = tiles * g.cuts;
   const int mine = blocks < kKv8MaxUnits ? (int)blocks : kKv8MaxUnits;
-  u = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(u, d);
-    if (lane >= d) u = kv8_add(u, o);
-  }
+  const int u = wave_scan(mine, add);
   g.base = u - mine;
   g.blocks = __builtin_amdgcn_readlane(u, 63);
   return g;
@@ -1209,18 +1199,35 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   const int row = blockIdx.x, t = threadIdx.x;
   const int *pre = kv8_plan_at<HD, NC>(a, runs);
   const int per = kv8_units_per_block(pre[nseq], runs, 1);
+  // a sequence a lane, where that is all of them, beside the search below: its group, the
+  // tokens it takes from it and its place there
+  Kv8ShareAt sh;
+  Kv8Groups gs;
+  int group = -1, pos = 0, shared = 0, unit0 = 0;
+  auto load = [&](int i) {
+    group = sh.group[i];
+    pos = sh.pos[i];
+    shared = kv8_shared_tokens(c, sh, i);
+    unit0 = pre[i];
+  };
+  if constexpr (PART == KV8_OWN) {
+    sh = kv8_share_at(c, a.share);
+    gs = kv8_groups(c, sh, a.shared_target);
+    if (nseq <= 64) load(min(t & 63, nseq - 1));
+  }
   // the sequence of this row: the last one that begins at it or before
   const SeqAt at = find_seq(c.cu, c.len, nseq, c.rows, row, 1, 0);
   const int lo = at.i, j = row - at.r0;
   Kv8Seq sq = kv8_seq(at.r0, at.r1, at.len, c.rows, c.maxpages * c.page, grp, NC);
   // the group's records of this row: cuts of them, from block `cut0` on
-  int group = -1, cuts = 0, cut0 = 0, place = 0;
+  int cuts = 0, cut0 = 0, place = 0;
   if constexpr (PART == KV8_OWN) {
-    const Kv8ShareAt sh = kv8_share_at(c, a.share);
-    const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
-    const int pos = sh.pos[lo];
-    kv8_from(sq, kv8_shared_tokens(c, sh, lo), c.maxpages * c.page);
-    group = __builtin_amdgcn_readfirstlane(sh.group[lo]);
+    const int from = nseq <= 64 ? lo : 0;
+    if (nseq > 64) load(lo);
+    group = __builtin_amdgcn_readlane(group, from);
+    pos = __builtin_amdgcn_readlane(pos, from);
+    unit0 = __builtin_amdgcn_readlane(unit0, from);
+    kv8_from(sq, __builtin_amdgcn_readlane(shared, from), c.maxpages * c.page);
     if (group < 0 || group >= sh.groups) group = -1;
     if (group >= 0) {
       cuts = __builtin_amdgcn_readlane(gs.cuts, group);
@@ -1228,6 +1235,8 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
       place = clamp_i((int64_t)pos + j - __builtin_amdgcn_readlane(gs.row0, group), 0,
                       max(0, __builtin_amdgcn_readlane(gs.n, group) - 1));
     }
+  } else {
+    unit0 = pre[lo];
   }
   if (j < 0 || j >= sq.n) return;             // behind the last sequence
   constexpr int IPH = HD / 4;
@@ -1236,7 +1245,7 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   {
     const int hh = blockIdx.z * hb + item / IPH, d = 4 * (item % IPH);
     const int lin = j * grp + hh, rt = lin / NC, cc = lin % NC;
-    const int64_t ua = pre[lo] + (int64_t)rt * sq.key_units;
+    const int64_t ua = unit0 + (int64_t)rt * sq.key_units;
     const int b0 = clamp_i(ua / per, 0, runs - 1);
     const int b1 = clamp_i((ua + sq.key_units - 1) / per, 0, runs - 1);
     float m = -INFINITY, l = 0.0f;

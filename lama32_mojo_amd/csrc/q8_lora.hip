@@ -98,11 +98,7 @@ __device__ __forceinline__ int rank8(int rank, int max_rank) {
 // Inclusive sum over the block's threads; *total the whole one.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *wsum, uint32_t *total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v = wave_scan(v, [](uint32_t a, uint32_t b) { return a + b; });
   if (lane == 63) wsum[w] = v;
   __syncthreads();
   uint32_t base = 0, all = 0;

@@ -101,25 +101,9 @@ template <class T> __device__ __forceinline__ T uniform(T v) {
   return __builtin_bit_cast(T, x);
 }
 
-// Inclusive sums over a wave's lanes (rows of 16, then the rows' last lanes into the
-// rows behind), in one fixed order.
-template <int CTRL, int ROWS, class T> __device__ __forceinline__ T from_lanes(T v) {
-  constexpr int W = sizeof(T) / 4;
-  struct Words {
-    int w[W];
-  } x = __builtin_bit_cast(Words, v), y;
-#pragma unroll
-  for (int i = 0; i < W; ++i) y.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], CTRL, ROWS, 0xf, false);
-  return __builtin_bit_cast(T, y);                    // (0 where there is no such lane)
-}
+// Inclusive sums over a wave's lanes, in one fixed order.
 template <class T> __device__ __forceinline__ T wave_sums(T v) {
-  v += from_lanes<0x111, 0xf>(v);                     // row_shr 1, 2, 4, 8
-  v += from_lanes<0x112, 0xf>(v);
-  v += from_lanes<0x114, 0xf>(v);
-  v += from_lanes<0x118, 0xf>(v);
-  v += from_lanes<0x142, 0xa>(v);                     // row_bcast 15 to rows 1, 3
-  v += from_lanes<0x143, 0xc>(v);                     // row_bcast 31 to rows 2, 3
-  return v;
+  return wave_scan(v, [](T a, T b) { return a + b; });
 }
 // Over the block's threads; *all: the last one's.  wsum: a value a wave; the caller
 // waits before it writes there again.
