@@ -1163,7 +1163,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
     if (j < n) {
       const bool whole = WHOLE || (cu.t0 == 0 && cu.t1 == cu.units);
       float *rec = a.ws + (((int64_t)run * c.nkv + g) * 2 + (cu.t0 == 0)) * kv8_record<HD, NC>();
-      const float il = whole ? 1.0f / l : 1.0f;
+      // (as it is where the join with the group's part follows)
+      const float il = whole && !(PART == KV8_OWN && cu.k0 > 0) ? 1.0f / l : 1.0f;
       float *out = whole ? a.out + ((int64_t)(row0 + j) * c.nheads + g * grp + lin % grp) * HD
                          : rec + cc * HD;
 #pragma unroll
@@ -1227,8 +1228,9 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
     group = __builtin_amdgcn_readlane(group, from);
     pos = __builtin_amdgcn_readlane(pos, from);
     unit0 = __builtin_amdgcn_readlane(unit0, from);
-    kv8_from(sq, __builtin_amdgcn_readlane(shared, from), c.maxpages * c.page);
-    if (group < 0 || group >= sh.groups) group = -1;
+    shared = __builtin_amdgcn_readlane(shared, from);
+    kv8_from(sq, shared, c.maxpages * c.page);
+    if (shared == 0) group = -1;
     if (group >= 0) {
       cuts = __builtin_amdgcn_readlane(gs.cuts, group);
       cut0 = __builtin_amdgcn_readlane(gs.base, group);
@@ -1254,40 +1256,40 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
     const bool on = grp_id < sg && hh < grp && (b0 != b1 || (PART == KV8_OWN && group >= 0));
     if constexpr (PART == KV8_OWN) {
       if (on && group >= 0) {
-        // the group's cuts, then the row's own run where it has one
+        // the group's cuts, then the row's own run where it has one (three at a time: four
+        // take more than 64 registers)
         const int slin = place * grp + hh;
         constexpr int cols = kKv8ShareCols;
         const int64_t first = (int64_t)cut0 + (int64_t)(slin / cols) * cuts;
         const int all = cuts + (b0 == b1 && sq.key_units > 0);
         const int64_t h = (int64_t)row * c.nheads + g * grp + hh;
-        for (int z0 = grp_id; z0 < all; z0 += 4 * sg) {
-          float zm[4], zl[4], zw[4];
-          f32x4 zo[4];
+        for (int z0 = grp_id; z0 < all; z0 += 3 * sg) {
+          float zm[3], zl[3];
+          f32x4 zo[3];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 3; ++x) {
             const int z = z0 + x * sg < all ? z0 + x * sg : z0;
             const int64_t rb = min(first + z, (int64_t)a.shared_blocks - 1);
             const float *r = a.shared_rec + (rb * c.nkv + g) * kv8_record<HD, cols>();
             const bool rec = z < cuts;
             zm[x] = rec ? r[cols * HD + slin % cols] : a.ml[2 * h];
             zl[x] = rec ? r[cols * HD + cols + slin % cols] : a.ml[2 * h + 1];
-            zw[x] = rec ? 1.0f : zl[x];
             zo[x] = *reinterpret_cast<const f32x4_u *>(rec ? r + slin % cols * HD + d : a.out + h * HD + d);
           }
           float mx = m;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) mx = fmaxf(mx, zm[x]);
+          for (int x = 0; x < 3; ++x) mx = fmaxf(mx, zm[x]);
           const float ms = mx == -INFINITY ? 0.0f : mx;
           const float f0 = __builtin_amdgcn_exp2f(m - ms);
           l *= f0;
           o *= f0;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 3; ++x) {
             if (z0 + x * sg >= all) continue;
-            const float f = __builtin_amdgcn_exp2f(zm[x] - ms), fw = f * zw[x];
+            const float f = __builtin_amdgcn_exp2f(zm[x] - ms);
             l = __builtin_fmaf(f, zl[x], l);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(fw, zo[x][v], o[v]);
+            for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(f, zo[x][v], o[v]);
           }
           m = mx;
         }
@@ -1326,13 +1328,17 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
     *reinterpret_cast<f32x4 *>(so + 4 * t) = o;
     __syncthreads();
     if (grp_id != 0 || !on) return;
+    // groups of threads that took any
+    const int with = min(sg, max(b1 - b0, PART == KV8_OWN && group >= 0 ? cuts : 0) + 1);
     float mx = m;
-    for (int x = 1; x < sg; ++x) mx = fmaxf(mx, sm[x * hb * IPH + item]);
+#pragma unroll 4
+    for (int x = 1; x < with; ++x) mx = fmaxf(mx, sm[x * hb * IPH + item]);
     const float ms = mx == -INFINITY ? 0.0f : mx;
     const float f0 = __builtin_amdgcn_exp2f(m - ms);
     l *= f0;
     o *= f0;
-    for (int x = 1; x < sg; ++x) {
+#pragma unroll 2
+    for (int x = 1; x < with; ++x) {
       const int y = x * hb * IPH + item;
       const float f = __builtin_amdgcn_exp2f(sm[y] - ms);
       l = __builtin_fmaf(f, sl[y], l);
