@@ -35,6 +35,9 @@ constexpr int kList = 8192;                           // members of a bin kept i
 constexpr double kTie = 0x1p-45;
 constexpr int kMaxSlices = 64;
 constexpr int kTop = 256;                             // tokens of a slice that are listed
+// Members of a bin that are compared with each other (up to 256 took 8 to 11 us, a
+// narrowing step before takes 3).
+constexpr uint32_t kCompared = 64;
 
 // A slice's part of its row: sums and counts of the bins below its own maximum.
 // Behind them its largest tokens: all those of its first `upto` bins.
@@ -156,10 +159,10 @@ __device__ __forceinline__ void load16(const float *x, int64_t i, int64_t end, f
 }
 
 struct RowSettings {
-  bool greedy;
   double inv_t;
   int64_t k;
   double top_p, min_p, u;
+  int greedy, pad;
 };
 __device__ __forceinline__ RowSettings settings(const SampleArgs &a, int64_t row) {
   const float *p = a.param + row;
@@ -332,10 +335,10 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
 // ---- pass 2: one block of kBins threads per row --------------------------------
 // The slices' bins are added up; where the kept tokens are few they are sorted and
 // the filters and the draw are one running sum, else each border's bin is looked into.
-// Bound: the chain of dependent reads, searches and block-wide sums (17 us where few
+// Bound: the chain of dependent reads, searches and block-wide sums (15 us where few
 // tokens are kept), and for rows that keep many the second read of their logits by one
-// CU: 16 us for 128256, with two selections behind it 43 us (64 rows) to 73 us (256 rows
-// of 151936).
+// CU: 12 us for 128256, with the selections behind it 35 us (64 rows) to 58 us (256 rows
+// of 151936, whose read alone takes 23 us, 6.8 TB/s).
 
 // The bin that a border falls into, the sums before it and up to it, its own.
 struct BorderBin {
@@ -346,7 +349,7 @@ struct BorderBin {
 };
 
 struct SelectLds {
-  uint64_t mass[kBins];                               // (sorting: places; sums as f64)
+  __attribute__((aligned(16))) uint64_t mass[kBins];                               // (sorting: places; sums as f64)
   uint32_t count[kBins];
   uint64_t list[kList];                               // places of the members
   uint64_t wsum64[kBins / 64];
@@ -566,29 +569,30 @@ __device__ __forceinline__ uint64_t select(const RowAt &r, const Values &bin, Se
   uint32_t count0 = 0, left = l.n;
   __syncthreads();
   while (lo < hi) {
-    if (l.n <= kList && left <= kBins / 4) {
-      // a thread a member, against all: places in l.mass, weights behind them
+    if (l.n <= kList && left <= kCompared) {
+      // a thread a member, against all: places and weights in l.mass
       __syncthreads();
       if (t == 0) l.where = 0;
       __syncthreads();
       members(r, bin, l, [&](uint64_t p) {
         if (p < lo || p > hi) return;
         const uint32_t i = atomicAdd(&l.where, 1u);
-        l.mass[i] = p;
-        l.mass[kBins / 2 + i] = weight(bin_of(value_of(p), r.inv_t));
+        l.mass[2 * i] = p;
+        l.mass[2 * i + 1] = weight(bin_of(value_of(p), r.inv_t));
       });
       __syncthreads();
       left = l.where;
       bool is = false;
       uint64_t p = 0, m = mass0;
       if (t < (int)left) {
-        p = l.mass[t];
-        const uint64_t w = l.mass[kBins / 2 + t];
+        p = l.mass[2 * t];
+        const uint64_t w = l.mass[2 * t + 1];
         uint32_t c = count0;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t j = 0; j < left; ++j) {
-          const bool first = l.mass[j] < p;
-          m += first ? l.mass[kBins / 2 + j] : 0;
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&l.mass[2 * j]);
+          const bool first = o.x < p;
+          m += first ? o.y : 0;
           c += first;
         }
         is = reached(m + w, c + 1) && !reached(m, c);
@@ -697,12 +701,12 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
   const SampleSlice *sl = reinterpret_cast<const SampleSlice *>(a.ws) + (int64_t)blockIdx.x * slices;
   static_assert(kMaxSlices <= 64, "a slice a lane");
   const SampleSlice &mine = sl[min(lane, slices - 1)];
-  const RowSettings s = settings(a, row);
+  const RowSettings s = uniform(settings(a, row));    // (vector registers are short)
   const RowAt r = {a.x + row * a.ldx, a.n, s.inv_t, sl, slices, mine.top, mine.max, mine.upto, mine.listed};
   int index = mine.index;
   const float top = wave_max(r.max);                  // the row's maximum
   const uint64_t tops = __builtin_amdgcn_ballot_w64(r.max == top);
-  const double top_bin = __shfl(r.top, __builtin_ctzll(tops));
+  const double top_bin = uniform(__shfl(r.top, __builtin_ctzll(tops)));
   if (top == -INFINITY || s.greedy) {                 // (the whole block)
     if (r.max != top) index = INT32_MAX;
 #pragma unroll
@@ -736,15 +740,17 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
   }
   // (without a count: about as many, weights are within 1 / 32 of 2^40)
   if (!counts) c = (uint32_t)((m + ((uint64_t)1 << 39)) >> 40);
-  const double ymax = bin_of(top, s.inv_t).y;
+  const double ymax = uniform(bin_of(top, s.inv_t).y);
   // (y of the maximum from its bin's middle on, exact)
-  const double rest = __builtin_isinf(ymax) ? 0.0 : ymax - top_bin / kBinsPerUnit;
+  const double rest = uniform(__builtin_isinf(ymax) ? 0.0 : ymax - top_bin / kBinsPerUnit);
   const double unit = exp(-(double)t / kBinsPerUnit - rest) * 0x1p-40;  // weight of 1 in this bin
   const double here = (double)m * unit;
-  double total;
-  uint32_t tokens;
-  const double upto = block_sums<kBins>(here, l.wsumd[0], &total);     // this bin included
-  const uint32_t cupto = block_sums<kBins>(c, l.wsum32, &tokens);
+  double mass_all;
+  uint32_t count_all;
+  const double upto = block_sums<kBins>(here, l.wsumd[0], &mass_all);     // this bin included
+  const uint32_t cupto = block_sums<kBins>(c, l.wsum32, &count_all);
+  const double total = uniform(mass_all);
+  const uint32_t tokens = uniform(count_all);
   // the bin that a border falls into: the first one that reaches it; the last one with
   // tokens where rounding leaves none.  (Two places in turn: a barrier lies between two
   // uses of the same.)
@@ -775,7 +781,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
     turn ^= 1;
     return f;
   };
-  auto bin_at = [&](int b) { return b == 0 ? top_bin : top_bin - (double)b; };
+  auto bin_at = [&](int b) { return uniform(b == 0 ? top_bin : top_bin - (double)b); };
   const bool by_k = counts && s.k < (int64_t)tokens;
   // the last bin of min_p: weights from min_p on
   int last = kBins - 1;
@@ -807,7 +813,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
         (stage == BY_WEIGHT && !(s.min_p > 0.0 && last < kBins - 1)))
       continue;
     double more = NAN;
-    const double want = stage == BY_MASS ? fmax(s.top_p, 0.0) * W * (1.0 - kTie) : s.u * W * (1.0 + kTie);
+    const double want = uniform(stage == BY_MASS ? fmax(s.top_p, 0.0) * W * (1.0 - kTie) : s.u * W * (1.0 + kTie));
     BorderBin f = {};
     if (stage != FEW)
       f = border(stage == BY_K        ? (int64_t)cupto >= s.k
@@ -822,7 +828,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
       if ((both >> 40) + (both >> 45) < kList) more = bin_at(draw.bin);
     }
     if (stage == BY_WEIGHT && f.bin != last) {        // (no token there)
-      if (e_upto > 0.0) W = fmin(W, e_upto);
+      if (e_upto > 0.0) W = uniform(fmin(W, e_upto));
       continue;
     }
     const double before = f.before, u = f.unit;
@@ -872,7 +878,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
       if (part) atomicAdd(reinterpret_cast<unsigned long long *>(&l.found), (unsigned long long)part);
       __syncthreads();
       const double kept = before + (double)l.found * u;
-      if (kept > 0.0) W = fmin(W, kept);
+      if (kept > 0.0) W = uniform(fmin(W, kept));
       __syncthreads();
       continue;
     }
@@ -880,7 +886,7 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
     uint64_t J;
     const uint64_t p = select(r, in_bin, l, reached, &J);
     if (stage != DRAW) {
-      W = fmin(W, before + (double)J * u);
+      W = uniform(fmin(W, before + (double)J * u));
     } else if (t == 0) {
       a.ids[row] = (int)(uint32_t)p;
       const double y = bin_of(value_of(p), s.inv_t).y;
