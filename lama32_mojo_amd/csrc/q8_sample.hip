@@ -69,17 +69,16 @@ __device__ __forceinline__ int below(double top, double a) {
   return top == a ? 0 : d < (double)kBins ? (int)d : kBins;
 }
 // exp(y - middle of the bin) 2^40 as a whole number, from 16 times that difference, at
-// most 1 / 2: the series to the 5th power is 2^-39 off at most.  Adding 2^52 leaves the
-// integer in the low bits.
+// most 1 / 2: the series to the 5th power is 2^-39 off at most.  The last step adds 2^52 as
+// well, which leaves the integer in the low bits.
 __device__ __forceinline__ uint64_t weight16(double z) {
-  constexpr double h = 1.0 / kBinsPerUnit;
-  double p = h * h * h * h * h / 120.0;
-  p = __builtin_fma(p, z, h * h * h * h / 24.0);
-  p = __builtin_fma(p, z, h * h * h / 6.0);
-  p = __builtin_fma(p, z, h * h / 2.0);
-  p = __builtin_fma(p, z, h);
-  p = __builtin_fma(p, z, 1.0);
-  const double w = __builtin_fma(p, 0x1p40, 0x1p52);
+  constexpr double h = 1.0 / kBinsPerUnit, one = 0x1p40;
+  double p = one * h * h * h * h * h / 120.0;
+  p = __builtin_fma(p, z, one * h * h * h * h / 24.0);
+  p = __builtin_fma(p, z, one * h * h * h / 6.0);
+  p = __builtin_fma(p, z, one * h * h / 2.0);
+  p = __builtin_fma(p, z, one * h);
+  const double w = __builtin_fma(p, z, 0x1p52 + one);
   return __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
 }
 __device__ __forceinline__ uint64_t weight(const BinOf &b) {
