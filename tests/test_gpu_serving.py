@@ -280,3 +280,70 @@ def test_all_together(ctx):
     assert not np.array_equal(logits[0], logits[1])
     for x in (*pair, ad, m):
         x.close()
+
+
+def test_graphs_share_scratch(ctx):
+    """Captured draws, adapters and shared attention of one context, replayed in turn on three
+    streams beside eager calls: every replay as the eager result."""
+    torch = pytest.importorskip("torch")
+    from lama32_mojo_amd import q8hip
+    from test_gpu_lora import Setup
+    from test_gpu_share import Step, queries
+    say("serving graphs share scratch")
+    rng = np.random.default_rng(21)
+    # (arrays, the call on them, where the result lies): buffers stay as long as the graphs
+    R, n = 5, 20001
+    logits = (rng.standard_normal((R, n)) * 2).astype(np.float32)
+    par = np.array([[1.0] * R, [0.9, 1, 1, 0.99, 1], [0, 0.1, 0, 0, 0], rng.random(R)], np.float32)
+    sa, sids = ctx.alloc(4 * (R * n + 4 * R)), ctx.alloc(8 * R)
+    sa.upload(np.concatenate([logits.reshape(-1), par.reshape(-1)]))
+    sids.upload(np.array([0, 0, 50, 0, 0], np.int32))
+
+    su = Setup(rng, [300, 1, 40], [0, 1, 0], [40, 8], 512, [600], dtype="bf16")
+    m, w = 512, 600
+    la, lw, lx = ctx.alloc(4 * (su.rows * (m + 2 * w) + 2)), ctx.alloc(su.w.nbytes), ctx.alloc(4 * 9)
+    la.upload(np.concatenate([su.x.reshape(-1), su.base.reshape(-1), np.zeros(su.rows * w, np.float32), su.scale]))
+    lw.upload(su.w)
+    lx.upload(np.concatenate([su.cu, su.ids, su.ranks]).astype(np.int32))
+
+    st = Step(rng, [1] * 9, [0] * 7 + [-1, -1], [30], rng.integers(0, 200, 9), 16, 2, 64)
+    q = queries(rng, 9, 8, 64)
+    at = 2 * 9 + 1 + 9 * st.maxpages
+    aa, ap, ax = ctx.alloc(2 * q.nbytes), ctx.alloc(st.c.to_bytes().nbytes), ctx.alloc(4 * (at + q8hip.kv8_share_ints(9, 9)))
+    aa.upload(q)
+    ap.upload(st.c.to_bytes())
+    ax.upload(np.concatenate([st.cu, st.old, st.table.reshape(-1)]).astype(np.int32))
+    where = (ax, 0, 10, 19, 9, 9, st.maxpages)
+
+    def share():
+        q8hip.kv8_share(ctx, *where, st.c.npages, 16, at)
+        q8hip.kv8_attention_shared(ctx, aa, 0, q.size, ap, 0, st.c.npages, 16, *where, 8, 2, 64, at)
+    calls = [
+        (lambda: q8hip.sample(ctx, sa, 0, R, n, R * n, sids, 0, R), sids, (R,), np.int32, 4 * R),
+        (lambda: q8hip.lora(ctx, lw, 0, su.sa, 2 * su.sa, su.sb, 2, 40, la, 0, su.rows * m, su.rows * (m + w),
+                            su.rows * (m + 2 * w), lx, 0, 4, 7, 3, su.rows, m, [w]), la, (su.rows, w), np.float32,
+         4 * su.rows * (m + w)),
+        (share, aa, q.shape, np.float32, q.nbytes)]
+    eager, graphs = [], []
+    for call, buf, shape, dtype, off in calls:
+        call()
+        eager.append(buf.download(shape, dtype, off))
+        ctx.graph_begin()
+        call()
+        graphs.append(ctx.graph_end())
+    streams = [torch.cuda.Stream() for _ in calls]
+    for i in range(9):
+        for _, buf, shape, dtype, off in calls:
+            buf.upload(np.full(shape, -3, dtype), off)
+        for k in range(3):
+            ctx.set_stream(streams[(i + k) % 3].cuda_stream)
+            graphs[(k + i // 3) % 3].launch()
+        torch.cuda.synchronize()
+        ctx.set_stream(None)
+        for (call, buf, shape, dtype, off), y in zip(calls, eager):
+            assert np.array_equal(buf.download(shape, dtype, off), y), i
+        calls[i % 3][0]()
+    for g in graphs:
+        g.destroy()
+    for b in (sa, sids, la, lw, lx, aa, ap, ax):
+        b.free()
