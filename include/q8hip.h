@@ -575,8 +575,8 @@ int q8_pages_compact(q8_ctx *ctx, q8_buf *ix, uint64_t otab_i32, uint64_t oheld_
  * (row stride ldy, 0: dense), y = base in place allowed; scale f32 [nadapters].
  * m a multiple of 8; ranks up to 256, up to 4096 adapters and 4096 sequences, more
  * than one with the same adapter.  f32 accuracy: x, A x and f32 weights enter as they
- * are, sums are f32.  A row with infinities or NaN in x has NaN in its y and leaves
- * others as they are.  The context's scratch is used (q8_set_stream). */
+ * are, sums are f32.  A row with an adapter and infinities or NaN in x has NaN in its y
+ * and leaves others as they are.  The context's scratch is used (q8_set_stream). */
 int q8_lora(q8_ctx *ctx, q8_buf *w, int w_dtype, uint64_t oa, int64_t a_stride, uint64_t ob,
             int64_t b_stride, int64_t nadapters, int max_rank, q8_buf *a, uint64_t ox_f32, int64_t ldx,
             uint64_t obase_f32, uint64_t oy_f32, int64_t ldy, uint64_t oscale_f32, q8_buf *ix,

@@ -334,8 +334,8 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
 // ---- pass 2: one block of kBins threads per row --------------------------------
 // The slices' bins are added up; where the kept tokens are few they are sorted and
 // the filters and the draw are one running sum, else each border's bin is looked into.
-// Bound: the chain of dependent reads, searches and block-wide sums (15 us where few
-// tokens are kept), and for rows that keep many the second read of their logits by one
+// Bound: the chain of dependent reads, searches and block-wide sums (13 us where few
+// tokens are kept, a third of it fetching code for its first use), and for rows that keep many the second read of their logits by one
 // CU: 12 us for 128256, with the selections behind it 35 us (64 rows) to 58 us (256 rows
 // of 151936, whose read alone takes 23 us, 6.8 TB/s).
 
