@@ -493,7 +493,7 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
  * q8_kv8_attention_shared: as q8_kv8_attention of the same arrays, within the same
  * bounds.  Sequences without a group are served as there.  The context's scratch
  * is used; where the rows of a call leave no room for the groups' records
- * there (some 1500 rows of 32 heads of 128), each sequence reads its own tokens. */
+ * there (some 1800 rows of 32 heads of 128), each sequence reads its own tokens. */
 uint64_t q8_kv8_share_ints(int64_t nseq, int64_t rows);
 int q8_kv8_share(q8_ctx *ctx, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32,
                  int64_t nseq, int64_t rows, int64_t maxpages, int64_t npages, int page,
