@@ -179,7 +179,8 @@ __device__ __forceinline__ RowSettings settings(const SampleArgs &a, int64_t row
 }
 
 // ---- pass 1: the histogram of a slice, grid (slices, rows) ---------------------
-// Bound: VALU, 12 f64 operations and an LDS atomic a logit, beside one read of the logits
+// Bound: an LDS atomic and 12 f64 operations a logit (without a branch each where no lane
+// needs one: no change), beside one read of the logits
 // (256 rows of 151936, 156 MB, 42 us: 3.7 TB/s, half of what a plain read reaches; 64
 // rows of 128256 21.6 us; a row alone 9 us, its chain).  A block walks its slice in chunks that it holds in registers; the
 // bins are a ring whose head is the slice's largest value so far, so the row's
