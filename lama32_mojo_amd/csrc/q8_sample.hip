@@ -31,7 +31,9 @@ constexpr int kPerThread = 16;                        // logits a thread holds
 constexpr int kChunk = kHistThreads * kPerThread;
 constexpr int kList = 8192;                           // members of a bin kept in LDS
 // A sum that meets a border exactly (equal logits, a power of two of the mass) has met
-// it, whatever the last bits of the f64 sums say.
+// it, whatever the last bits of the f64 sums say.  The margin covers f64 additions only, so
+// both sides of a comparison are sums of the same weights: a histogram's, which are up to
+// 2^-39 off in one direction, are not compared with those of exp.
 constexpr double kTie = 0x1p-45;
 constexpr int kMaxSlices = 64;
 constexpr int kTop = 256;                             // tokens of a slice that are listed
@@ -811,9 +813,12 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
     b = by_k ? at : min(b, at);
   }
   // a bin's running sums
-  __shared__ double e_upto;
+  __shared__ double e_upto, e_few;
   __shared__ uint32_t e_count;
-  if (t == b) e_count = cupto;
+  if (t == b) {
+    e_count = cupto;
+    e_few = upto;
+  }
   if (t == last) e_upto = upto;
   __syncthreads();
   double W = total;
@@ -866,7 +871,10 @@ __global__ __launch_bounds__(kBins) void sample_draw_kernel(SampleArgs a, int64_
       double *sums = reinterpret_cast<double *>(l.mass);
       sums[t] = sum;
       __syncthreads();
-      const double S = by_k ? sums[min((int64_t)n, s.k) - 1] : total;
+      // top_p's sum: of the first k, or of all that were gathered and of the bins behind
+      // them (the histogram's: off by 2^-39 of what is not here, and by some last bits of
+      // the whole where nothing is, which kTie covers)
+      const double S = by_k ? sums[min((int64_t)n, s.k) - 1] : sums[n - 1] + (total - e_few);
       const bool keep = in && t < s.k && (t == 0 || ((s.top_p >= 1.0 || sum - w < s.top_p * S * (1.0 - kTie)) &&
                                                      w >= s.min_p));
       const int kept = __syncthreads_count(keep);     // (a head of the order)
