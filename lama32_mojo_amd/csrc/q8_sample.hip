@@ -59,6 +59,7 @@ struct BinOf {
   double y, a;
 };
 __device__ __forceinline__ BinOf bin_of(float x, double inv_t) {
+#pragma clang fp contract(off)                        // (the histogram's loop rounds alike)
   BinOf b;
   b.y = (double)x * inv_t;
   if (x == INFINITY) b.y = INFINITY;                  // (T = inf: inf * 0)
@@ -254,6 +255,9 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
     // Adding 1.5 2^52 rounds to a whole number, whose low bits are the bin's; further
     // from 0 than that allows, the plain way.
     if (!s.greedy && __builtin_fabs(top_bin) < 0x1p30) {
+      // The product is rounded before the addition, as bin_of rounds it: one fused operation
+      // would put a logit between two bins into another one than the maximum's says.
+#pragma clang fp contract(off)
       const double scale = s.inv_t * kBinsPerUnit, least = top_bin - kBins + 0.5;
       const uint32_t from = (uint32_t)(head + (int)top_bin);
 #pragma unroll

@@ -53,3 +53,18 @@ def test_tokens_behind_the_border(ctx, temp):
         for u in (0.0, 0.5, 0.999):
             check(ctx, x, temp=temp, top_p=0.5, u=u)
             check(ctx, x, temp=temp, top_p=0.5, min_p=0.5, u=u)
+
+
+@pytest.mark.parametrize("temp", [0.75, 1.25, 1.5, 0.7, 3.0])
+@pytest.mark.parametrize("n", [40, 5000, 20000])
+def test_half_bins(ctx, n, temp):
+    """Logits halfway between two bins' middles, the largest among them."""
+    say("sample half bins", n, temp)
+    rng = np.random.default_rng(n)
+    j = rng.integers(-200, 100, (12, n))
+    x = (np.float64(np.float32(temp)) * (2 * j + 1) / 32).astype(np.float32)
+    for r in range(12):
+        x[r, rng.integers(0, n)] = np.float32(np.float64(np.float32(temp)) * (2 * (100 + 7 * r) + 1) / 32)
+    u = rng.random(12).astype(np.float32)
+    for kw in (dict(), dict(top_p=0.9), dict(k=30, top_p=0.8), dict(min_p=0.03), dict(k=n // 2)):
+        check(ctx, x, temp=temp, u=u, **kw)
