@@ -57,7 +57,10 @@ class Adapters:
     def load(self, i: int, tensors: Mapping[str, np.ndarray], alpha: float) -> None:
         """Adapter i from its lora_A [rank, m] and lora_B [n, rank] matrices (floating
         values, or bf16 bits as uint16) by name; linears that are not named are left
-        alone.  scale = alpha / rank, the largest rank among them."""
+        alone.  The scale of a linear is alpha / its own rank.  (The device has one scale an
+        adapter, that of the largest rank; the B of others are multiplied by the quotient of
+        the two ranks before they are rounded to `dtype`, so in bf16 an update of another rank
+        is off by up to half a step of bf16, 2^-8, unless the quotient is a power of two.)"""
         if not 0 <= i < self.count:
             raise ValueError(f"load: adapter {i} of {self.count}")
         found: dict[tuple, dict] = {}
@@ -96,7 +99,7 @@ class Adapters:
                 if ab is not None:
                     r = ab["lora_A"].shape[0]
                     A[z, :r] = ab["lora_A"]
-                    B[first:first + n, :r] = ab["lora_B"]
+                    B[first:first + n, :r] = ab["lora_B"] * np.float32(rank / r)
                 first += n
             for off, x in ((oa + i * sa, A), (ob + i * sb, B)):
                 x = _bf16_bits(x) if self.dtype == "bf16" else x
