@@ -310,6 +310,9 @@ class Q8Batch:
         if u is not None and (len(u) != len(out_rows) or not set(sample) <= set(slots)):
             raise ValueError(f"forward: {len(u)} random numbers for {len(out_rows)} ids, or settings of a slot "
                              "without tokens")
+        if sample is not None:
+            of = [s for s in slots for _ in (tokens[s] if every else (0,))]
+            settings = self._settings([sample.get(s, Sampling(0.0)) for s in of], u)
         lora = self._adapters_of(slots)
         p.reserve([n + c for n, c in zip(old, counts)])
         p.ix.upload(cu, 4 * p.at["cu"])
@@ -334,8 +337,7 @@ class Q8Batch:
             if logits:
                 flat = self.a.read(olg, len(out_rows) * V).reshape(-1, V)
             elif sample is not None:
-                of = [s for s in slots for _ in (tokens[s] if every else (0,))]
-                flat = self._draw(olg, [sample.get(s, Sampling(0.0)) for s in of], u)
+                flat = self._draw(olg, *settings)
             else:
                 for i in range(len(out_rows)):
                     q8hip.argmax(self.ctx, self.a.buf, olg + i * V, V, self.ids, i)
@@ -363,13 +365,18 @@ class Q8Batch:
             self.loaded = now
         return frozenset().union(*(ad.has[i] for i in used))
 
-    def _draw(self, olg: int, how: Sequence[Sampling], u: Sequence[float]) -> list:
+    @staticmethod
+    def _settings(how: Sequence[Sampling], u: Sequence[float]):
+        """The arrays of q8_sample for rows of these settings: f32 [4 * rows], k."""
+        return (np.array([[h.temperature for h in how], [h.top_p for h in how], [h.min_p for h in how], list(u)],
+                         np.float32).reshape(-1), np.array([h.top_k for h in how], np.int32))
+
+    def _draw(self, olg: int, par: np.ndarray, k: np.ndarray) -> list:
         """(id, log-probability) of each row of logits at olg."""
-        n, V, p = len(how), self.m.cfg.vocab, self.pages
+        n, V, p = len(k), self.m.cfg.vocab, self.pages
         opar = self.a.alloc(5 * n)
-        self.a.write(opar, np.array([[h.temperature for h in how], [h.top_p for h in how], [h.min_p for h in how],
-                                     list(u)], np.float32).reshape(-1))
-        p.ix.upload(np.array([h.top_k for h in how], np.int32), 4 * p.at["k"])
+        self.a.write(opar, par)
+        p.ix.upload(k, 4 * p.at["k"])
         q8hip.sample(self.ctx, self.a.buf, olg, n, V, opar, p.ix, p.at["k"], p.at["drawn"], self.a.buf, opar + 4 * n)
         ids = p.ix.download((n,), np.int32, 4 * p.at["drawn"])
         return list(zip(ids.tolist(), self.a.read(opar + 4 * n, n).tolist()))
