@@ -403,10 +403,10 @@ class Q8Batch:
         """Slot s continues slot source[s], sharing its pages, with its adapter."""
         if any(not 0 <= x < self.slots for pair in source.items() for x in pair):
             raise ValueError("fork: no such slot")
+        self.pages.fork([source.get(s, -1) for s in range(self.slots)])
         was = list(self.adapter)
         for s, f in source.items():
             self.adapter[s] = was[f]
-        self.pages.fork([source.get(s, -1) for s in range(self.slots)])
 
     def compact(self) -> int:
         return self.pages.compact()

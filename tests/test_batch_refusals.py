@@ -6,6 +6,7 @@ import pytest
 
 from lama32_mojo_amd import batch
 from lama32_mojo_amd.batch import Q8Batch, Sampling
+from lama32_mojo_amd.q8hip import Q8_ERR_HIP, Q8Error
 
 
 class Touched(Exception):
@@ -15,6 +16,9 @@ class Touched(Exception):
 class NoDevice:
     length = [3, 4, 0]
     forked = set()
+
+    def fork(self, source):
+        raise Q8Error(Q8_ERR_HIP, "refused")
 
     def reserve(self, want):
         raise Touched
@@ -30,6 +34,18 @@ def a_batch():
             hidden, vocab = 64, 50
     b.m = m
     return b
+
+
+def test_fork():
+    b = a_batch()
+    b.adapter = [0, 1, -1]
+    with pytest.raises(Q8Error):
+        b.fork({2: 0, 1: 0})
+    assert b.adapter == [0, 1, -1]
+    taken = []
+    b.pages.fork = taken.append
+    b.fork({2: 0, 0: 1})
+    assert b.adapter == [1, 1, 0] and taken == [[1, -1, 0]]
 
 
 @pytest.mark.parametrize("how,u", [(Sampling(top_k=1 << 31), 0.5), (Sampling(top_k=-(1 << 31) - 1), 0.5),
