@@ -1447,9 +1447,10 @@ template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream
   const int64_t groups = kv8_most_groups(c.nseq, c.rows);
   const int64_t tiles = cols / NC + groups, rec = c.nkv * kv8_record<HD, NC>();
   // maxima and sums per (row, head), the groups' records (three quarters of the space
-  // at most), then what the sequences' own parts leave
+  // at most), then the sequences' own parts (a block of these, whose runs have two records of
+  // all columns, at least)
   const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4;
-  const int64_t room = (a.ws_floats / 4 * 3 - ml) / rec;
+  const int64_t room = (std::min(a.ws_floats / 4 * 3, a.ws_floats - 2 * rec - c.nseq - 1) - ml) / rec;
   const int64_t units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit * ((cols + NC - 1) / NC) * c.nkv;
   const bool together = units <= kKv8TogetherUnits<HD>;
   // as many blocks as are resident
