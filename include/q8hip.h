@@ -492,8 +492,12 @@ int q8_kv8_attention(q8_ctx *ctx, q8_buf *a, uint64_t oq_f32, int64_t ldq, uint6
  * to the cu, len and table that it was found from: find it again when they change.
  * q8_kv8_attention_shared: as q8_kv8_attention of the same arrays, within the same
  * bounds.  Sequences without a group are served as there.  The context's scratch
- * is used; where the rows of a call leave no room for the groups' records
- * there (some 1800 rows of 32 heads of 128), each sequence reads its own tokens. */
+ * is used, and holds 64 columns (row, query head) of a group by nkv * 64 * (head_dim + 2)
+ * f32 for each part that its tokens are cut into.  It has room for all groups that a call
+ * may have up to some 1800 rows of 32 query and 8 KV heads of 128 or 77 of 32 KV heads; with
+ * more KV heads or sequences (32 KV heads: up to some 1400 rows), groups of more than four
+ * rows for each 64 columns are taken in their order as far as there is room.  Sequences of
+ * the others, and all where one group of all rows would not fit, read their own tokens. */
 uint64_t q8_kv8_share_ints(int64_t nseq, int64_t rows);
 int q8_kv8_share(q8_ctx *ctx, q8_buf *ix, uint64_t ocu_i32, uint64_t olen_i32, uint64_t otab_i32,
                  int64_t nseq, int64_t rows, int64_t maxpages, int64_t npages, int page,

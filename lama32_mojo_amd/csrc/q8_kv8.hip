@@ -472,19 +472,21 @@ __device__ __forceinline__ Kv8ShareAt kv8_share_at(const Kv8Args &c, const int *
 __device__ __forceinline__ int kv8_tokens(const Kv8Args &c, int tok) {
   return clamp_i(tok, 0, c.maxpages * c.page) & ~(c.page - 1);
 }
-// Tokens of sequence i that its group's part of the attention covers.
-__device__ __forceinline__ int kv8_shared_tokens(const Kv8Args &c, const Kv8ShareAt &sh, int i) {
+// Tokens of sequence i that its group's part of the attention covers (kept: the groups
+// that have one).
+__device__ __forceinline__ int kv8_shared_tokens(const Kv8Args &c, const Kv8ShareAt &sh, int i, uint64_t kept) {
   const int g = sh.group[i], tok = sh.tok[i];
-  return g >= 0 && g < sh.groups ? kv8_tokens(c, tok) : 0;
+  return g >= 0 && g < sh.groups && (kept >> g & 1) ? kv8_tokens(c, tok) : 0;
 }
+static_assert(kKv8ShareGroups <= 64, "a group a bit, a group a lane");
 
 // What of a sequence a launch goes through: all its keys, or the ones behind the
 // shared tokens.
 enum { KV8_ALL = 0, KV8_OWN = 1 };
 
 template <bool WHOLE, int NT, int PART>
-__device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, int cols, const Kv8Plan &pl,
-                                        int *wsum) {
+__device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, uint64_t kept, int cols,
+                                        const Kv8Plan &pl, int *wsum) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, nseq = (int)c.nseq;
   const int grp = c.nheads / c.nkv;
   int base = 0;
@@ -496,7 +498,7 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &c, const int *share, int 
       const int a = c.cu[i];
       Kv8Seq s = kv8_seq(a, c.cu[i + 1], c.len[i], c.rows, c.maxpages * c.page, grp, cols);
       if (PART == KV8_OWN) {
-        const int k0 = kv8_shared_tokens(c, kv8_share_at(c, share), i);
+        const int k0 = kv8_shared_tokens(c, kv8_share_at(c, share), i, kept);
         kv8_from(s, k0, c.maxpages * c.page);
         pl.k0[i] = k0;
       }
@@ -565,11 +567,19 @@ struct Kv8Place {
 // The groups' part, a group a lane (whole waves): a block goes through `per` units at most
 // of one row tile of a group, cut so that about `target` blocks have work.  The blocks of
 // group g are base .. base + tiles * cuts - 1, its tiles' cuts one after the other.
+// A call with a limit (kv8_share_room) keeps to `limit` blocks: fewer cuts where it must, and
+// where row tiles alone are more, the first groups that fit.  Of its groups it takes those
+// that save work: a row alone costs a wave a unit, a row tile kKv8Waves.  (32 KV heads of 128,
+// two layers, us with groups / each sequence for itself, behind 400 and 2000 tokens: one group
+// of 160 171 / 217, 205 / 728; 20 groups of 8 190 / 199, 343 / 603; 40 of 4 taken 253 / 203,
+// 647 / 631, left out 233, 660; 64 of 2 taken 299 / 178, 798 / 549, left out 196, 566.)
+// The others have no part (n = 0).
 struct Kv8Groups {
   int lead, tokens, row0, n, units, cuts, base;
   int per, blocks;                       // the same in all lanes
+  uint64_t kept;
 };
-__device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8ShareAt &sh, int target) {
+__device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8ShareAt &sh, int target, int limit) {
   const int lane = threadIdx.x & 63, at = clamp_i(lane, 0, c.nseq - 1);
   Kv8Groups g;
   g.lead = clamp_i(sh.lead[at], 0, c.nseq - 1);
@@ -578,17 +588,31 @@ __device__ __forceinline__ Kv8Groups kv8_groups(const Kv8Args &c, const Kv8Share
   const int end = clamp_i(sh.gcu[at + 1], 0, c.rows);
   g.n = lane < sh.groups && end > g.row0 ? end - g.row0 : 0;
   g.units = (g.tokens + kKv8Unit - 1) / kKv8Unit;
-  const int64_t tiles = ((int64_t)g.n * (c.nheads / c.nkv) + kKv8ShareCols - 1) / kKv8ShareCols;
+  int64_t tiles = ((int64_t)g.n * (c.nheads / c.nkv) + kKv8ShareCols - 1) / kKv8ShareCols;
+  if (limit < kKv8MaxUnits && g.n <= kKv8Waves * tiles) g.n = tiles = 0;
   const int64_t work = tiles * g.units;
   auto add = [](int a, int b) { return kv8_add(a, b); };
-  const int all = wave_scan(work < kKv8MaxUnits ? (int)work : kKv8MaxUnits, add);
-  g.per = kv8_units_per_block(__builtin_amdgcn_readlane(all, 63), target, 1);
-  g.cuts = (g.units + g.per - 1) / g.per;
-  const int64_t blocks = tiles * g.cuts;
-  const int mine = blocks < kKv8MaxUnits ? (int)blocks : kKv8MaxUnits;
-  const int u = wave_scan(mine, add);
-  g.base = u - mine;
-  g.blocks = __builtin_amdgcn_readlane(u, 63);
+  const int all = __builtin_amdgcn_readlane(wave_scan(work < kKv8MaxUnits ? (int)work : kKv8MaxUnits, add), 63);
+  int u;
+  auto cut = [&](int target) {
+    g.per = kv8_units_per_block(all, target, 1);
+    g.cuts = (g.units + g.per - 1) / g.per;
+    const int64_t blocks = tiles * g.cuts;
+    const int mine = blocks < kKv8MaxUnits ? (int)blocks : kKv8MaxUnits;
+    u = wave_scan(mine, add);
+    g.base = u - mine;
+    g.blocks = __builtin_amdgcn_readlane(u, 63);
+  };
+  cut(target);
+  g.kept = ~(uint64_t)0;
+  if (limit < kKv8MaxUnits) {
+    if (g.blocks > limit)
+      cut(kv8_fewer_blocks(limit, __builtin_amdgcn_readlane(
+          wave_scan(tiles < kKv8MaxUnits ? (int)tiles : kKv8MaxUnits, add), 63)));
+    if (u > limit) g.n = 0;              // (u ascends over the lanes)
+    g.kept = __builtin_amdgcn_ballot_w64(g.n > 0);
+    g.blocks = g.kept ? __builtin_amdgcn_readlane(u, 63 - __builtin_clzll(g.kept)) : 0;
+  }
   return g;
 }
 
@@ -618,7 +642,7 @@ template <int HD> __device__ __forceinline__ void kv8_shared_block(const Kv8Attn
   const int64_t k_at = (int64_t)g * P * HD, v_at = (int64_t)(c.nkv + g) * P * HD;
   const float qscale = 1.44269504088896341f / sqrtf((float)HD);
   const Kv8ShareAt sh = kv8_share_at(c, a.share);
-  const Kv8Groups gs = kv8_groups(c, sh, a.shared_target);
+  const Kv8Groups gs = kv8_groups(c, sh, a.shared_target, a.shared_limit);
   const int b = blockIdx.x;
   if (b >= gs.blocks) return;             // (the whole block)
   // the last group that begins at this block or before and has any
@@ -884,7 +908,12 @@ __global__ __launch_bounds__(WHOLE ? 512 : 64 * kKv8Waves, 2) void kv8_attn_kern
   pl.old = pl.n + nseq;
   pl.k0 = pl.old + nseq;
 
-  const int units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, NC, pl, wsum);
+  uint64_t kept = ~(uint64_t)0;           // groups that have a part of their own
+  if constexpr (PART == KV8_OWN) {
+    if (a.shared_limit < kKv8MaxUnits)
+      kept = kv8_groups(c, kv8_share_at(c, a.share), a.shared_target, a.shared_limit).kept;
+  }
+  const int units = kv8_plan<WHOLE, 64 * NW, PART>(c, a.share, kept, NC, pl, wsum);
   const int runs = ((int)gridDim.x - first) * RW, run = bx * RW + w;
   const int per = WHOLE ? 1 : kv8_units_per_block(units, runs, 1);
   // the merge reads the plan behind the records
@@ -1208,12 +1237,12 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(Kv8AttnArgs a, int runs,
   auto load = [&](int i) {
     group = sh.group[i];
     pos = sh.pos[i];
-    shared = kv8_shared_tokens(c, sh, i);
+    shared = kv8_shared_tokens(c, sh, i, gs.kept);
     unit0 = pre[i];
   };
   if constexpr (PART == KV8_OWN) {
     sh = kv8_share_at(c, a.share);
-    gs = kv8_groups(c, sh, a.shared_target);
+    gs = kv8_groups(c, sh, a.shared_target, a.shared_limit);
     if (nseq <= 64) load(min(t & 63, nseq - 1));
   }
   // the sequence of this row: the last one that begins at it or before
@@ -1446,26 +1475,29 @@ template <int HD> static hipError_t launch_kv8_shared_t(Kv8AttnArgs a, hipStream
   const int64_t grp = c.nheads / c.nkv, cols = c.rows * grp;
   const int64_t groups = kv8_most_groups(c.nseq, c.rows);
   const int64_t tiles = cols / NC + groups, rec = c.nkv * kv8_record<HD, NC>();
-  // maxima and sums per (row, head), the groups' records (three quarters of the space
-  // at most), then the sequences' own parts (a block of these, whose runs have two records of
-  // all columns, at least)
+  // maxima and sums per (row, head), the groups' records, then the sequences' own parts (a
+  // block of these, whose runs have two records of all columns, at least)
   const int64_t ml = (2 * c.rows * c.nheads + 3) / 4 * 4;
-  const int64_t room = (std::min(a.ws_floats / 4 * 3, a.ws_floats - 2 * rec - c.nseq - 1) - ml) / rec;
   const int64_t units = (c.maxpages * c.page + kKv8Unit - 1) / kKv8Unit * ((cols + NC - 1) / NC) * c.nkv;
   const bool together = units <= kKv8TogetherUnits<HD>;
   // as many blocks as are resident
   const int64_t want = ((together ? 512 : 768) + c.nkv - 1) / c.nkv;
-  a.shared_target = (int)std::min(want, room - tiles);
+  const Kv8Room room = kv8_share_room(a.ws_floats, ml, rec, 2 * rec, c.nseq + 1, (512 + c.nkv - 1) / c.nkv,
+                                      (cols + NC - 1) / NC, tiles, want);
   // (more rows than there is room for: every sequence for itself)
-  if (a.shared_target < std::min<int64_t>(want, 8) || groups == 0) return launch_kv8_attention(a, st);
-  const int64_t blocks = a.shared_target + tiles, recs = blocks * rec;
+  if (room.blocks == 0 || groups == 0) return launch_kv8_attention(a, st);
+  const int64_t blocks = room.blocks, recs = blocks * rec;
+  a.shared_target = room.target;
+  a.shared_limit = room.limit;
   a.ml = a.ws;
   a.shared_rec = a.ws + ml;
   a.shared_blocks = (int)blocks;
-  a.shared_first = together ? (int)blocks : 0;
+  // (blocks that leave at once would only be in the way of the sequences' own: 64 groups of 2
+  // rows, see kv8_groups, 745 / 573 us in one launch / in two)
+  a.shared_first = together && room.limit == kKv8MaxUnits ? (int)blocks : 0;
   a.ws += ml + recs;
   a.ws_floats -= ml + recs;
-  if (!together) {
+  if (a.shared_first == 0) {
     hipLaunchKernelGGL(kv8_shared_kernel<HD>, dim3((unsigned)blocks, (unsigned)c.nkv), dim3(64 * kKv8Waves), 0, st,
                        a);
     const hipError_t e = hipGetLastError();

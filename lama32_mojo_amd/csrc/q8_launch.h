@@ -294,7 +294,7 @@ struct Kv8AttnArgs {
   // shared prefixes: what q8_kv8_share wrote; the others are set by the launch
   const int *share;
   float *ml, *shared_rec;
-  int shared_target, shared_blocks, shared_first;
+  int shared_target, shared_limit, shared_blocks, shared_first;
 };
 // Sequences of one call: their unit counts are summed in LDS.
 constexpr int kKv8MaxSeq = 4096;

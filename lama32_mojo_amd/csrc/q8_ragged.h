@@ -86,4 +86,31 @@ Q8_HD int kv8_units_per_block(int64_t units, int nruns, int least) {
   return (int)(per < least ? least : per);
 }
 
+// Blocks that the groups' parts of a call with shared prefixes are cut into: about
+// `target`, of which there is room for `blocks` records.  limit: what a call's groups
+// must keep to (kKv8MaxUnits: they do so whatever they are).
+struct Kv8Room {
+  int blocks, target, limit;             // blocks 0: no room
+};
+// rec: a block's record; ml: what else lies there; own, plan: records of a block of the
+// sequences' own parts and what is behind them; all in floats.  nb: such blocks that a call
+// would have.  one: row tiles of a group that has all rows, most: of as many groups as there
+// may be (cut into `target` parts of equal work, t row tiles are target + t blocks at most).
+// Three quarters of the space are the groups'.  Where these do not hold the tiles that there
+// may be and 8 cuts (32 KV heads of 128: from 78 sequences of a row on), the call has a limit:
+// what the nb blocks leave, if that holds one group of all rows and 8 cuts.
+Q8_HD Kv8Room kv8_share_room(int64_t ws, int64_t ml, int64_t rec, int64_t own, int64_t plan, int64_t nb,
+                             int64_t one, int64_t most, int64_t want) {
+  const int64_t least = want < 8 ? want : 8;
+  const int64_t part = ws / 4 * 3 < ws - own - plan ? ws / 4 * 3 : ws - own - plan;
+  int64_t room = part > ml ? (part - ml) / rec : 0;
+  const int64_t target = room - most < want ? room - most : want;
+  if (target >= least) return {(int)(target + most), (int)target, kKv8MaxUnits};
+  room = (ws - ml - nb * own - plan) / rec;
+  if (room - one < least) return {0, 0, 0};
+  return {(int)room, (int)(want < room ? want : room), (int)room};
+}
+// The target with which `tiles` row tiles keep to `limit` blocks (tiles alone, from there on).
+Q8_HD int kv8_fewer_blocks(int limit, int tiles) { return limit - tiles > 1 ? limit - tiles : 1; }
+
 }  // namespace q8
