@@ -603,9 +603,11 @@ int q8_lora(q8_ctx *ctx, q8_buf *w, int w_dtype, uint64_t oa, int64_t a_stride, 
  * T <= 0 takes the first token of the order.  Settings that are NaN are off (u: 0, T:
  * the first token).  With lp non-null, lp[r] at olp is the log of the id's w over
  * the kept sum (f32).  Logits that are -inf or NaN are never drawn; of a row with
- * +inf, only those are; a row without any token gives id -1 and -inf.  Weights and
- * sums are held to 2^-40 and f64, in an order that depends on the inputs alone, so
- * equal inputs give equal ids.  1 <= n <= 2^22.  The context's scratch is used
+ * +inf, only those are; a row without any token gives id -1 and -inf.  Weights are
+ * within 2^-39 of exp's and summed to f64, in an order that depends on the inputs alone:
+ * equal inputs give equal ids, the ones above unless u or a border lies within 2^-39
+ * of a running sum (at most one draw in two million where 10^5 tokens are kept).  Sums of equal logits
+ * that meet a border exactly have met it.  1 <= n <= 2^22.  The context's scratch is used
  * (q8_set_stream). */
 int q8_sample(q8_ctx *ctx, q8_buf *a, uint64_t ox_f32, int64_t ldx, int64_t rows, int64_t n,
               uint64_t oparam_f32, q8_buf *ids, uint64_t otopk_i32, uint64_t oid_i32, q8_buf *lp,

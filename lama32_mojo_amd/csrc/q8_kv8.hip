@@ -1461,8 +1461,10 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t st) {
 }
 
 // The groups' part (a row tile of 64 columns cut over blocks), each sequence's own
-// part, and the merge that joins them.  Little work in the groups (by its bound, units of
-// row tiles and KV heads) takes one launch with the sequences' parts: a launch less,
+// part, and the merge that joins them.  Little work in the groups (units of row tiles and
+// KV heads) takes one launch with the sequences' parts.  The rule goes by what the tables can
+// hold, not by what they do: a launch is sized without the arrays, so that a captured one fits
+// all of them, and a table with room to spare takes two launches.  One is a launch less,
 // but two blocks a CU where alone it has three (us together / apart, 8 KV heads: 64
 // sequences of 500 tokens behind 8000, heads of 128, 128 / 137; 64 behind 8000 with
 // pages of 128 73 / 72, behind 16000 98 / 90; 128 behind 32000 252 / 227; heads of 64:

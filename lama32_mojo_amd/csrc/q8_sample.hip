@@ -12,8 +12,10 @@
 // numbers of 2^-40: integer sums, so the order of the atomics does not matter and
 // equal inputs give equal ids; over bins they are summed in f64 in a fixed order.
 // Bins reach 64 below the maximum (e^-64 of the largest weight: 2^22 such tokens
-// are 2^-70 of the sum, less than a f64 sum can hold).  Sums in f32 would be off
-// by 2^-24 of the mass, as much as the step of a f32 u.
+// are 2^-70 of the sum, less than a f64 sum can hold).  With the series' error they are
+// within 2^-39 of exp, so an id is not the definition's where u or a border lies that close
+// to a running sum.  Sums in f32 would be off by 2^-24 of the mass, as much as the step of
+// a f32 u.
 #include "q8_device.h"
 #include "q8_launch.h"
 
@@ -184,8 +186,8 @@ __device__ __forceinline__ RowSettings settings(const SampleArgs &a, int64_t row
 // ---- pass 1: the histogram of a slice, grid (slices, rows) ---------------------
 // Bound: an LDS atomic and 12 f64 operations a logit (without a branch each where no lane
 // needs one: no change), beside one read of the logits
-// (256 rows of 151936, 156 MB, 42 us: 3.7 TB/s, half of what a plain read reaches; 64
-// rows of 128256 21.6 us; a row alone 9 us, its chain).  A block walks its slice in chunks that it holds in registers; the
+// (medians: 256 rows of 151936, 156 MB, 43 us: 3.6 TB/s, half of what a plain read reaches;
+// 64 rows of 128256 21 us; a row alone 9.8 us, its chain).  A block walks its slice in chunks that it holds in registers; the
 // bins are a ring whose head is the slice's largest value so far, so the row's
 // maximum need not be known first.
 __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs a, int64_t row0,
@@ -341,10 +343,11 @@ __global__ __launch_bounds__(kHistThreads, 8) void sample_hist_kernel(SampleArgs
 // ---- pass 2: one block of kBins threads per row --------------------------------
 // The slices' bins are added up; where the kept tokens are few they are sorted and
 // the filters and the draw are one running sum, else each border's bin is looked into.
-// Bound: the chain of dependent reads, searches and block-wide sums (13 us where few
-// tokens are kept, a third of it fetching code for its first use), and for rows that keep many the second read of their logits by one
-// CU: 12 us for 128256, with the selections behind it 35 us (64 rows) to 58 us (256 rows
-// of 151936, whose read alone takes 23 us, 6.8 TB/s).
+// Bound: the chain of dependent reads, searches and block-wide sums (14 us where few
+// tokens are kept, a third of it fetching code for its first use), and for rows that keep many
+// the second read of their logits by one CU: 12 us for 128256, with the selections behind it
+// 46 us (median of 64 mixed rows; 35 where the draws are easy) to 67 us (256 rows of 151936
+// with top-p, 58 at best; their read alone takes 23 us, 6.8 TB/s).
 
 // The bin that a border falls into, the sums before it and up to it, its own.
 struct BorderBin {
