@@ -54,6 +54,23 @@ def test_many_kv_heads(ctx, monkeypatch, ns, nh, nkv):
     assert max_rel_err(s.run(ctx, q), ref) <= 1e-5
 
 
+@pytest.mark.parametrize("P,nkv,hd,ns,most", [(128, 32, 128, 90, 1), (64, 32, 128, 60, 5), (16, 32, 64, 700, 3)])
+def test_pages_and_rows(ctx, monkeypatch, P, nkv, hd, ns, most):
+    """The same with other pages and heads, several rows a sequence, tables with room to spare,
+    rows behind the last sequence and q inside wider rows."""
+    say("shared limit", P, hd, ns)
+    rng = np.random.default_rng(ns)
+    lens = rng.integers(1, most + 1, ns).tolist()
+    s = Step(rng, lens, [0 if i % 5 else -1 for i in range(ns)], [2], rng.integers(0, 20, ns), P, nkv, hd)
+    s.table = np.concatenate([s.table, np.full((ns, 300), -1, np.int32)], axis=1)
+    s.maxpages += 300
+    q = queries(rng, s.T, nkv, hd)
+    y, members = hidden(ctx, monkeypatch, s, q)
+    ref = s.ref(q)
+    assert members and max_rel_err(y, ref) <= 1e-5
+    assert np.array_equal(s.check(ctx, q, dead=3, off=3, extra=7), s.run(ctx, q, dead=3))
+
+
 def outside(y, members, groups):
     """The groups whose members read their own tables; every other group is read by its leader."""
     nan = np.isnan(y).any((1, 2))
